@@ -375,6 +375,65 @@ int rka_adamw_step(float* const* params, const float* const* grads, float* const
                    float* const* exp_avg_sqs, const size_t* numels, int count, double lr, double beta1,
                    double beta2, double eps, double weight_decay, int step, void* stream);
 
+/*
+ * The gated delta rule, a recurrence whose state is a matrix.  Per batch row and
+ * value head, with the state S [key_dim, value_dim] in float32:
+ *
+ *   S~ = exp(g_t) S_{t-1};  e_t = v_t - S~^T k_t;  S_t = S~ + k_t (beta_t e_t)^T;
+ *   o_t = scale S_t^T q_t.
+ *
+ * q, k [batch, tokens, key_heads, key_dim], v [batch, tokens, value_heads,
+ * value_dim] and o (as v, dense) are of `dtype`; g (the logarithm of the decay, at
+ * most 0; -infinity empties the state) and beta [batch, tokens, value_heads] of
+ * `gate_dtype`.  Value head h uses key head h / (value_heads / key_heads).
+ * key_dim is at most 256.  With `normalize` q and k are divided by
+ * sqrt(|.|^2 + 1e-6) first.  States [batch, value_heads, key_dim, value_dim] are
+ * dense float32.  `strides` is a host array of 15 element strides: (batch row,
+ * token, head) of q, k, v, g and beta in turn; a head's elements are contiguous.
+ * (No counterpart in the reference, whose one recurrence is the GRU.)
+ */
+#define RKA_DTYPE_F32 0
+#define RKA_DTYPE_BF16 1
+
+/* Workspace of the calls below, and what a forward saves for its backward
+ * (0 for sizes that the calls refuse). */
+size_t rka_gated_delta_forward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
+                                               int value_dim);
+size_t rka_gated_delta_reserve_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim, int value_dim);
+size_t rka_gated_delta_backward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
+                                                int value_dim);
+
+/* Whole sequences.  initial_state NULL: zeros.  lengths (device, [batch], or NULL):
+ * row b ends after lengths[b] tokens (clamped to 0 .. tokens); what lies behind is
+ * not read, its outputs are 0.  `reserve` non-NULL saves what the backward needs. */
+int rka_gated_delta_forward(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                            const float* initial_state, const int* lengths, void* o, float* final_state, void* reserve,
+                            void* workspace, size_t workspace_bytes, int batch, int tokens, int key_heads,
+                            int value_heads, int key_dim, int value_dim, const long long* strides, int dtype,
+                            int gate_dtype, int normalize, double scale, void* stream);
+
+/* Its gradients, dense, of the inputs' types; those of tokens behind a row's length
+ * are 0.  grad_o and grad_final_state may be NULL (zeros), grad_initial_state NULL
+ * (not wanted).  dq and dk are summed over the value heads that share a key head in a
+ * fixed order. */
+int rka_gated_delta_backward(const void* q, const void* k, const void* g, const void* beta, const int* lengths,
+                             const void* reserve, const void* grad_o, const float* grad_final_state, void* grad_q,
+                             void* grad_k, void* grad_v, void* grad_g, void* grad_beta, float* grad_initial_state,
+                             void* workspace, size_t workspace_bytes, int batch, int tokens, int key_heads,
+                             int value_heads, int key_dim, int value_dim, const long long* strides, int dtype,
+                             int gate_dtype, int normalize, double scale, void* stream);
+
+/* One token of each of `batch` requests (q, k [batch, key_heads, key_dim] and so on;
+ * the token strides are not used).  state [num_slots, value_heads, key_dim, value_dim]
+ * is updated in place: request b has state slots[b] (device, [batch]), or b if slots is
+ * NULL.  Slots have to be distinct.  A negative slot is a request without a state
+ * (padding of the batch): its output is 0; one from num_slots up gives NaN.  Neither
+ * touches a state. */
+int rka_gated_delta_step(const void* q, const void* k, const void* v, const void* g, const void* beta, float* state,
+                         const int* slots, int num_slots, void* o, int batch, int key_heads, int value_heads,
+                         int key_dim, int value_dim, const long long* strides, int dtype, int gate_dtype, int normalize,
+                         double scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 """MI355X (gfx950) fp32 GRU training path: hand-written HIP kernels behind a
 C ABI (librnn_kernel_amd.so), with an nn.GRU-compatible PyTorch front end."""
+from .delta import GatedDeltaFunction, gated_delta_rule, gated_delta_step
 from .gru import (
     GRU,
     GRUFunction,
@@ -15,6 +16,9 @@ from .gru import (
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "GatedDeltaFunction",
+    "gated_delta_rule",
+    "gated_delta_step",
     "AdamW",
     "HeadFunction",
     "LinearHead",

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_PKG_DIR, "librnn_kernel_amd.so")
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LLP = ctypes.POINTER(ctypes.c_longlong)
 SIGNATURES = {
     "rka_version": (_I, []),
     "rka_last_error": (ctypes.c_char_p, []),
@@ -59,6 +60,12 @@ SIGNATURES = {
     "rka_head_backward_workspace_bytes": (_SZ, [_I, _I]),
     "rka_head_backward": (_I, [_P] * 7 + [_SZ, _I, _I, _P]),
     "rka_adamw_step": (_I, [ctypes.POINTER(_P)] * 4 + [ctypes.POINTER(_SZ), _I] + [ctypes.c_double] * 5 + [_I, _P]),
+    "rka_gated_delta_forward_workspace_bytes": (_SZ, [_I] * 6),
+    "rka_gated_delta_reserve_bytes": (_SZ, [_I] * 6),
+    "rka_gated_delta_backward_workspace_bytes": (_SZ, [_I] * 6),
+    "rka_gated_delta_forward": (_I, [_P] * 11 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
+    "rka_gated_delta_backward": (_I, [_P] * 15 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
+    "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
 }
 NUM_STAGES = 6
 
