@@ -434,6 +434,35 @@ int rka_gated_delta_step(const void* q, const void* k, const void* v, const void
                          int key_dim, int value_dim, const long long* strides, int dtype, int gate_dtype, int normalize,
                          double scale, void* stream);
 
+/*
+ * The matrix product with its epilogue, y = act(x W^T + b) + r: x [rows, inputs],
+ * W [outputs, inputs], b [outputs] or NULL, r [rows, outputs] or NULL and y [rows,
+ * outputs], all of `dtype`; y and z are dense, the others' rows lie ldx, ldw and ldr
+ * elements apart (at most 2^21).  Sums, bias, activation and residual are in float32.
+ * (The reference's F.linear, src/rnn_kernel/a100/prod/gru.py:519-523, has neither.)
+ */
+#define RKA_ACT_NONE 0
+#define RKA_ACT_RELU 1
+#define RKA_ACT_GELU 2 /* z Phi(z), by the error function */
+#define RKA_ACT_SILU 3
+#define RKA_ACT_SIGMOID 4
+#define RKA_ACT_LOGSIGMOID 5
+
+size_t rka_linear_forward_workspace_bytes(int rows, int outputs, int inputs, int dtype);
+size_t rka_linear_backward_workspace_bytes(int rows, int outputs, int inputs, int dtype);
+
+/* `z` non-NULL receives x W^T + b (dense, of `dtype`) for the backward. */
+int rka_linear_forward(const void* x, long long ldx, const void* weight, long long ldw, const void* bias,
+                       const void* residual, long long ldr, void* y, void* z, void* workspace, size_t workspace_bytes,
+                       int rows, int outputs, int inputs, int act, int dtype, void* stream);
+
+/* dz = dy act'(z) (z may be NULL without an activation); grad_x = dz W, grad_weight =
+ * dz^T x, grad_bias = the sum of dz's rows, each dense, or NULL if it is not wanted.
+ * Every sum has a fixed order. */
+int rka_linear_backward(const void* grad_y, long long ldy, const void* x, long long ldx, const void* weight, long long ldw,
+                        const void* z, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                        size_t workspace_bytes, int rows, int outputs, int inputs, int act, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

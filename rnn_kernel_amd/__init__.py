@@ -13,9 +13,13 @@ from .gru import (
     is_supported_gru,
     set_strict,
 )
+from .linear import Linear, LinearFunction, linear
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "Linear",
+    "LinearFunction",
+    "linear",
     "GatedDeltaFunction",
     "gated_delta_rule",
     "gated_delta_step",

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_PKG_DIR, "librnn_kernel_amd.so")
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
 _LLP = ctypes.POINTER(ctypes.c_longlong)
 SIGNATURES = {
     "rka_version": (_I, []),
@@ -65,6 +66,10 @@ SIGNATURES = {
     "rka_gated_delta_backward_workspace_bytes": (_SZ, [_I] * 6),
     "rka_gated_delta_forward": (_I, [_P] * 11 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
     "rka_gated_delta_backward": (_I, [_P] * 15 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
+    "rka_linear_forward_workspace_bytes": (_SZ, [_I] * 4),
+    "rka_linear_backward_workspace_bytes": (_SZ, [_I] * 4),
+    "rka_linear_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
+    "rka_linear_backward": (_I, [_P, _LL, _P, _LL, _P, _LL] + [_P] * 5 + [_SZ] + [_I] * 5 + [_P]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
 }
 NUM_STAGES = 6
