@@ -398,10 +398,10 @@ int rka_adamw_step(float* const* params, const float* const* grads, float* const
 /* Workspace of the calls below, and what a forward saves for its backward
  * (0 for sizes that the calls refuse). */
 size_t rka_gated_delta_forward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
-                                               int value_dim);
+                                               int value_dim, int dtype);
 size_t rka_gated_delta_reserve_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim, int value_dim);
 size_t rka_gated_delta_backward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
-                                                int value_dim);
+                                                int value_dim, int dtype);
 
 /* Whole sequences.  initial_state NULL: zeros.  lengths (device, [batch], or NULL):
  * row b ends after lengths[b] tokens (clamped to 0 .. tokens); what lies behind is

@@ -61,9 +61,9 @@ SIGNATURES = {
     "rka_head_backward_workspace_bytes": (_SZ, [_I, _I]),
     "rka_head_backward": (_I, [_P] * 7 + [_SZ, _I, _I, _P]),
     "rka_adamw_step": (_I, [ctypes.POINTER(_P)] * 4 + [ctypes.POINTER(_SZ), _I] + [ctypes.c_double] * 5 + [_I, _P]),
-    "rka_gated_delta_forward_workspace_bytes": (_SZ, [_I] * 6),
+    "rka_gated_delta_forward_workspace_bytes": (_SZ, [_I] * 7),
     "rka_gated_delta_reserve_bytes": (_SZ, [_I] * 6),
-    "rka_gated_delta_backward_workspace_bytes": (_SZ, [_I] * 6),
+    "rka_gated_delta_backward_workspace_bytes": (_SZ, [_I] * 7),
     "rka_gated_delta_forward": (_I, [_P] * 11 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
     "rka_gated_delta_backward": (_I, [_P] * 15 + [_SZ] + [_I] * 6 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
     "rka_linear_forward_workspace_bytes": (_SZ, [_I] * 4),

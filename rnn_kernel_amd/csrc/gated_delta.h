@@ -1,6 +1,8 @@
-// Declarations shared by the gated delta rule's translation units
-// (gated_delta.hip: entry points, per-chunk products and gradients;
-// gated_delta_chain.hip: the chains over chunks; gated_delta_step.hip: one token).
+// Declarations shared by the gated delta rule's translation units: gated_delta.hip
+// (entry points, what is made for all chunks at once before the chains),
+// gated_delta_chain.h (the chains over chunks), gated_delta_grad.hip (the gradients
+// made for all chunks at once after the backward's chain), gated_delta_step.hip (one
+// token).
 //
 // Per batch row and value head, with S [Dk, Dv] in float32:
 //   S~ = exp(g_t) S_{t-1};  e_t = v_t - S~^T k_t;  S_t = S~ + k_t (beta_t e_t)^T;
@@ -13,9 +15,8 @@
 //   E = T (V - diag(exp G) K S)
 //   O = scale diag(exp G) Q S + P E,          P = lower part of scale (Q K^T * L) diag(beta)
 //   S' = exp(G_C) S + K^T diag(exp(G_C - G) beta) E
-// T and P hang on no state, so they are made for all chunks at once ("prepare");
-// only E, O and S' go from chunk to chunk ("chain").  Columns of S, V, E and O do
-// not mix, so a wavefront takes 16 of them through all chunks on its own.
+// T and P hang on no state, so they are made for all chunks at once; only E, O and S'
+// go from chunk to chunk.  Columns of S, V, E and O do not mix.
 //
 // With dS' the gradient of S' and dO that of O:
 //   B dU = P^T dO + diag(exp(G_C - G) beta) K dS'          (B = diag(beta))
@@ -30,6 +31,14 @@
 //   dG_i = q_i . dq_i + k_i . dk_i(read) - beta_i dbeta_i, and for the chunk's last
 //   token also sum_j beta_j k_j . W_j + exp(G_C) <S, dS'>;  dg = dG summed from the end.
 // beta is never divided by: it may be zero.
+//
+// All products run on the bf16 matrix cores.  A float32 is the sum of three bf16 values
+// (24 bits in three rounded pieces of 8), a bf16 is one; of the products of pieces
+// those up to 2^-16 of the largest are taken, smallest first, each exact and summed in
+// float32: three where one operand is bf16, six where neither is.  The error is that
+// of a float32 product (lower pieces of numbers under some 2^-110 are lost).  One
+// 16x16x32 bf16 instruction takes 16 clocks, the eight 16x16x4 float32 ones for the same
+// block 256.
 #pragma once
 
 #include "rka_internal.h"
@@ -43,6 +52,8 @@ constexpr int kMaxKeyDim = 256;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // Element types of q, k, v, o and their gradients.
 struct bf16 {
@@ -62,6 +73,9 @@ __device__ __forceinline__ bf16 from_f32<bf16>(float x) {
     const __bf16 y = (__bf16)x;
     return bf16{__builtin_bit_cast(unsigned short, y)};
 }
+// bf16 pieces of a value of type T
+template <typename T>
+constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
 
 // A call's sizes and where its tensors lie (strides in elements: batch row,
 // token, head; the head's elements are contiguous).
@@ -90,25 +104,104 @@ __device__ __forceinline__ void store_gate(void* p, long long i, float v, int is
 // NaN stays NaN.
 __device__ __forceinline__ float floor_gate(float g) { return g < -200.f ? -200.f : g; }
 
+// Running sums of the floored gates of a chunk (by one wavefront; lane = token).
+// In 64 bits: a difference of sums is as exact after a closed gate as before it.
+__device__ __forceinline__ double chunk_sum(float g, int lane) {
+    double s = floor_gate(g);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const double up = __shfl_up(s, o);
+        if (lane >= o) s += up;
+    }
+    return s;
+}
+
 __device__ __forceinline__ int row_length(const int* lengths, int b, int T) {
     return lengths ? max(0, min(T, lengths[b])) : T;
 }
 
-// Per chunk and head, made by `prepare` (a chunk past the row's length has none):
-// kCoefs rows of 64 floats, then exp(G_C).
-enum Coef { RK = 0, WK, RQ, BETA, CK, CQ, NCOEF };
+// ------------------------------------------------- pieces and products ---
+// Four values as N pieces of four bf16 each.
+template <int N>
+__device__ __forceinline__ void split(f32x4 x, u32x2 (&p)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bf16x2 v = {(__bf16)x[2 * h], (__bf16)x[2 * h + 1]};
+            p[c][h] = __builtin_bit_cast(unsigned, v);
+            if (c + 1 < N) {
+                x[2 * h] -= __uint_as_float(p[c][h] << 16);
+                x[2 * h + 1] -= __uint_as_float(p[c][h] & 0xffff0000u);
+            }
+        }
+}
+// Eight values as N fragments of a lane.
+template <int N>
+__device__ __forceinline__ void split8(f32x4 lo, f32x4 hi, u32x4 (&p)[N]) {
+    u32x2 a[N], b[N];
+    split<N>(lo, a);
+    split<N>(hi, b);
+#pragma unroll
+    for (int c = 0; c < N; ++c) p[c] = u32x4{a[c][0], a[c][1], b[c][0], b[c][1]};
+}
+
+// c += A B for a 16x16x32 block in NA and NB pieces.  Lane l holds row (A) or column
+// (B) l % 16 at the sum's indices 8 (l / 16) .. + 7; of the result column l % 16, rows 4
+// (l / 16) .. + 3.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mul(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
+    constexpr int most = (NA < NB ? NB : NA) - 1;
+#pragma unroll
+    for (int s = most; s >= 0; --s)
+#pragma unroll
+        for (int i = NA - 1; i >= 0; --i) {
+            const int j = s - i;
+            if (j < 0 || j >= NB) continue;
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[j]),
+                                                        c, 0, 0, 0);
+        }
+    return c;
+}
+
+// ------------------------------------------------------- chunk operands ---
+// A "fragment" is what one matrix instruction takes of an operand: 64 lanes x 16 bytes.
+constexpr int kFragLanes = 64;
+
+// 32-wide steps over Dk.
+inline __host__ __device__ int key_steps(int Dk) { return (Dk + 31) / 32; }
+// The steps that the chains' instances are made for: 2, 4, 6 or 8.
+inline __host__ __device__ int chain_steps(int Dk) { return (Dk + 63) / 64 * 2; }
+
+// Of a chunk's q or k, per key head, in kPieces<T> pieces: rows for the products over
+// Dk, [16-token block][step][piece], and transposed for those over tokens,
+// [16-wide block of Dk][32-token step][piece].  Each 4 steps (8 blocks x 2) fragments.
+template <typename T>
+inline __host__ __device__ size_t row_frags(int Dk) {
+    return (size_t)4 * chain_steps(Dk) * kPieces<T>;
+}
+
+// The fragments of a lower triangular 64x64 matrix (or, transposed, of an upper one)
+// that are not all zero, of 16 rows x 32 of the sum: six.
+//   lower: rows 0, 1: step 0; rows 2, 3: steps 0, 1.   (i, w) at i + w * 2 (w = 1: i >= 2)
+//   upper: rows 0, 1: steps 0, 1; rows 2, 3: step 1.
+constexpr int kTriFrags = 6;
+inline __host__ __device__ constexpr int lower_frag(int i, int w) { return w == 0 ? i : i + 2; }
+inline __host__ __device__ constexpr int upper_frag(int i, int w) { return w == 0 ? i : i + 2; }
+
+// Per chunk and value head (a chunk past the row's length has none): rows of 64
+// floats, then exp(G_C).
 //   RK: exp(G) ck;  WK: exp(G_C - G) ck beta;  RQ: scale exp(G) cq;  CK, CQ: what
 //   normalises k and q (1 if nothing does)
+enum Coef { RK = 0, WK, RQ, BETA, CK, CQ, NCOEF };
 constexpr int kCoefFloats = NCOEF * kChunk + 4;
-// T and P as 16x16 blocks of the lower triangle, block (i, j) at i (i + 1) / 2 + j,
-// each 256 floats in the order that a matrix instruction's operand takes them.
-constexpr int kBlocks = 10;
-constexpr int kTriFloats = kBlocks * 256;
 
 struct ChunkData {
-    float* coef;  // [chunk-head][kCoefFloats]
-    float* t;     // [chunk-head][kTriFloats]
-    float* p;
+    float* coef;        // [value chunk-head][kCoefFloats]
+    float* norm;        // [key chunk-head][2][64]: CK, CQ
+    u32x4 *k, *q;       // [key chunk-head] row fragments
+    u32x4 *kt, *qt;     // [key chunk-head] transposed (qt: backward only)
+    u32x4 *t, *p;       // [value chunk-head][kTriFrags][3]: T and P, or their transposes
 };
 
 // Gradients' inputs and outputs that pass between the backward's launches.
@@ -122,19 +215,19 @@ struct BackwardData {
 };
 
 // The launches below take lengths == nullptr for rows of T tokens each.
-// Forward operands (transpose false) or the backward's transposed ones (true).
-template <typename T>
-int launch_prepare(const Dims& d, const T* q, const T* k, const void* g, const void* beta, const int* lengths,
-                   const ChunkData& out, bool transpose, hipStream_t stream);
 // states, e: saved for the backward, or both null.
 template <typename T>
-int launch_chain_forward(const Dims& d, const T* q, const T* k, const T* v, const float* s0, const int* lengths,
-                         const ChunkData& in, T* o, float* state_out, float* states, float* e, hipStream_t stream);
+int launch_chain_forward(const Dims& d, const T* v, const float* s0, const int* lengths, const ChunkData& in, T* o,
+                         float* state_out, float* states, float* e, hipStream_t stream);
 // dstate_out (of the final state), dO: either may be null (zeros).
 template <typename T>
-int launch_chain_backward(const Dims& d, const T* q, const T* k, const T* dout, const float* dstate_out,
-                          const int* lengths, const ChunkData& in, T* dv, float* ds0, const BackwardData& bd,
-                          hipStream_t stream);
+int launch_chain_backward(const Dims& d, const T* dout, const float* dstate_out, const int* lengths, const ChunkData& in,
+                          T* dv, float* ds0, const BackwardData& bd, hipStream_t stream);
+// dq, dk, dg, dbeta after the chain.
+template <typename T>
+int launch_gradients(const Dims& d, const T* q, const T* k, const T* dout, const void* g, const int* lengths,
+                     const ChunkData& in, const BackwardData& bd, T* dq, T* dk, void* dg, void* dbeta,
+                     hipStream_t stream);
 
 // A call's sizes and its other arguments, checked (the errors of the C entries).
 int make_dims(const char* what, int B, int T, int Hk, int Hv, int Dk, int Dv, Dims* d);

@@ -1,6 +1,5 @@
-// The gated delta rule (gated_delta.h has the formulas): entry points, what is made
-// for all chunks at once before the chains (prepare) and the gradients made after
-// the backward's chain.
+// The gated delta rule (gated_delta.h has the formulas): entry points, and what is made
+// for all chunks at once before the chains.
 #include "gated_delta.h"
 
 #include <algorithm>
@@ -10,58 +9,103 @@ namespace delta {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLd = 68;  // row of a 64-wide LDS tile: 16 bytes past a multiple of all banks
+
+// A chunk's q (which = 1) or k (0) as fragments, by rows and transposed, and what
+// normalises its rows.  The chunk is staged in LDS once, as it is.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void rows_kernel(Dims d, const T* q, const T* k, const int* lengths, ChunkData out) {
+    constexpr int NP = kPieces<T>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    T* rows = reinterpret_cast<T*>(lds);
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, hi = lane / 16;
+    const int which = blockIdx.x % 2, kch = blockIdx.x / 2, c = kch % d.chunks, bk = kch / d.chunks;
+    const int b = bk / d.Hk, hk = bk % d.Hk, t0 = c * kChunk;
+    const int live = min(kChunk, row_length(lengths, b, d.T) - t0);
+    if (live <= 0) return;
+    const int steps = chain_steps(d.Dk), width = steps * 32, ld = width + 8;
+    const long long* st = which ? d.q_s : d.k_s;
+    const T* src = (which ? q : k) + b * st[0] + t0 * st[1] + hk * st[2];
+    for (int i = tid; i < kChunk * width; i += kThreads) {
+        const int r = i / width, e = i % width;
+        rows[r * ld + e] = r < live && e < d.Dk ? src[r * st[1] + e] : from_f32<T>(0.f);
+    }
+    __syncthreads();
+    {
+        float x2 = 0.f;
+        for (int e = tid % 4; e < d.Dk; e += 4) {
+            const float x = to_f32(rows[tid / 4 * ld + e]);
+            x2 += x * x;
+        }
+        x2 += __shfl_xor(x2, 1);
+        x2 += __shfl_xor(x2, 2);
+        if (tid % 4 == 0)
+            out.norm[((size_t)kch * 2 + which) * kChunk + tid / 4] = d.normalize ? 1.f / sqrtf(x2 + kNormEps) : 1.f;
+    }
+    const size_t at = (size_t)kch * row_frags<T>(d.Dk) * kFragLanes;
+    u32x4* byrow = (which ? out.q : out.k) + at;
+    for (int f = wave; f < 4 * steps; f += kThreads / 64) {
+        const T* p = rows + (f / steps * 16 + n) * ld + f % steps * 32 + 8 * hi;
+        u32x4 x[NP];
+        split8<NP>(f32x4{to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])},
+                   f32x4{to_f32(p[4]), to_f32(p[5]), to_f32(p[6]), to_f32(p[7])}, x);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) byrow[(f * NP + i) * kFragLanes + lane] = x[i];
+    }
+    u32x4* turned = which ? out.qt : out.kt;
+    if (!turned) return;
+    turned += at;
+    for (int f = wave; f < 4 * steps; f += kThreads / 64) {  // 2 steps blocks of Dk x 2 steps of tokens
+        const T* p = rows + (f % 2 * 32 + 8 * hi) * ld + f / 2 * 16 + n;
+        u32x4 x[NP];
+        split8<NP>(f32x4{to_f32(p[0]), to_f32(p[ld]), to_f32(p[2 * ld]), to_f32(p[3 * ld])},
+                   f32x4{to_f32(p[4 * ld]), to_f32(p[5 * ld]), to_f32(p[6 * ld]), to_f32(p[7 * ld])}, x);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) turned[(f * NP + i) * kFragLanes + lane] = x[i];
+    }
+}
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// rows x 64 elements (from column d0 of `width`) of a strided matrix as float32 in
-// LDS; zero past `live` rows and the width.
-template <typename T>
-__device__ __forceinline__ void stage64(float* lds, const T* src, long long stride, int live, int d0, int width,
-                                        int tid) {
+constexpr int kLd = 68;  // row of a 64-wide LDS tile: 16 bytes past a multiple of all banks
+
+// c += A B of 16x16 blocks in LDS in float32: rows of A at a, rows of B at b.
+__device__ __forceinline__ f32x4 block_product(const float* a, const float* b, int n, int hi, f32x4 c) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a + n * kLd + 4 * hi);
 #pragma unroll
-    for (int i = 0; i < kChunk * 16 / kThreads; ++i) {
-        const int r = (tid + i * kThreads) / 16, c = (tid + i * kThreads) % 16 * 4;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (r < live) {
+    for (int r = 0; r < 4; ++r) c = mfma4(x[r], b[(4 * hi + r) * kLd + n], c);
+    return c;
+}
+// The same with B as a result block in registers.
+__device__ __forceinline__ f32x4 block_product(const float* a, f32x4 b, int n, int hi, f32x4 c) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a + n * kLd + 4 * hi);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (d0 + c + j < width) x[j] = to_f32(src[r * stride + d0 + c + j]);
-        }
-        *reinterpret_cast<f32x4*>(lds + r * kLd + c) = x;
-    }
+    for (int r = 0; r < 4; ++r) c = mfma4(x[r], b[r], c);
+    return c;
+}
+__device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) to[(4 * hi + r) * kLd + n] = x[r];
 }
 
-// Running sums of the floored gates of a chunk (by one wavefront; lane = token).
-// In 64 bits: a difference of sums is as exact after a closed gate as before it.
-__device__ __forceinline__ double chunk_sum(float g, int lane) {
-    double s = floor_gate(g);
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const double up = __shfl_up(s, o);
-        if (lane >= o) s += up;
-    }
-    return s;
-}
-
-// T and P of a chunk.  K K^T and Q K^T on fp32 matrix instructions, then the inverse of the
-// unit lower triangular I + N diag(beta) by forward substitution, one column per
-// lane (backward stable, which a series of powers of N is not).
+// T and P of a chunk and value head.  The inverse of I + N diag(beta) in float32: its
+// 16x16 diagonal blocks by forward substitution (a column per lane), then the blocks
+// below from theirs, [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1], for 32 and 64 rows.
+// (Backward stable; a series of powers of N is not where keys are alike.)
 template <typename T, bool TRANSPOSE>
-__global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* q, const T* k, const void* g,
-                                                           const void* beta, const int* lengths, ChunkData out) {
-    __shared__ float ks[kChunk * kLd], qs[kChunk * kLd], nb[kChunk * kLd], ps[kChunk * kLd];
+__global__ __launch_bounds__(kThreads) void triangles_kernel(Dims d, const void* g, const void* beta, const int* lengths,
+                                                             ChunkData out) {
+    constexpr int NP = kPieces<T>;
+    __shared__ __attribute__((aligned(16))) float nb[kChunk * kLd], ti[kChunk * kLd];
     __shared__ double gsum[kChunk];
     __shared__ float bet[kChunk], ck[kChunk], cq[kChunk];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, hi = lane / 16;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, hi = lane / 16;
     const int c = blockIdx.x % d.chunks, bh = blockIdx.x / d.chunks;
     const int b = bh / d.Hv, h = bh % d.Hv, hk = h / (d.Hv / d.Hk);
     const int t0 = c * kChunk, live = min(kChunk, row_length(lengths, b, d.T) - t0);
     if (live <= 0) return;
-    const T* kb = k + b * d.k_s[0] + t0 * d.k_s[1] + hk * d.k_s[2];
-    const T* qb = q + b * d.q_s[0] + t0 * d.q_s[1] + hk * d.q_s[2];
+    const size_t ch = blockIdx.x, kch = ((size_t)b * d.Hk + hk) * d.chunks + c;
     if (wave == 0) {
         float gv = 0.f, bv = 0.f;
         if (lane < live) {
@@ -70,46 +114,33 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* q, c
         }
         gsum[lane] = chunk_sum(gv, lane);
         bet[lane] = bv;
+    } else if (wave == 1) {
+        ck[lane] = out.norm[kch * 2 * kChunk + lane];
+        cq[lane] = out.norm[(kch * 2 + 1) * kChunk + lane];
     }
+    const int steps = chain_steps(d.Dk);
+    const u32x4* fk = out.k + kch * row_frags<T>(d.Dk) * kFragLanes + lane;
+    const u32x4* fq = out.q + kch * row_frags<T>(d.Dk) * kFragLanes + lane;
     f32x4 kk[4] = {}, qk[4] = {};
-    float k2 = 0.f, q2 = 0.f;
-    for (int d0 = 0; d0 < d.Dk; d0 += 64) {
-        __syncthreads();
-        stage64(ks, kb, d.k_s[1], live, d0, d.Dk, tid);
-        stage64(qs, qb, d.q_s[1], live, d0, d.Dk, tid);
-        __syncthreads();
-        // a quarter of a row's squares per thread
+    for (int u = 0; u < steps; ++u) {
+        u32x4 a[NP], aq[NP];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float x = ks[tid / 4 * kLd + tid % 4 * 16 + j], y = qs[tid / 4 * kLd + tid % 4 * 16 + j];
-            k2 += x * x;
-            q2 += y * y;
+        for (int i = 0; i < NP; ++i) {
+            a[i] = fk[((wave * steps + u) * NP + i) * kFragLanes];
+            aq[i] = fq[((wave * steps + u) * NP + i) * kFragLanes];
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const f32x4 ak = *reinterpret_cast<const f32x4*>(ks + (16 * wave + n) * kLd + s * 16 + hi * 4);
-            const f32x4 aq = *reinterpret_cast<const f32x4*>(qs + (16 * wave + n) * kLd + s * 16 + hi * 4);
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) break;
+            u32x4 x[NP];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j > wave) break;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(ks + (16 * j + n) * kLd + s * 16 + hi * 4);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    kk[j] = mfma4(ak[r], x[r], kk[j]);
-                    qk[j] = mfma4(aq[r], x[r], qk[j]);
-                }
-            }
+            for (int i = 0; i < NP; ++i) x[i] = fk[((j * steps + u) * NP + i) * kFragLanes];
+            kk[j] = mul(a, x, kk[j]);
+            qk[j] = mul(aq, x, qk[j]);
         }
-    }
-    k2 += __shfl_xor(k2, 1);
-    q2 += __shfl_xor(q2, 1);
-    k2 += __shfl_xor(k2, 2);
-    q2 += __shfl_xor(q2, 2);
-    if (tid % 4 == 0) {
-        ck[tid / 4] = d.normalize ? 1.f / sqrtf(k2 + kNormEps) : 1.f;
-        cq[tid / 4] = d.normalize ? 1.f / sqrtf(q2 + kNormEps) : 1.f;
     }
     __syncthreads();
+    f32x4 p[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -122,9 +153,9 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* q, c
                 pv = d.scale * qk[j][r] * cq[row] * w;
             }
             nb[row * kLd + col] = nv;
-            ps[row * kLd + col] = pv;
+            ti[row * kLd + col] = 0.f;
+            p[j][r] = pv;
         }
-    const size_t ch = blockIdx.x;
     if (tid < kChunk) {
         float* coef = out.coef + ch * kCoefFloats;
         const float eg = expf((float)gsum[tid]), el = expf((float)(gsum[kChunk - 1] - gsum[tid]));
@@ -138,326 +169,92 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* q, c
         if (tid == 0) coef[NCOEF * kChunk] = expf((float)gsum[kChunk - 1]);
     }
     __syncthreads();
-    if (wave == 0) {
-        float x[kChunk];
+    {
+        // the wavefront's own diagonal block (the four 16-lane groups alike)
+        const float* a = nb + 16 * wave * kLd + 16 * wave;
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            float v = i == lane ? 1.f : 0.f;
+        for (int i = 0; i < 16; ++i) {
+            float v = i == n ? 1.f : 0.f;
 #pragma unroll
-            for (int m = 0; m < i; ++m) v = fmaf(-nb[i * kLd + m], x[m], v);
+            for (int m = 0; m < i; ++m) v = fmaf(-a[i * kLd + m], x[m], v);
             x[i] = v;
         }
-        __builtin_amdgcn_wave_barrier();
+        if (hi == 0) {
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) nb[i * kLd + lane] = x[i];
+            for (int i = 0; i < 16; ++i) ti[(16 * wave + i) * kLd + 16 * wave + n] = x[i];
+        }
     }
     __syncthreads();
-    float* tt = out.t + ch * kTriFloats;
-    float* pp = out.p + ch * kTriFloats;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j > wave) break;
-        const int blk = (wave * (wave + 1) / 2 + j) * 256 + lane * 4;
-        f32x4 tv, pv;
-        if constexpr (TRANSPOSE) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                tv[r] = nb[(16 * wave + 4 * hi + r) * kLd + 16 * j + n];
-                pv[r] = ps[(16 * wave + 4 * hi + r) * kLd + 16 * j + n];
-            }
-        } else {
-            tv = *reinterpret_cast<const f32x4*>(nb + (16 * wave + n) * kLd + 16 * j + 4 * hi);
-            pv = *reinterpret_cast<const f32x4*>(ps + (16 * wave + n) * kLd + 16 * j + 4 * hi);
-        }
-        *reinterpret_cast<f32x4*>(tt + blk) = tv;
-        *reinterpret_cast<f32x4*>(pp + blk) = pv;
+    auto at = [&](float* m, int i, int j) { return m + 16 * i * kLd + 16 * j; };
+    if (wave == 1 || wave == 3) {
+        const f32x4 y = block_product(at(nb, wave, wave - 1), at(ti, wave - 1, wave - 1), n, hi, f32x4{});
+        put_result(at(ti, wave, wave - 1), -block_product(at(ti, wave, wave), y, n, hi, f32x4{}), n, hi);
     }
-}
-
-
-constexpr int kLdV = 36;  // row of a 32-wide LDS tile
-
-// 64 rows x 32 columns (from v0 of Dv) of a dense matrix of row stride `stride` as
-// float32 in LDS, zero past `rows` rows and Dv.
-template <typename T>
-__device__ __forceinline__ void stage32(float* lds, const T* src, long long stride, int rows, int v0, int Dv, int tid) {
-#pragma unroll
-    for (int i = 0; i < kChunk * 8 / kThreads; ++i) {
-        const int r = (tid + i * kThreads) / 8, c = (tid + i * kThreads) % 8 * 4;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (src && r < rows) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (v0 + c + j < Dv) x[j] = to_f32(src[r * stride + v0 + c + j]);
-        }
-        *reinterpret_cast<f32x4*>(lds + r * kLdV + c) = x;
-    }
-}
-
-// Sum over the 16 lanes that hold a row of a 16x16 block.
-__device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 1);
-    x += __shfl_xor(x, 2);
-    x += __shfl_xor(x, 4);
-    x += __shfl_xor(x, 8);
-    return x;
-}
-
-// The gradients of q, k, g and beta of a chunk and value head.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void gradients_kernel(Dims d, const T* q, const T* k, const T* dout, const void* g,
-                                                             const int* lengths, ChunkData in, BackwardData bd, void* dg,
-                                                             void* dbeta) {
-    __shared__ float f1[kChunk * kLd], f2[kChunk * kLd], ks[kChunk * kLd], qs[kChunk * kLd];
-    __shared__ float sdo[kChunk * kLdV], sdx[kChunk * kLdV], se[kChunk * kLdV], ss[kChunk * kLdV], sds[kChunk * kLdV];
-    __shared__ double gsum[kChunk];
-    __shared__ float sums[4][kChunk], dots[4];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, hi = lane / 16;
-    const int c = blockIdx.x % d.chunks, bh = blockIdx.x / d.chunks;
-    const int b = bh / d.Hv, h = bh % d.Hv, hk = h / (d.Hv / d.Hk);
-    const int t0 = c * kChunk, live = min(kChunk, row_length(lengths, b, d.T) - t0);
-    const size_t ch = blockIdx.x;
-    const size_t row0 = ((size_t)b * d.T + t0) * d.Hv + h;  // token row of the [B, T, Hv] tensors
-    if (live <= 0) {
-        if (tid < min(kChunk, d.T - t0)) {
-            store_gate(dg, row0 + (size_t)tid * d.Hv, 0.f, d.gate_bf16);
-            store_gate(dbeta, row0 + (size_t)tid * d.Hv, 0.f, d.gate_bf16);
-        }
-        return;
-    }
-    const float* coef = in.coef + ch * kCoefFloats;
-    if (wave == 0)
-        gsum[lane] = chunk_sum(
-            lane < live ? load_gate(g, b * d.g_s[0] + (t0 + lane) * d.g_s[1] + h * d.g_s[2], d.gate_bf16) : 0.f, lane);
-    const T* pdo = dout ? dout + row0 * d.Dv : nullptr;
-    const float* pdx = bd.dx + row0 * d.Dv;
-    const float* pe = bd.e + row0 * d.Dv;
-    const float* ps = bd.states + ch * d.Dk * d.Dv;
-    const float* pds = bd.dstates + ch * d.Dk * d.Dv;
-    const long long vrow = (long long)d.Hv * d.Dv;
+    __syncthreads();
     {
-        f32x4 a1[4] = {}, a2[4] = {};
-        for (int v0 = 0; v0 < d.Dv; v0 += 32) {
-            __syncthreads();
-            stage32(sdo, pdo, vrow, live, v0, d.Dv, tid);
-            stage32(sdx, pdx, vrow, live, v0, d.Dv, tid);
-            stage32(se, pe, vrow, live, v0, d.Dv, tid);
-            __syncthreads();
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const f32x4 x1 = *reinterpret_cast<const f32x4*>(sdo + (16 * wave + n) * kLdV + s * 16 + hi * 4);
-                const f32x4 x2 = *reinterpret_cast<const f32x4*>(sdx + (16 * wave + n) * kLdV + s * 16 + hi * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j > wave) break;
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(se + (16 * j + n) * kLdV + s * 16 + hi * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        a1[j] = mfma4(x1[r], y[r], a1[j]);
-                        a2[j] = mfma4(x2[r], y[r], a2[j]);
-                    }
-                }
-            }
+        // block (2 + i, j) of the lower left quarter
+        const int i = wave / 2, j = wave % 2;
+        f32x4 sum{};
+        for (int m = 0; m <= i; ++m) {
+            f32x4 y{};
+            for (int l = j; l < 2; ++l) y = block_product(at(nb, 2 + m, l), at(ti, l, j), n, hi, y);
+            sum = block_product(at(ti, 2 + i, 2 + m), y, n, hi, sum);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                const float w = row >= col ? expf((float)(gsum[row] - gsum[col])) : 0.f;
-                f1[row * kLd + col] = row >= col ? d.scale * a1[j][r] * w : 0.f;
-                f2[row * kLd + col] = row > col ? -a2[j][r] * w : 0.f;
-            }
+        put_result(at(ti, 2 + i, j), -sum, n, hi);
     }
-    const T* kb = k + b * d.k_s[0] + t0 * d.k_s[1] + hk * d.k_s[2];
-    const T* qb = q + b * d.q_s[0] + t0 * d.q_s[1] + hk * d.q_s[2];
-    // exp(G) and exp(G_C - G) of the thread's rows
-    float eg[4], el[4], cki[4], cqi[4], bi[4], rq[4] = {}, rk[4] = {}, rz[4] = {}, rw[4] = {}, dot = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = 16 * wave + 4 * hi + r;
-        eg[r] = expf((float)gsum[row]);
-        el[r] = expf((float)(gsum[kChunk - 1] - gsum[row]));
-        cki[r] = coef[CK * kChunk + row];
-        cqi[r] = coef[CQ * kChunk + row];
-        bi[r] = coef[BETA * kChunk + row];
-    }
-    for (int d0 = 0; d0 < d.Dk; d0 += 64) {
-        f32x4 aq[4] = {}, ar[4] = {}, az[4] = {};
-        for (int v0 = 0; v0 < d.Dv; v0 += 32) {
-            __syncthreads();
-            if (v0 == 0) {
-                stage64(ks, kb, d.k_s[1], live, d0, d.Dk, tid);
-                stage64(qs, qb, d.q_s[1], live, d0, d.Dk, tid);
-            }
-            stage32(sdo, pdo, vrow, live, v0, d.Dv, tid);
-            stage32(sdx, pdx, vrow, live, v0, d.Dv, tid);
-            stage32(se, pe, vrow, live, v0, d.Dv, tid);
-            stage32(ss, ps + (size_t)d0 * d.Dv, d.Dv, d.Dk - d0, v0, d.Dv, tid);
-            stage32(sds, pds + (size_t)d0 * d.Dv, d.Dv, d.Dk - d0, v0, d.Dv, tid);
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kChunk * 32 / kThreads; ++i) {
-                const int r = (tid + i * kThreads) / 32, cc = (tid + i * kThreads) % 32;
-                dot += ss[r * kLdV + cc] * sds[r * kLdV + cc];
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int at = (16 * wave + n) * kLdV + s * 16 + hi * 4;
-                const f32x4 xo = *reinterpret_cast<const f32x4*>(sdo + at);
-                const f32x4 xx = *reinterpret_cast<const f32x4*>(sdx + at);
-                const f32x4 xe = *reinterpret_cast<const f32x4*>(se + at);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 ys = *reinterpret_cast<const f32x4*>(ss + (16 * j + n) * kLdV + s * 16 + hi * 4);
-                    const f32x4 yd = *reinterpret_cast<const f32x4*>(sds + (16 * j + n) * kLdV + s * 16 + hi * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        aq[j] = mfma4(xo[r], ys[r], aq[j]);
-                        ar[j] = mfma4(xx[r], ys[r], ar[j]);
-                        az[j] = mfma4(xe[r], yd[r], az[j]);
-                    }
-                }
-            }
-        }
-        // now in terms of the normalised keys and queries
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                aq[j][r] *= d.scale * eg[r];
-                ar[j][r] *= -eg[r];
-                az[j][r] *= el[r];
-                rw[r] += az[j][r] * ks[row * kLd + col] * cki[r];
-            }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {  // 16 tokens of the sum
-            const f32x4 ckm = *reinterpret_cast<const f32x4*>(coef + CK * kChunk + 16 * m + 4 * hi);
-            const f32x4 cqm = *reinterpret_cast<const f32x4*>(coef + CQ * kChunk + 16 * m + 4 * hi);
-            const f32x4 bm = *reinterpret_cast<const f32x4*>(coef + BETA * kChunk + 16 * m + 4 * hi);
-            const f32x4 x1 = *reinterpret_cast<const f32x4*>(f1 + (16 * wave + n) * kLd + 16 * m + 4 * hi);
-            const f32x4 x2 = *reinterpret_cast<const f32x4*>(f2 + (16 * wave + n) * kLd + 16 * m + 4 * hi);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int tok = 16 * m + 4 * hi + r;
-                const float xt1 = f1[tok * kLd + 16 * wave + n], xt2 = f2[tok * kLd + 16 * wave + n];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float kv = ks[tok * kLd + 16 * j + n] * ckm[r], qv = qs[tok * kLd + 16 * j + n] * cqm[r];
-                    aq[j] = mfma4(x1[r] * bm[r], kv, aq[j]);
-                    ar[j] = mfma4(x2[r] * bm[r], kv, ar[j]);
-                    az[j] = mfma4(xt1, qv, az[j]);
-                    az[j] = mfma4(xt2, kv, az[j]);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                const float kv = ks[row * kLd + col] * cki[r], qv = qs[row * kLd + col] * cqi[r];
-                rq[r] += aq[j][r] * qv;
-                rk[r] += ar[j][r] * kv;
-                rz[r] += az[j][r] * kv;
-                if (row < live && d0 + col < d.Dk) {
-                    const size_t at = (row0 + (size_t)row * d.Hv) * d.Dk + d0 + col;
-                    bd.dq[at] = aq[j][r];
-                    bd.dk[at] = ar[j][r] + bi[r] * az[j][r];
-                }
-            }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = 16 * wave + 4 * hi + r;
-        const float a = row_sum(rq[r]), bb = row_sum(rk[r]), z = row_sum(rz[r]), w = row_sum(rw[r]);
-        if (n == 0) {
-            sums[0][row] = a;
-            sums[1][row] = bb;
-            sums[2][row] = z;
-            sums[3][row] = w * bi[r];
-        }
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) dot += __shfl_xor(dot, o);
-    if (lane == 0) dots[wave] = dot;
     __syncthreads();
-    if (wave != 0) return;
-    float w = sums[3][lane];
+    // P where N was (which nobody reads any more)
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) w += __shfl_xor(w, o);
-    const float db = sums[2][lane];
-    float dgv = sums[0][lane] + sums[1][lane] - coef[BETA * kChunk + lane] * db;
-    if (lane == 63) dgv += w + expf((float)gsum[kChunk - 1]) * (dots[0] + dots[1] + dots[2] + dots[3]);
+    for (int j = 0; j < 4; ++j) put_result(at(nb, wave, j), p[j], n, hi);
+    __syncthreads();
+    u32x4* ft = out.t + ch * (size_t)(kTriFrags * 3 * kFragLanes) + lane;
+    u32x4* fp = out.p + ch * (size_t)(kTriFrags * 3 * kFragLanes) + lane;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const float down = __shfl_down(dgv, o);
-        if (lane + o < 64) dgv += down;
-    }
-    if (lane < min(kChunk, d.T - t0)) {
-        store_gate(dg, row0 + (size_t)lane * d.Hv, lane < live ? dgv : 0.f, d.gate_bf16);
-        store_gate(dbeta, row0 + (size_t)lane * d.Hv, lane < live ? db : 0.f, d.gate_bf16);
-    }
-}
-
-__device__ __forceinline__ float wave_sum(float x) {
+    for (int w = 0; w < 2; ++w) {
+        if (TRANSPOSE ? w < wave / 2 : w > wave / 2) continue;
+        const int f = TRANSPOSE ? upper_frag(wave, w) : lower_frag(wave, w);
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
-    return x;
-}
-
-// dq and dk of the key heads: the sum over the value heads that share one, then
-// the normalisation's gradient, dx = c (dy - y (y . dy)) with y = c x.  A wavefront
-// per token and key head.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void finish_kernel(Dims d, const T* q, const T* k, const int* lengths,
-                                                          BackwardData bd, T* dq, T* dk) {
-    constexpr int M = kMaxKeyDim / 64;
-    const long long row = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
-    if (row >= (long long)d.B * d.T * d.Hk) return;
-    const int lane = threadIdx.x % 64, hk = (int)(row % d.Hk), rep = d.Hv / d.Hk;
-    const long long bt = row / d.Hk;
-    const int b = (int)(bt / d.T), t = (int)(bt % d.T);
-    const bool on = t < row_length(lengths, b, d.T);
+        for (int m = 0; m < 2; ++m) {
+            const float* from = m ? nb : ti;
+            f32x4 x[2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const float* part = (which ? bd.dk : bd.dq) + (bt * d.Hv + (long long)hk * rep) * d.Dk;
-        const T* x = which ? k + b * d.k_s[0] + t * d.k_s[1] + hk * d.k_s[2] : q + b * d.q_s[0] + t * d.q_s[1] + hk * d.q_s[2];
-        T* out = (which ? dk : dq) + row * d.Dk;
-        float v[M], xv[M], x2 = 0.f, xd = 0.f;
+            for (int e = 0; e < 8; ++e)
+                x[e / 4][e % 4] = TRANSPOSE ? from[(32 * w + 8 * hi + e) * kLd + 16 * wave + n]
+                                            : from[(16 * wave + n) * kLd + 32 * w + 8 * hi + e];
+            u32x4 y[3];
+            split8<3>(x[0], x[1], y);
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const int i = lane + 64 * m;
-            v[m] = xv[m] = 0.f;
-            if (!on || i >= d.Dk) continue;
-            for (int r = 0; r < rep; ++r) v[m] += part[(long long)r * d.Dk + i];
-            xv[m] = to_f32(x[i]);
-            x2 += xv[m] * xv[m];
-            xd += xv[m] * v[m];
+            for (int i = 0; i < 3; ++i) (m ? fp : ft)[(f * 3 + i) * kFragLanes] = y[i];
         }
-        if (d.normalize) {
-            x2 = wave_sum(x2);
-            xd = wave_sum(xd);
-            const float c = 1.f / sqrtf(x2 + kNormEps);
-#pragma unroll
-            for (int m = 0; m < M; ++m) v[m] = c * (v[m] - c * c * xd * xv[m]);
-        }
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-            if (lane + 64 * m < d.Dk) out[lane + 64 * m] = from_f32<T>(v[m]);
     }
 }
 
-struct ForwardLayout {
-    size_t coef, t, p, total;
+// ---------------------------------------------------------- workspaces ---
+struct ChunkLayout {
+    size_t coef, norm, k, q, kt, qt, t, p, total;
 };
-ForwardLayout forward_layout(long long chunk_heads) {
-    ForwardLayout l{};
-    l.coef = 0;
-    l.t = align_up((size_t)chunk_heads * kCoefFloats * sizeof(float), 256);
-    l.p = l.t + align_up((size_t)chunk_heads * kTriFloats * sizeof(float), 256);
-    l.total = l.p + align_up((size_t)chunk_heads * kTriFloats * sizeof(float), 256);
+// `qt` only where the backward wants it.  Sized for float32 pieces where `wide`.
+ChunkLayout chunk_layout(const Dims& d, bool wide, bool backward) {
+    ChunkLayout l{};
+    const size_t ch = (size_t)d.B * d.Hv * d.chunks, kch = (size_t)d.B * d.Hk * d.chunks;
+    const size_t rows = kch * (wide ? row_frags<float>(d.Dk) : row_frags<bf16>(d.Dk)) * kFragLanes * 16;
+    const size_t tri = ch * kTriFrags * 3 * kFragLanes * 16;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t was = at;
+        at += align_up(bytes, 256);
+        return was;
+    };
+    l.coef = take(ch * kCoefFloats * sizeof(float));
+    l.norm = take(kch * 2 * kChunk * sizeof(float));
+    l.k = take(rows);
+    l.q = take(rows);
+    l.kt = take(rows);
+    l.qt = backward ? take(rows) : 0;
+    l.t = take(tri);
+    l.p = take(tri);
+    l.total = at;
     return l;
 }
 struct ReserveLayout {
@@ -471,12 +268,12 @@ ReserveLayout reserve_layout(const Dims& d) {
     return l;
 }
 struct BackwardLayout {
-    ForwardLayout f;
+    ChunkLayout f;
     size_t dstates, dx, dq, dk, total;
 };
-BackwardLayout backward_layout(const Dims& d) {
+BackwardLayout backward_layout(const Dims& d, bool wide) {
     BackwardLayout l{};
-    l.f = forward_layout((long long)d.B * d.Hv * d.chunks);
+    l.f = chunk_layout(d, wide, true);
     l.dstates = l.f.total;
     l.dx = l.dstates + align_up((size_t)d.B * d.Hv * d.chunks * d.Dk * d.Dv * sizeof(float), 256);
     l.dq = l.dx + align_up((size_t)d.B * d.T * d.Hv * d.Dv * sizeof(float), 256);
@@ -485,19 +282,45 @@ BackwardLayout backward_layout(const Dims& d) {
     return l;
 }
 
-ChunkData chunk_data(char* ws, const ForwardLayout& l) {
-    return ChunkData{reinterpret_cast<float*>(ws + l.coef), reinterpret_cast<float*>(ws + l.t),
-                     reinterpret_cast<float*>(ws + l.p)};
+ChunkData chunk_data(char* ws, const ChunkLayout& l) {
+    ChunkData c{};
+    c.coef = reinterpret_cast<float*>(ws + l.coef);
+    c.norm = reinterpret_cast<float*>(ws + l.norm);
+    c.k = reinterpret_cast<u32x4*>(ws + l.k);
+    c.q = reinterpret_cast<u32x4*>(ws + l.q);
+    c.kt = reinterpret_cast<u32x4*>(ws + l.kt);
+    c.qt = l.qt ? reinterpret_cast<u32x4*>(ws + l.qt) : nullptr;
+    c.t = reinterpret_cast<u32x4*>(ws + l.t);
+    c.p = reinterpret_cast<u32x4*>(ws + l.p);
+    return c;
+}
+
+template <typename T>
+int prepare(const Dims& d, const T* q, const T* k, const void* g, const void* beta, const int* lengths,
+            const ChunkData& out, bool transpose, hipStream_t stream) {
+    const long long blocks = (long long)d.B * d.Hv * d.chunks, rows = (long long)d.B * d.Hk * d.chunks * 2;
+    if (blocks == 0) return 0;
+    RKA_RETURN_IF_ERR(check_grid(std::max(blocks, rows), kThreads, "gated_delta"));
+    const size_t lds = (size_t)kChunk * (chain_steps(d.Dk) * 32 + 8) * sizeof(T);
+    RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T>),
+                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)rows), dim3(kThreads), lds, stream, d, q, k, lengths, out);
+    RKA_RETURN_IF_HIP(hipGetLastError());
+    if (transpose)
+        hipLaunchKernelGGL((triangles_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, g, beta, lengths, out);
+    else
+        hipLaunchKernelGGL((triangles_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, g, beta, lengths, out);
+    RKA_RETURN_IF_HIP(hipGetLastError());
+    return 0;
 }
 
 template <typename T>
 int forward(const Dims& d, const void* q, const void* k, const void* v, const void* g, const void* beta, const float* s0,
             const int* lengths, void* o, float* state_out, char* reserve, char* ws, hipStream_t s) {
-    const ChunkData cd = chunk_data(ws, forward_layout((long long)d.B * d.Hv * d.chunks));
-    const T *tq = static_cast<const T*>(q), *tk = static_cast<const T*>(k), *tv = static_cast<const T*>(v);
-    RKA_RETURN_IF_ERR(launch_prepare<T>(d, tq, tk, g, beta, lengths, cd, false, s));
+    const ChunkData cd = chunk_data(ws, chunk_layout(d, sizeof(T) == 4, false));
+    RKA_RETURN_IF_ERR(prepare<T>(d, static_cast<const T*>(q), static_cast<const T*>(k), g, beta, lengths, cd, false, s));
     const ReserveLayout r = reserve_layout(d);
-    return launch_chain_forward<T>(d, tq, tk, tv, s0, lengths, cd, static_cast<T*>(o), state_out,
+    return launch_chain_forward<T>(d, static_cast<const T*>(v), s0, lengths, cd, static_cast<T*>(o), state_out,
                                    reserve ? reinterpret_cast<float*>(reserve + r.states) : nullptr,
                                    reserve ? reinterpret_cast<float*>(reserve + r.e) : nullptr, s);
 }
@@ -506,28 +329,16 @@ template <typename T>
 int backward(const Dims& d, const void* q, const void* k, const void* g, const void* beta, const int* lengths,
              const char* reserve, const void* dout, const float* dstate_out, void* dq, void* dk, void* dv, void* dg,
              void* dbeta, float* ds0, char* ws, hipStream_t s) {
-    const BackwardLayout l = backward_layout(d);
+    const BackwardLayout l = backward_layout(d, sizeof(T) == 4);
     const ReserveLayout r = reserve_layout(d);
     const ChunkData cd = chunk_data(ws, l.f);
     const T *tq = static_cast<const T*>(q), *tk = static_cast<const T*>(k), *tdo = static_cast<const T*>(dout);
     const BackwardData bd{reinterpret_cast<const float*>(reserve + r.states), reinterpret_cast<const float*>(reserve + r.e),
                           reinterpret_cast<float*>(ws + l.dstates), reinterpret_cast<float*>(ws + l.dx),
                           reinterpret_cast<float*>(ws + l.dq), reinterpret_cast<float*>(ws + l.dk)};
-    RKA_RETURN_IF_ERR(launch_prepare<T>(d, tq, tk, g, beta, lengths, cd, true, s));
-    RKA_RETURN_IF_ERR(
-        launch_chain_backward<T>(d, tq, tk, tdo, dstate_out, lengths, cd, static_cast<T*>(dv), ds0, bd, s));
-    const long long blocks = (long long)d.B * d.Hv * d.chunks;
-    if (blocks == 0) return 0;
-    RKA_RETURN_IF_ERR(check_grid(blocks, kThreads, "gated_delta_backward"));
-    hipLaunchKernelGGL((gradients_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, s, d, tq, tk, tdo, g, lengths, cd,
-                       bd, dg, dbeta);
-    RKA_RETURN_IF_HIP(hipGetLastError());
-    const long long rows = (long long)d.B * d.T * d.Hk, fin = (rows + kThreads / 64 - 1) / (kThreads / 64);
-    RKA_RETURN_IF_ERR(check_grid(fin, kThreads, "gated_delta_backward"));
-    hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)fin), dim3(kThreads), 0, s, d, tq, tk, lengths, bd,
-                       static_cast<T*>(dq), static_cast<T*>(dk));
-    RKA_RETURN_IF_HIP(hipGetLastError());
-    return 0;
+    RKA_RETURN_IF_ERR(prepare<T>(d, tq, tk, g, beta, lengths, cd, true, s));
+    RKA_RETURN_IF_ERR(launch_chain_backward<T>(d, tdo, dstate_out, lengths, cd, static_cast<T*>(dv), ds0, bd, s));
+    return launch_gradients<T>(d, tq, tk, tdo, g, lengths, cd, bd, static_cast<T*>(dq), static_cast<T*>(dk), dg, dbeta, s);
 }
 
 }  // namespace
@@ -577,22 +388,6 @@ int check_grid(long long blocks, int threads, const char* what) {
     return 0;
 }
 
-template <typename T>
-int launch_prepare(const Dims& d, const T* q, const T* k, const void* g, const void* beta, const int* lengths,
-                   const ChunkData& out, bool transpose, hipStream_t stream) {
-    const long long blocks = (long long)d.B * d.Hv * d.chunks;
-    if (blocks == 0) return 0;
-    RKA_RETURN_IF_ERR(check_grid(blocks, kThreads, "gated_delta"));
-    if (transpose)
-        hipLaunchKernelGGL((prepare_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, q, k, g, beta,
-                           lengths, out);
-    else
-        hipLaunchKernelGGL((prepare_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, q, k, g, beta,
-                           lengths, out);
-    RKA_RETURN_IF_HIP(hipGetLastError());
-    return 0;
-}
-
 }  // namespace delta
 }  // namespace rka
 
@@ -602,10 +397,10 @@ using namespace rka::delta;
 extern "C" {
 
 size_t rka_gated_delta_forward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
-                                               int value_dim) {
+                                               int value_dim, int dtype) {
     Dims d;
     if (make_dims("gated_delta", batch, tokens, key_heads, value_heads, key_dim, value_dim, &d) != 0) return 0;
-    return forward_layout((long long)d.B * d.Hv * d.chunks).total;
+    return chunk_layout(d, dtype == RKA_DTYPE_F32, false).total;
 }
 
 size_t rka_gated_delta_reserve_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim, int value_dim) {
@@ -615,10 +410,10 @@ size_t rka_gated_delta_reserve_bytes(int batch, int tokens, int key_heads, int v
 }
 
 size_t rka_gated_delta_backward_workspace_bytes(int batch, int tokens, int key_heads, int value_heads, int key_dim,
-                                                int value_dim) {
+                                                int value_dim, int dtype) {
     Dims d;
     if (make_dims("gated_delta", batch, tokens, key_heads, value_heads, key_dim, value_dim, &d) != 0) return 0;
-    return backward_layout(d).total;
+    return backward_layout(d, dtype == RKA_DTYPE_F32).total;
 }
 
 int rka_gated_delta_forward(const void* q, const void* k, const void* v, const void* g, const void* beta,
@@ -633,7 +428,7 @@ int rka_gated_delta_forward(const void* q, const void* k, const void* v, const v
     if (d.B == 0) return 0;
     if (!final_state || (d.T > 0 && (!q || !k || !v || !g || !beta || !o)))
         return fail(RKA_ERR_INVALID_ARGUMENT, "gated_delta_forward: null tensor pointer");
-    const size_t need = forward_layout((long long)d.B * d.Hv * d.chunks).total;
+    const size_t need = chunk_layout(d, dtype == RKA_DTYPE_F32, false).total;
     if (workspace_bytes < need || (need > 0 && !workspace))
         return fail(RKA_ERR_WORKSPACE_TOO_SMALL, "gated_delta_forward: workspace needs " + std::to_string(need) +
                                                      " bytes, got " + std::to_string(workspace_bytes));
@@ -656,7 +451,7 @@ int rka_gated_delta_backward(const void* q, const void* k, const void* g, const 
     if (d.B == 0) return 0;
     if (d.T > 0 && (!q || !k || !g || !beta || !reserve || !grad_q || !grad_k || !grad_v || !grad_g || !grad_beta))
         return fail(RKA_ERR_INVALID_ARGUMENT, "gated_delta_backward: null tensor pointer");
-    const size_t need = backward_layout(d).total;
+    const size_t need = backward_layout(d, dtype == RKA_DTYPE_F32).total;
     if (workspace_bytes < need || (need > 0 && !workspace))
         return fail(RKA_ERR_WORKSPACE_TOO_SMALL, "gated_delta_backward: workspace needs " + std::to_string(need) +
                                                      " bytes, got " + std::to_string(workspace_bytes));

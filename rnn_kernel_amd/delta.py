@@ -101,7 +101,7 @@ def _forward(q, k, v, g, beta, initial_state, lengths, scale: float, normalize: 
     sizes = (batch, tokens, key_heads, v.size(2), key_dim, v.size(3))
     o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     final_state = torch.empty(batch, v.size(2), key_dim, v.size(3), dtype=torch.float32, device=v.device)
-    ws_bytes = lib.rka_gated_delta_forward_workspace_bytes(*sizes)
+    ws_bytes = lib.rka_gated_delta_forward_workspace_bytes(*sizes, _DTYPES[q.dtype])
     ws = _bytes(ws_bytes, v.device)
     reserve = _bytes(lib.rka_gated_delta_reserve_bytes(*sizes), v.device) if training else None
     _lib.call(_index_of(v.device), "rka_gated_delta_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
@@ -139,7 +139,7 @@ class GatedDeltaFunction(torch.autograd.Function):
         ds0 = None
         if ctx.has_state and ctx.needs_input_grad[5]:
             ds0 = torch.empty(batch, value_heads, key_dim, value_dim, dtype=torch.float32, device=device)
-        ws_bytes = lib.rka_gated_delta_backward_workspace_bytes(*ctx.sizes)
+        ws_bytes = lib.rka_gated_delta_backward_workspace_bytes(*ctx.sizes, _DTYPES[q.dtype])
         ws = _bytes(ws_bytes, device)
         _lib.call(_index_of(device), "rka_gated_delta_backward", q.data_ptr(), k.data_ptr(), g.data_ptr(),
                   beta.data_ptr(), _lib.ptr(lengths), reserve.data_ptr(), _lib.ptr(grad_o), _lib.ptr(grad_state),
