@@ -77,7 +77,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
 
     // the operands' registers and what fills them
     u32x4 kf[KU][NP], qf[KU][NP], tf[2][3], pf[2][PO], ktf[TW][2][NP];
-    float vv[NC][4];
+    T vv[NC][4];
     const size_t kch0 = ((size_t)b * d.Hk + hk) * d.chunks, ch0 = (size_t)bh * d.chunks;
     const size_t rows = row_frags<T>(d.Dk) * kFragLanes;
     auto load_rows = [&](int c) {
@@ -96,8 +96,9 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = c * kChunk + 16 * wave + 4 * hi + r, col = col0 + 16 * j;
-                vv[j][r] = t < len && col < d.Dv ? to_f32(v[b * d.v_s[0] + t * d.v_s[1] + h * d.v_s[2] + col]) : 0.f;
+                // (clamped, not guarded: a load under a branch is waited for there)
+                const int t = min(c * kChunk + 16 * wave + 4 * hi + r, len - 1), col = min(col0 + 16 * j, d.Dv - 1);
+                vv[j][r] = v[b * d.v_s[0] + t * d.v_s[1] + h * d.v_s[2] + col];
             }
     };
     auto load_tri = [&](int c) {
@@ -161,7 +162,11 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
                     out[j] = mul(qf[u], f, out[j]);
                 }
             }
-            const f32x4 x = f32x4{vv[j][0], vv[j][1], vv[j][2], vv[j][3]} - rk * (y[0] + y[1]);
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                x[r] = t0 + 16 * wave + 4 * hi + r < len && col0 + 16 * j < d.Dv ? to_f32(vv[j][r]) : 0.f;
+            x -= rk * (y[0] + y[1]);
             out[j] *= rq;
             u32x2 p[3];
             split<3>(x, p);
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         }
 
     u32x4 kf[KU][NP], tf[2][3], pf[2][3], ktf[TW][2][NP], qtf[TW][2][NP];
-    f32x4 go[NC];  // dO of the wavefront's rows
+    T go[NC][4] = {};  // dO of the wavefront's rows
     const size_t kch0 = ((size_t)b * d.Hk + hk) * d.chunks, ch0 = (size_t)bh * d.chunks;
     const size_t rows = row_frags<T>(d.Dk) * kFragLanes;
     auto load_rows = [&](int c) {
@@ -287,16 +292,23 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = c * kChunk + 16 * wave + 4 * hi + r, col = col0 + 16 * j;
-                go[j][r] = dout && t < len && col < d.Dv ? to_f32(dout[(((size_t)b * d.T + t) * d.Hv + h) * d.Dv + col]) : 0.f;
+                const int t = min(c * kChunk + 16 * wave + 4 * hi + r, len - 1), col = min(col0 + 16 * j, d.Dv - 1);
+                if (dout) go[j][r] = dout[(((size_t)b * d.T + t) * d.Hv + h) * d.Dv + col];
             }
     };
+    auto masked_do = [&](int c, int j) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            x[r] = c * kChunk + 16 * wave + 4 * hi + r < len && col0 + 16 * j < d.Dv ? to_f32(go[j][r]) : 0.f;
+        return x;
+    };
     // (exact in the pieces of its type)
-    auto put_do = [&]() {
+    auto put_do = [&](int c) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             u32x2 p[NP];
-            split<NP>(go[j], p);
+            split<NP>(masked_do(c, j), p);
             put_block(fo[j], NP, wave, hi, n, p);
         }
     };
@@ -330,7 +342,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         load_tri(in.t, c, tf);
         load_tri(in.p, c, pf);
         load_transposed(c);
-        put_do();
+        put_do(c);
     }
     for (int c = live_chunks - 1; c >= 0; --c) {
         const int t0 = c * kChunk, next = max(c - 1, 0);
@@ -366,7 +378,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
             u32x2 p[3];
             split<3>(u + wk * (y[0] + y[1]), p);
             put_block(fx[j], 3, wave, hi, n, p);
-            split<3>(rq * go[j], p);
+            split<3>(rq * masked_do(c, j), p);
             put_block(fq[j], 3, wave, hi, n, p);
         }
         load_rows(next);
@@ -424,7 +436,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                     bd.dx[at] = x[j][r];
                 }
             }
-        put_do();
+        put_do(next);
     }
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
