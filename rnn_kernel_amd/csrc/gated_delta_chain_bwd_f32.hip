@@ -9,7 +9,7 @@ int launch_chain_backward<float>(const Dims& d, const float* dout, const float* 
                                  const ChunkData& in, float* dv, float* ds0, const BackwardData& bd, hipStream_t stream) {
     return with_chain<float>(d, [&](auto ku, auto nc) {
         constexpr int KU = decltype(ku)::value, NC = decltype(nc)::value;
-        const long long blocks = (long long)d.B * d.Hv * ((d.Dv - 1) / (16 * NC) + 1);
+        const long long blocks = chain_blocks(d, NC);
         RKA_RETURN_IF_ERR(check_grid(blocks, kChainThreads, "gated_delta_backward"));
         hipLaunchKernelGGL((chain_backward_kernel<float, KU, NC>), dim3((unsigned)blocks), dim3(kChainThreads), 0, stream,
                            d, dout, dstate_out, lengths, in, dv, ds0, bd);

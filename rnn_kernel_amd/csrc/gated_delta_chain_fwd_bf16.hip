@@ -10,7 +10,7 @@ int launch_chain_forward<bf16>(const Dims& d, const bf16* v, const float* s0, co
                                 bf16* o, float* state_out, float* states, float* e, hipStream_t stream) {
     return with_chain<bf16>(d, [&](auto ku, auto nc) {
         constexpr int KU = decltype(ku)::value, NC = decltype(nc)::value;
-        const long long blocks = (long long)d.B * d.Hv * ((d.Dv - 1) / (16 * NC) + 1);
+        const long long blocks = chain_blocks(d, NC);
         RKA_RETURN_IF_ERR(check_grid(blocks, kChainThreads, "gated_delta_forward"));
         hipLaunchKernelGGL((chain_forward_kernel<bf16, KU, NC>), dim3((unsigned)blocks), dim3(kChainThreads), 0, stream, d,
                            v, s0, lengths, in, o, state_out, states, e);
