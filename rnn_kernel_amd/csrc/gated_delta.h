@@ -12,18 +12,20 @@
 // sum of g in the chunk, L_ij = exp(G_i - G_j) for i >= j, and K, Q, V, E the
 // tokens' rows:
 //   N = strictly lower part of (K K^T * L),   T = (I + N diag(beta))^-1
-//   E = T (V - diag(exp G) K S)
+//   E = T (V - diag(exp G) K S) = T V - (T diag(exp G) K) S
 //   O = scale diag(exp G) Q S + P E,          P = lower part of scale (Q K^T * L) diag(beta)
 //   S' = exp(G_C) S + K^T diag(exp(G_C - G) beta) E
-// T and P hang on no state, so they are made for all chunks at once; only E, O and S'
-// go from chunk to chunk.  Columns of S, V, E and O do not mix.
+// T V, T diag(exp G) K and P hang on no state, so they are made for all chunks at once
+// ("prepare"); E, O and S' go from chunk to chunk ("chain"): two products that wait for
+// one another.  Columns of S, V, E and O do not mix.
 //
-// With dS' the gradient of S' and dO that of O:
-//   B dU = P^T dO + diag(exp(G_C - G) beta) K dS'          (B = diag(beta))
-//   dX = T^T (B dU)                                        (= dV)
+// With dS' the gradient of S' and dO that of O (B = diag(beta)):
+//   B dU = P^T dO + diag(exp(G_C - G) beta) K dS'
+//   dX = T^T (B dU) = (P T)^T dO + (T^T diag(exp(G_C - G) beta) K) dS'       (= dV)
 //   dS = exp(G_C) dS' + scale Q^T diag(exp G) dO - K^T diag(exp G) dX
-// goes through the chunks backwards; the rest of the gradients is again made for
-// all chunks at once, from S, dS', E and dX of each:
+// goes through the chunks backwards, again with the factors of dO and dS' made before;
+// the rest of the gradients is made for all chunks at once, from S, dS', E and dX of
+// each:
 //   F1 = scale dO E^T * L,  F2 = -(dX E^T * L) strictly lower,  W = diag(exp(G_C - G)) E dS'^T
 //   dQ = scale diag(exp G) dO S^T + F1 B K
 //   Z  = W + F1^T Q + F2^T K;  dK (as a written key) = B Z;  dbeta_j = k_j . Z_j
@@ -197,12 +199,26 @@ enum Coef { RK = 0, WK, RQ, BETA, CK, CQ, NCOEF };
 constexpr int kCoefFloats = NCOEF * kChunk + 4;
 
 struct ChunkData {
-    float* coef;        // [value chunk-head][kCoefFloats]
-    float* norm;        // [key chunk-head][2][64]: CK, CQ
-    u32x4 *k, *q;       // [key chunk-head] row fragments
-    u32x4 *kt, *qt;     // [key chunk-head] transposed (qt: backward only)
-    u32x4 *t, *p;       // [value chunk-head][kTriFrags][3]: T and P, or their transposes
+    float* coef;      // [value chunk-head][kCoefFloats]
+    float* norm;      // [key chunk-head][2][64]: CK, CQ
+    u32x4 *k, *q;     // [key chunk-head] row fragments
+    u32x4 *kt, *qt;   // [key chunk-head] transposed (qt: backward only)
+    u32x4* read;      // [value chunk-head][16-token block][step][3]: T diag(exp G) K, or (backward)
+                      // T^T diag(exp(G_C - G) beta) K
+    u32x4* p;         // [value chunk-head][kTriFrags][3]: P (forward only)
+    f32x4* own;       // [value chunk-head][16-column block][16-token block][lane], as a product leaves it: T V, or
+                      // (backward) (P T)^T dO
 };
+inline __host__ __device__ size_t read_frags(int Dk) { return (size_t)4 * chain_steps(Dk) * 3; }
+inline __host__ __device__ int column_blocks(int Dv) { return (Dv + 15) / 16; }
+
+// Where a 16x16 result block goes among the fragments over its rows: block x of 16
+// rows, lane (hi, n): eight bytes of step x / 2 at lane (2 (x % 2) + hi / 2, n).
+__device__ __forceinline__ void put_block(u32x4* frags, int pieces, int x, int hi, int n, const u32x2* p) {
+    u32x2* at = reinterpret_cast<u32x2*>(frags + (size_t)(x / 2) * pieces * kFragLanes) +
+                ((2 * (x % 2) + hi / 2) * 16 + n) * 2 + hi % 2;
+    for (int c = 0; c < pieces; ++c) at[c * kFragLanes * 2] = p[c];
+}
 
 // Gradients' inputs and outputs that pass between the backward's launches.
 struct BackwardData {
@@ -217,8 +233,8 @@ struct BackwardData {
 // The launches below take lengths == nullptr for rows of T tokens each.
 // states, e: saved for the backward, or both null.
 template <typename T>
-int launch_chain_forward(const Dims& d, const T* v, const float* s0, const int* lengths, const ChunkData& in, T* o,
-                         float* state_out, float* states, float* e, hipStream_t stream);
+int launch_chain_forward(const Dims& d, const float* s0, const int* lengths, const ChunkData& in, T* o, float* state_out,
+                         float* states, float* e, hipStream_t stream);
 // dstate_out (of the final state), dO: either may be null (zeros).
 template <typename T>
 int launch_chain_backward(const Dims& d, const T* dout, const float* dstate_out, const int* lengths, const ChunkData& in,

@@ -89,17 +89,19 @@ __device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
     for (int r = 0; r < 4; ++r) to[(4 * hi + r) * kLd + n] = x[r];
 }
 
-// T and P of a chunk and value head.  The inverse of I + N diag(beta) in float32: its
-// 16x16 diagonal blocks by forward substitution (a column per lane), then the blocks
-// below from theirs, [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1], for 32 and 64 rows.
-// (Backward stable; a series of powers of N is not where keys are alike.)
-template <typename T, bool TRANSPOSE>
-__global__ __launch_bounds__(kThreads) void triangles_kernel(Dims d, const void* g, const void* beta, const int* lengths,
-                                                             ChunkData out) {
+// What the chains read of a chunk and value head.  The inverse of I + N diag(beta) in
+// float32: its 16x16 diagonal blocks by forward substitution (a column per lane), then
+// the blocks below from theirs, [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1], for 32 and 64
+// rows.  (Backward stable; a series of powers of N is not where keys are alike.)
+// `x`: v, or (backward) dO, which may be null.
+template <typename T, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, const void* g, const void* beta,
+                                                           const int* lengths, ChunkData out) {
     constexpr int NP = kPieces<T>;
+    constexpr int kLdX = sizeof(T) == 4 ? 68 : 72;  // row of 64 columns of x
     __shared__ __attribute__((aligned(16))) float nb[kChunk * kLd], ti[kChunk * kLd];
     __shared__ double gsum[kChunk];
-    __shared__ float bet[kChunk], ck[kChunk], cq[kChunk];
+    __shared__ float bet[kChunk], ck[kChunk], cq[kChunk], scaled[kChunk];
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, hi = lane / 16;
     const int c = blockIdx.x % d.chunks, bh = blockIdx.x / d.chunks;
     const int b = bh / d.Hv, h = bh % d.Hv, hk = h / (d.Hv / d.Hk);
@@ -132,11 +134,11 @@ __global__ __launch_bounds__(kThreads) void triangles_kernel(Dims d, const void*
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j > wave) break;
-            u32x4 x[NP];
+            u32x4 y[NP];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) x[i] = fk[((j * steps + u) * NP + i) * kFragLanes];
-            kk[j] = mul(a, x, kk[j]);
-            qk[j] = mul(aq, x, qk[j]);
+            for (int i = 0; i < NP; ++i) y[i] = fk[((j * steps + u) * NP + i) * kFragLanes];
+            kk[j] = mul(a, y, kk[j]);
+            qk[j] = mul(aq, y, qk[j]);
         }
     }
     __syncthreads();
@@ -160,29 +162,31 @@ __global__ __launch_bounds__(kThreads) void triangles_kernel(Dims d, const void*
         float* coef = out.coef + ch * kCoefFloats;
         const float eg = expf((float)gsum[tid]), el = expf((float)(gsum[kChunk - 1] - gsum[tid]));
         const bool on = tid < live;
-        coef[RK * kChunk + tid] = on ? eg * ck[tid] : 0.f;
-        coef[WK * kChunk + tid] = on ? el * ck[tid] * bet[tid] : 0.f;
+        const float rk = on ? eg * ck[tid] : 0.f, wk = on ? el * ck[tid] * bet[tid] : 0.f;
+        coef[RK * kChunk + tid] = rk;
+        coef[WK * kChunk + tid] = wk;
         coef[RQ * kChunk + tid] = on ? d.scale * eg * cq[tid] : 0.f;
         coef[BETA * kChunk + tid] = bet[tid];
         coef[CK * kChunk + tid] = ck[tid];
         coef[CQ * kChunk + tid] = cq[tid];
         if (tid == 0) coef[NCOEF * kChunk] = expf((float)gsum[kChunk - 1]);
+        scaled[tid] = BACKWARD ? wk : rk;
     }
     __syncthreads();
     {
         // the wavefront's own diagonal block (the four 16-lane groups alike)
         const float* a = nb + 16 * wave * kLd + 16 * wave;
-        float x[16];
+        float y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float v = i == n ? 1.f : 0.f;
 #pragma unroll
-            for (int m = 0; m < i; ++m) v = fmaf(-a[i * kLd + m], x[m], v);
-            x[i] = v;
+            for (int m = 0; m < i; ++m) v = fmaf(-a[i * kLd + m], y[m], v);
+            y[i] = v;
         }
         if (hi == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) ti[(16 * wave + i) * kLd + 16 * wave + n] = x[i];
+            for (int i = 0; i < 16; ++i) ti[(16 * wave + i) * kLd + 16 * wave + n] = y[i];
         }
     }
     __syncthreads();
@@ -208,38 +212,114 @@ __global__ __launch_bounds__(kThreads) void triangles_kernel(Dims d, const void*
 #pragma unroll
     for (int j = 0; j < 4; ++j) put_result(at(nb, wave, j), p[j], n, hi);
     __syncthreads();
-    u32x4* ft = out.t + ch * (size_t)(kTriFrags * 3 * kFragLanes) + lane;
-    u32x4* fp = out.p + ch * (size_t)(kTriFrags * 3 * kFragLanes) + lane;
+    // Operands of the wavefront's 16 rows: of T with its columns (backward: of T^T with
+    // them) scaled for the keys, and of what x is multiplied by: T (backward: (P T)^T).
+    // T and T^T differ in which 32-wide steps are not all zero.
+    u32x4 tk[2][3], tx[2][3];
+    auto operand = [&](const float* m, int w, bool scale, u32x4 (&f)[3]) {
+        f32x4 y[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = 32 * w + 8 * hi + e;
+            const float v = BACKWARD ? m[i * kLd + 16 * wave + n] : m[(16 * wave + n) * kLd + i];
+            y[e / 4][e % 4] = scale ? v * scaled[i] : v;
+        }
+        split8<3>(y[0], y[1], f);
+    };
+    auto live_step = [&](int w) { return BACKWARD ? w >= wave / 2 : w <= wave / 2; };
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        if (TRANSPOSE ? w < wave / 2 : w > wave / 2) continue;
-        const int f = TRANSPOSE ? upper_frag(wave, w) : lower_frag(wave, w);
+        if (!live_step(w)) continue;
+        operand(ti, w, true, tk[w]);
+        if constexpr (!BACKWARD) {
+            operand(ti, w, false, tx[w]);
+            u32x4 f[3];
+            operand(nb, w, false, f);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const float* from = m ? nb : ti;
-            f32x4 x[2];
+            for (int i = 0; i < 3; ++i)
+                out.p[(ch * kTriFrags * 3 + lower_frag(wave, w) * 3 + i) * kFragLanes + lane] = f[i];
+        }
+    }
+    if constexpr (BACKWARD) {
+        f32x4 m[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e / 4][e % 4] = TRANSPOSE ? from[(32 * w + 8 * hi + e) * kLd + 16 * wave + n]
-                                            : from[(16 * wave + n) * kLd + 32 * w + 8 * hi + e];
-            u32x4 y[3];
-            split8<3>(x[0], x[1], y);
+        for (int j = 0; j < 4; ++j) {
+            m[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int l = j; l <= wave; ++l) m[j] = block_product(at(nb, wave, l), at(ti, l, j), n, hi, m[j]);
+        }
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 3; ++i) (m ? fp : ft)[(f * 3 + i) * kFragLanes] = y[i];
+        for (int j = 0; j < 4; ++j) put_result(at(nb, wave, j), m[j], n, hi);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+            if (live_step(w)) operand(nb, w, false, tx[w]);
+    }
+    // transposed: rows of Dk, columns the wavefront's tokens
+    u32x4* read = out.read + (ch * read_frags(d.Dk) + (size_t)wave * steps * 3) * kFragLanes;
+    const u32x4* fkt = out.kt + kch * row_frags<T>(d.Dk) * kFragLanes + lane;
+    for (int blk = 0; blk < 2 * steps; ++blk) {
+        f32x4 y{};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            if (!live_step(w)) continue;
+            u32x4 a[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) a[i] = fkt[((blk * 2 + w) * NP + i) * kFragLanes];
+            y = mul(a, tk[w], y);
+        }
+        u32x2 pieces[3];
+        split<3>(y, pieces);
+        put_block(read, 3, blk, hi, n, pieces);
+    }
+    // the products with x, 64 columns of it at a time in LDS
+    T* xs = reinterpret_cast<T*>(ti);
+    const T* px = x;
+    long long stride = 0;
+    if constexpr (BACKWARD) {
+        stride = (long long)d.Hv * d.Dv;
+        if (px) px += (((size_t)b * d.T + t0) * d.Hv + h) * d.Dv;
+    } else {
+        stride = d.v_s[1];
+        px += b * d.v_s[0] + t0 * d.v_s[1] + h * d.v_s[2];
+    }
+    const int blocks = column_blocks(d.Dv);
+    for (int v0 = 0; v0 < d.Dv; v0 += 64) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunk * 64 / kThreads; ++i) {
+            const int r = (tid + i * kThreads) / 64, e = tid % 64;
+            xs[r * kLdX + e] = px && r < live && v0 + e < d.Dv ? px[r * stride + v0 + e] : from_f32<T>(0.f);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (v0 + 16 * j >= d.Dv) break;
+            f32x4 y{};
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                if (!live_step(w)) continue;
+                const T* q = xs + (32 * w + 8 * hi) * kLdX + 16 * j + n;
+                u32x4 f[NP];
+                split8<NP>(f32x4{to_f32(q[0]), to_f32(q[kLdX]), to_f32(q[2 * kLdX]), to_f32(q[3 * kLdX])},
+                           f32x4{to_f32(q[4 * kLdX]), to_f32(q[5 * kLdX]), to_f32(q[6 * kLdX]), to_f32(q[7 * kLdX])}, f);
+                y = mul(tx[w], f, y);
+            }
+            out.own[((ch * blocks + v0 / 16 + j) * 4 + wave) * kFragLanes + lane] = y;
         }
     }
 }
 
 // ---------------------------------------------------------- workspaces ---
 struct ChunkLayout {
-    size_t coef, norm, k, q, kt, qt, t, p, total;
+    size_t coef, norm, k, q, kt, qt, read, p, own, total;
 };
-// `qt` only where the backward wants it.  Sized for float32 pieces where `wide`.
+// Of the backward (with qt, without p) or the forward.  Sized for float32 pieces
+// where `wide`.
 ChunkLayout chunk_layout(const Dims& d, bool wide, bool backward) {
     ChunkLayout l{};
     const size_t ch = (size_t)d.B * d.Hv * d.chunks, kch = (size_t)d.B * d.Hk * d.chunks;
     const size_t rows = kch * (wide ? row_frags<float>(d.Dk) : row_frags<bf16>(d.Dk)) * kFragLanes * 16;
-    const size_t tri = ch * kTriFrags * 3 * kFragLanes * 16;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t was = at;
@@ -252,8 +332,9 @@ ChunkLayout chunk_layout(const Dims& d, bool wide, bool backward) {
     l.q = take(rows);
     l.kt = take(rows);
     l.qt = backward ? take(rows) : 0;
-    l.t = take(tri);
-    l.p = take(tri);
+    l.read = take(ch * read_frags(d.Dk) * kFragLanes * 16);
+    l.p = backward ? 0 : take(ch * kTriFrags * 3 * kFragLanes * 16);
+    l.own = take(ch * column_blocks(d.Dv) * 4 * kFragLanes * 16);
     l.total = at;
     return l;
 }
@@ -290,14 +371,16 @@ ChunkData chunk_data(char* ws, const ChunkLayout& l) {
     c.q = reinterpret_cast<u32x4*>(ws + l.q);
     c.kt = reinterpret_cast<u32x4*>(ws + l.kt);
     c.qt = l.qt ? reinterpret_cast<u32x4*>(ws + l.qt) : nullptr;
-    c.t = reinterpret_cast<u32x4*>(ws + l.t);
-    c.p = reinterpret_cast<u32x4*>(ws + l.p);
+    c.read = reinterpret_cast<u32x4*>(ws + l.read);
+    c.p = l.p ? reinterpret_cast<u32x4*>(ws + l.p) : nullptr;
+    c.own = reinterpret_cast<f32x4*>(ws + l.own);
     return c;
 }
 
-template <typename T>
-int prepare(const Dims& d, const T* q, const T* k, const void* g, const void* beta, const int* lengths,
-            const ChunkData& out, bool transpose, hipStream_t stream) {
+// x: v, or (backward) dO.
+template <typename T, bool BACKWARD>
+int prepare(const Dims& d, const T* q, const T* k, const T* x, const void* g, const void* beta, const int* lengths,
+            const ChunkData& out, hipStream_t stream) {
     const long long blocks = (long long)d.B * d.Hv * d.chunks, rows = (long long)d.B * d.Hk * d.chunks * 2;
     if (blocks == 0) return 0;
     RKA_RETURN_IF_ERR(check_grid(std::max(blocks, rows), kThreads, "gated_delta"));
@@ -306,10 +389,8 @@ int prepare(const Dims& d, const T* q, const T* k, const void* g, const void* be
                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)rows), dim3(kThreads), lds, stream, d, q, k, lengths, out);
     RKA_RETURN_IF_HIP(hipGetLastError());
-    if (transpose)
-        hipLaunchKernelGGL((triangles_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, g, beta, lengths, out);
-    else
-        hipLaunchKernelGGL((triangles_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, g, beta, lengths, out);
+    hipLaunchKernelGGL((prepare_kernel<T, BACKWARD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, x, g, beta,
+                       lengths, out);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
@@ -318,9 +399,10 @@ template <typename T>
 int forward(const Dims& d, const void* q, const void* k, const void* v, const void* g, const void* beta, const float* s0,
             const int* lengths, void* o, float* state_out, char* reserve, char* ws, hipStream_t s) {
     const ChunkData cd = chunk_data(ws, chunk_layout(d, sizeof(T) == 4, false));
-    RKA_RETURN_IF_ERR(prepare<T>(d, static_cast<const T*>(q), static_cast<const T*>(k), g, beta, lengths, cd, false, s));
+    RKA_RETURN_IF_ERR((prepare<T, false>(d, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), g,
+                                         beta, lengths, cd, s)));
     const ReserveLayout r = reserve_layout(d);
-    return launch_chain_forward<T>(d, static_cast<const T*>(v), s0, lengths, cd, static_cast<T*>(o), state_out,
+    return launch_chain_forward<T>(d, s0, lengths, cd, static_cast<T*>(o), state_out,
                                    reserve ? reinterpret_cast<float*>(reserve + r.states) : nullptr,
                                    reserve ? reinterpret_cast<float*>(reserve + r.e) : nullptr, s);
 }
@@ -336,7 +418,7 @@ int backward(const Dims& d, const void* q, const void* k, const void* g, const v
     const BackwardData bd{reinterpret_cast<const float*>(reserve + r.states), reinterpret_cast<const float*>(reserve + r.e),
                           reinterpret_cast<float*>(ws + l.dstates), reinterpret_cast<float*>(ws + l.dx),
                           reinterpret_cast<float*>(ws + l.dq), reinterpret_cast<float*>(ws + l.dk)};
-    RKA_RETURN_IF_ERR(prepare<T>(d, tq, tk, g, beta, lengths, cd, true, s));
+    RKA_RETURN_IF_ERR((prepare<T, true>(d, tq, tk, tdo, g, beta, lengths, cd, s)));
     RKA_RETURN_IF_ERR(launch_chain_backward<T>(d, tdo, dstate_out, lengths, cd, static_cast<T*>(dv), ds0, bd, s));
     return launch_gradients<T>(d, tq, tk, tdo, g, lengths, cd, bd, static_cast<T*>(dq), static_cast<T*>(dk), dg, dbeta, s);
 }

@@ -3,16 +3,16 @@
 // gated_delta_chain_*.hip files.
 //
 // A workgroup of eight wavefronts takes NC blocks of 16 columns of one head's state
-// through all chunks.  A step has three products that wait for one another: K S, T X
-// and K^T (..) E.  Four wavefronts make the first two, 16 tokens' rows each; the other
-// four make what the step does not wait for (forward: Q S and, a step later, P E and o;
-// backward: P^T dO a step ahead, and the pieces of dO); the third is shared by all
-// eight, a part of Dk's rows each.  The rows of K, Q, T, P and K^T come straight from
-// memory into the operand registers of the wavefront that uses them, each loaded again
-// for a later chunk as soon as it has been used; what the products hand on (S, X, E,
-// each split into bf16 pieces by the wavefront that made it) passes through LDS in
-// operand order, one barrier apiece.  The workgroups of a head are eight apart, on one
-// XCD, whose L2 then answers all but the first of them.
+// through all chunks.  A step has two products that wait for one another: that of S
+// (or dS') which gives E (or dX), and that which updates the state.  Four wavefronts make
+// the first, 16 tokens' rows each; the other four make what the step does not wait for
+// (forward: Q S and, a step later, P E and o; backward: the pieces of scale exp(G) dO);
+// the second is shared by all eight, a part of Dk's rows each.  The rows of the prepared
+// factors come straight from memory into the operand registers of the wavefront that
+// uses them, each loaded again for the next chunk as soon as it has been used; what the
+// products hand on (S, E, each split into bf16 pieces by the wavefront that made it)
+// passes through LDS in operand order, one barrier apiece.  The workgroups of a head are
+// eight apart, on one XCD, whose L2 then answers all but the first of them.
 //
 #pragma once
 
@@ -25,14 +25,6 @@ namespace delta {
 namespace {
 
 constexpr int kChainThreads = 512;
-
-// Where a 16x16 result block goes among the fragments over its rows: block x of 16
-// rows, lane (hi, n): eight bytes of step x / 2 at lane (2 (x % 2) + hi / 2, n).
-__device__ __forceinline__ void put_block(u32x4* frags, int pieces, int x, int hi, int n, const u32x2* p) {
-    u32x2* at = reinterpret_cast<u32x2*>(frags + (size_t)(x / 2) * pieces * kFragLanes) +
-                ((2 * (x % 2) + hi / 2) * 16 + n) * 2 + hi % 2;
-    for (int c = 0; c < pieces; ++c) at[c * kFragLanes * 2] = p[c];
-}
 
 template <int N>
 __device__ __forceinline__ void get_frag(const u32x4* frags, int step, int stride, int lane, u32x4 (&f)[N]) {
@@ -60,7 +52,7 @@ inline long long chain_blocks(const Dims& d, int nc) {
 template <int KU, int NC>
 struct Place {
     static constexpr int TW = (2 * KU + 7) / 8;  // blocks of 16 rows of the state per wavefront, at most
-    int lane, wave, n, hi, w4, bh, b, h, hk, col0, len, live_chunks;
+    int lane, wave, n, hi, w4, bh, blk, b, h, hk, col0, len, live_chunks;
     bool chain;  // of the wavefronts that the step waits for
     size_t head;
     __device__ __forceinline__ bool init(const Dims& d, const int* lengths) {
@@ -70,7 +62,6 @@ struct Place {
         hi = lane / 16;
         w4 = wave % 4;
         chain = wave < 4;
-        int blk;
         if (!head_and_block(d.B * d.Hv, &bh, &blk)) return false;
         b = bh / d.Hv;
         h = bh % d.Hv;
@@ -158,13 +149,12 @@ __device__ __forceinline__ f32x4 token_values(const T (&x)[4], int c, int first,
 
 // KU: 32-wide steps over Dk (even).
 template <typename T, int KU, int NC>
-__global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d, const T* v, const float* s0,
-                                                                         const int* lengths, ChunkData in, T* o,
-                                                                         float* state_out, float* states, float* e_out) {
+__global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d, const float* s0, const int* lengths,
+                                                                         ChunkData in, T* o, float* state_out,
+                                                                         float* states, float* e_out) {
     constexpr int NP = kPieces<T>, TW = Place<KU, NC>::TW;
     constexpr int PO = NP == 1 ? 2 : 3;  // pieces for what only reaches o: bf16 keeps 8 bits, two pieces 16
-    __shared__ u32x4 fs[NC][KU * 3 * kFragLanes], fx[NC][2 * 3 * kFragLanes], fe[2][NC][2 * PO * kFragLanes],
-        fw[NC][2 * 3 * kFragLanes];
+    __shared__ u32x4 fs[NC][KU * 3 * kFragLanes], fe[2][NC][2 * PO * kFragLanes], fw[NC][2 * 3 * kFragLanes];
     Place<KU, NC> at;
     if (!at.init(d, lengths)) return;
     const int lane = at.lane, n = at.n, hi = at.hi, w4 = at.w4, len = at.len, col0 = at.col0;
@@ -186,25 +176,37 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
     at.load_state(d, s0 ? s0 + at.head : nullptr, s);
     put_state();
 
-    // rows: of K and T (chain), of Q and P (others)
-    u32x4 row[KU][NP], tri[2][3], turned[TW][2][NP];
-    T vv[NC][4];
-    f32x4 rc, wk;  // RK (chain) or RQ (others); WK
+    // chain: rows of T diag(exp G) K; others: of Q (kPieces<T>) and P
+    u32x4 row[KU][3], tri[2][PO], turned[TW][2][NP];
+    f32x4 own[NC];  // T V (chain)
+    f32x4 coef;     // WK (chain) or RQ (others)
     float last;
     const size_t kch0 = ((size_t)at.b * d.Hk + at.hk) * d.chunks, ch0 = (size_t)at.bh * d.chunks;
-    const size_t rows = row_frags<T>(d.Dk) * kFragLanes;
-    const u32x4* prow = (chain ? in.k : in.q) + kch0 * rows + (size_t)w4 * KU * NP * kFragLanes + lane;
-    const u32x4* ptri = (chain ? in.t : in.p) + ch0 * (kTriFrags * 3 * kFragLanes) + lane;
+    const size_t rows = row_frags<T>(d.Dk) * kFragLanes, reads = read_frags(d.Dk) * kFragLanes;
+    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC;
+    const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
+    const u32x4* pq = in.q + kch0 * rows + (size_t)w4 * KU * NP * kFragLanes + lane;
+    const u32x4* ptri = in.p + ch0 * (kTriFrags * 3 * kFragLanes) + lane;
     const u32x4* pturned = in.kt + kch0 * rows + lane;
-    const T* pv = v + at.b * d.v_s[0] + first * d.v_s[1] + at.h * d.v_s[2] + col0;
     T* po = o + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0;
     const size_t orow = (size_t)d.Hv * d.Dv;
     auto load_rows = [&](int c) {
-        const u32x4* p = prow + c * rows;
+        if (chain) {
+            const u32x4* p = pread + c * reads;
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int i = 0; i < NP; ++i) row[u][i] = p[(u * NP + i) * kFragLanes];
+                for (int i = 0; i < 3; ++i) row[u][i] = p[(u * 3 + i) * kFragLanes];
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
+        } else {
+            const u32x4* p = pq + c * rows;
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) row[u][i] = p[(u * NP + i) * kFragLanes];
+        }
     };
     auto load_tri = [&](int c) {
         const u32x4* p = ptri + (size_t)c * (kTriFrags * 3 * kFragLanes);
@@ -212,8 +214,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         for (int w = 0; w < 2; ++w) {
             if (w > w4 / 2) break;
 #pragma unroll
-            for (int i = 0; i < 3; ++i)
-                if (PO == 3 || i < 2 || chain) tri[w][i] = p[(lower_frag(w4, w) * 3 + i) * kFragLanes];
+            for (int i = 0; i < PO; ++i) tri[w][i] = p[(lower_frag(w4, w) * 3 + i) * kFragLanes];
         }
     };
     auto load_turned = [&](int c) {
@@ -228,10 +229,9 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         }
     };
     auto load_coef = [&](int c) {
-        const float* coef = in.coef + (ch0 + c) * kCoefFloats;
-        rc = coef4(coef, chain ? RK : RQ, w4, hi);
-        if (chain) wk = coef4(coef, WK, w4, hi);
-        last = coef[NCOEF * kChunk];
+        const float* p = in.coef + (ch0 + c) * kCoefFloats;
+        coef = coef4(p, chain ? WK : RQ, w4, hi);
+        last = p[NCOEF * kChunk];
     };
     // P E of chunk c, whose E is in fe[c % 2], and its outputs
     auto finish = [&](int c, f32x4 (&out)[NC]) {
@@ -240,11 +240,9 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 if (w > w4 / 2) break;
-                u32x4 f[PO], a[PO];
+                u32x4 f[PO];
                 get_frag(fe[c % 2][j], w, PO, lane, f);
-#pragma unroll
-                for (int i = 0; i < PO; ++i) a[i] = tri[w][i];
-                out[j] = mul(a, f, out[j]);
+                out[j] = mul(tri[w], f, out[j]);
             }
             if (col0 + 16 * j >= d.Dv) continue;
             T* p = po + (size_t)c * kChunk * orow + 16 * j;
@@ -256,56 +254,28 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
     const int final = at.live_chunks - 1;
     if (final >= 0) {
         load_rows(0);
-        load_tri(0);
+        if (!chain) load_tri(0);
         load_turned(0);
         load_coef(0);
-        if (chain) load_tokens<T, NC>(pv, d.v_s[1], 0, first, len, col0, d.Dv, vv);
     }
     f32x4 out[NC];
     for (int c = 0; c <= final; ++c) {
         const int next = min(c + 1, final);
         if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
         __syncthreads();
-        f32x4 y[NC];
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            f32x4 part[2] = {};
-#pragma unroll
-            for (int u = 0; u < KU; ++u) {
-                if (chain || PO == 3) {
-                    u32x4 f[3];
-                    get_frag(fs[j], u, 3, lane, f);
-                    part[u % 2] = mul(row[u], f, part[u % 2]);
-                } else {
-                    u32x4 f[2];
-                    get_frag(fs[j], u, 3, lane, f);
-                    part[u % 2] = mul(row[u], f, part[u % 2]);
-                }
-            }
-            y[j] = rc * (part[0] + part[1]);
-            if (chain) {
-                u32x2 p[3];
-                split<3>(token_values(vv[j], c, first, len) - y[j], p);
-                put_block(fx[j], 3, w4, hi, n, p);
-            }
-        }
-        load_rows(next);
-        if (chain) load_tokens<T, NC>(pv, d.v_s[1], next, first, len, col0, d.Dv, vv);
-        __syncthreads();
         if (chain) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                f32x4 a[2] = {};
+                f32x4 part[2] = {};
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    if (w > w4 / 2) break;
+                for (int u = 0; u < KU; ++u) {
                     u32x4 f[3];
-                    get_frag(fx[j], w, 3, lane, f);
-                    a[w] = mul(tri[w], f, a[w]);
+                    get_frag(fs[j], u, 3, lane, f);
+                    part[u % 2] = mul(row[u], f, part[u % 2]);
                 }
-                const f32x4 e = a[0] + a[1];
+                const f32x4 e = own[j] - (part[0] + part[1]);
                 u32x2 pw[3], pe[PO];
-                split<3>(wk * e, pw);
+                split<3>(coef * e, pw);
                 put_block(fw[j], 3, w4, hi, n, pw);
                 split<PO>(e, pe);
                 put_block(fe[c % 2][j], PO, w4, hi, n, pe);
@@ -316,11 +286,29 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
                         if ((c + 1) * kChunk <= len || c * kChunk + first + r < len) p[r * orow] = e[r];
                 }
             }
-            load_tri(next);
-        } else if (c > 0) {
-            finish(c - 1, out);
-            load_tri(c);
+        } else {
+            f32x4 y[NC];
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                f32x4 part[2] = {};
+#pragma unroll
+                for (int u = 0; u < KU; ++u) {
+                    u32x4 f[PO], a[NP];
+                    get_frag(fs[j], u, 3, lane, f);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) a[i] = row[u][i];
+                    part[u % 2] = mul(a, f, part[u % 2]);
+                }
+                y[j] = coef * (part[0] + part[1]);
+            }
+            if (c > 0) {
+                finish(c - 1, out);
+                load_tri(c);
+            }
+#pragma unroll
+            for (int j = 0; j < NC; ++j) out[j] = y[j];
         }
+        load_rows(next);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
@@ -333,7 +321,6 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
                 s[j][t] = mul(turned[t][0], f[0], s[j][t] * last);
                 s[j][t] = mul(turned[t][1], f[1], s[j][t]);
             }
-            out[j] = y[j];
         }
         put_state();
         load_turned(next);
@@ -355,9 +342,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                                                                           const int* lengths, ChunkData in, T* dv,
                                                                           float* ds0, BackwardData bd) {
     constexpr int NP = kPieces<T>, TW = Place<KU, NC>::TW;
-    __shared__ u32x4 fs[NC][KU * 3 * kFragLanes], fx[NC][2 * 3 * kFragLanes], fo[NC][2 * NP * kFragLanes],
-        fw[NC][2 * 3 * kFragLanes], fq[NC][2 * 3 * kFragLanes];
-    __shared__ f32x4 pd[NC][4][kFragLanes];  // P^T dO, as its makers hold it
+    __shared__ u32x4 fs[NC][KU * 3 * kFragLanes], fw[NC][2 * 3 * kFragLanes], fq[NC][2 * 3 * kFragLanes];
     Place<KU, NC> at;
     if (!at.init(d, lengths)) return;
     const int lane = at.lane, n = at.n, hi = at.hi, w4 = at.w4, len = at.len, col0 = at.col0;
@@ -379,31 +364,29 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
     at.load_state(d, dstate_out ? dstate_out + at.head : nullptr, s);
     put_state();
 
-    u32x4 row[KU][NP], tri[2][3], kt[TW][2][NP], qt[TW][2][NP];  // row: chain only; tri: T^T (chain), P^T (others)
-    T go[NC][4], go1[NC][4];                                      // dO of this chunk and the next (others)
-    f32x4 rc, wk;                                                 // RK (chain) or RQ (others); WK
+    u32x4 row[KU][3], kt[TW][2][NP], qt[TW][2][NP];  // row: T^T diag(exp(G_C - G) beta) K (chain)
+    f32x4 own[NC];                                   // (P T)^T dO (chain)
+    T go[NC][4];                                     // dO (others)
+    f32x4 coef;                                      // RK (chain) or RQ (others)
     float last;
     const size_t kch0 = ((size_t)at.b * d.Hk + at.hk) * d.chunks, ch0 = (size_t)at.bh * d.chunks;
-    const size_t rows = row_frags<T>(d.Dk) * kFragLanes;
-    const u32x4* prow = in.k + kch0 * rows + (size_t)w4 * KU * NP * kFragLanes + lane;
-    const u32x4* ptri = (chain ? in.t : in.p) + ch0 * (kTriFrags * 3 * kFragLanes) + lane;
+    const size_t rows = row_frags<T>(d.Dk) * kFragLanes, reads = read_frags(d.Dk) * kFragLanes;
+    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC;
+    const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
     const size_t token = (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0;
     const size_t orow = (size_t)d.Hv * d.Dv;
     auto load_rows = [&](int c) {
-        const u32x4* p = prow + c * rows;
+        if (chain) {
+            const u32x4* p = pread + c * reads;
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int i = 0; i < NP; ++i) row[u][i] = p[(u * NP + i) * kFragLanes];
-    };
-    // rows `w4` of the transposes, steps w4 / 2 and up
-    auto load_tri = [&](int c) {
-        const u32x4* p = ptri + (size_t)c * (kTriFrags * 3 * kFragLanes);
+                for (int i = 0; i < 3; ++i) row[u][i] = p[(u * 3 + i) * kFragLanes];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            if (w < w4 / 2) continue;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) tri[w][i] = p[(upper_frag(w4, w) * 3 + i) * kFragLanes];
+            for (int j = 0; j < NC; ++j)
+                own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
+        } else if (dout) {
+            load_tokens<T, NC>(dout + token, orow, c, first, len, col0, d.Dv, go);
         }
     };
     auto load_turned = [&](int c) {
@@ -421,63 +404,16 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                 }
         }
     };
-    auto load_do = [&](int c, T (&x)[NC][4]) {
-        if (dout) load_tokens<T, NC>(dout + token, orow, c, first, len, col0, d.Dv, x);
-    };
-    // the pieces of dO of chunk c (exact in its type), and those of scale exp(G) dO
-    auto put_do = [&](int c, const T (&x)[NC][4]) {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            u32x2 p[NP];
-            split<NP>(dout ? token_values(x[j], c, first, len) : f32x4{0.f, 0.f, 0.f, 0.f}, p);
-            put_block(fo[j], NP, w4, hi, n, p);
-        }
-    };
-    auto put_query = [&](int c) {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            u32x2 p[3];
-            split<3>(rc * (dout ? token_values(go[j], c, first, len) : f32x4{0.f, 0.f, 0.f, 0.f}), p);
-            put_block(fq[j], 3, w4, hi, n, p);
-        }
-    };
-    auto put_pd = [&]() {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            f32x4 u{};
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                if (w < w4 / 2) continue;
-                u32x4 f[NP];
-                get_frag(fo[j], w, NP, lane, f);
-                u = mul(tri[w], f, u);
-            }
-            pd[j][w4][lane] = u;
-        }
-    };
     auto load_coef = [&](int c) {
-        const float* coef = in.coef + (ch0 + c) * kCoefFloats;
-        rc = coef4(coef, chain ? RK : RQ, w4, hi);
-        if (chain) wk = coef4(coef, WK, w4, hi);
-        last = coef[NCOEF * kChunk];
+        const float* p = in.coef + (ch0 + c) * kCoefFloats;
+        coef = coef4(p, chain ? RK : RQ, w4, hi);
+        last = p[NCOEF * kChunk];
     };
     const int final = at.live_chunks - 1;
     if (final >= 0) {
-        load_coef(final);
+        load_rows(final);
         load_turned(final);
-        load_tri(final);
-        if (chain) {
-            load_rows(final);
-        } else {
-            load_do(final, go);
-            load_do(max(final - 1, 0), go1);
-            put_do(final, go);
-        }
-        __syncthreads();
-        if (!chain) {
-            put_pd();
-            load_tri(max(final - 1, 0));
-        }
+        load_coef(final);
     }
     for (int c = final; c >= 0; --c) {
         const int next = max(c - 1, 0);
@@ -486,42 +422,16 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         if (chain) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                f32x4 y[2] = {};
+                f32x4 y[2] = {own[j], f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
                 for (int u = 0; u < KU; ++u) {
                     u32x4 f[3];
                     get_frag(fs[j], u, 3, lane, f);
                     y[u % 2] = mul(row[u], f, y[u % 2]);
                 }
+                const f32x4 x = y[0] + y[1];
                 u32x2 p[3];
-                split<3>(pd[j][w4][lane] + wk * (y[0] + y[1]), p);
-                put_block(fx[j], 3, w4, hi, n, p);
-            }
-            load_rows(next);
-        } else {
-            put_query(c);
-            put_do(next, go1);
-#pragma unroll
-            for (int j = 0; j < NC; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) go[j][r] = go1[j][r];
-            load_do(max(c - 2, 0), go1);
-        }
-        __syncthreads();
-        if (chain) {
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 a[2] = {};
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    if (w < w4 / 2) continue;
-                    u32x4 f[3];
-                    get_frag(fx[j], w, 3, lane, f);
-                    a[w] = mul(tri[w], f, a[w]);
-                }
-                const f32x4 x = a[0] + a[1];
-                u32x2 p[3];
-                split<3>(-rc * x, p);
+                split<3>(-coef * x, p);
                 put_block(fw[j], 3, w4, hi, n, p);
                 if (col0 + 16 * j < d.Dv) {
                     const size_t to = token + (size_t)c * kChunk * orow + 16 * j;
@@ -533,11 +443,15 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                         }
                 }
             }
-            load_tri(next);
         } else {
-            put_pd();
-            load_tri(max(c - 2, 0));
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                u32x2 p[3];
+                split<3>(coef * (dout ? token_values(go[j], c, first, len) : f32x4{0.f, 0.f, 0.f, 0.f}), p);
+                put_block(fq[j], 3, w4, hi, n, p);
+            }
         }
+        load_rows(next);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
@@ -550,12 +464,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
                 if (!at.has(t)) continue;
+                f32x4 other{0.f, 0.f, 0.f, 0.f};
                 s[j][t] *= last;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    s[j][t] = mul(qt[t][w], g[w], s[j][t]);
+                    other = mul(qt[t][w], g[w], other);
                     s[j][t] = mul(kt[t][w], f[w], s[j][t]);
                 }
+                s[j][t] += other;
             }
         }
         put_state();

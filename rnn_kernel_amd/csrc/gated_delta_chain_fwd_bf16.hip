@@ -6,14 +6,14 @@ namespace rka {
 namespace delta {
 
 template <>
-int launch_chain_forward<bf16>(const Dims& d, const bf16* v, const float* s0, const int* lengths, const ChunkData& in,
-                                bf16* o, float* state_out, float* states, float* e, hipStream_t stream) {
+int launch_chain_forward<bf16>(const Dims& d, const float* s0, const int* lengths, const ChunkData& in, bf16* o,
+                                float* state_out, float* states, float* e, hipStream_t stream) {
     return with_chain<bf16>(d, [&](auto ku, auto nc) {
         constexpr int KU = decltype(ku)::value, NC = decltype(nc)::value;
         const long long blocks = chain_blocks(d, NC);
         RKA_RETURN_IF_ERR(check_grid(blocks, kChainThreads, "gated_delta_forward"));
         hipLaunchKernelGGL((chain_forward_kernel<bf16, KU, NC>), dim3((unsigned)blocks), dim3(kChainThreads), 0, stream, d,
-                           v, s0, lengths, in, o, state_out, states, e);
+                           s0, lengths, in, o, state_out, states, e);
         RKA_RETURN_IF_HIP(hipGetLastError());
         return 0;
     });
