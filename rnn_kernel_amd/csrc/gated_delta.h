@@ -166,6 +166,12 @@ __device__ __forceinline__ f32x4 mul(const u32x4 (&a)[NA], const u32x4 (&b)[NB],
     return c;
 }
 
+// Waits until the last product of a sum is in its registers.  The compiler counts the
+// wait states between a matrix instruction and the reader of its result only within a
+// basic block (clang 22 of ROCm 7.2; where a branch came between, the reader saw the old
+// value now and then), so every sum that is read behind a branch ends with this.
+__device__ __forceinline__ void settle(f32x4& c) { asm volatile("s_nop 9" : "+v"(c)); }
+
 // ------------------------------------------------------- chunk operands ---
 // A "fragment" is what one matrix instruction takes of an operand: 64 lanes x 16 bytes.
 constexpr int kFragLanes = 64;

@@ -75,6 +75,8 @@ struct Place {
     // The wavefront's block t of the state's rows; whether there is one.
     __device__ __forceinline__ int block(int t) const { return wave + 8 * t; }
     __device__ __forceinline__ bool has(int t) const { return 8 * t + 8 <= 2 * KU || block(t) < 2 * KU; }
+    // That block, or the last one in its place (whose result is not used).
+    __device__ __forceinline__ int near(int t) const { return min(block(t), 2 * KU - 1); }
 
     // The state, from and to [Dk][Dv] in memory.
     __device__ __forceinline__ void load_state(const Dims& d, const float* from, f32x4 (&s)[NC][TW]) const {
@@ -135,6 +137,19 @@ __device__ __forceinline__ void load_tokens(const T* p, long long stride, int c,
         }
     }
 }
+// Their stores, of one column.
+template <typename T>
+__device__ __forceinline__ void store_tokens(T* p, long long stride, int c, int first, int len, f32x4 x) {
+    p += (long long)c * kChunk * stride;
+    if ((c + 1) * kChunk <= len) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r * stride] = from_f32<T>(x[r]);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (c * kChunk + first + r < len) p[r * stride] = from_f32<T>(x[r]);
+    }
+}
 // As float32, zero past the row's end.
 template <typename T>
 __device__ __forceinline__ f32x4 token_values(const T (&x)[4], int c, int first, int len) {
@@ -146,6 +161,11 @@ __device__ __forceinline__ f32x4 token_values(const T (&x)[4], int c, int first,
     }
     return y;
 }
+
+// Sets of row registers, which take the chunks in turn: with two, a load has a whole
+// step more to arrive.  Where the operands leave room for two.
+template <typename T, int KU>
+constexpr int kRowSets = kPieces<T> == 1 && KU <= 4 ? 2 : 1;
 
 // KU: 32-wide steps over Dk (even).
 template <typename T, int KU, int NC>
@@ -177,139 +197,26 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
     put_state();
 
     // chain: rows of T diag(exp G) K; others: of Q (kPieces<T>) and P
-    u32x4 row[KU][3], tri[2][PO], turned[TW][2][NP];
-    f32x4 own[NC];  // T V (chain)
-    f32x4 coef;     // WK (chain) or RQ (others)
-    float last;
     const size_t kch0 = ((size_t)at.b * d.Hk + at.hk) * d.chunks, ch0 = (size_t)at.bh * d.chunks;
     const size_t rows = row_frags<T>(d.Dk) * kFragLanes, reads = read_frags(d.Dk) * kFragLanes;
-    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC;
-    const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
-    const u32x4* pq = in.q + kch0 * rows + (size_t)w4 * KU * NP * kFragLanes + lane;
-    const u32x4* ptri = in.p + ch0 * (kTriFrags * 3 * kFragLanes) + lane;
-    const u32x4* pturned = in.kt + kch0 * rows + lane;
-    T* po = o + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0;
+    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC, final = at.live_chunks - 1;
     const size_t orow = (size_t)d.Hv * d.Dv;
-    auto load_rows = [&](int c) {
-        if (chain) {
-            const u32x4* p = pread + c * reads;
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-                for (int i = 0; i < 3; ++i) row[u][i] = p[(u * 3 + i) * kFragLanes];
-#pragma unroll
-            for (int j = 0; j < NC; ++j)
-                own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
-        } else {
-            const u32x4* p = pq + c * rows;
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-                for (int i = 0; i < NP; ++i) row[u][i] = p[(u * NP + i) * kFragLanes];
-        }
-    };
-    auto load_tri = [&](int c) {
-        const u32x4* p = ptri + (size_t)c * (kTriFrags * 3 * kFragLanes);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            if (w > w4 / 2) break;
-#pragma unroll
-            for (int i = 0; i < PO; ++i) tri[w][i] = p[(lower_frag(w4, w) * 3 + i) * kFragLanes];
-        }
-    };
+    constexpr int NS = kRowSets<T, KU>;
+
+    u32x4 turned[TW][2][NP];
+    float last;
     auto load_turned = [&](int c) {
-        const u32x4* p = pturned + c * rows;
+        const u32x4* p = in.kt + (kch0 + c) * rows + lane;
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
-            if (!at.has(t)) continue;
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) turned[t][w][i] = p[((at.block(t) * 2 + w) * NP + i) * kFragLanes];
-        }
+                for (int i = 0; i < NP; ++i) turned[t][w][i] = p[((at.near(t) * 2 + w) * NP + i) * kFragLanes];
+        last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
     };
-    auto load_coef = [&](int c) {
-        const float* p = in.coef + (ch0 + c) * kCoefFloats;
-        coef = coef4(p, chain ? WK : RQ, w4, hi);
-        last = p[NCOEF * kChunk];
-    };
-    // P E of chunk c, whose E is in fe[c % 2], and its outputs
-    auto finish = [&](int c, f32x4 (&out)[NC]) {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                if (w > w4 / 2) break;
-                u32x4 f[PO];
-                get_frag(fe[c % 2][j], w, PO, lane, f);
-                out[j] = mul(tri[w], f, out[j]);
-            }
-            if (col0 + 16 * j >= d.Dv) continue;
-            T* p = po + (size_t)c * kChunk * orow + 16 * j;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if ((c + 1) * kChunk <= len || c * kChunk + first + r < len) p[r * orow] = from_f32<T>(out[j][r]);
-        }
-    };
-    const int final = at.live_chunks - 1;
-    if (final >= 0) {
-        load_rows(0);
-        if (!chain) load_tri(0);
-        load_turned(0);
-        load_coef(0);
-    }
-    f32x4 out[NC];
-    for (int c = 0; c <= final; ++c) {
-        const int next = min(c + 1, final);
-        if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
-        __syncthreads();
-        if (chain) {
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 part[2] = {};
-#pragma unroll
-                for (int u = 0; u < KU; ++u) {
-                    u32x4 f[3];
-                    get_frag(fs[j], u, 3, lane, f);
-                    part[u % 2] = mul(row[u], f, part[u % 2]);
-                }
-                const f32x4 e = own[j] - (part[0] + part[1]);
-                u32x2 pw[3], pe[PO];
-                split<3>(coef * e, pw);
-                put_block(fw[j], 3, w4, hi, n, pw);
-                split<PO>(e, pe);
-                put_block(fe[c % 2][j], PO, w4, hi, n, pe);
-                if (e_out && col0 + 16 * j < d.Dv) {
-                    float* p = e_out + (((size_t)at.b * d.T + c * kChunk + first) * d.Hv + at.h) * d.Dv + col0 + 16 * j;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if ((c + 1) * kChunk <= len || c * kChunk + first + r < len) p[r * orow] = e[r];
-                }
-            }
-        } else {
-            f32x4 y[NC];
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 part[2] = {};
-#pragma unroll
-                for (int u = 0; u < KU; ++u) {
-                    u32x4 f[PO], a[NP];
-                    get_frag(fs[j], u, 3, lane, f);
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) a[i] = row[u][i];
-                    part[u % 2] = mul(a, f, part[u % 2]);
-                }
-                y[j] = coef * (part[0] + part[1]);
-            }
-            if (c > 0) {
-                finish(c - 1, out);
-                load_tri(c);
-            }
-#pragma unroll
-            for (int j = 0; j < NC; ++j) out[j] = y[j];
-        }
-        load_rows(next);
-        __syncthreads();
+    // the second product, all wavefronts' part of a step
+    auto update = [&](int c) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             u32x4 f[2][3];
@@ -317,24 +224,154 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
             get_frag(fw[j], 1, 3, lane, f[1]);
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
-                if (!at.has(t)) continue;
                 s[j][t] = mul(turned[t][0], f[0], s[j][t] * last);
                 s[j][t] = mul(turned[t][1], f[1], s[j][t]);
+                settle(s[j][t]);
             }
         }
         put_state();
-        load_turned(next);
-        load_coef(next);
-    }
-    if (final >= 0 && !chain) finish(final, out);
-    at.store_state(d, state_out + at.head, s);
-    if (!chain) {
+        load_turned(min(c + 1, final));
+    };
+
+    // The two kinds of wavefront in loops of their own: the compiler waits for what may
+    // have been loaded on either side of a branch.
+    if (final >= 0) load_turned(0);
+    if (chain) {
+        struct Rows {
+            u32x4 row[KU][3];  // of T diag(exp G) K
+            f32x4 own[NC];     // of T V
+            f32x4 wk;
+        } sets[NS];
+        const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
+        float* pe = e_out ? e_out + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0 : nullptr;
+        auto load = [&](Rows& x, int c) {
+            const u32x4* p = pread + c * reads;
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                x.own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
+            x.wk = coef4(in.coef + (ch0 + c) * kCoefFloats, WK, w4, hi);
+        };
+        auto step = [&](Rows& x, int c) {
+            if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                f32x4 part[2] = {};
+#pragma unroll
+                for (int u = 0; u < KU; ++u) {
+                    u32x4 f[3];
+                    get_frag(fs[j], u, 3, lane, f);
+                    part[u % 2] = mul(x.row[u], f, part[u % 2]);
+                }
+                settle(part[0]);
+                settle(part[1]);
+                const f32x4 e = x.own[j] - (part[0] + part[1]);
+                u32x2 pw[3], pp[PO];
+                split<3>(x.wk * e, pw);
+                put_block(fw[j], 3, w4, hi, n, pw);
+                split<PO>(e, pp);
+                put_block(fe[c % 2][j], PO, w4, hi, n, pp);
+                if (pe && col0 + 16 * j < d.Dv) store_tokens(pe + 16 * j, orow, c, first, len, e);
+            }
+            load(x, min(c + NS, final));
+            __syncthreads();
+            update(c);
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (final >= 0) load(sets[i], min(i, final));
+        for (int c = 0; c <= final; c += NS) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c + i <= final) step(sets[i], c + i);
+        }
+    } else {
+        struct Rows {
+            u32x4 row[KU][NP];  // of Q
+            f32x4 rq;
+        } sets[NS];
+        u32x4 tri[2][PO];
+        f32x4 out[NC];
+        const u32x4* pq = in.q + kch0 * rows + (size_t)w4 * KU * NP * kFragLanes + lane;
+        const u32x4* ptri = in.p + ch0 * (kTriFrags * 3 * kFragLanes) + lane;
+        T* po = o + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0;
+        auto load = [&](Rows& x, int c) {
+            const u32x4* p = pq + c * rows;
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) x.row[u][i] = p[(u * NP + i) * kFragLanes];
+            x.rq = coef4(in.coef + (ch0 + c) * kCoefFloats, RQ, w4, hi);
+        };
+        // rows w4 of P; their second step is zero for the first two (and not taken)
+        auto load_tri = [&](int c) {
+            const u32x4* p = ptri + (size_t)c * (kTriFrags * 3 * kFragLanes);
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int i = 0; i < PO; ++i) tri[w][i] = p[(lower_frag(w4, w4 / 2 < w ? 0 : w) * 3 + i) * kFragLanes];
+        };
+        // P E of chunk c, whose E is in fe[c % 2], and its outputs
+        auto finish = [&](int c) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                u32x4 f[PO];
+                get_frag(fe[c % 2][j], 0, PO, lane, f);
+                out[j] = mul(tri[0], f, out[j]);
+                settle(out[j]);
+                if (w4 >= 2) {
+                    get_frag(fe[c % 2][j], 1, PO, lane, f);
+                    out[j] = mul(tri[1], f, out[j]);
+                    settle(out[j]);
+                }
+                if (col0 + 16 * j < d.Dv) store_tokens(po + 16 * j, orow, c, first, len, out[j]);
+            }
+        };
+        auto step = [&](Rows& x, int c) {
+            if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
+            __syncthreads();
+            f32x4 y[NC];
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                f32x4 part[2] = {};
+#pragma unroll
+                for (int u = 0; u < KU; ++u) {
+                    u32x4 f[PO];
+                    get_frag(fs[j], u, 3, lane, f);
+                    part[u % 2] = mul(x.row[u], f, part[u % 2]);
+                }
+                settle(part[0]);
+                settle(part[1]);
+                y[j] = x.rq * (part[0] + part[1]);
+            }
+            load(x, min(c + NS, final));
+            if (c > 0) finish(c - 1);
+            load_tri(c);
+#pragma unroll
+            for (int j = 0; j < NC; ++j) out[j] = y[j];
+            __syncthreads();
+            update(c);
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (final >= 0) load(sets[i], min(i, final));
+        for (int c = 0; c <= final; c += NS) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c + i <= final) step(sets[i], c + i);
+        }
+        if (final >= 0) finish(final);
 #pragma unroll
         for (int j = 0; j < NC; ++j)
             if (col0 + 16 * j < d.Dv)
                 for (int t = len + w4 * 4 + hi; t < d.T; t += 16)
                     o[((size_t)at.b * d.T + t) * orow + (size_t)at.h * d.Dv + col0 + 16 * j] = from_f32<T>(0.f);
     }
+    at.store_state(d, state_out + at.head, s);
 }
 
 template <typename T, int KU, int NC>
@@ -364,95 +401,30 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
     at.load_state(d, dstate_out ? dstate_out + at.head : nullptr, s);
     put_state();
 
-    u32x4 row[KU][3], kt[TW][2][NP], qt[TW][2][NP];  // row: T^T diag(exp(G_C - G) beta) K (chain)
-    f32x4 own[NC];                                   // (P T)^T dO (chain)
-    T go[NC][4];                                     // dO (others)
-    f32x4 coef;                                      // RK (chain) or RQ (others)
-    float last;
     const size_t kch0 = ((size_t)at.b * d.Hk + at.hk) * d.chunks, ch0 = (size_t)at.bh * d.chunks;
     const size_t rows = row_frags<T>(d.Dk) * kFragLanes, reads = read_frags(d.Dk) * kFragLanes;
-    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC;
-    const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
+    const int blocks = column_blocks(d.Dv), block0 = at.blk * NC, final = at.live_chunks - 1;
     const size_t token = (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0;
     const size_t orow = (size_t)d.Hv * d.Dv;
-    auto load_rows = [&](int c) {
-        if (chain) {
-            const u32x4* p = pread + c * reads;
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-                for (int i = 0; i < 3; ++i) row[u][i] = p[(u * 3 + i) * kFragLanes];
-#pragma unroll
-            for (int j = 0; j < NC; ++j)
-                own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
-        } else if (dout) {
-            load_tokens<T, NC>(dout + token, orow, c, first, len, col0, d.Dv, go);
-        }
-    };
+    constexpr int NS = kRowSets<T, KU>;
+
+    u32x4 kt[TW][2][NP], qt[TW][2][NP];
+    float last;
     auto load_turned = [&](int c) {
         const u32x4 *pk = in.kt + (kch0 + c) * rows + lane, *pq = in.qt + (kch0 + c) * rows + lane;
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
-            if (!at.has(t)) continue;
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
-                    const int f = ((at.block(t) * 2 + w) * NP + i) * kFragLanes;
+                    const int f = ((at.near(t) * 2 + w) * NP + i) * kFragLanes;
                     kt[t][w][i] = pk[f];
                     qt[t][w][i] = pq[f];
                 }
-        }
+        last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
     };
-    auto load_coef = [&](int c) {
-        const float* p = in.coef + (ch0 + c) * kCoefFloats;
-        coef = coef4(p, chain ? RK : RQ, w4, hi);
-        last = p[NCOEF * kChunk];
-    };
-    const int final = at.live_chunks - 1;
-    if (final >= 0) {
-        load_rows(final);
-        load_turned(final);
-        load_coef(final);
-    }
-    for (int c = final; c >= 0; --c) {
-        const int next = max(c - 1, 0);
-        at.store_state(d, bd.dstates + (ch0 + c) * d.Dk * d.Dv, s);
-        __syncthreads();
-        if (chain) {
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 y[2] = {own[j], f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int u = 0; u < KU; ++u) {
-                    u32x4 f[3];
-                    get_frag(fs[j], u, 3, lane, f);
-                    y[u % 2] = mul(row[u], f, y[u % 2]);
-                }
-                const f32x4 x = y[0] + y[1];
-                u32x2 p[3];
-                split<3>(-coef * x, p);
-                put_block(fw[j], 3, w4, hi, n, p);
-                if (col0 + 16 * j < d.Dv) {
-                    const size_t to = token + (size_t)c * kChunk * orow + 16 * j;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if ((c + 1) * kChunk <= len || c * kChunk + first + r < len) {
-                            dv[to + r * orow] = from_f32<T>(x[r]);
-                            bd.dx[to + r * orow] = x[r];
-                        }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                u32x2 p[3];
-                split<3>(coef * (dout ? token_values(go[j], c, first, len) : f32x4{0.f, 0.f, 0.f, 0.f}), p);
-                put_block(fq[j], 3, w4, hi, n, p);
-            }
-        }
-        load_rows(next);
-        __syncthreads();
+    auto update = [&](int c) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             u32x4 f[2][3], g[2][3];
@@ -463,7 +435,6 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
             }
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
-                if (!at.has(t)) continue;
                 f32x4 other{0.f, 0.f, 0.f, 0.f};
                 s[j][t] *= last;
 #pragma unroll
@@ -471,21 +442,107 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                     other = mul(qt[t][w], g[w], other);
                     s[j][t] = mul(kt[t][w], f[w], s[j][t]);
                 }
+                settle(other);
+                settle(s[j][t]);
                 s[j][t] += other;
             }
         }
         put_state();
-        load_turned(next);
-        load_coef(next);
-    }
-    if (ds0) at.store_state(d, ds0 + at.head, s);
-    if (!chain) {
+        load_turned(max(c - 1, 0));
+    };
+
+    // (loops of their own, as in the forward)
+    if (final >= 0) load_turned(final);
+    if (chain) {
+        struct Rows {
+            u32x4 row[KU][3];  // of T^T diag(exp(G_C - G) beta) K
+            f32x4 own[NC];     // of (P T)^T dO
+            f32x4 rk;
+        } sets[NS];
+        const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
+        auto load = [&](Rows& x, int c) {
+            const u32x4* p = pread + c * reads;
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                x.own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
+            x.rk = coef4(in.coef + (ch0 + c) * kCoefFloats, RK, w4, hi);
+        };
+        auto step = [&](Rows& x, int c) {
+            at.store_state(d, bd.dstates + (ch0 + c) * d.Dk * d.Dv, s);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                f32x4 y[2] = {x.own[j], f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int u = 0; u < KU; ++u) {
+                    u32x4 f[3];
+                    get_frag(fs[j], u, 3, lane, f);
+                    y[u % 2] = mul(x.row[u], f, y[u % 2]);
+                }
+                settle(y[0]);
+                settle(y[1]);
+                const f32x4 dx = y[0] + y[1];
+                u32x2 p[3];
+                split<3>(-x.rk * dx, p);
+                put_block(fw[j], 3, w4, hi, n, p);
+                if (col0 + 16 * j < d.Dv) {
+                    store_tokens(dv + token + 16 * j, orow, c, first, len, dx);
+                    store_tokens(bd.dx + token + 16 * j, orow, c, first, len, dx);
+                }
+            }
+            load(x, max(c - NS, 0));
+            __syncthreads();
+            update(c);
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (final >= 0) load(sets[i], max(final - i, 0));
+        for (int c = final; c >= 0; c -= NS) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c - i >= 0) step(sets[i], c - i);
+        }
+    } else {
+        struct Rows {
+            T go[NC][4];  // dO
+            f32x4 rq;
+        } sets[NS];
+        auto load = [&](Rows& x, int c) {
+            if (dout) load_tokens<T, NC>(dout + token, orow, c, first, len, col0, d.Dv, x.go);
+            x.rq = coef4(in.coef + (ch0 + c) * kCoefFloats, RQ, w4, hi);
+        };
+        auto step = [&](Rows& x, int c) {
+            at.store_state(d, bd.dstates + (ch0 + c) * d.Dk * d.Dv, s);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                u32x2 p[3];
+                split<3>(x.rq * (dout ? token_values(x.go[j], c, first, len) : f32x4{0.f, 0.f, 0.f, 0.f}), p);
+                put_block(fq[j], 3, w4, hi, n, p);
+            }
+            load(x, max(c - NS, 0));
+            __syncthreads();
+            update(c);
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (final >= 0) load(sets[i], max(final - i, 0));
+        for (int c = final; c >= 0; c -= NS) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c - i >= 0) step(sets[i], c - i);
+        }
 #pragma unroll
         for (int j = 0; j < NC; ++j)
             if (col0 + 16 * j < d.Dv)
                 for (int t = len + w4 * 4 + hi; t < d.T; t += 16)
                     dv[((size_t)at.b * d.T + t) * orow + (size_t)at.h * d.Dv + col0 + 16 * j] = from_f32<T>(0.f);
     }
+    if (ds0) at.store_state(d, ds0 + at.head, s);
 }
 
 // Calls f with the chain's steps over Dk and its column blocks as integral constants.
