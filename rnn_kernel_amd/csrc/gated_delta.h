@@ -172,6 +172,13 @@ __device__ __forceinline__ f32x4 mul(const u32x4 (&a)[NA], const u32x4 (&b)[NB],
 // value now and then), so every sum that is read behind a branch ends with this.
 __device__ __forceinline__ void settle(f32x4& c) { asm volatile("s_nop 9" : "+v"(c)); }
 
+// A value that is made whether or not it is used: without this the compiler puts loads
+// and exponentials whose result is then selected away under branches, one each.
+__device__ __forceinline__ float made(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // ------------------------------------------------------- chunk operands ---
 // A "fragment" is what one matrix instruction takes of an operand: 64 lanes x 16 bytes.
 constexpr int kFragLanes = 64;
@@ -232,8 +239,6 @@ struct BackwardData {
     const float* e;       // [B][T][Hv][Dv]
     float* dstates;       // [chunk-head][Dk][Dv]: dS' of each chunk
     float* dx;            // [B][T][Hv][Dv]
-    float* dq;            // [B][T][Hv][Dk]: of each value head
-    float* dk;
 };
 
 // The launches below take lengths == nullptr for rows of T tokens each.

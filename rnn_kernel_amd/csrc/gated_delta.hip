@@ -148,12 +148,9 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-            float nv = 0.f, pv = 0.f;
-            if (row >= col) {
-                const float w = expf((float)(gsum[row] - gsum[col])) * ck[col] * bet[col];
-                if (row > col) nv = kk[j][r] * ck[row] * w;
-                pv = d.scale * qk[j][r] * cq[row] * w;
-            }
+            const float w = made(expf((float)(gsum[row] - gsum[col]))) * ck[col] * bet[col];
+            const float nv = row > col ? kk[j][r] * ck[row] * w : 0.f;
+            const float pv = row >= col ? d.scale * qk[j][r] * cq[row] * w : 0.f;
             nb[row * kLd + col] = nv;
             ti[row * kLd + col] = 0.f;
             p[j][r] = pv;
@@ -350,16 +347,14 @@ ReserveLayout reserve_layout(const Dims& d) {
 }
 struct BackwardLayout {
     ChunkLayout f;
-    size_t dstates, dx, dq, dk, total;
+    size_t dstates, dx, total;
 };
 BackwardLayout backward_layout(const Dims& d, bool wide) {
     BackwardLayout l{};
     l.f = chunk_layout(d, wide, true);
     l.dstates = l.f.total;
     l.dx = l.dstates + align_up((size_t)d.B * d.Hv * d.chunks * d.Dk * d.Dv * sizeof(float), 256);
-    l.dq = l.dx + align_up((size_t)d.B * d.T * d.Hv * d.Dv * sizeof(float), 256);
-    l.dk = l.dq + align_up((size_t)d.B * d.T * d.Hv * d.Dk * sizeof(float), 256);
-    l.total = l.dk + align_up((size_t)d.B * d.T * d.Hv * d.Dk * sizeof(float), 256);
+    l.total = l.dx + align_up((size_t)d.B * d.T * d.Hv * d.Dv * sizeof(float), 256);
     return l;
 }
 
@@ -416,8 +411,7 @@ int backward(const Dims& d, const void* q, const void* k, const void* g, const v
     const ChunkData cd = chunk_data(ws, l.f);
     const T *tq = static_cast<const T*>(q), *tk = static_cast<const T*>(k), *tdo = static_cast<const T*>(dout);
     const BackwardData bd{reinterpret_cast<const float*>(reserve + r.states), reinterpret_cast<const float*>(reserve + r.e),
-                          reinterpret_cast<float*>(ws + l.dstates), reinterpret_cast<float*>(ws + l.dx),
-                          reinterpret_cast<float*>(ws + l.dq), reinterpret_cast<float*>(ws + l.dk)};
+                          reinterpret_cast<float*>(ws + l.dstates), reinterpret_cast<float*>(ws + l.dx)};
     RKA_RETURN_IF_ERR((prepare<T, true>(d, tq, tk, tdo, g, beta, lengths, cd, s)));
     RKA_RETURN_IF_ERR(launch_chain_backward<T>(d, tdo, dstate_out, lengths, cd, static_cast<T*>(dv), ds0, bd, s));
     return launch_gradients<T>(d, tq, tk, tdo, g, lengths, cd, bd, static_cast<T*>(dq), static_cast<T*>(dk), dg, dbeta, s);

@@ -1,53 +1,74 @@
 // The gradients of the gated delta rule that are made for all chunks at once after the
 // backward's chain (gated_delta.h has the formulas).
+//
+// A workgroup of eight wavefronts takes a chunk of a key head through its value heads
+// and keeps the sums of dq and dk in registers: they are rounded once, in a fixed
+// order, and nothing of a value head goes through memory.  A wavefront has 16 tokens'
+// rows and half of Dk.  Over Dv, 32 columns at a time: the rows of dO and dX come from
+// memory to the operand registers, the blocks of S, dS' and E are split into bf16 pieces
+// once and shared through LDS, loaded a step ahead.
+//
+// Bound by memory: of S, dS', E, dX and dO some 12 bytes per state element and chunk are
+// read once, against 15 products of pieces on each.
 #include "gated_delta.h"
 
 namespace rka {
 namespace delta {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kLd = 68;  // row of a 64-wide LDS tile: 16 bytes past a multiple of all banks
 
-__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+struct __attribute__((packed, aligned(4))) Float4U {
+    float x, y, z, w;
+};
+struct __attribute__((packed, aligned(2))) Bytes16 {
+    unsigned w[4];
+};
+
+// Loads of neighbouring columns, from column c of a row of `width` in memory, zero past
+// it: without branches (clamped addresses), and for the widths that are multiples of
+// eight (VEC) in 16-byte loads.
+template <bool VEC>
+__device__ __forceinline__ f32x4 load4(const float* row, int c, int width) {
+    f32x4 x;
+    if constexpr (VEC) {
+        const Float4U v = *reinterpret_cast<const Float4U*>(row + min(c, width - 4));
+        x = f32x4{v.x, v.y, v.z, v.w};
+        if (c >= width) x = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v = row[min(c + j, width - 1)];
+            x[j] = c + j < width ? v : 0.f;
+        }
+    }
+    return x;
 }
 
-// rows x 64 elements (from column d0 of `width`) of a strided matrix as float32 in
-// LDS; zero past `live` rows and the width.
-template <typename T>
-__device__ __forceinline__ void stage64(float* lds, const T* src, long long stride, int live, int d0, int width,
-                                        int tid) {
-#pragma unroll
-    for (int i = 0; i < kChunk * 16 / kThreads; ++i) {
-        const int r = (tid + i * kThreads) / 16, c = (tid + i * kThreads) % 16 * 4;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (r < live) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (d0 + c + j < width) x[j] = to_f32(src[r * stride + d0 + c + j]);
-        }
-        *reinterpret_cast<f32x4*>(lds + r * kLd + c) = x;
-    }
+// Eight columns of a row that is read or, where `on` is false, zero: a lane's part of an
+// operand.
+template <bool VEC>
+__device__ __forceinline__ void load_operand(const float* row, int c, int width, bool on, u32x4 (&p)[3]) {
+    f32x4 a = load4<VEC>(row, c, width), b = load4<VEC>(row, c + 4, width);
+    if (!on) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+    split8<3>(a, b, p);
 }
-
-constexpr int kLdV = 36;  // row of a 32-wide LDS tile
-
-// 64 rows x 32 columns (from v0 of Dv) of a dense matrix of row stride `stride` as
-// float32 in LDS, zero past `rows` rows and Dv.
-template <typename T>
-__device__ __forceinline__ void stage32(float* lds, const T* src, long long stride, int rows, int v0, int Dv, int tid) {
+template <bool VEC>
+__device__ __forceinline__ void load_operand(const bf16* row, int c, int width, bool on, u32x4 (&p)[1]) {
+    if constexpr (VEC) {
+        const Bytes16 v = *reinterpret_cast<const Bytes16*>(row + min(c, width - 8));
+        p[0] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+        if (c >= width) p[0] = u32x4{0, 0, 0, 0};
+    } else {
+        p[0] = u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < kChunk * 8 / kThreads; ++i) {
-        const int r = (tid + i * kThreads) / 8, c = (tid + i * kThreads) % 8 * 4;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (src && r < rows) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (v0 + c + j < Dv) x[j] = to_f32(src[r * stride + v0 + c + j]);
+        for (int j = 0; j < 8; ++j) {
+            const unsigned v = row[min(c + j, width - 1)].bits;
+            p[0][j / 2] |= (c + j < width ? v : 0u) << (j % 2 * 16);
         }
-        *reinterpret_cast<f32x4*>(lds + r * kLdV + c) = x;
     }
+    if (!on) p[0] = u32x4{0, 0, 0, 0};
 }
 
 // Sum over the 16 lanes that hold a row of a 16x16 block.
@@ -59,249 +80,313 @@ __device__ __forceinline__ float row_sum(float x) {
     return x;
 }
 
-// The gradients of q, k, g and beta of a chunk and value head.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void gradients_kernel(Dims d, const T* q, const T* k, const T* dout, const void* g,
-                                                             const int* lengths, ChunkData in, BackwardData bd, void* dg,
-                                                             void* dbeta) {
-    __shared__ float f1[kChunk * kLd], f2[kChunk * kLd], ks[kChunk * kLd], qs[kChunk * kLd];
-    __shared__ float sdo[kChunk * kLdV], sdx[kChunk * kLdV], se[kChunk * kLdV], ss[kChunk * kLdV], sds[kChunk * kLdV];
+// Where four neighbouring columns (c of 32) of row `row` go among the fragments of a
+// 32-wide step: 8 bytes per piece.
+__device__ __forceinline__ void put_columns(u32x4* frags, int row, int c, f32x4 x) {
+    u32x2 p[3];
+    split<3>(x, p);
+    u32x2* at = reinterpret_cast<u32x2*>(frags + (size_t)(row / 16) * 3 * kFragLanes + c / 8 * 16 + row % 16) + c / 4 % 2;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) at[i * kFragLanes * 2] = p[i];
+}
+
+// KU: 32-wide steps over Dk (even).  VEC: Dv is a multiple of eight.
+template <typename T, int KU, bool VEC>
+__global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T* q, const T* k, const T* dout, const void* g,
+                                                                const int* lengths, ChunkData in, BackwardData bd, T* dq,
+                                                                T* dk, void* dg, void* dbeta) {
+    constexpr int NP = kPieces<T>, TB = 2 * KU, TH = KU;  // blocks of 16 rows of the state; a wavefront's
+    constexpr int kRows = TB * 16, kN = kRows * 8 / kThreads;  // float4 of S (and dS') per thread and step
+    constexpr int kFrags = (2 * TB + 4) * 3;                   // of a step: S, dS', E
+    constexpr int kShared = kFrags * kFragLanes * 16 > 2 * kChunk * kLd * 4 ? kFrags * kFragLanes * 16 : 2 * kChunk * kLd * 4;
+    __shared__ __attribute__((aligned(16))) char shared[kShared];
     __shared__ double gsum[kChunk];
-    __shared__ float sums[4][kChunk], dots[4];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, hi = lane / 16;
-    const int c = blockIdx.x % d.chunks, bh = blockIdx.x / d.chunks;
-    const int b = bh / d.Hv, h = bh % d.Hv, hk = h / (d.Hv / d.Hk);
-    const int t0 = c * kChunk, live = min(kChunk, row_length(lengths, b, d.T) - t0);
-    const size_t ch = blockIdx.x;
-    const size_t row0 = ((size_t)b * d.T + t0) * d.Hv + h;  // token row of the [B, T, Hv] tensors
+    __shared__ float bet[kChunk], sums[2][4][kChunk], dots[8];
+    u32x4* fs = reinterpret_cast<u32x4*>(shared);
+    u32x4* fd = fs + TB * 3 * kFragLanes;
+    u32x4* fe = fd + TB * 3 * kFragLanes;
+    float* f1 = reinterpret_cast<float*>(shared);  // (after the steps)
+    float* f2 = f1 + kChunk * kLd;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, hi = lane / 16;
+    const int w4 = wave % 4, half = wave / 4;
+    const int c = blockIdx.x % d.chunks, bk = blockIdx.x / d.chunks, b = bk / d.Hk, hk = bk % d.Hk, rep = d.Hv / d.Hk;
+    const int t0 = c * kChunk, live = min(kChunk, row_length(lengths, b, d.T) - t0), here = min(kChunk, d.T - t0);
+    const size_t kch = blockIdx.x;
     if (live <= 0) {
-        if (tid < min(kChunk, d.T - t0)) {
-            store_gate(dg, row0 + (size_t)tid * d.Hv, 0.f, d.gate_bf16);
-            store_gate(dbeta, row0 + (size_t)tid * d.Hv, 0.f, d.gate_bf16);
+        for (int i = tid; i < here * rep; i += kThreads) {
+            const size_t at = ((size_t)b * d.T + t0 + i / rep) * d.Hv + hk * rep + i % rep;
+            store_gate(dg, at, 0.f, d.gate_bf16);
+            store_gate(dbeta, at, 0.f, d.gate_bf16);
+        }
+        for (int i = tid; i < here * d.Dk; i += kThreads) {
+            const size_t at = (((size_t)b * d.T + t0 + i / d.Dk) * d.Hk + hk) * d.Dk + i % d.Dk;
+            dq[at] = from_f32<T>(0.f);
+            dk[at] = from_f32<T>(0.f);
         }
         return;
     }
-    const float* coef = in.coef + ch * kCoefFloats;
-    if (wave == 0)
-        gsum[lane] = chunk_sum(
-            lane < live ? load_gate(g, b * d.g_s[0] + (t0 + lane) * d.g_s[1] + h * d.g_s[2], d.gate_bf16) : 0.f, lane);
-    const T* pdo = dout ? dout + row0 * d.Dv : nullptr;
-    const float* pdx = bd.dx + row0 * d.Dv;
-    const float* pe = bd.e + row0 * d.Dv;
-    const float* ps = bd.states + ch * d.Dk * d.Dv;
-    const float* pds = bd.dstates + ch * d.Dk * d.Dv;
+    const float* norm = in.norm + kch * 2 * kChunk;
+    const size_t turned = kch * row_frags<T>(d.Dk) * kFragLanes + lane;
     const long long vrow = (long long)d.Hv * d.Dv;
-    {
-        f32x4 a1[4] = {}, a2[4] = {};
+    const int first = 16 * w4 + 4 * hi;
+    const f32x4 ck = *reinterpret_cast<const f32x4*>(norm + first), cq = *reinterpret_cast<const f32x4*>(norm + kChunk + first);
+    f32x4 sum_q[TH] = {}, sum_k[TH] = {}, dot_q{}, dot_k{};
+
+    for (int r = 0; r < rep; ++r) {
+        const int h = hk * rep + r;
+        const size_t ch = ((size_t)b * d.Hv + h) * d.chunks + c;
+        const size_t row0 = ((size_t)b * d.T + t0) * d.Hv + h;  // token row of the [B, T, Hv] tensors
+        const float* coef = in.coef + ch * kCoefFloats;
+        // (a zero that the compiler does not know: what hangs on it stays in the loop,
+        // where the addresses of every block of Dk would fill the registers)
+        size_t zero = 0;
+        asm volatile("" : "+s"(zero));
+        if (wave == 0) {
+            gsum[lane] = chunk_sum(
+                lane < live ? load_gate(g, b * d.g_s[0] + (t0 + lane) * d.g_s[1] + h * d.g_s[2], d.gate_bf16) : 0.f, lane);
+            bet[lane] = coef[BETA * kChunk + lane];
+        }
+        // of the lane's rows as operands
+        const bool on = 16 * w4 + n < live;
+        const int token = min(16 * w4 + n, live - 1);
+        const T* pdo = dout ? dout + row0 * d.Dv + token * vrow : nullptr;
+        const float* pdx = bd.dx + row0 * d.Dv + token * vrow;
+        const float* pe = bd.e + row0 * d.Dv;
+        const float* ps = bd.states + ch * d.Dk * d.Dv;
+        const float* pd = bd.dstates + ch * d.Dk * d.Dv;
+        // of the next step: S, dS' and E as they will go to LDS, dO and dX
+        f32x4 ns[kN], nd[kN], ne;
+        auto load = [&](int v0) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const int x = tid + i * kThreads, row = min(x / 8, d.Dk - 1);
+                ns[i] = load4<VEC>(ps + (size_t)row * d.Dv, v0 + x % 8 * 4, d.Dv);
+                nd[i] = load4<VEC>(pd + (size_t)row * d.Dv, v0 + x % 8 * 4, d.Dv);
+            }
+            ne = load4<VEC>(pe + min(tid / 8, live - 1) * vrow, v0 + tid % 8 * 4, d.Dv);
+        };
+        f32x4 aq[TH] = {}, ar[TH] = {}, az[TH] = {}, af[4] = {};
+        float dot = 0.f;
+        load(0);
         for (int v0 = 0; v0 < d.Dv; v0 += 32) {
+            u32x4 xo[NP], xx[3], xe[3];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) xo[i] = u32x4{0, 0, 0, 0};
+            if (dout) load_operand<VEC>(pdo, v0 + 8 * hi, d.Dv, on, xo);
+            load_operand<VEC>(pdx, v0 + 8 * hi, d.Dv, on, xx);
             __syncthreads();
-            stage32(sdo, pdo, vrow, live, v0, d.Dv, tid);
-            stage32(sdx, pdx, vrow, live, v0, d.Dv, tid);
-            stage32(se, pe, vrow, live, v0, d.Dv, tid);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const int x = tid + i * kThreads;
+                if (x / 8 >= d.Dk) ns[i] = nd[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dot += ns[i][j] * nd[i][j];
+                put_columns(fs, x / 8, x % 8 * 4, ns[i]);
+                put_columns(fd, x / 8, x % 8 * 4, nd[i]);
+            }
+            put_columns(fe, tid / 8, tid % 8 * 4, tid / 8 < live ? ne : f32x4{0.f, 0.f, 0.f, 0.f});
             __syncthreads();
+            if (v0 + 32 < d.Dv) load(v0 + 32);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const f32x4 x1 = *reinterpret_cast<const f32x4*>(sdo + (16 * wave + n) * kLdV + s * 16 + hi * 4);
-                const f32x4 x2 = *reinterpret_cast<const f32x4*>(sdx + (16 * wave + n) * kLdV + s * 16 + hi * 4);
+            for (int i = 0; i < 3; ++i) xe[i] = fe[(w4 * 3 + i) * kFragLanes + lane];
+            // dO E^T by the one half of the wavefronts, dX E^T by the other
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j > wave) break;
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(se + (16 * j + n) * kLdV + s * 16 + hi * 4);
+            for (int j = 0; j < 4; ++j) {
+                if (j > w4) break;
+                u32x4 y[3];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        a1[j] = mfma4(x1[r], y[r], a1[j]);
-                        a2[j] = mfma4(x2[r], y[r], a2[j]);
-                    }
+                for (int i = 0; i < 3; ++i) y[i] = fe[(j * 3 + i) * kFragLanes + lane];
+                af[j] = half ? mul(xx, y, af[j]) : mul(xo, y, af[j]);
+                settle(af[j]);
+            }
+#pragma unroll
+            for (int t = 0; t < TH; ++t) {
+                u32x4 ys[3], yd[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    ys[i] = fs[((half * TH + t) * 3 + i) * kFragLanes + lane];
+                    yd[i] = fd[((half * TH + t) * 3 + i) * kFragLanes + lane];
                 }
+                aq[t] = mul(xo, ys, aq[t]);
+                ar[t] = mul(xx, ys, ar[t]);
+                az[t] = mul(xe, yd, az[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 0; t < TH; ++t) {
+                settle(aq[t]);
+                settle(ar[t]);
+                settle(az[t]);
+            }
+        }
+        __syncthreads();
+        {
+            float* f = half ? f2 : f1;
+            const float by = half ? -1.f : d.scale;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = first + i, col = 16 * j + n;
+                    const bool in_f = half ? row > col : row >= col;
+                    const float w = made(expf((float)(gsum[row] - gsum[col])));
+                    f[row * kLd + col] = in_f ? by * af[j][i] * w : 0.f;
+                }
+        }
+        f32x4 eg, el, beta;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            eg[i] = expf((float)gsum[first + i]);
+            el[i] = expf((float)(gsum[kChunk - 1] - gsum[first + i]));
+            beta[i] = bet[first + i];
+        }
+        __syncthreads();
+        // Rows of F1 B and F2 B (of the normalised keys), then of F1^T and F2^T (of the
+        // normalised queries and keys): two at a time, and a block of Dk at a time, for
+        // the registers' sake.  (The half of a triangle that is zero is multiplied too:
+        // no branch between the products.)
+        f32x4 rq{}, rk{}, rz{}, rw{};
+        u32x4 x[2][2][3];
+        auto operands = [&](auto value) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    f32x4 a[2];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a[i / 4][i % 4] = value(m, 32 * w + 8 * hi + i);
+                    split8<3>(a[0], a[1], x[m][w]);
+                }
+        };
+        auto turned_frag = [&](const u32x4* from, int blk, int w, u32x4 (&y)[NP]) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) y[i] = from[zero + turned + ((size_t)(blk * 2 + w) * NP + i) * kFragLanes];
+        };
+        // the normalised rows of q or k, as a product leaves its block
+        auto values = [&](const T* from, const long long* st, int blk, f32x4 by) {
+            const int dim = 16 * blk + n;
+            const T* p = from + zero + b * st[0] + t0 * st[1] + hk * st[2] + min(dim, d.Dk - 1);
+            f32x4 y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = made(to_f32(p[min(first + i, live - 1) * st[1]]));
+                y[i] = first + i < live && dim < d.Dk ? v * by[i] : 0.f;
+            }
+            return y;
+        };
+        operands([&](int m, int t) { return (m ? f2 : f1)[(16 * w4 + n) * kLd + t] * (bet[t] * norm[t]); });
+#pragma unroll
+        for (int t = 0; t < TH; ++t) {
+            const int blk = half * TH + t;
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            aq[t] *= d.scale * eg;
+            ar[t] *= -eg;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                u32x4 y[NP];
+                turned_frag(in.kt, blk, w, y);
+                aq[t] = mul(x[0][w], y, aq[t]);
+                ar[t] = mul(x[1][w], y, ar[t]);
+            }
+            settle(aq[t]);
+            settle(ar[t]);
+            sum_q[t] += aq[t];
+            sum_k[t] += ar[t];
+            rq += aq[t] * values(q, d.q_s, blk, cq);
+            rk += ar[t] * values(k, d.k_s, blk, ck);
+        }
+        operands([&](int m, int t) { return (m ? f2 : f1)[t * kLd + 16 * w4 + n] * norm[m ? t : kChunk + t]; });
+#pragma unroll
+        for (int t = 0; t < TH; ++t) {
+            const int blk = half * TH + t;
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            const f32x4 kv = values(k, d.k_s, blk, ck);
+            az[t] *= el;
+            rw += az[t] * kv;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                u32x4 y[NP];
+                turned_frag(in.qt, blk, w, y);
+                az[t] = mul(x[0][w], y, az[t]);
+                turned_frag(in.kt, blk, w, y);
+                az[t] = mul(x[1][w], y, az[t]);
+            }
+            settle(az[t]);
+            rz += az[t] * kv;
+            sum_k[t] += beta * az[t];
+        }
+        dot_q += rq;
+        dot_k += rk + beta * rz;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = row_sum(rq[i]), bb = row_sum(rk[i]), z = row_sum(rz[i]), w = row_sum(rw[i]);
+            if (n == 0) {
+                sums[half][0][first + i] = a;
+                sums[half][1][first + i] = bb;
+                sums[half][2][first + i] = z;
+                sums[half][3][first + i] = w * beta[i];
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int o = 1; o < 64; o *= 2) dot += __shfl_xor(dot, o);
+        if (lane == 0) dots[wave] = dot;
+        __syncthreads();
+        if (wave == 0) {
+            float w = sums[0][3][lane] + sums[1][3][lane];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                const float w = row >= col ? expf((float)(gsum[row] - gsum[col])) : 0.f;
-                f1[row * kLd + col] = row >= col ? d.scale * a1[j][r] * w : 0.f;
-                f2[row * kLd + col] = row > col ? -a2[j][r] * w : 0.f;
-            }
-    }
-    const T* kb = k + b * d.k_s[0] + t0 * d.k_s[1] + hk * d.k_s[2];
-    const T* qb = q + b * d.q_s[0] + t0 * d.q_s[1] + hk * d.q_s[2];
-    // exp(G) and exp(G_C - G) of the thread's rows
-    float eg[4], el[4], cki[4], cqi[4], bi[4], rq[4] = {}, rk[4] = {}, rz[4] = {}, rw[4] = {}, dot = 0.f;
+            for (int o = 1; o < 64; o *= 2) w += __shfl_xor(w, o);
+            const float db = sums[0][2][lane] + sums[1][2][lane];
+            float v = (sums[0][0][lane] + sums[1][0][lane]) + (sums[0][1][lane] + sums[1][1][lane]) - bet[lane] * db;
+            if (lane == 63) {
+                float all = 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = 16 * wave + 4 * hi + r;
-        eg[r] = expf((float)gsum[row]);
-        el[r] = expf((float)(gsum[kChunk - 1] - gsum[row]));
-        cki[r] = coef[CK * kChunk + row];
-        cqi[r] = coef[CQ * kChunk + row];
-        bi[r] = coef[BETA * kChunk + row];
-    }
-    for (int d0 = 0; d0 < d.Dk; d0 += 64) {
-        f32x4 aq[4] = {}, ar[4] = {}, az[4] = {};
-        for (int v0 = 0; v0 < d.Dv; v0 += 32) {
-            __syncthreads();
-            if (v0 == 0) {
-                stage64(ks, kb, d.k_s[1], live, d0, d.Dk, tid);
-                stage64(qs, qb, d.q_s[1], live, d0, d.Dk, tid);
-            }
-            stage32(sdo, pdo, vrow, live, v0, d.Dv, tid);
-            stage32(sdx, pdx, vrow, live, v0, d.Dv, tid);
-            stage32(se, pe, vrow, live, v0, d.Dv, tid);
-            stage32(ss, ps + (size_t)d0 * d.Dv, d.Dv, d.Dk - d0, v0, d.Dv, tid);
-            stage32(sds, pds + (size_t)d0 * d.Dv, d.Dv, d.Dk - d0, v0, d.Dv, tid);
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kChunk * 32 / kThreads; ++i) {
-                const int r = (tid + i * kThreads) / 32, cc = (tid + i * kThreads) % 32;
-                dot += ss[r * kLdV + cc] * sds[r * kLdV + cc];
+                for (int i = 0; i < 8; ++i) all += dots[i];
+                v += w + expf((float)gsum[kChunk - 1]) * all;
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int at = (16 * wave + n) * kLdV + s * 16 + hi * 4;
-                const f32x4 xo = *reinterpret_cast<const f32x4*>(sdo + at);
-                const f32x4 xx = *reinterpret_cast<const f32x4*>(sdx + at);
-                const f32x4 xe = *reinterpret_cast<const f32x4*>(se + at);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 ys = *reinterpret_cast<const f32x4*>(ss + (16 * j + n) * kLdV + s * 16 + hi * 4);
-                    const f32x4 yd = *reinterpret_cast<const f32x4*>(sds + (16 * j + n) * kLdV + s * 16 + hi * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        aq[j] = mfma4(xo[r], ys[r], aq[j]);
-                        ar[j] = mfma4(xx[r], ys[r], ar[j]);
-                        az[j] = mfma4(xe[r], yd[r], az[j]);
-                    }
-                }
+            for (int o = 1; o < 64; o *= 2) {
+                const float down = __shfl_down(v, o);
+                if (lane + o < 64) v += down;
+            }
+            if (lane < here) {
+                store_gate(dg, row0 + (size_t)lane * d.Hv, lane < live ? v : 0.f, d.gate_bf16);
+                store_gate(dbeta, row0 + (size_t)lane * d.Hv, lane < live ? db : 0.f, d.gate_bf16);
             }
         }
-        // now in terms of the normalised keys and queries
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                aq[j][r] *= d.scale * eg[r];
-                ar[j][r] *= -eg[r];
-                az[j][r] *= el[r];
-                rw[r] += az[j][r] * ks[row * kLd + col] * cki[r];
-            }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {  // 16 tokens of the sum
-            const f32x4 ckm = *reinterpret_cast<const f32x4*>(coef + CK * kChunk + 16 * m + 4 * hi);
-            const f32x4 cqm = *reinterpret_cast<const f32x4*>(coef + CQ * kChunk + 16 * m + 4 * hi);
-            const f32x4 bm = *reinterpret_cast<const f32x4*>(coef + BETA * kChunk + 16 * m + 4 * hi);
-            const f32x4 x1 = *reinterpret_cast<const f32x4*>(f1 + (16 * wave + n) * kLd + 16 * m + 4 * hi);
-            const f32x4 x2 = *reinterpret_cast<const f32x4*>(f2 + (16 * wave + n) * kLd + 16 * m + 4 * hi);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int tok = 16 * m + 4 * hi + r;
-                const float xt1 = f1[tok * kLd + 16 * wave + n], xt2 = f2[tok * kLd + 16 * wave + n];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float kv = ks[tok * kLd + 16 * j + n] * ckm[r], qv = qs[tok * kLd + 16 * j + n] * cqm[r];
-                    aq[j] = mfma4(x1[r] * bm[r], kv, aq[j]);
-                    ar[j] = mfma4(x2[r] * bm[r], kv, ar[j]);
-                    az[j] = mfma4(xt1, qv, az[j]);
-                    az[j] = mfma4(xt2, kv, az[j]);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * hi + r, col = 16 * j + n;
-                const float kv = ks[row * kLd + col] * cki[r], qv = qs[row * kLd + col] * cqi[r];
-                rq[r] += aq[j][r] * qv;
-                rk[r] += ar[j][r] * kv;
-                rz[r] += az[j][r] * kv;
-                if (row < live && d0 + col < d.Dk) {
-                    const size_t at = (row0 + (size_t)row * d.Hv) * d.Dk + d0 + col;
-                    bd.dq[at] = aq[j][r];
-                    bd.dk[at] = ar[j][r] + bi[r] * az[j][r];
-                }
-            }
+        __syncthreads();
     }
+    // The normalisation's gradient, dx = c (dy - y (y . dy)) with y = c x.
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = 16 * wave + 4 * hi + r;
-        const float a = row_sum(rq[r]), bb = row_sum(rk[r]), z = row_sum(rz[r]), w = row_sum(rw[r]);
+    for (int i = 0; i < 4; ++i) {
+        const float a = row_sum(dot_q[i]), bb = row_sum(dot_k[i]);
         if (n == 0) {
-            sums[0][row] = a;
-            sums[1][row] = bb;
-            sums[2][row] = z;
-            sums[3][row] = w * bi[r];
+            sums[half][0][first + i] = a;
+            sums[half][1][first + i] = bb;
         }
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) dot += __shfl_xor(dot, o);
-    if (lane == 0) dots[wave] = dot;
     __syncthreads();
-    if (wave != 0) return;
-    float w = sums[3][lane];
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) w += __shfl_xor(w, o);
-    const float db = sums[2][lane];
-    float dgv = sums[0][lane] + sums[1][lane] - coef[BETA * kChunk + lane] * db;
-    if (lane == 63) dgv += w + expf((float)gsum[kChunk - 1]) * (dots[0] + dots[1] + dots[2] + dots[3]);
+    for (int i = 0; i < 4; ++i) {
+        const int tok = first + i;
+        if (tok >= here) continue;
+        const float yq = sums[0][0][tok] + sums[1][0][tok], yk = sums[0][1][tok] + sums[1][1][tok];
+        const size_t to = (((size_t)b * d.T + t0 + tok) * d.Hk + hk) * d.Dk;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const float down = __shfl_down(dgv, o);
-        if (lane + o < 64) dgv += down;
-    }
-    if (lane < min(kChunk, d.T - t0)) {
-        store_gate(dg, row0 + (size_t)lane * d.Hv, lane < live ? dgv : 0.f, d.gate_bf16);
-        store_gate(dbeta, row0 + (size_t)lane * d.Hv, lane < live ? db : 0.f, d.gate_bf16);
-    }
-}
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
-    return x;
-}
-
-// dq and dk of the key heads: the sum over the value heads that share one, then
-// the normalisation's gradient, dx = c (dy - y (y . dy)) with y = c x.  A wavefront
-// per token and key head.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void finish_kernel(Dims d, const T* q, const T* k, const int* lengths,
-                                                          BackwardData bd, T* dq, T* dk) {
-    constexpr int M = kMaxKeyDim / 64;
-    const long long row = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
-    if (row >= (long long)d.B * d.T * d.Hk) return;
-    const int lane = threadIdx.x % 64, hk = (int)(row % d.Hk), rep = d.Hv / d.Hk;
-    const long long bt = row / d.Hk;
-    const int b = (int)(bt / d.T), t = (int)(bt % d.T);
-    const bool on = t < row_length(lengths, b, d.T);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const float* part = (which ? bd.dk : bd.dq) + (bt * d.Hv + (long long)hk * rep) * d.Dk;
-        const T* x = which ? k + b * d.k_s[0] + t * d.k_s[1] + hk * d.k_s[2] : q + b * d.q_s[0] + t * d.q_s[1] + hk * d.q_s[2];
-        T* out = (which ? dk : dq) + row * d.Dk;
-        float v[M], xv[M], x2 = 0.f, xd = 0.f;
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const int i = lane + 64 * m;
-            v[m] = xv[m] = 0.f;
-            if (!on || i >= d.Dk) continue;
-            for (int r = 0; r < rep; ++r) v[m] += part[(long long)r * d.Dk + i];
-            xv[m] = to_f32(x[i]);
-            x2 += xv[m] * xv[m];
-            xd += xv[m] * v[m];
+        for (int t = 0; t < TH; ++t) {
+            const int dim = 16 * (half * TH + t) + n;
+            if (dim >= d.Dk) continue;
+            float vq = sum_q[t][i], vk = sum_k[t][i];
+            if (d.normalize && tok < live) {
+                const float x = to_f32(k[b * d.k_s[0] + (t0 + tok) * d.k_s[1] + hk * d.k_s[2] + dim]);
+                const float y = to_f32(q[b * d.q_s[0] + (t0 + tok) * d.q_s[1] + hk * d.q_s[2] + dim]);
+                vq = cq[i] * (vq - cq[i] * y * yq);
+                vk = ck[i] * (vk - ck[i] * x * yk);
+            }
+            dq[to + dim] = from_f32<T>(tok < live ? vq : 0.f);
+            dk[to + dim] = from_f32<T>(tok < live ? vk : 0.f);
         }
-        if (d.normalize) {
-            x2 = wave_sum(x2);
-            xd = wave_sum(xd);
-            const float c = 1.f / sqrtf(x2 + kNormEps);
-#pragma unroll
-            for (int m = 0; m < M; ++m) v[m] = c * (v[m] - c * c * xd * xv[m]);
-        }
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-            if (lane + 64 * m < d.Dk) out[lane + 64 * m] = from_f32<T>(v[m]);
     }
 }
 
@@ -311,15 +396,24 @@ template <typename T>
 int launch_gradients(const Dims& d, const T* q, const T* k, const T* dout, const void* g, const int* lengths,
                      const ChunkData& in, const BackwardData& bd, T* dq, T* dk, void* dg, void* dbeta,
                      hipStream_t stream) {
-    const long long blocks = (long long)d.B * d.Hv * d.chunks;
+    const long long blocks = (long long)d.B * d.Hk * d.chunks;
     if (blocks == 0) return 0;
     RKA_RETURN_IF_ERR(check_grid(blocks, kThreads, "gated_delta_backward"));
-    hipLaunchKernelGGL((gradients_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, q, k, dout, g, lengths,
-                       in, bd, dg, dbeta);
-    RKA_RETURN_IF_HIP(hipGetLastError());
-    const long long rows = (long long)d.B * d.T * d.Hk, fin = (rows + kThreads / 64 - 1) / (kThreads / 64);
-    RKA_RETURN_IF_ERR(check_grid(fin, kThreads, "gated_delta_backward"));
-    hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)fin), dim3(kThreads), 0, stream, d, q, k, lengths, bd, dq, dk);
+    auto go = [&](auto ku) {
+        constexpr int KU = decltype(ku)::value;
+        if (d.Dv % 8 == 0)
+            hipLaunchKernelGGL((gradients_kernel<T, KU, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, q, k,
+                               dout, g, lengths, in, bd, dq, dk, dg, dbeta);
+        else
+            hipLaunchKernelGGL((gradients_kernel<T, KU, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, q, k,
+                               dout, g, lengths, in, bd, dq, dk, dg, dbeta);
+    };
+    switch (chain_steps(d.Dk)) {
+        case 2: go(std::integral_constant<int, 2>{}); break;
+        case 4: go(std::integral_constant<int, 4>{}); break;
+        case 6: go(std::integral_constant<int, 6>{}); break;
+        default: go(std::integral_constant<int, 8>{}); break;
+    }
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
