@@ -46,30 +46,70 @@ __device__ __forceinline__ f32x4 load4(const float* row, int c, int width) {
     return x;
 }
 
-// Eight columns of a row that is read or, where `on` is false, zero: a lane's part of an
-// operand.
-template <bool VEC>
-__device__ __forceinline__ void load_operand(const float* row, int c, int width, bool on, u32x4 (&p)[3]) {
-    f32x4 a = load4<VEC>(row, c, width), b = load4<VEC>(row, c + 4, width);
-    if (!on) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
-    split8<3>(a, b, p);
-}
-template <bool VEC>
-__device__ __forceinline__ void load_operand(const bf16* row, int c, int width, bool on, u32x4 (&p)[1]) {
-    if constexpr (VEC) {
-        const Bytes16 v = *reinterpret_cast<const Bytes16*>(row + min(c, width - 8));
-        p[0] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
-        if (c >= width) p[0] = u32x4{0, 0, 0, 0};
-    } else {
-        p[0] = u32x4{0, 0, 0, 0};
+// Eight columns of a row: a lane's part of an operand, as loaded and in pieces (zero
+// where the row is not `on`).
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+    f32x4 a, b;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const float* row, int c, int width) {
+        a = load4<VEC>(row, c, width);
+        b = load4<VEC>(row, c + 4, width);
+    }
+    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[3]) {
+        if (!on) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        split8<3>(a, b, p);
+    }
+};
+template <>
+struct Eight<bf16> {
+    u32x4 x;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const bf16* row, int c, int width) {
+        if constexpr (VEC) {
+            const Bytes16 v = *reinterpret_cast<const Bytes16*>(row + min(c, width - 8));
+            x = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+            if (c >= width) x = u32x4{0, 0, 0, 0};
+        } else {
+            x = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned v = row[min(c + j, width - 1)].bits;
-            p[0][j / 2] |= (c + j < width ? v : 0u) << (j % 2 * 16);
+            for (int j = 0; j < 8; ++j) {
+                const unsigned v = row[min(c + j, width - 1)].bits;
+                x[j / 2] |= (c + j < width ? v : 0u) << (j % 2 * 16);
+            }
         }
     }
-    if (!on) p[0] = u32x4{0, 0, 0, 0};
-}
+    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[1]) { p[0] = on ? x : u32x4{0, 0, 0, 0}; }
+};
+
+// An element of q and one of k.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<float> {
+    float x, y;
+    __device__ __forceinline__ void set(float a, float b) {
+        x = a;
+        y = b;
+    }
+    __device__ __forceinline__ float q() const { return made(x); }
+    __device__ __forceinline__ float k() const { return made(y); }
+};
+template <>
+struct Pair<bf16> {
+    unsigned x;
+    __device__ __forceinline__ void set(bf16 a, bf16 b) { x = (unsigned)b.bits << 16 | a.bits; }
+    // (unpacked where it is used, not ahead of the loop into twice the registers)
+    __device__ __forceinline__ unsigned here() const {
+        unsigned y = x;
+        asm volatile("" : "+v"(y));
+        return y;
+    }
+    __device__ __forceinline__ float q() const { return __uint_as_float(here() << 16); }
+    __device__ __forceinline__ float k() const { return __uint_as_float(here() & 0xffff0000u); }
+};
 
 // Sum over the 16 lanes that hold a row of a 16x16 block.
 __device__ __forceinline__ float row_sum(float x) {
@@ -100,6 +140,16 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
     constexpr int kFrags = (2 * TB + 4) * 3;                   // of a step: S, dS', E
     constexpr int kShared = kFrags * kFragLanes * 16 > 2 * kChunk * kLd * 4 ? kFrags * kFragLanes * 16 : 2 * kChunk * kLd * 4;
     __shared__ __attribute__((aligned(16))) char shared[kShared];
+    // sums of dq and dk over the value heads, a lane's own: in LDS where they fit
+    constexpr bool kSumsInLds = KU <= 4;
+    __shared__ f32x4 lds_sums[kSumsInLds ? 2 * TH * kThreads : 1];
+    f32x4 reg_sums[kSumsInLds ? 1 : 2 * TH];
+    auto sum = [&](int which, int t) -> f32x4& {
+        if constexpr (kSumsInLds)
+            return lds_sums[(which * TH + t) * kThreads + threadIdx.x];
+        else
+            return reg_sums[which * TH + t];
+    };
     __shared__ double gsum[kChunk];
     __shared__ float bet[kChunk], sums[2][4][kChunk], dots[8];
     u32x4* fs = reinterpret_cast<u32x4*>(shared);
@@ -130,7 +180,30 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
     const long long vrow = (long long)d.Hv * d.Dv;
     const int first = 16 * w4 + 4 * hi;
     const f32x4 ck = *reinterpret_cast<const f32x4*>(norm + first), cq = *reinterpret_cast<const f32x4*>(norm + kChunk + first);
-    f32x4 sum_q[TH] = {}, sum_k[TH] = {}, dot_q{}, dot_k{};
+    // the rows of q and k, as a product leaves its blocks
+    Pair<T> qk[TH][4];
+#pragma unroll
+    for (int t = 0; t < TH; ++t) {
+        const int dim = min(16 * (half * TH + t) + n, d.Dk - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tok = t0 + min(first + i, live - 1);
+            const T none = from_f32<T>(0.f);
+            const bool real = first + i < live && 16 * (half * TH + t) + n < d.Dk;
+            const T x = q[b * d.q_s[0] + tok * d.q_s[1] + hk * d.q_s[2] + dim];
+            const T y = k[b * d.k_s[0] + tok * d.k_s[1] + hk * d.k_s[2] + dim];
+            qk[t][i].set(real ? x : none, real ? y : none);
+        }
+    }
+    auto values = [&](int which, int t) {
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = which ? qk[t][i].k() * ck[i] : qk[t][i].q() * cq[i];
+        return y;
+    };
+    f32x4 dot_q{}, dot_k{};
+#pragma unroll
+    for (int t = 0; t < TH; ++t) sum(0, t) = sum(1, t) = f32x4{0.f, 0.f, 0.f, 0.f};
 
     for (int r = 0; r < rep; ++r) {
         const int h = hk * rep + r;
@@ -141,11 +214,9 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
         // where the addresses of every block of Dk would fill the registers)
         size_t zero = 0;
         asm volatile("" : "+s"(zero));
-        if (wave == 0) {
-            gsum[lane] = chunk_sum(
-                lane < live ? load_gate(g, b * d.g_s[0] + (t0 + lane) * d.g_s[1] + h * d.g_s[2], d.gate_bf16) : 0.f, lane);
-            bet[lane] = coef[BETA * kChunk + lane];
-        }
+        float gate = 0.f;
+        if (wave == 0)
+            gate = load_gate(g, b * d.g_s[0] + (t0 + min(lane, live - 1)) * d.g_s[1] + h * d.g_s[2], d.gate_bf16);
         // of the lane's rows as operands
         const bool on = 16 * w4 + n < live;
         const int token = min(16 * w4 + n, live - 1);
@@ -156,6 +227,8 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
         const float* pd = bd.dstates + ch * d.Dk * d.Dv;
         // of the next step: S, dS' and E as they will go to LDS, dO and dX
         f32x4 ns[kN], nd[kN], ne;
+        Eight<T> no{};
+        Eight<float> nx;
         auto load = [&](int v0) {
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
@@ -164,16 +237,16 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
                 nd[i] = load4<VEC>(pd + (size_t)row * d.Dv, v0 + x % 8 * 4, d.Dv);
             }
             ne = load4<VEC>(pe + min(tid / 8, live - 1) * vrow, v0 + tid % 8 * 4, d.Dv);
+            if (dout) no.template load<VEC>(pdo, v0 + 8 * hi, d.Dv);
+            nx.template load<VEC>(pdx, v0 + 8 * hi, d.Dv);
         };
         f32x4 aq[TH] = {}, ar[TH] = {}, az[TH] = {}, af[4] = {};
         float dot = 0.f;
         load(0);
         for (int v0 = 0; v0 < d.Dv; v0 += 32) {
             u32x4 xo[NP], xx[3], xe[3];
-#pragma unroll
-            for (int i = 0; i < NP; ++i) xo[i] = u32x4{0, 0, 0, 0};
-            if (dout) load_operand<VEC>(pdo, v0 + 8 * hi, d.Dv, on, xo);
-            load_operand<VEC>(pdx, v0 + 8 * hi, d.Dv, on, xx);
+            no.pieces(on && dout, xo);
+            nx.pieces(on, xx);
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
@@ -219,6 +292,10 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
                 settle(az[t]);
             }
         }
+        if (wave == 0) {
+            gsum[lane] = chunk_sum(lane < live ? gate : 0.f, lane);
+            bet[lane] = coef[BETA * kChunk + lane];
+        }
         __syncthreads();
         {
             float* f = half ? f2 : f1;
@@ -258,64 +335,57 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
                     split8<3>(a[0], a[1], x[m][w]);
                 }
         };
-        auto turned_frag = [&](const u32x4* from, int blk, int w, u32x4 (&y)[NP]) {
+        auto turned_frags = [&](const u32x4* from, int t, u32x4 (&y)[2][NP]) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) y[i] = from[zero + turned + ((size_t)(blk * 2 + w) * NP + i) * kFragLanes];
-        };
-        // the normalised rows of q or k, as a product leaves its block
-        auto values = [&](const T* from, const long long* st, int blk, f32x4 by) {
-            const int dim = 16 * blk + n;
-            const T* p = from + zero + b * st[0] + t0 * st[1] + hk * st[2] + min(dim, d.Dk - 1);
-            f32x4 y;
+            for (int w = 0; w < 2; ++w)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = made(to_f32(p[min(first + i, live - 1) * st[1]]));
-                y[i] = first + i < live && dim < d.Dk ? v * by[i] : 0.f;
-            }
-            return y;
+                for (int i = 0; i < NP; ++i)
+                    y[w][i] = from[zero + turned + ((size_t)((half * TH + t) * 2 + w) * NP + i) * kFragLanes];
         };
+        // (loaded a block ahead)
+        u32x4 yk[2][2][NP], yq[2][2][NP];
+        turned_frags(in.kt, 0, yk[0]);
         operands([&](int m, int t) { return (m ? f2 : f1)[(16 * w4 + n) * kLd + t] * (bet[t] * norm[t]); });
 #pragma unroll
         for (int t = 0; t < TH; ++t) {
-            const int blk = half * TH + t;
+            turned_frags(in.kt, (t + 1) % TH, yk[(t + 1) % 2]);
+            if (t + 1 == TH) turned_frags(in.qt, 0, yq[0]);
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
             aq[t] *= d.scale * eg;
             ar[t] *= -eg;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                u32x4 y[NP];
-                turned_frag(in.kt, blk, w, y);
-                aq[t] = mul(x[0][w], y, aq[t]);
-                ar[t] = mul(x[1][w], y, ar[t]);
+                aq[t] = mul(x[0][w], yk[t % 2][w], aq[t]);
+                ar[t] = mul(x[1][w], yk[t % 2][w], ar[t]);
             }
             settle(aq[t]);
             settle(ar[t]);
-            sum_q[t] += aq[t];
-            sum_k[t] += ar[t];
-            rq += aq[t] * values(q, d.q_s, blk, cq);
-            rk += ar[t] * values(k, d.k_s, blk, ck);
+            sum(0, t) += aq[t];
+            sum(1, t) += ar[t];
+            rq += aq[t] * values(0, t);
+            rk += ar[t] * values(1, t);
         }
         operands([&](int m, int t) { return (m ? f2 : f1)[t * kLd + 16 * w4 + n] * norm[m ? t : kChunk + t]; });
 #pragma unroll
         for (int t = 0; t < TH; ++t) {
-            const int blk = half * TH + t;
+            if (t + 1 < TH) {
+                turned_frags(in.kt, t + 1, yk[(t + 1) % 2]);
+                turned_frags(in.qt, t + 1, yq[(t + 1) % 2]);
+            }
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
-            const f32x4 kv = values(k, d.k_s, blk, ck);
+            const f32x4 y = values(1, t);
             az[t] *= el;
-            rw += az[t] * kv;
+            rw += az[t] * y;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                u32x4 y[NP];
-                turned_frag(in.qt, blk, w, y);
-                az[t] = mul(x[0][w], y, az[t]);
-                turned_frag(in.kt, blk, w, y);
-                az[t] = mul(x[1][w], y, az[t]);
+                az[t] = mul(x[0][w], yq[t % 2][w], az[t]);
+                az[t] = mul(x[1][w], yk[t % 2][w], az[t]);
             }
             settle(az[t]);
-            rz += az[t] * kv;
-            sum_k[t] += beta * az[t];
+            rz += az[t] * y;
+            sum(1, t) += beta * az[t];
         }
         dot_q += rq;
         dot_k += rk + beta * rz;
@@ -377,12 +447,10 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
         for (int t = 0; t < TH; ++t) {
             const int dim = 16 * (half * TH + t) + n;
             if (dim >= d.Dk) continue;
-            float vq = sum_q[t][i], vk = sum_k[t][i];
+            float vq = sum(0, t)[i], vk = sum(1, t)[i];
             if (d.normalize && tok < live) {
-                const float x = to_f32(k[b * d.k_s[0] + (t0 + tok) * d.k_s[1] + hk * d.k_s[2] + dim]);
-                const float y = to_f32(q[b * d.q_s[0] + (t0 + tok) * d.q_s[1] + hk * d.q_s[2] + dim]);
-                vq = cq[i] * (vq - cq[i] * y * yq);
-                vk = ck[i] * (vk - ck[i] * x * yk);
+                vq = cq[i] * (vq - cq[i] * qk[t][i].q() * yq);
+                vk = ck[i] * (vk - ck[i] * qk[t][i].k() * yk);
             }
             dq[to + dim] = from_f32<T>(tok < live ? vq : 0.f);
             dk[to + dim] = from_f32<T>(tok < live ? vk : 0.f);
