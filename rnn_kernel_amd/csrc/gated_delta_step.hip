@@ -14,10 +14,9 @@ constexpr int kThreads = 256;
 constexpr int kColThreads = 8;                       // threads of a row, four columns each
 constexpr int kCols = 4 * kColThreads;
 constexpr int kRowGroups = kThreads / kColThreads;   // rows in flight
-constexpr int kRows = kMaxKeyDim / kRowGroups;       // rows of a thread
 
-// VEC: the state's rows are aligned float4.
-template <typename T, bool VEC>
+// VEC: the state's rows are aligned float4.  kRows: rows of a thread, at most.
+template <typename T, bool VEC, int kRows>
 __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, const T* q, const T* k, const T* v, const void* g,
                                                         const void* beta, float* state, const int* slots, int num_slots,
                                                         T* o) {
@@ -41,27 +40,35 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, const T* q, cons
     float* sb = state + ((size_t)slot * d.Hv + h) * d.Dk * d.Dv;
     const T* qb = q + b * d.q_s[0] + hk * d.q_s[2];
     const T* kb = k + b * d.k_s[0] + hk * d.k_s[2];
+    // Everything is loaded at once, from clamped addresses: a load under a branch would
+    // be waited for there.
     f32x4 s[kRows];
-    float kv[kRows], qv[kRows];
-    const float decay = expf(floor_gate(load_gate(g, b * d.g_s[0] + h * d.g_s[2], d.gate_bf16)));
+    T kr[kRows], qr[kRows], vr[4];
+    const float gate = load_gate(g, b * d.g_s[0] + h * d.g_s[2], d.gate_bf16);
+    const float bt = load_gate(beta, b * d.b_s[0] + h * d.b_s[2], d.gate_bf16);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        const int r = row + i * kRowGroups;
-        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        kv[i] = qv[i] = 0.f;
-        if (i * kRowGroups >= d.Dk) continue;
-        if (r < d.Dk) {
-            const float* p = sb + (size_t)r * d.Dv + col;
-            if constexpr (VEC) {
-                if (col < d.Dv) s[i] = *reinterpret_cast<const f32x4*>(p);
-            } else {
+        const int r = min(row + i * kRowGroups, d.Dk - 1);
+        const float* p = sb + (size_t)r * d.Dv;
+        if constexpr (VEC) {
+            s[i] = *reinterpret_cast<const f32x4*>(p + min(col, d.Dv - 4));
+        } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col + j < d.Dv) s[i][j] = p[j];
-            }
-            kv[i] = to_f32(kb[r]);
-            qv[i] = to_f32(qb[r]);
+            for (int j = 0; j < 4; ++j) s[i][j] = p[min(col + j, d.Dv - 1)];
         }
+        kr[i] = kb[r];
+        qr[i] = qb[r];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vr[j] = v[b * d.v_s[0] + h * d.v_s[2] + min(col + j, d.Dv - 1)];
+    const float decay = expf(floor_gate(gate));
+    float kv[kRows], qv[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const bool on = row + i * kRowGroups < d.Dk;
+        kv[i] = on ? to_f32(kr[i]) : 0.f;
+        qv[i] = on ? to_f32(qr[i]) : 0.f;
+        if (!on) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     f32x4 ak{0.f, 0.f, 0.f, 0.f}, aq{0.f, 0.f, 0.f, 0.f};
     float k2 = 0.f, q2 = 0.f, qk = 0.f;
@@ -102,14 +109,13 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, const T* q, cons
     const float ck = d.normalize ? 1.f / sqrtf(ck_q[0][0] + ck_q[0][1] + ck_q[0][2] + ck_q[0][3] + kNormEps) : 1.f;
     const float cq = d.normalize ? 1.f / sqrtf(ck_q[1][0] + ck_q[1][1] + ck_q[1][2] + ck_q[1][3] + kNormEps) : 1.f;
     qk = (ck_q[2][0] + ck_q[2][1] + ck_q[2][2] + ck_q[2][3]) * ck;
-    const float bt = load_gate(beta, b * d.b_s[0] + h * d.b_s[2], d.gate_bf16);
     f32x4 u{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = tid % kColThreads * 4 + j;
         if (col + j >= d.Dv) continue;
         const float ks = part[0][0][c] + part[0][1][c] + part[0][2][c] + part[0][3][c];
-        u[j] = bt * (to_f32(v[b * d.v_s[0] + h * d.v_s[2] + col + j]) - ck * ks);
+        u[j] = bt * (to_f32(vr[j]) - ck * ks);
         if (row == 0) {
             const float qs = part[1][0][c] + part[1][1][c] + part[1][2][c] + part[1][3][c];
             ob[col + j] = from_f32<T>(d.scale * cq * (qs + qk * u[j]));
@@ -139,12 +145,23 @@ int launch_step(const Dims& d, const void* q, const void* k, const void* v, cons
     const bool vec = d.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15u) == 0;
     const T *tq = static_cast<const T*>(q), *tk = static_cast<const T*>(k), *tv = static_cast<const T*>(v);
     T* to = static_cast<T*>(o);
-    if (vec)
-        hipLaunchKernelGGL((step_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, tq, tk, tv, g,
-                           beta, state, slots, num_slots, to);
+    auto go = [&](auto rows) {
+        constexpr int R = decltype(rows)::value;
+        if (vec)
+            hipLaunchKernelGGL((step_kernel<T, true, R>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, tq, tk, tv,
+                               g, beta, state, slots, num_slots, to);
+        else
+            hipLaunchKernelGGL((step_kernel<T, false, R>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, tq, tk, tv,
+                               g, beta, state, slots, num_slots, to);
+    };
+    if (d.Dk <= kRowGroups)
+        go(std::integral_constant<int, 1>{});
+    else if (d.Dk <= 2 * kRowGroups)
+        go(std::integral_constant<int, 2>{});
+    else if (d.Dk <= 4 * kRowGroups)
+        go(std::integral_constant<int, 4>{});
     else
-        hipLaunchKernelGGL((step_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, tq, tk, tv, g,
-                           beta, state, slots, num_slots, to);
+        go(std::integral_constant<int, kMaxKeyDim / kRowGroups>{});
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
