@@ -11,8 +11,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // A chunk's q (which = 1) or k (0) as fragments, by rows and transposed, and what
-// normalises its rows.  The chunk is staged in LDS once, as it is.
-template <typename T>
+// normalises its rows.  The chunk is staged in LDS once, as it is.  VEC: Dk is a multiple
+// of eight.
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void rows_kernel(Dims d, const T* q, const T* k, const int* lengths, ChunkData out) {
     constexpr int NP = kPieces<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -25,9 +26,19 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Dims d, const T* q, cons
     const int steps = chain_steps(d.Dk), width = steps * 32, ld = width + 8;
     const long long* st = which ? d.q_s : d.k_s;
     const T* src = (which ? q : k) + b * st[0] + t0 * st[1] + hk * st[2];
-    for (int i = tid; i < kChunk * width; i += kThreads) {
-        const int r = i / width, e = i % width;
-        rows[r * ld + e] = r < live && e < d.Dk ? src[r * st[1] + e] : from_f32<T>(0.f);
+    // (four loads at a time)
+    for (int i = tid; i < kChunk * width / 8; i += 4 * kThreads) {
+        Eight<T> x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = min(i + j * kThreads, kChunk * width / 8 - 1), r = min(at / (width / 8), live - 1);
+            x[j].template load<VEC>(src + r * st[1], at % (width / 8) * 8, d.Dk);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = i + j * kThreads, r = at / (width / 8);
+            if (at < kChunk * width / 8) x[j].store(r < live, rows + r * ld + at % (width / 8) * 8);
+        }
     }
     __syncthreads();
     {
@@ -93,8 +104,8 @@ __device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
 // float32: its 16x16 diagonal blocks by forward substitution (a column per lane), then
 // the blocks below from theirs, [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1], for 32 and 64
 // rows.  (Backward stable; a series of powers of N is not where keys are alike.)
-// `x`: v, or (backward) dO, which may be null.
-template <typename T, bool BACKWARD>
+// `x`: v, or (backward) dO, which may be null.  VEC: Dv is a multiple of eight.
+template <typename T, bool BACKWARD, bool VEC>
 __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, const void* g, const void* beta,
                                                            const int* lengths, ChunkData out) {
     constexpr int NP = kPieces<T>;
@@ -108,14 +119,29 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
     const int t0 = c * kChunk, live = min(kChunk, row_length(lengths, b, d.T) - t0);
     if (live <= 0) return;
     const size_t ch = blockIdx.x, kch = ((size_t)b * d.Hk + hk) * d.chunks + c;
+    // the rows of x, 64 columns at a time, the first loaded now
+    const T* px = x;
+    long long stride = 0;
+    if constexpr (BACKWARD) {
+        stride = (long long)d.Hv * d.Dv;
+        if (px) px += (((size_t)b * d.T + t0) * d.Hv + h) * d.Dv;
+    } else {
+        stride = d.v_s[1];
+        px += b * d.v_s[0] + t0 * d.v_s[1] + h * d.v_s[2];
+    }
+    Eight<T> next[2] = {};
+    auto load_x = [&](int v0) {
+        if (!px) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            next[i].template load<VEC>(px + min(tid / 8 + 32 * i, live - 1) * stride, v0 + tid % 8 * 8, d.Dv);
+    };
+    load_x(0);
     if (wave == 0) {
-        float gv = 0.f, bv = 0.f;
-        if (lane < live) {
-            gv = load_gate(g, b * d.g_s[0] + (t0 + lane) * d.g_s[1] + h * d.g_s[2], d.gate_bf16);
-            bv = load_gate(beta, b * d.b_s[0] + (t0 + lane) * d.b_s[1] + h * d.b_s[2], d.gate_bf16);
-        }
-        gsum[lane] = chunk_sum(gv, lane);
-        bet[lane] = bv;
+        float gv = load_gate(g, b * d.g_s[0] + (t0 + min(lane, live - 1)) * d.g_s[1] + h * d.g_s[2], d.gate_bf16);
+        float bv = load_gate(beta, b * d.b_s[0] + (t0 + min(lane, live - 1)) * d.b_s[1] + h * d.b_s[2], d.gate_bf16);
+        gsum[lane] = chunk_sum(lane < live ? gv : 0.f, lane);
+        bet[lane] = lane < live ? bv : 0.f;
     } else if (wave == 1) {
         ck[lane] = out.norm[kch * 2 * kChunk + lane];
         cq[lane] = out.norm[(kch * 2 + 1) * kChunk + lane];
@@ -255,39 +281,39 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
     // transposed: rows of Dk, columns the wavefront's tokens
     u32x4* read = out.read + (ch * read_frags(d.Dk) + (size_t)wave * steps * 3) * kFragLanes;
     const u32x4* fkt = out.kt + kch * row_frags<T>(d.Dk) * kFragLanes + lane;
-    for (int blk = 0; blk < 2 * steps; ++blk) {
-        f32x4 y{};
+    for (int b0 = 0; b0 < 2 * steps; b0 += 4) {  // (a multiple of four; their loads at once)
+        u32x4 a[4][2][NP];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            if (!live_step(w)) continue;
-            u32x4 a[NP];
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < NP; ++i) a[i] = fkt[((blk * 2 + w) * NP + i) * kFragLanes];
-            y = mul(a, tk[w], y);
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) a[j][w][i] = fkt[(((b0 + j) * 2 + w) * NP + i) * kFragLanes];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f32x4 y{};
+            if (live_step(0)) {
+                y = mul(a[j][0], tk[0], y);
+                settle(y);
+            }
+            if (live_step(1)) {
+                y = mul(a[j][1], tk[1], y);
+                settle(y);
+            }
+            u32x2 pieces[3];
+            split<3>(y, pieces);
+            put_block(read, 3, b0 + j, hi, n, pieces);
         }
-        u32x2 pieces[3];
-        split<3>(y, pieces);
-        put_block(read, 3, blk, hi, n, pieces);
     }
     // the products with x, 64 columns of it at a time in LDS
     T* xs = reinterpret_cast<T*>(ti);
-    const T* px = x;
-    long long stride = 0;
-    if constexpr (BACKWARD) {
-        stride = (long long)d.Hv * d.Dv;
-        if (px) px += (((size_t)b * d.T + t0) * d.Hv + h) * d.Dv;
-    } else {
-        stride = d.v_s[1];
-        px += b * d.v_s[0] + t0 * d.v_s[1] + h * d.v_s[2];
-    }
     const int blocks = column_blocks(d.Dv);
     for (int v0 = 0; v0 < d.Dv; v0 += 64) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kChunk * 64 / kThreads; ++i) {
-            const int r = (tid + i * kThreads) / 64, e = tid % 64;
-            xs[r * kLdX + e] = px && r < live && v0 + e < d.Dv ? px[r * stride + v0 + e] : from_f32<T>(0.f);
-        }
+        for (int i = 0; i < 2; ++i)
+            next[i].store(px && tid / 8 + 32 * i < live, xs + (tid / 8 + 32 * i) * kLdX + tid % 8 * 8);
+        if (v0 + 64 < d.Dv) load_x(v0 + 64);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -301,6 +327,7 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
                 split8<NP>(f32x4{to_f32(q[0]), to_f32(q[kLdX]), to_f32(q[2 * kLdX]), to_f32(q[3 * kLdX])},
                            f32x4{to_f32(q[4 * kLdX]), to_f32(q[5 * kLdX]), to_f32(q[6 * kLdX]), to_f32(q[7 * kLdX])}, f);
                 y = mul(tx[w], f, y);
+                settle(y);
             }
             out.own[((ch * blocks + v0 / 16 + j) * 4 + wave) * kFragLanes + lane] = y;
         }
@@ -380,12 +407,20 @@ int prepare(const Dims& d, const T* q, const T* k, const T* x, const void* g, co
     if (blocks == 0) return 0;
     RKA_RETURN_IF_ERR(check_grid(std::max(blocks, rows), kThreads, "gated_delta"));
     const size_t lds = (size_t)kChunk * (chain_steps(d.Dk) * 32 + 8) * sizeof(T);
-    RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T>),
-                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)rows), dim3(kThreads), lds, stream, d, q, k, lengths, out);
-    RKA_RETURN_IF_HIP(hipGetLastError());
-    hipLaunchKernelGGL((prepare_kernel<T, BACKWARD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, x, g, beta,
-                       lengths, out);
+    auto by_rows = [&](auto kernel) {
+        RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(kThreads), lds, stream, d, q, k, lengths, out);
+        RKA_RETURN_IF_HIP(hipGetLastError());
+        return 0;
+    };
+    RKA_RETURN_IF_ERR(d.Dk % 8 == 0 ? by_rows(&rows_kernel<T, true>) : by_rows(&rows_kernel<T, false>));
+    if (d.Dv % 8 == 0)
+        hipLaunchKernelGGL((prepare_kernel<T, BACKWARD, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, x, g,
+                           beta, lengths, out);
+    else
+        hipLaunchKernelGGL((prepare_kernel<T, BACKWARD, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, d, x, g,
+                           beta, lengths, out);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }

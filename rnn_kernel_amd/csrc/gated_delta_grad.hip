@@ -19,71 +19,6 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kLd = 68;  // row of a 64-wide LDS tile: 16 bytes past a multiple of all banks
 
-struct __attribute__((packed, aligned(4))) Float4U {
-    float x, y, z, w;
-};
-struct __attribute__((packed, aligned(2))) Bytes16 {
-    unsigned w[4];
-};
-
-// Loads of neighbouring columns, from column c of a row of `width` in memory, zero past
-// it: without branches (clamped addresses), and for the widths that are multiples of
-// eight (VEC) in 16-byte loads.
-template <bool VEC>
-__device__ __forceinline__ f32x4 load4(const float* row, int c, int width) {
-    f32x4 x;
-    if constexpr (VEC) {
-        const Float4U v = *reinterpret_cast<const Float4U*>(row + min(c, width - 4));
-        x = f32x4{v.x, v.y, v.z, v.w};
-        if (c >= width) x = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float v = row[min(c + j, width - 1)];
-            x[j] = c + j < width ? v : 0.f;
-        }
-    }
-    return x;
-}
-
-// Eight columns of a row: a lane's part of an operand, as loaded and in pieces (zero
-// where the row is not `on`).
-template <typename T>
-struct Eight;
-template <>
-struct Eight<float> {
-    f32x4 a, b;
-    template <bool VEC>
-    __device__ __forceinline__ void load(const float* row, int c, int width) {
-        a = load4<VEC>(row, c, width);
-        b = load4<VEC>(row, c + 4, width);
-    }
-    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[3]) {
-        if (!on) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
-        split8<3>(a, b, p);
-    }
-};
-template <>
-struct Eight<bf16> {
-    u32x4 x;
-    template <bool VEC>
-    __device__ __forceinline__ void load(const bf16* row, int c, int width) {
-        if constexpr (VEC) {
-            const Bytes16 v = *reinterpret_cast<const Bytes16*>(row + min(c, width - 8));
-            x = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
-            if (c >= width) x = u32x4{0, 0, 0, 0};
-        } else {
-            x = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const unsigned v = row[min(c + j, width - 1)].bits;
-                x[j / 2] |= (c + j < width ? v : 0u) << (j % 2 * 16);
-            }
-        }
-    }
-    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[1]) { p[0] = on ? x : u32x4{0, 0, 0, 0}; }
-};
-
 // An element of q and one of k.
 template <typename T>
 struct Pair;
