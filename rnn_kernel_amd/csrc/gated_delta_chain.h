@@ -9,7 +9,9 @@
 // (forward: Q S and, a step later, P E and o; backward: the pieces of scale exp(G) dO);
 // the second is shared by all eight, a part of Dk's rows each.  The rows of the prepared
 // factors come straight from memory into the operand registers of the wavefront that
-// uses them, each loaded again for the next chunk as soon as it has been used; what the
+// uses them, each loaded again for a later chunk as soon as it has been used, one by one
+// between the products: a load takes 16 clocks to issue, and a step's hundred in one go
+// hold up the wavefronts longer than its products; what the
 // products hand on (S, E, each split into bf16 pieces by the wavefront that made it)
 // passes through LDS in operand order, one barrier apiece.  The workgroups of a head are
 // eight apart, on one XCD, whose L2 then answers all but the first of them.
@@ -217,20 +219,22 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
     };
     // the second product, all wavefronts' part of a step
     auto update = [&](int c) {
+        u32x4 f[NC][2][3];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            u32x4 f[2][3];
-            get_frag(fw[j], 0, 3, lane, f[0]);
-            get_frag(fw[j], 1, 3, lane, f[1]);
+            get_frag(fw[j], 0, 3, lane, f[j][0]);
+            get_frag(fw[j], 1, 3, lane, f[j][1]);
+        }
 #pragma unroll
-            for (int t = 0; t < TW; ++t) {
-                s[j][t] = mul(turned[t][0], f[0], s[j][t] * last);
-                s[j][t] = mul(turned[t][1], f[1], s[j][t]);
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                s[j][t] = mul(turned[t][0], f[j][0], s[j][t] * last);
+                s[j][t] = mul(turned[t][1], f[j][1], s[j][t]);
                 settle(s[j][t]);
             }
-        }
-        put_state();
         load_turned(min(c + 1, final));
+        put_state();
     };
 
     // The two kinds of wavefront in loops of their own: the compiler waits for what may
@@ -244,12 +248,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         } sets[NS];
         const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
         float* pe = e_out ? e_out + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0 : nullptr;
-        auto load = [&](Rows& x, int c) {
+        auto load_rows = [&](Rows& x, int c) {
             const u32x4* p = pread + c * reads;
 #pragma unroll
             for (int u = 0; u < KU; ++u)
 #pragma unroll
                 for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+        };
+        auto load_rest = [&](Rows& x, int c) {
 #pragma unroll
             for (int j = 0; j < NC; ++j)
                 x.own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
@@ -258,18 +264,26 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         auto step = [&](Rows& x, int c) {
             if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
             __syncthreads();
+            const u32x4* p = pread + min(c + NS, final) * reads;
+            f32x4 part[NC][2] = {};
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 part[2] = {};
+            for (int u = 0; u < KU; ++u) {
 #pragma unroll
-                for (int u = 0; u < KU; ++u) {
+                for (int j = 0; j < NC; ++j) {
                     u32x4 f[3];
                     get_frag(fs[j], u, 3, lane, f);
-                    part[u % 2] = mul(x.row[u], f, part[u % 2]);
+                    part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]);
                 }
-                settle(part[0]);
-                settle(part[1]);
-                const f32x4 e = x.own[j] - (part[0] + part[1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                settle(part[j][0]);
+                settle(part[j][1]);
+                const f32x4 e = x.own[j] - (part[j][0] + part[j][1]);
                 u32x2 pw[3], pp[PO];
                 split<3>(x.wk * e, pw);
                 put_block(fw[j], 3, w4, hi, n, pw);
@@ -277,13 +291,16 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
                 put_block(fe[c % 2][j], PO, w4, hi, n, pp);
                 if (pe && col0 + 16 * j < d.Dv) store_tokens(pe + 16 * j, orow, c, first, len, e);
             }
-            load(x, min(c + NS, final));
+            load_rest(x, min(c + NS, final));
             __syncthreads();
             update(c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            if (final >= 0) load(sets[i], min(i, final));
+            if (final >= 0) {
+                load_rows(sets[i], min(i, final));
+                load_rest(sets[i], min(i, final));
+            }
         for (int c = 0; c <= final; c += NS) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
@@ -334,21 +351,28 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         auto step = [&](Rows& x, int c) {
             if (states) at.store_state(d, states + (ch0 + c) * d.Dk * d.Dv, s);
             __syncthreads();
-            f32x4 y[NC];
+            const int then = min(c + NS, final);
+            f32x4 part[NC][2] = {}, y[NC];
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                f32x4 part[2] = {};
+            for (int u = 0; u < KU; ++u) {
 #pragma unroll
-                for (int u = 0; u < KU; ++u) {
+                for (int j = 0; j < NC; ++j) {
                     u32x4 f[PO];
                     get_frag(fs[j], u, 3, lane, f);
-                    part[u % 2] = mul(x.row[u], f, part[u % 2]);
+                    part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]);
                 }
-                settle(part[0]);
-                settle(part[1]);
-                y[j] = x.rq * (part[0] + part[1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) x.row[u][i] = pq[then * rows + (u * NP + i) * kFragLanes];
+                __builtin_amdgcn_sched_barrier(0);
             }
-            load(x, min(c + NS, final));
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                settle(part[j][0]);
+                settle(part[j][1]);
+                y[j] = x.rq * (part[j][0] + part[j][1]);
+            }
+            x.rq = coef4(in.coef + (ch0 + then) * kCoefFloats, RQ, w4, hi);
             if (c > 0) finish(c - 1);
             load_tri(c);
 #pragma unroll
@@ -447,8 +471,8 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                 s[j][t] += other;
             }
         }
-        put_state();
         load_turned(max(c - 1, 0));
+        put_state();
     };
 
     // (loops of their own, as in the forward)
@@ -460,12 +484,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
             f32x4 rk;
         } sets[NS];
         const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
-        auto load = [&](Rows& x, int c) {
+        auto load_rows = [&](Rows& x, int c) {
             const u32x4* p = pread + c * reads;
 #pragma unroll
             for (int u = 0; u < KU; ++u)
 #pragma unroll
                 for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+        };
+        auto load_rest = [&](Rows& x, int c) {
 #pragma unroll
             for (int j = 0; j < NC; ++j)
                 x.own[j] = in.own[(((ch0 + c) * blocks + min(block0 + j, blocks - 1)) * 4 + w4) * kFragLanes + lane];
@@ -474,33 +500,49 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         auto step = [&](Rows& x, int c) {
             at.store_state(d, bd.dstates + (ch0 + c) * d.Dk * d.Dv, s);
             __syncthreads();
+            const u32x4* p = pread + max(c - NS, 0) * reads;
+            f32x4 y[NC][2];
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                f32x4 y[2] = {x.own[j], f32x4{0.f, 0.f, 0.f, 0.f}};
+                y[j][0] = x.own[j];
+                y[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
-                for (int u = 0; u < KU; ++u) {
+            for (int u = 0; u < KU; ++u) {
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
                     u32x4 f[3];
                     get_frag(fs[j], u, 3, lane, f);
-                    y[u % 2] = mul(x.row[u], f, y[u % 2]);
+                    y[j][u % 2] = mul(x.row[u], f, y[j][u % 2]);
                 }
-                settle(y[0]);
-                settle(y[1]);
-                const f32x4 dx = y[0] + y[1];
-                u32x2 p[3];
-                split<3>(-x.rk * dx, p);
-                put_block(fw[j], 3, w4, hi, n, p);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                settle(y[j][0]);
+                settle(y[j][1]);
+                const f32x4 dx = y[j][0] + y[j][1];
+                u32x2 pw[3];
+                split<3>(-x.rk * dx, pw);
+                put_block(fw[j], 3, w4, hi, n, pw);
                 if (col0 + 16 * j < d.Dv) {
                     store_tokens(dv + token + 16 * j, orow, c, first, len, dx);
                     store_tokens(bd.dx + token + 16 * j, orow, c, first, len, dx);
                 }
             }
-            load(x, max(c - NS, 0));
+            load_rest(x, max(c - NS, 0));
             __syncthreads();
             update(c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            if (final >= 0) load(sets[i], max(final - i, 0));
+            if (final >= 0) {
+                load_rows(sets[i], max(final - i, 0));
+                load_rest(sets[i], max(final - i, 0));
+            }
         for (int c = final; c >= 0; c -= NS) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
