@@ -34,6 +34,28 @@ __device__ __forceinline__ void get_frag(const u32x4* frags, int step, int strid
     for (int c = 0; c < N; ++c) f[c] = frags[((size_t)step * stride + c) * kFragLanes + lane];
 }
 
+// Sums of KU steps for NC column blocks, from the blocks' fragments in LDS (NF pieces of
+// them, three apart): the reads run two products ahead, pinned there, as the compiler
+// would put each right before its use and wait for it.  `use(u, j, f)` makes a product,
+// `done(u)` follows the last of a step.
+template <int KU, int NC, int NF, int FRAGS, typename Use, typename Done>
+__device__ __forceinline__ void steps_ahead(const u32x4 (&from)[NC][FRAGS], int lane, Use use, Done done) {
+    constexpr int kAhead = 2, kAll = KU * NC;
+    u32x4 f[kAhead + 1][NF];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < kAll) get_frag(from[i % NC], i / NC, 3, lane, f[i % (kAhead + 1)]);
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+        if (i + kAhead < kAll)
+            get_frag(from[(i + kAhead) % NC], (i + kAhead) / NC, 3, lane, f[(i + kAhead) % (kAhead + 1)]);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i / NC, i % NC, f[i % (kAhead + 1)]);
+        if (i % NC == NC - 1) done(i / NC);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 __device__ __forceinline__ f32x4 coef4(const float* coef, int which, int block, int hi) {
     return *reinterpret_cast<const f32x4*>(coef + which * kChunk + 16 * block + 4 * hi);
 }
@@ -205,46 +227,50 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
     const size_t orow = (size_t)d.Hv * d.Dv;
     constexpr int NS = kRowSets<T, KU>;
 
-    u32x4 turned[TW][2][NP];
-    float last;
-    auto load_turned = [&](int c) {
+    // of K^T, and exp(G_C)
+    struct Turned {
+        u32x4 frag[TW][2][NP];
+        float last;
+    };
+    auto load_turned = [&](Turned& x, int c) {
         const u32x4* p = in.kt + (kch0 + c) * rows + lane;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) turned[t][w][i] = p[((at.near(t) * 2 + w) * NP + i) * kFragLanes];
-        last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
+                for (int i = 0; i < NP; ++i) x.frag[t][w][i] = p[((at.near(t) * 2 + w) * NP + i) * kFragLanes];
+        x.last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
     };
     // the second product, all wavefronts' part of a step
-    auto update = [&](int c) {
+    auto update = [&](Turned& x, int c) {
         u32x4 f[NC][2][3];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             get_frag(fw[j], 0, 3, lane, f[j][0]);
             get_frag(fw[j], 1, 3, lane, f[j][1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                s[j][t] = mul(turned[t][0], f[j][0], s[j][t] * last);
-                s[j][t] = mul(turned[t][1], f[j][1], s[j][t]);
+                s[j][t] = mul(x.frag[t][0], f[j][0], s[j][t] * x.last);
+                s[j][t] = mul(x.frag[t][1], f[j][1], s[j][t]);
                 settle(s[j][t]);
             }
-        load_turned(min(c + 1, final));
+        load_turned(x, min(c + NS, final));
         put_state();
     };
 
     // The two kinds of wavefront in loops of their own: the compiler waits for what may
     // have been loaded on either side of a branch.
-    if (final >= 0) load_turned(0);
     if (chain) {
         struct Rows {
             u32x4 row[KU][3];  // of T diag(exp G) K
             f32x4 own[NC];     // of T V
             f32x4 wk;
+            Turned turned;
         } sets[NS];
         const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
         float* pe = e_out ? e_out + (((size_t)at.b * d.T + first) * d.Hv + at.h) * d.Dv + col0 : nullptr;
@@ -266,19 +292,12 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
             __syncthreads();
             const u32x4* p = pread + min(c + NS, final) * reads;
             f32x4 part[NC][2] = {};
+            steps_ahead<KU, NC, 3>(
+                fs, lane, [&](int u, int j, const u32x4(&f)[3]) { part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]); },
+                [&](int u) {
 #pragma unroll
-            for (int u = 0; u < KU; ++u) {
-#pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    u32x4 f[3];
-                    get_frag(fs[j], u, 3, lane, f);
-                    part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+                });
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
                 settle(part[j][0]);
@@ -293,13 +312,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
             }
             load_rest(x, min(c + NS, final));
             __syncthreads();
-            update(c);
+            update(x.turned, c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             if (final >= 0) {
                 load_rows(sets[i], min(i, final));
                 load_rest(sets[i], min(i, final));
+                load_turned(sets[i].turned, min(i, final));
             }
         for (int c = 0; c <= final; c += NS) {
 #pragma unroll
@@ -310,6 +330,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         struct Rows {
             u32x4 row[KU][NP];  // of Q
             f32x4 rq;
+            Turned turned;
         } sets[NS];
         u32x4 tri[2][PO];
         f32x4 out[NC];
@@ -336,13 +357,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
         auto finish = [&](int c) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                u32x4 f[PO];
-                get_frag(fe[c % 2][j], 0, PO, lane, f);
-                out[j] = mul(tri[0], f, out[j]);
+                u32x4 f[2][PO];
+                get_frag(fe[c % 2][j], 0, PO, lane, f[0]);
+                get_frag(fe[c % 2][j], 1, PO, lane, f[1]);
+                __builtin_amdgcn_sched_barrier(0);
+                out[j] = mul(tri[0], f[0], out[j]);
                 settle(out[j]);
                 if (w4 >= 2) {
-                    get_frag(fe[c % 2][j], 1, PO, lane, f);
-                    out[j] = mul(tri[1], f, out[j]);
+                    out[j] = mul(tri[1], f[1], out[j]);
                     settle(out[j]);
                 }
                 if (col0 + 16 * j < d.Dv) store_tokens(po + 16 * j, orow, c, first, len, out[j]);
@@ -353,19 +375,12 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
             __syncthreads();
             const int then = min(c + NS, final);
             f32x4 part[NC][2] = {}, y[NC];
+            steps_ahead<KU, NC, PO>(
+                fs, lane, [&](int u, int j, const u32x4(&f)[PO]) { part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]); },
+                [&](int u) {
 #pragma unroll
-            for (int u = 0; u < KU; ++u) {
-#pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    u32x4 f[PO];
-                    get_frag(fs[j], u, 3, lane, f);
-                    part[j][u % 2] = mul(x.row[u], f, part[j][u % 2]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < NP; ++i) x.row[u][i] = pq[then * rows + (u * NP + i) * kFragLanes];
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    for (int i = 0; i < NP; ++i) x.row[u][i] = pq[then * rows + (u * NP + i) * kFragLanes];
+                });
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
                 settle(part[j][0]);
@@ -378,11 +393,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_forward_kernel(Dims d,
 #pragma unroll
             for (int j = 0; j < NC; ++j) out[j] = y[j];
             __syncthreads();
-            update(c);
+            update(x.turned, c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            if (final >= 0) load(sets[i], min(i, final));
+            if (final >= 0) {
+                load(sets[i], min(i, final));
+                load_turned(sets[i].turned, min(i, final));
+            }
         for (int c = 0; c <= final; c += NS) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
@@ -432,9 +450,12 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
     const size_t orow = (size_t)d.Hv * d.Dv;
     constexpr int NS = kRowSets<T, KU>;
 
-    u32x4 kt[TW][2][NP], qt[TW][2][NP];
-    float last;
-    auto load_turned = [&](int c) {
+    // of K^T and Q^T, and exp(G_C)
+    struct Turned {
+        u32x4 kt[TW][2][NP], qt[TW][2][NP];
+        float last;
+    };
+    auto load_turned = [&](Turned& x, int c) {
         const u32x4 *pk = in.kt + (kch0 + c) * rows + lane, *pq = in.qt + (kch0 + c) * rows + lane;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
@@ -443,12 +464,12 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
                     const int f = ((at.near(t) * 2 + w) * NP + i) * kFragLanes;
-                    kt[t][w][i] = pk[f];
-                    qt[t][w][i] = pq[f];
+                    x.kt[t][w][i] = pk[f];
+                    x.qt[t][w][i] = pq[f];
                 }
-        last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
+        x.last = in.coef[(ch0 + c) * kCoefFloats + NCOEF * kChunk];
     };
-    auto update = [&](int c) {
+    auto update = [&](Turned& x, int c) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             u32x4 f[2][3], g[2][3];
@@ -457,31 +478,32 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                 get_frag(fq[j], w, 3, lane, g[w]);
                 get_frag(fw[j], w, 3, lane, f[w]);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
                 f32x4 other{0.f, 0.f, 0.f, 0.f};
-                s[j][t] *= last;
+                s[j][t] *= x.last;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    other = mul(qt[t][w], g[w], other);
-                    s[j][t] = mul(kt[t][w], f[w], s[j][t]);
+                    other = mul(x.qt[t][w], g[w], other);
+                    s[j][t] = mul(x.kt[t][w], f[w], s[j][t]);
                 }
                 settle(other);
                 settle(s[j][t]);
                 s[j][t] += other;
             }
         }
-        load_turned(max(c - 1, 0));
+        load_turned(x, max(c - NS, 0));
         put_state();
     };
 
     // (loops of their own, as in the forward)
-    if (final >= 0) load_turned(final);
     if (chain) {
         struct Rows {
             u32x4 row[KU][3];  // of T^T diag(exp(G_C - G) beta) K
             f32x4 own[NC];     // of (P T)^T dO
             f32x4 rk;
+            Turned turned;
         } sets[NS];
         const u32x4* pread = in.read + ch0 * reads + (size_t)w4 * KU * 3 * kFragLanes + lane;
         auto load_rows = [&](Rows& x, int c) {
@@ -507,19 +529,12 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
                 y[j][0] = x.own[j];
                 y[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
+            steps_ahead<KU, NC, 3>(
+                fs, lane, [&](int u, int j, const u32x4(&f)[3]) { y[j][u % 2] = mul(x.row[u], f, y[j][u % 2]); },
+                [&](int u) {
 #pragma unroll
-            for (int u = 0; u < KU; ++u) {
-#pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    u32x4 f[3];
-                    get_frag(fs[j], u, 3, lane, f);
-                    y[j][u % 2] = mul(x.row[u], f, y[j][u % 2]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    for (int i = 0; i < 3; ++i) x.row[u][i] = p[(u * 3 + i) * kFragLanes];
+                });
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
                 settle(y[j][0]);
@@ -535,13 +550,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
             }
             load_rest(x, max(c - NS, 0));
             __syncthreads();
-            update(c);
+            update(x.turned, c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             if (final >= 0) {
                 load_rows(sets[i], max(final - i, 0));
                 load_rest(sets[i], max(final - i, 0));
+                load_turned(sets[i].turned, max(final - i, 0));
             }
         for (int c = final; c >= 0; c -= NS) {
 #pragma unroll
@@ -552,6 +568,7 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
         struct Rows {
             T go[NC][4];  // dO
             f32x4 rq;
+            Turned turned;
         } sets[NS];
         auto load = [&](Rows& x, int c) {
             if (dout) load_tokens<T, NC>(dout + token, orow, c, first, len, col0, d.Dv, x.go);
@@ -568,11 +585,14 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
             }
             load(x, max(c - NS, 0));
             __syncthreads();
-            update(c);
+            update(x.turned, c);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            if (final >= 0) load(sets[i], max(final - i, 0));
+            if (final >= 0) {
+                load(sets[i], max(final - i, 0));
+                load_turned(sets[i].turned, max(final - i, 0));
+            }
         for (int c = final; c >= 0; c -= NS) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
