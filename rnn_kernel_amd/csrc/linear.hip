@@ -49,6 +49,8 @@ __device__ __forceinline__ u32x4 load16(const void* p) {
 __device__ __forceinline__ void store16(void* p, u32x4 v) {
     *static_cast<Bytes16*>(p) = Bytes16{{v[0], v[1], v[2], v[3]}};
 }
+__device__ __forceinline__ f32x4 load4(const float* p) { return __builtin_bit_cast(f32x4, load16(p)); }
+__device__ __forceinline__ void store4(float* p, f32x4 v) { store16(p, __builtin_bit_cast(u32x4, v)); }
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);  // elements of 16 bytes
 
@@ -59,28 +61,67 @@ union Piece {
 };
 
 // ---------------------------------------------------------- activations ---
+// exp and 1/x for results of type T: for bf16 the hardware's own, whose relative error (1e-6
+// at |z| = 20) is far below its last bit.
+template <typename T>
+__device__ __forceinline__ float exp_for(float x) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_amdgcn_exp2f(1.4426950408889634f * x);
+    else
+        return expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float inverse_for(float x) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_amdgcn_rcpf(x);
+    else
+        return 1.f / x;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+    return inverse_for<T>(1.f + exp_for<T>(-z));
+}
+// The normal distribution's function, half of erfc(x) at x = -z / sqrt(2).  For x >= 0,
+// erfc(x) = exp(-x^2) t P(t) with t = 1 / (1 + 0.4 x) and P fitted over all of t in (0, 1]
+// for the least relative error, 1.3e-7: no branch on z, where the library's erfc has three.
+template <typename T>
+__device__ __forceinline__ float normal(float z, float gauss) {  // gauss: exp(-z^2 / 2)
+    const float t = inverse_for<T>(1.f + (0.4f * 0.70710678118654752f) * fabsf(z));
+    float p = 0.05026539f;
+    p = fmaf(p, t, -0.18291503f);
+    p = fmaf(p, t, 0.16910847f);
+    p = fmaf(p, t, -0.00562818f);
+    p = fmaf(p, t, 0.14144189f);
+    p = fmaf(p, t, 0.168539f);
+    p = fmaf(p, t, 0.20784314f);
+    p = fmaf(p, t, 0.22566957f);
+    p = fmaf(p, t, 0.22567586f);
+    const float tail = 0.5f * gauss * (p * t);
+    return z < 0.f ? tail : 1.f - tail;
+}
+template <typename T>
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case RKA_ACT_RELU: return z < 0.f ? 0.f : z;  // NaN stays
-        case RKA_ACT_GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
-        case RKA_ACT_SILU: return z / (1.f + expf(-z));
-        case RKA_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
+        case RKA_ACT_GELU: return z * normal<T>(z, exp_for<T>(-0.5f * z * z));
+        case RKA_ACT_SILU: return z * sigmoid<T>(z);
+        case RKA_ACT_SIGMOID: return sigmoid<T>(z);
         case RKA_ACT_LOGSIGMOID: return (z < 0.f ? z : z != z ? z : 0.f) - log1pf(expf(-fabsf(z)));
         default: return z;
     }
 }
 // dy act'(z)
+template <typename T>
 __device__ __forceinline__ float slope(float dy, float z, int act) {
     switch (act) {
         case RKA_ACT_RELU: return z <= 0.f ? 0.f : dy;
-        case RKA_ACT_GELU:
-            return dy * (0.5f * erfcf(-0.70710678118654752f * z) + z * 0.3989422804014327f * expf(-0.5f * z * z));
-        case RKA_ACT_SILU: {
-            const float s = 1.f / (1.f + expf(-z));
-            return dy * s * (1.f + z * (1.f / (1.f + expf(z))));
+        case RKA_ACT_GELU: {
+            const float gauss = exp_for<T>(-0.5f * z * z);
+            return dy * (normal<T>(z, gauss) + z * 0.3989422804014327f * gauss);
         }
-        case RKA_ACT_SIGMOID: return dy * (1.f / (1.f + expf(-z))) * (1.f / (1.f + expf(z)));
-        case RKA_ACT_LOGSIGMOID: return dy * (1.f / (1.f + expf(z)));
+        case RKA_ACT_SILU: return dy * sigmoid<T>(z) * (1.f + z * sigmoid<T>(-z));
+        case RKA_ACT_SIGMOID: return dy * sigmoid<T>(z) * sigmoid<T>(-z);
+        case RKA_ACT_LOGSIGMOID: return dy * sigmoid<T>(-z);
         default: return dy;
     }
 }
@@ -255,7 +296,7 @@ __device__ __forceinline__ void finish(const Args& p, long long row, int col, co
             float x = sum[j];
             if (bias) x += to_f32(pb.e[j]);
             pz.e[j] = from_f32<T>(x);
-            x = activate(x, p.ep.act);
+            x = activate<T>(x, p.ep.act);
             if (res) x += to_f32(pr.e[j]);
             pc.e[j] = from_f32<T>(x);
         }
@@ -269,7 +310,7 @@ __device__ __forceinline__ void finish(const Args& p, long long row, int col, co
         float x = sum[j];
         if (bias) x += to_f32(bias[j]);
         if (z) z[j] = from_f32<T>(x);
-        x = activate(x, p.ep.act);
+        x = activate<T>(x, p.ep.act);
         if (res) x += to_f32(res[j]);
         c[j] = from_f32<T>(x);
     }
@@ -288,6 +329,54 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int slices, in
     const int group = t / (G * tiles_n), first = group * G, rows = min(G, tiles_m - first), in = t - group * G * tiles_n;
     *tm = first + in % rows;
     *tn = in / rows;
+}
+
+// A wavefront's WM x WN of the output, from row0 and col0.  Through LDS (`out`), 32 rows
+// at a time: a lane holds four neighbouring columns of one row, memory wants whole rows.
+template <int WN>
+constexpr int kOutBytes = 32 * (WN + 4) * 4;
+template <typename T, int WM, int WN>
+__device__ __forceinline__ void put_out(const Args& p, const f32x16 (&acc)[WM / 32][WN / 32], float* out, int row0, int col0,
+                                        int slice) {
+    constexpr int kLd = WN + 4, kV = kVec<T>, kLanes = WN / kV, kRows = 64 / kLanes, MB = WM / 32, NB = WN / 32;
+    const int lane = threadIdx.x % 64, i32 = lane % 32, hi = lane / 32;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x4*>(out + i32 * kLd + 32 * j + 8 * r + 4 * hi) =
+                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int x = 0; x < 32 / kRows; ++x) {
+            const int r = x * kRows + lane / kLanes, c = lane % kLanes * kV;
+            const int row = row0 + 32 * i + r, col = col0 + c;
+            float sum[kV];
+#pragma unroll
+            for (int e = 0; e < kV; e += 4) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(out + r * kLd + c + e);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[e + y] = q[y];
+            }
+            if (row >= p.m) continue;
+            if (p.slices > 1) {
+                float* part = p.partial + ((size_t)slice * p.m + row) * p.n + col;
+                if (col + kV <= p.n) {
+#pragma unroll
+                    for (int e = 0; e < kV; e += 4) store4(part + e, f32x4{sum[e], sum[e + 1], sum[e + 2], sum[e + 3]});
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < kV; ++e)
+                    if (col + e < p.n) part[e] = sum[e];
+            } else {
+                finish<T, kV>(p, row, col, sum);
+            }
+        }
+    }
 }
 
 // BM x BN tiles, WM x WN of them per wavefront.
@@ -343,42 +432,105 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(Args p) {
         }
         __syncthreads();
     }
-    // Through LDS, 32 rows of the wavefront at a time: a lane holds four
-    // neighbouring columns of one row, memory wants whole rows.
-    constexpr int kLd = WN + 4, kV = kVec<T>, kLanes = WN / kV, kRows = 64 / kLanes;
-    float* out = reinterpret_cast<float*>(lds) + wave * 32 * kLd;
+    put_out<T, WM, WN>(p, acc, reinterpret_cast<float*>(lds + wave * kOutBytes<WN>), m0 + wm, n0 + wn, slice);
+}
+
+// Order of the 16-byte pieces of a row: sixteen rows' pieces of one number are on
+// different banks, and 32 rows further the order is the same.
+__device__ __forceinline__ int direct_turn(int row) { return (row ^ (row >> 3 & 3)) & 7; }
+
+// The same for operands that both lie along the sum, in whole stages and on 16 bytes:
+// they go from memory to LDS without registers between, which leaves those for the
+// fragments of the next products.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(Args p) {
+    constexpr int W = BM / WM * BN / WN, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;
+    constexpr int kStage = (BM + BN) * kRowBytes, kLoads = (BM + BN) / 8 / W;  // a wavefront's, 8 rows each
+    constexpr int kBuffer = kStage > W / 2 * kOutBytes<WN> ? kStage : W / 2 * kOutBytes<WN>;
+    // (two variables, by which the compiler knows that reads of the one need not wait for
+    // loads into the other)
+    __shared__ __attribute__((aligned(16))) char even[kBuffer];
+    __shared__ __attribute__((aligned(16))) char odd[kBuffer];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), i32 = lane % 32, hi = lane / 32;
+    int tm, tn, slice;
+    tile_of((p.m - 1) / BM + 1, (p.n - 1) / BN + 1, p.slices, &tm, &tn, &slice);
+    const int m0 = tm * BM, n0 = tn * BN, wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+    const int kbeg = min(p.k, slice * p.stages * kK), kend = min(p.k, kbeg + p.stages * kK);
+    const int stages = (kend - kbeg) / kK;
+    // What lane l loads goes to LDS's l-th 16 bytes of 8 rows: it is the piece that
+    // belongs there.  A wavefront loads rows of one operand.
+    const bool of_a = wave < W / 2;
+    const Operand& op = of_a ? p.a : p.b;
+    const int row0 = of_a ? m0 : n0, rows = of_a ? p.m : p.n, first = wave % (W / 2) * kLoads * 8;
+    const auto memory = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(static_cast<const char*>(op.ptr)) + ((long long)row0 * op.ld + kbeg) * (long long)sizeof(T), 0,
+        (int)0xffffffffu, 0x27000);
+    unsigned from[kLoads];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<f32x4*>(out + i32 * kLd + 32 * j + 8 * r + 4 * hi) =
-                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int x = 0; x < 32 / kRows; ++x) {
-            const int r = x * kRows + lane / kLanes, c = lane % kLanes * kV;
-            const int row = m0 + wm + 32 * i + r, col = n0 + wn + c;
-            float sum[kV];
-#pragma unroll
-            for (int e = 0; e < kV; e += 4) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(out + r * kLd + c + e);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) sum[e + y] = q[y];
-            }
-            if (row >= p.m) continue;
-            if (p.slices > 1) {
-                float* part = p.partial + ((size_t)slice * p.m + row) * p.n + col;
-#pragma unroll
-                for (int e = 0; e < kV; ++e)
-                    if (col + e < p.n) part[e] = sum[e];
-            } else {
-                finish<T, kV>(p, row, col, sum);
-            }
-        }
+    for (int i = 0; i < kLoads; ++i) {
+        const int row = first + i * 8 + lane / 8;
+        from[i] = (unsigned)min(row, rows - 1 - row0) * ((unsigned)op.ld * (unsigned)sizeof(T)) + (lane % 8 ^ direct_turn(row)) * 16;
     }
+    auto load = [&](char* to, int stage, int i0, int i1) {
+#pragma unroll
+        for (int i = i0; i < i1; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                memory, (__attribute__((address_space(3))) void*)(to + (wave * kLoads + i) * 8 * kRowBytes), 16, (int)from[i],
+                stage * kRowBytes, 0, 0);
+    };
+    f32x16 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = f32x16{};
+    // (the next stage's loads are issued in two lots, 1.5% faster than in one)
+    auto compute = [&](const char* cur, char* next, int stage) {
+        u32x4 fa[2][MB], fb[2][NB];
+        // (made here each time: the addresses of all stages would fill the registers)
+        unsigned at = i32 * kRowBytes + ((hi ^ direct_turn(i32)) << 4);
+        asm volatile("" : "+v"(at));
+        auto read = [&](int kk) {
+            const char* of = cur + (at ^ (unsigned)kk << 5);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                fb[kk % 2][j] = *reinterpret_cast<const u32x4*>(of + (BM + wn + 32 * j) * kRowBytes);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) fa[kk % 2][i] = *reinterpret_cast<const u32x4*>(of + (wm + 32 * i) * kRowBytes);
+        };
+        read(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (kk < 3) read(kk + 1);
+            if (next && kk < 2) load(next, stage, kk * kLoads / 2, (kk + 1) * kLoads / 2);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = multiply<T>(fb[kk % 2][j], fa[kk % 2][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // all of the wavefront's loads are in LDS, then everyone's
+    auto arrive = [&] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    load(even, 0, 0, kLoads);
+    arrive();
+    int s = 0;
+    for (; s + 2 < stages; s += 2) {
+        compute(even, odd, s + 1);
+        arrive();
+        compute(odd, even, s + 2);
+        arrive();
+    }
+    if (s + 1 < stages) load(odd, s + 1, 0, kLoads);
+    compute(even, nullptr, 0);
+    arrive();
+    if (s + 1 < stages) compute(odd, nullptr, 0);
+    __syncthreads();
+    float* out = reinterpret_cast<float*>((wave < W / 2 ? even : odd) + wave % (W / 2) * kOutBytes<WN>);
+    put_out<T, WM, WN>(p, acc, out, m0 + wm, n0 + wn, slice);
 }
 
 // The slices' sums, always in their order, and the epilogue.
@@ -392,10 +544,22 @@ __global__ __launch_bounds__(256) void slices_kernel(Args p) {
         const int col = (int)(i % groups) * kV;
         float sum[kV] = {};
         const float* part = p.partial + (size_t)row * p.n + col;
-        for (int s = 0; s < p.slices; ++s, part += (size_t)p.m * p.n) {
+        if (col + kV <= p.n) {
+#pragma unroll 4
+            for (int s = 0; s < p.slices; ++s, part += (size_t)p.m * p.n) {
 #pragma unroll
-            for (int e = 0; e < kV; ++e)
-                if (col + e < p.n) sum[e] += part[e];
+                for (int e = 0; e < kV; e += 4) {
+                    const f32x4 q = load4(part + e);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) sum[e + y] += q[y];
+                }
+            }
+        } else {
+            for (int s = 0; s < p.slices; ++s, part += (size_t)p.m * p.n) {
+#pragma unroll
+                for (int e = 0; e < kV; ++e)
+                    if (col + e < p.n) sum[e] += part[e];
+            }
         }
         finish<T, kV>(p, row, col, sum);
     }
@@ -497,7 +661,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long long lddy,
             }
 #pragma unroll
             for (int j = 0; j < kV; ++j) {
-                const float g = slope(to_f32(a.e[j]), pb ? to_f32(b.e[j]) : 0.f, act);
+                const float g = slope<T>(to_f32(a.e[j]), pb ? to_f32(b.e[j]) : 0.f, act);
                 o.e[j] = from_f32<T>(g);
                 if (j < left) sum[j] += g;
             }
@@ -549,25 +713,38 @@ struct Plan {
     int slices, stages;
 };
 
-// Tile and slices of a product.
-Plan plan_product(int m, int n, int k, int esize) {
+// Tile and slices of a product: the least of a model of the time in us.  A stage of a
+// tile takes a CU `work` of its time and, alone there, `least` (the loads' latency);
+// measured with 1, 2 and 4 workgroups to a CU, bf16: 256: 1.8; 128: 0.7, 1.1; 64: 0.25-0.5,
+// 0.4, 0.73.  `across`: an operand is turned on its way.  Slices write and read float32 sums.
+// Of 24 products measured with every choice, the one taken costs at most a tenth more than
+// the best: 8192 x 2048 x 2048's gradient of the weight 92 us with 256 tiles in 4 slices,
+// 147 and 234 with 64 and 256 tiles unsliced; 8192 x 32 over 2048 12 and 17 us with 64 tiles
+// in 4 slices and one.
+Plan plan_product(int m, int n, int k, int esize, bool across) {
     const int kk = kRowBytes / esize, all = std::max(1, (k + kk - 1) / kk);
+    struct Cost {
+        Tile tile;
+        int edge;
+        double share, least, work, turn, f32;
+    };
+    static const Cost costs[] = {
+        {TILE_256, 256, 1, 1.8, 1.8, 1.2, 4}, {TILE_128, 128, 2, 0.7, 0.55, 1.2, 3.1}, {TILE_64, 64, 4, 0.35, 0.165, 1.25, 2.95}};
     Plan best{TILE_64, 1, all};
     double least = 1e30;
-    for (const Tile tile : {TILE_256, TILE_128, TILE_64}) {
-        const int edge = tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64;
-        const double per_cu = tile == TILE_256 ? 1 : tile == TILE_128 ? 2 : 4;
-        // a stage of as many workgroups as share a CU, in us
-        const double stage = (tile == TILE_256 ? 1.25 : tile == TILE_128 ? 0.75 : 0.5) * (esize == 4 ? 8 : 1);
-        const double tiles = (double)((m - 1) / edge + 1) * ((n - 1) / edge + 1);
+    for (const Cost& c : costs) {
+        const double tiles = (double)((m - 1) / c.edge + 1) * ((n - 1) / c.edge + 1);
         for (int want = 1; want <= 64 && want <= all; want *= 2) {
             const int stages = (all + want - 1) / want, slices = (all + stages - 1) / stages;
-            const double rounds = std::ceil(tiles * slices / (256 * per_cu));
-            double cost = rounds * (stages + 3) * stage;
-            if (slices > 1) cost += 4 + (double)slices * m * n * 8 / 4e6;
+            const double to_a_cu = std::ceil(tiles * slices / 256), rounds = std::floor(to_a_cu / c.share), rest = to_a_cu - rounds * c.share;
+            double stage = rounds * std::max(c.least, c.share * c.work) + (rest > 0 ? std::max(c.least, rest * c.work) : 0);
+            if (across) stage *= c.turn;
+            if (esize == 4) stage *= c.f32;
+            double cost = (stages + 3) * stage;
+            if (slices > 1) cost += 3 + 0.15 * slices + (double)slices * m * n * 8 / 6e6;
             if (cost < least) {
                 least = cost;
-                best = Plan{tile, slices, stages};
+                best = Plan{c.tile, slices, stages};
             }
         }
     }
@@ -578,25 +755,44 @@ size_t partial_bytes(int m, int n, const Plan& p) {
 }
 constexpr int kFewRows = 64;  // up to here the rows' kernel
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 template <typename T, bool A, bool B>
 int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
-    auto go = [&](auto kernel, int edge, int wm, int wn) {
+    auto go = [&](auto kernel, bool direct, int edge, int wm, int wn) {
         const int threads = edge / wm * edge / wn * 64;
         const long long blocks = (long long)((p.m - 1) / edge + 1) * ((p.n - 1) / edge + 1) * p.slices;
         if (blocks * threads >= (1LL << 32)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, "linear: more workgroups than a launch may have");
-        const size_t lds = std::max<size_t>((size_t)4 * edge * kRowBytes, (size_t)threads / 64 * 32 * (wn + 4) * 4);
-        RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        const size_t lds = direct ? 0 : std::max<size_t>((size_t)4 * edge * kRowBytes, (size_t)threads / 64 * 32 * (wn + 4) * 4);
+        if (!direct)
+            RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, p);
         RKA_RETURN_IF_HIP(hipGetLastError());
         return 0;
     };
-    if (tile == TILE_256) {
-        RKA_RETURN_IF_ERR(go(&tile_kernel<T, 256, 256, 128, 64, A, B>, 256, 128, 64));
-    } else if (tile == TILE_128) {
-        RKA_RETURN_IF_ERR(go(&tile_kernel<T, 128, 128, 64, 64, A, B>, 128, 64, 64));
-    } else {
-        RKA_RETURN_IF_ERR(go(&tile_kernel<T, 64, 64, 32, 32, A, B>, 64, 32, 32));
+    auto either = [&](auto direct) {
+        constexpr bool D = decltype(direct)::value;
+        const auto kernel = [](auto bm, auto wm, auto wn) {
+            constexpr int BM = decltype(bm)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+            if constexpr (D)
+                return &direct_kernel<T, BM, BM, WM, WN>;
+            else
+                return &tile_kernel<T, BM, BM, WM, WN, A, B>;
+        };
+        if (tile == TILE_256) return go(kernel(Int<256>{}, Int<128>{}, Int<64>{}), D, 256, 128, 64);
+        if (tile == TILE_128) return go(kernel(Int<128>{}, Int<64>{}, Int<64>{}), D, 128, 64, 64);
+        return go(kernel(Int<64>{}, Int<32>{}, Int<32>{}), D, 64, 32, 32);
+    };
+    bool done = false;
+    if constexpr (!A && !B) {
+        const auto on16 = [](const Operand& o) { return (reinterpret_cast<uintptr_t>(o.ptr) | (size_t)o.ld * sizeof(T)) % 16 == 0; };
+        if (p.k % (8 * kVec<T>) == 0 && on16(p.a) && on16(p.b)) {
+            RKA_RETURN_IF_ERR(either(std::true_type{}));
+            done = true;
+        }
     }
+    if (!done) RKA_RETURN_IF_ERR(either(std::false_type{}));
     if (p.slices > 1) {
         const long long items = (long long)p.m * ((p.n + kVec<T> - 1) / kVec<T>);
         hipLaunchKernelGGL((slices_kernel<T>), dim3((unsigned)std::min<long long>((items + 255) / 256, 2048)), dim3(256), 0, s, p);
@@ -609,7 +805,7 @@ int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
 template <typename T, bool A, bool B>
 int product(int m, int n, int k, const Operand& a, const Operand& b, void* c, const Epilogue& ep, float* partial,
             hipStream_t s) {
-    const Plan plan = plan_product(m, n, k, sizeof(T));
+    const Plan plan = plan_product(m, n, k, sizeof(T), A || B);
     return launch_tiles<T, A, B>(Args{m, n, k, a, b, c, partial, plan.slices, plan.stages, ep}, plan.tile, s);
 }
 
@@ -629,11 +825,12 @@ int forward(int m, int n, int k, const Operand& x, const Operand& w, void* y, co
     return 0;
 }
 
-// Row ranges of the slope kernel: enough workgroups for the GPU, at least 64 rows each.
+// Row ranges of the slope kernel: enough workgroups for the GPU, at least two rows to a thread
+// (with eight, 1000 rows of 385 float32 took 18 us).
 int slope_ranges(int m, int n, int esize, int* rows) {
     const int cols = (n - 1) / (32 * (16 / esize)) + 1;
     const int want = std::max(1, 2048 / cols);
-    *rows = std::max(64, ((m - 1) / want + 8) / 8 * 8);
+    *rows = std::max(16, ((m - 1) / want + 8) / 8 * 8);
     return (m - 1) / *rows + 1;
 }
 
@@ -647,7 +844,7 @@ BackwardLayout backward_layout(int m, int n, int k, int esize) {
     l.sums = align_up((size_t)m * n * esize, 256);
     l.partial = l.sums + align_up((size_t)slope_ranges(m, n, esize, &rows) * n * sizeof(float), 256);
     // one after the other on the stream
-    l.total = l.partial + std::max(partial_bytes(m, k, plan_product(m, k, n, esize)), partial_bytes(n, k, plan_product(n, k, m, esize)));
+    l.total = l.partial + std::max(partial_bytes(m, k, plan_product(m, k, n, esize, true)), partial_bytes(n, k, plan_product(n, k, m, esize, true)));
     return l;
 }
 
@@ -699,7 +896,7 @@ extern "C" {
 
 size_t rka_linear_forward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {
     if (rows < 1 || outputs < 1 || inputs < 1 || rows <= kFewRows) return 0;
-    return partial_bytes(rows, outputs, plan_product(rows, outputs, inputs, dtype == RKA_DTYPE_F32 ? 4 : 2));
+    return partial_bytes(rows, outputs, plan_product(rows, outputs, inputs, dtype == RKA_DTYPE_F32 ? 4 : 2, false));
 }
 
 size_t rka_linear_backward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {

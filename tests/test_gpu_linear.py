@@ -100,6 +100,19 @@ def test_sizes(gpu, m, n, k, dtype):
     _check(gpu, m, n, k, dtype, "none", bias=False, residual=False)
 
 
+# operands that go to LDS directly (whole stages on 16 bytes): one stage, even and odd
+# numbers of them, slices, and each tile with an end inside
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(70, 1000, 64), (300, 200, 192), (129, 40, 2048), (257, 31, 128), (2048, 1030, 256)])
+def test_aligned_sizes(gpu, m, n, k, dtype):
+    _check(gpu, m, n, k, dtype, "gelu")
+
+
+@pytest.mark.parametrize("m,n,k", [(4100, 4104, 320), (16384, 1032, 64)])
+def test_aligned_large_tiles(gpu, m, n, k):
+    _check(gpu, m, n, k, torch.bfloat16, "silu")
+
+
 @pytest.mark.parametrize("m,n,k", [(4096, 4096, 200), (4100, 4100, 136), (8192, 256, 1000)])
 def test_large_tiles(gpu, m, n, k):
     _check(gpu, m, n, k, torch.bfloat16, "gelu")
