@@ -1,6 +1,7 @@
 """MI355X (gfx950) fp32 GRU training path: hand-written HIP kernels behind a
 C ABI (librnn_kernel_amd.so), with an nn.GRU-compatible PyTorch front end."""
 from .delta import GatedDeltaFunction, gated_delta_rule, gated_delta_step
+from .delta_layer import GatedDelta
 from .gru import (
     GRU,
     GRUFunction,
@@ -20,6 +21,7 @@ __all__ = [
     "Linear",
     "LinearFunction",
     "linear",
+    "GatedDelta",
     "GatedDeltaFunction",
     "gated_delta_rule",
     "gated_delta_step",
