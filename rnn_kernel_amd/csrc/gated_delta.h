@@ -187,16 +187,16 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
     unsigned w[4];
 };
 
-// Loads of neighbouring columns, from column c of a row of `width` in memory, zero past
-// it: without branches (clamped addresses), and for the widths that are multiples of
-// eight (VEC) in 16-byte loads.
+// Loads of neighbouring columns, from column c of a row of `width` in memory, without
+// branches (clamped addresses).  For the widths that are multiples of eight (VEC) in
+// 16-byte loads, and as they come: what lies past the width is made zero where it is
+// used, since a select beside the load would wait for it.
 template <bool VEC>
 __device__ __forceinline__ f32x4 load4(const float* row, int c, int width) {
     f32x4 x;
     if constexpr (VEC) {
         const Float4U v = *reinterpret_cast<const Float4U*>(row + min(c, width - 4));
         x = f32x4{v.x, v.y, v.z, v.w};
-        if (c >= width) x = f32x4{0.f, 0.f, 0.f, 0.f};
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -208,36 +208,39 @@ __device__ __forceinline__ f32x4 load4(const float* row, int c, int width) {
 }
 
 // Eight columns of a row: a lane's part of an operand, as loaded, in pieces, or put
-// where rows are kept (zero where the row is not `on`).
+// where rows are kept (zero where the row is not `on`, or past the width).
 template <typename T>
 struct Eight;
 template <>
 struct Eight<float> {
     f32x4 a, b;
+    bool in;
     template <bool VEC>
     __device__ __forceinline__ void load(const float* row, int c, int width) {
+        in = c < width;
         a = load4<VEC>(row, c, width);
         b = load4<VEC>(row, c + 4, width);
     }
     __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[3]) {
-        if (!on) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!on || !in) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
         split8<3>(a, b, p);
     }
     __device__ __forceinline__ void store(bool on, float* to) const {
         const f32x4 none{0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<f32x4*>(to) = on ? a : none;
-        *reinterpret_cast<f32x4*>(to + 4) = on ? b : none;
+        *reinterpret_cast<f32x4*>(to) = on && in ? a : none;
+        *reinterpret_cast<f32x4*>(to + 4) = on && in ? b : none;
     }
 };
 template <>
 struct Eight<bf16> {
     u32x4 x;
+    bool in;
     template <bool VEC>
     __device__ __forceinline__ void load(const bf16* row, int c, int width) {
+        in = c < width;
         if constexpr (VEC) {
             const Bytes16 v = *reinterpret_cast<const Bytes16*>(row + min(c, width - 8));
             x = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
-            if (c >= width) x = u32x4{0, 0, 0, 0};
         } else {
             x = u32x4{0, 0, 0, 0};
 #pragma unroll
@@ -247,9 +250,9 @@ struct Eight<bf16> {
             }
         }
     }
-    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[1]) { p[0] = on ? x : u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void pieces(bool on, u32x4 (&p)[1]) { p[0] = on && in ? x : u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void store(bool on, bf16* to) const {
-        *reinterpret_cast<u32x4*>(to) = on ? x : u32x4{0, 0, 0, 0};
+        *reinterpret_cast<u32x4*>(to) = on && in ? x : u32x4{0, 0, 0, 0};
     }
 };
 

@@ -149,9 +149,6 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
         // where the addresses of every block of Dk would fill the registers)
         size_t zero = 0;
         asm volatile("" : "+s"(zero));
-        float gate = 0.f;
-        if (wave == 0)
-            gate = load_gate(g, b * d.g_s[0] + (t0 + min(lane, live - 1)) * d.g_s[1] + h * d.g_s[2], d.gate_bf16);
         // of the lane's rows as operands
         const bool on = 16 * w4 + n < live;
         const int token = min(16 * w4 + n, live - 1);
@@ -176,8 +173,10 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
             nx.template load<VEC>(pdx, v0 + 8 * hi, d.Dv);
         };
         f32x4 aq[TH] = {}, ar[TH] = {}, az[TH] = {}, af[4] = {};
-        float dot = 0.f;
+        float dot = 0.f, gate = 0.f;
         load(0);
+        if (wave == 0)
+            gate = load_gate(g, b * d.g_s[0] + (t0 + min(lane, live - 1)) * d.g_s[1] + h * d.g_s[2], d.gate_bf16);
         for (int v0 = 0; v0 < d.Dv; v0 += 32) {
             u32x4 xo[NP], xx[3], xe[3];
             no.pieces(on && dout, xo);
@@ -186,13 +185,13 @@ __global__ __launch_bounds__(kThreads, 1) void gradients_kernel(Dims d, const T*
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 const int x = tid + i * kThreads;
-                if (x / 8 >= d.Dk) ns[i] = nd[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (x / 8 >= d.Dk || v0 + x % 8 * 4 >= d.Dv) ns[i] = nd[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dot += ns[i][j] * nd[i][j];
                 put_columns(fs, x / 8, x % 8 * 4, ns[i]);
                 put_columns(fd, x / 8, x % 8 * 4, nd[i]);
             }
-            put_columns(fe, tid / 8, tid % 8 * 4, tid / 8 < live ? ne : f32x4{0.f, 0.f, 0.f, 0.f});
+            put_columns(fe, tid / 8, tid % 8 * 4, tid / 8 < live && v0 + tid % 8 * 4 < d.Dv ? ne : f32x4{0.f, 0.f, 0.f, 0.f});
             __syncthreads();
             if (v0 + 32 < d.Dv) load(v0 + 32);
 #pragma unroll

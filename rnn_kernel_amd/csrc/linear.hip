@@ -765,7 +765,7 @@ int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
         const long long blocks = (long long)((p.m - 1) / edge + 1) * ((p.n - 1) / edge + 1) * p.slices;
         if (blocks * threads >= (1LL << 32)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, "linear: more workgroups than a launch may have");
         const size_t lds = direct ? 0 : std::max<size_t>((size_t)4 * edge * kRowBytes, (size_t)threads / 64 * 32 * (wn + 4) * 4);
-        if (!direct)
+        if (lds > (64 << 10))
             RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, p);
         RKA_RETURN_IF_HIP(hipGetLastError());
