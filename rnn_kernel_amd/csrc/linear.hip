@@ -379,7 +379,11 @@ __device__ __forceinline__ void put_out(const Args& p, const f32x16 (&acc)[WM / 
     }
 }
 
-// BM x BN tiles, WM x WN of them per wavefront.
+// BM x BN tiles, WM x WN of them per wavefront: through registers, for operands that are
+// turned on their way and for rows of any address and length.  Bound by its waits: the
+// registers that hold the next stage leave those of one k step's fragments, so that
+// LDS's latency shows between the products.  8192 x 2048 over 2048 bf16, one operand
+// turned: 87 us, 790 TFLOP/s; direct_kernel: 69 us.
 template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS>
 __global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(Args p) {
     constexpr int NT = BM / WM * BN / WN * 64, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;
@@ -441,7 +445,10 @@ __device__ __forceinline__ int direct_turn(int row) { return (row ^ (row >> 3 & 
 
 // The same for operands that both lie along the sum, in whole stages and on 16 bytes:
 // they go from memory to LDS without registers between, which leaves those for the
-// fragments of the next products.
+// fragments of the next products.  Bound by LDS: a 256 x 256 tile's stage reads 192 KB of
+// fragments and writes 64, as many clocks (2048) as its matrix instructions.  16384 x 4096
+// over 4096 bf16: 458 us, 1200 TFLOP/s (576 through registers; without its loads, in a copy,
+// 344); 128 x 128 to a wavefront, with fewer reads of LDS but one wavefront to a SIMD, 565.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(Args p) {
     constexpr int W = BM / WM * BN / WN, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;
@@ -567,7 +574,8 @@ __global__ __launch_bounds__(256) void slices_kernel(Args p) {
 
 // Few rows: 16 columns of the output per workgroup, whose wavefronts share the sum.
 // The weight goes from memory to the matrix instructions' operands directly, every
-// element once.
+// element once.  4 rows of 4096 over 2048 bf16 (16.8 MB, which the chip's caches hold
+// between calls): 5.7 us.
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void rows_kernel(Args p) {
     constexpr int kV = kVec<T>, kK = 4 * kV, kWaves = 8, kDeep = 4;
@@ -753,7 +761,16 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
 size_t partial_bytes(int m, int n, const Plan& p) {
     return p.slices > 1 ? align_up((size_t)p.slices * m * n * sizeof(float), 256) : 0;
 }
-constexpr int kFewRows = 64;  // up to here the rows' kernel
+// The rows' kernel, whose workgroup goes through the whole sum, or tiles, in slices where
+// those are few, which go through the weight at 6 TB/s (out of the caches; models of the
+// measured times in us).  Rows' kernel and tiles, bf16, 4096 columns over 2048: 1 row 4.9 and
+// 9.3, 16 5.8 and 10.1, 32 7.7 and 10.7, 64 12.1 and 10.4; 256 columns over 4096: 8 rows 7.5
+// and 10.0, 32 12.5 and 10.9.  float32, 64 columns over 4096: 1 row 11.8 and 9.6.
+bool few_rows(int m, int n, int k, int esize) {
+    if (m > 32) return false;
+    const double row = (double)k * esize;
+    return 4 + row / 1024 * (m <= 16 ? 0.5 : 1.15) < 9.3 + n * row / 6e6;
+}
 
 template <int N>
 using Int = std::integral_constant<int, N>;
@@ -812,15 +829,13 @@ int product(int m, int n, int k, const Operand& a, const Operand& b, void* c, co
 template <typename T>
 int forward(int m, int n, int k, const Operand& x, const Operand& w, void* y, const Epilogue& ep, float* partial,
             hipStream_t s) {
-    if (m > kFewRows) return product<T, false, false>(m, n, k, x, w, y, ep, partial, s);
+    if (!few_rows(m, n, k, sizeof(T))) return product<T, false, false>(m, n, k, x, w, y, ep, partial, s);
     const Args p{m, n, k, x, w, y, nullptr, 1, 0, ep};
     const dim3 grid((unsigned)((n - 1) / 16 + 1));
     if (m <= 16)
         hipLaunchKernelGGL((rows_kernel<T, 1>), grid, dim3(512), 0, s, p);
-    else if (m <= 32)
-        hipLaunchKernelGGL((rows_kernel<T, 2>), grid, dim3(512), 0, s, p);
     else
-        hipLaunchKernelGGL((rows_kernel<T, 4>), grid, dim3(512), 0, s, p);
+        hipLaunchKernelGGL((rows_kernel<T, 2>), grid, dim3(512), 0, s, p);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
@@ -895,8 +910,9 @@ using namespace rka;
 extern "C" {
 
 size_t rka_linear_forward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {
-    if (rows < 1 || outputs < 1 || inputs < 1 || rows <= kFewRows) return 0;
-    return partial_bytes(rows, outputs, plan_product(rows, outputs, inputs, dtype == RKA_DTYPE_F32 ? 4 : 2, false));
+    const int esize = dtype == RKA_DTYPE_F32 ? 4 : 2;
+    if (rows < 1 || outputs < 1 || inputs < 1 || few_rows(rows, outputs, inputs, esize)) return 0;
+    return partial_bytes(rows, outputs, plan_product(rows, outputs, inputs, esize, false));
 }
 
 size_t rka_linear_backward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {

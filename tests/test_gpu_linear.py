@@ -108,6 +108,13 @@ def test_aligned_sizes(gpu, m, n, k, dtype):
     _check(gpu, m, n, k, dtype, "gelu")
 
 
+# few rows on either side of the rule that takes the rows' kernel or tiles in slices
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 9000), (16, 70, 2000), (17, 300, 513), (32, 24, 1500), (32, 24, 5000), (33, 24, 1500)])
+def test_few_rows(gpu, m, n, k, dtype):
+    _check(gpu, m, n, k, dtype, "relu")
+
+
 @pytest.mark.parametrize("m,n,k", [(4100, 4104, 320), (16384, 1032, 64)])
 def test_aligned_large_tiles(gpu, m, n, k):
     _check(gpu, m, n, k, torch.bfloat16, "silu")
