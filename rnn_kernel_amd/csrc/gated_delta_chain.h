@@ -16,6 +16,12 @@
 // passes through LDS in operand order, one barrier apiece.  The workgroups of a head are
 // eight apart, on one XCD, whose L2 then answers all but the first of them.
 //
+// Bound by the latency of the chain.  bf16, 128x128, one column block to a workgroup,
+// 16384 tokens of 16 heads: 481 us, 4400 clocks per chunk, of which the wavefronts that
+// make E spend 1500 on its products with the loads between them, 250 on handing it on, 600
+// on the state's update and 1300 at the two barriers, where the other four arrive last.
+// Without its loads of rows (a copy, with wrong results) the same takes 280 us.
+// 64 heads of 2048 tokens with two blocks: 151 us forward and 155 backward.
 #pragma once
 
 #include <algorithm>
@@ -608,12 +614,16 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
 }
 
 // Calls f with the chain's steps over Dk and its column blocks as integral constants.
-// Two blocks halve what is read of K, Q, T and P per column, one has the shorter
-// chain: two once every CU has a workgroup anyway.  (Float32 operands of the largest
-// Dk leave no registers for two.)
+// Two blocks halve what is read of K, Q, T and P per column, one has the shorter chain:
+// two where one to a workgroup would not have a CU for each.  Measured, the whole forward
+// in us with one and two (bf16, 128x128): 256 workgroups of one (2048 tokens) 113 and 131,
+// 320 163 and 140, 512 260 and 225, 1024 (1024 tokens) 325 and 230; 128 (16384 tokens) 690
+// and 810.  float32 (512 tokens): 256 57 and 61, 384 84 and 71.  (Float32 operands of the
+// largest Dk leave no registers for two.)
 template <typename T, typename F>
 int with_chain(const Dims& d, F f) {
-    const bool two = d.Dv > 16 && (long long)d.B * d.Hv * ((d.Dv + 31) / 32) >= 256;
+    constexpr int kCus = 256;
+    const bool two = d.Dv > 16 && (long long)d.B * d.Hv * ((d.Dv + 15) / 16) > kCus;
     auto pick = [&](auto ku) {
         if constexpr (kPieces<T> == 1 || decltype(ku)::value < 8)
             if (two) return f(ku, std::integral_constant<int, 2>{});

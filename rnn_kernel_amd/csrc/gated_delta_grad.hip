@@ -8,8 +8,10 @@
 // memory to the operand registers, the blocks of S, dS' and E are split into bf16 pieces
 // once and shared through LDS, loaded a step ahead.
 //
-// Bound by memory: of S, dS', E, dX and dO some 12 bytes per state element and chunk are
-// read once, against 15 products of pieces on each.
+// Bound by latency, with one workgroup to a CU, as the sums and the operands fill its
+// registers and LDS: 8192 tokens of 16 heads of 128x128 bf16 282 us, of which the matrix
+// instructions are some 75 and the bytes (440 MB) 90.  Holding the next head's first
+// loads through what follows a head's last step spills registers and took 347 us.
 #include "gated_delta.h"
 
 namespace rka {

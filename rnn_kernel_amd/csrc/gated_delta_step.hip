@@ -4,6 +4,10 @@
 // A workgroup takes a block of columns of one state, in registers; k^T S~ and
 // q^T S~ come out of one reduction over the rows, since o = q^T S' needs only
 // q^T S~ and q . k besides the error e:  o = scale (q^T S~ + (q . k) beta e).
+//
+// Bound by memory: 256 requests on 32 heads of 128x128 (1.07 GB) 225 us, 4.8 TB/s, the rate of
+// a large copy.  Blocks of 32 columns give one request on 8 heads of 64x64 16 workgroups;
+// that call is 14 us of the host's time.
 #include "gated_delta.h"
 
 namespace rka {
