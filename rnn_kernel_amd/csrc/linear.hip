@@ -445,10 +445,12 @@ __device__ __forceinline__ int direct_turn(int row) { return (row ^ (row >> 3 & 
 
 // The same for operands that both lie along the sum, in whole stages and on 16 bytes:
 // they go from memory to LDS without registers between, which leaves those for the
-// fragments of the next products.  Bound by LDS: a 256 x 256 tile's stage reads 192 KB of
-// fragments and writes 64, as many clocks (2048) as its matrix instructions.  16384 x 4096
-// over 4096 bf16: 458 us, 1200 TFLOP/s (576 through registers; without its loads, in a copy,
-// 344); 128 x 128 to a wavefront, with fewer reads of LDS but one wavefront to a SIMD, 565.
+// fragments of the next products.  16384 x 4096 over 4096 bf16: 458 us, 1200 TFLOP/s (576
+// through registers).  Bound by how the loads and their arrival interleave with the products:
+// the matrix instructions are busy for 52% of the clocks, LDS for 21%; without the loads (a
+// copy, with wrong results) 344 us, with all of them from L2 461; half stages in a ring of four,
+// whose next fragments are read before the barrier, 494 (rows of 64 bytes); 128 x 128 to a
+// wavefront, with one wavefront to a SIMD, 565.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(Args p) {
     constexpr int W = BM / WM * BN / WN, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;
