@@ -109,8 +109,8 @@ __device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
 //
 // Bound by what it writes: of a chunk and head of 128x128 bf16 32 KB of `own` (float32, as
 // the chain adds it), 48 KB of `read` and 18 KB of `p` in three pieces; 16384 tokens of 16
-// heads (470 MB written and read) 162 us, 2.9 TB/s; the inverse, a chain of its own, is
-// hidden only by the other workgroups of the CU.  Written in the form that the chain's
+// heads (408 MB written, 219 read) 160 us, 3.9 TB/s; the inverse, a chain of its own, is
+// hidden by the other workgroups of the CU.  Written in the form that the chain's
 // registers take, since the chain, which is serial, would pay for every conversion.
 template <typename T, bool BACKWARD, bool VEC>
 __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, const void* g, const void* beta,

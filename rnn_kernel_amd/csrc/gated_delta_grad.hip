@@ -9,9 +9,10 @@
 // once and shared through LDS, loaded a step ahead.
 //
 // Bound by latency, with one workgroup to a CU, as the sums and the operands fill its
-// registers and LDS: 8192 tokens of 16 heads of 128x128 bf16 282 us, of which the matrix
-// instructions are some 75 and the bytes (440 MB) 90.  Holding the next head's first
-// loads through what follows a head's last step spills registers and took 347 us.
+// registers and LDS: 8192 tokens of 16 heads of 128x128 bf16 282 us, in which the matrix
+// instructions are busy for 16% of the clocks and 710 MB are read and written, 150 us of a
+// copy.  Holding the next head's first loads through what follows a head's last step
+// spills registers and took 347 us.
 #include "gated_delta.h"
 
 namespace rka {
