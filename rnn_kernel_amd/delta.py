@@ -36,29 +36,32 @@ def _check_inputs(q, k, v, g, beta, tokens: bool) -> None:
     """The checks that both entry points share; ``tokens``: with a token
     dimension."""
     lead = 2 if tokens else 1
-    shape = "[batch, tokens, heads, dim]" if tokens else "[batch, heads, dim]"
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
-        if not t.is_cuda:
-            raise RuntimeError(f"gated delta rule: {name} must be a CUDA/HIP tensor")
-        if t.device != q.device:
-            raise RuntimeError("gated delta rule: all tensors must be on one device")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    index = q.get_device()  # (a tensor's device as an int: a single step is a few us of the host)
+    if not (q.is_cuda and k.get_device() == v.get_device() == g.get_device() == beta.get_device() == index):
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
+            if not t.is_cuda:
+                raise RuntimeError(f"gated delta rule: {name} must be a CUDA/HIP tensor")
+        raise RuntimeError("gated delta rule: all tensors must be on one device")
+    dtype, gate = q.dtype, g.dtype
+    if dtype not in _DTYPES or k.dtype != dtype or v.dtype != dtype:
         raise RuntimeError("gated delta rule: q, k and v must be all float32 or all bfloat16")
-    if g.dtype != beta.dtype or g.dtype not in (torch.float32, q.dtype):
+    if beta.dtype != gate or gate not in (torch.float32, dtype):
         raise RuntimeError("gated delta rule: g and beta must be float32 or of q's dtype")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != lead + 2:
-            raise ValueError(f"gated delta rule: {name} must have shape {shape}")
-    if k.shape != q.shape:
+    qs, vs = q.shape, v.shape
+    if len(qs) != lead + 2 or k.dim() != lead + 2 or len(vs) != lead + 2:
+        name = "q" if len(qs) != lead + 2 else "k" if k.dim() != lead + 2 else "v"
+        shape = "[batch, tokens, heads, dim]" if tokens else "[batch, heads, dim]"
+        raise ValueError(f"gated delta rule: {name} must have shape {shape}")
+    if k.shape != qs:
         raise ValueError("gated delta rule: q and k must have the same shape")
-    if v.shape[:lead] != q.shape[:lead]:
+    if vs[0] != qs[0] or vs[lead - 1] != qs[lead - 1]:
         raise ValueError("gated delta rule: v must have q's batch and token dimensions")
-    heads = v.size(lead)
-    if q.size(lead) < 1 or heads < 1 or heads % q.size(lead) != 0:
+    if qs[lead] < 1 or vs[lead] < 1 or vs[lead] % qs[lead] != 0:
         raise ValueError("gated delta rule: v's heads must be a multiple of q's and k's")
-    if not 1 <= q.size(-1) <= MAX_KEY_DIM or v.size(-1) < 1:
+    if not 1 <= qs[-1] <= MAX_KEY_DIM or vs[-1] < 1:
         raise ValueError(f"gated delta rule: key dim must be in [1, {MAX_KEY_DIM}] and value dim at least 1")
-    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+    gates = vs[:-1]
+    if g.shape != gates or beta.shape != gates:
         raise ValueError("gated delta rule: g and beta must have v's shape without its last dimension")
 
 
@@ -208,8 +211,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     elif state.size(0) < batch:
         raise ValueError("gated delta rule: fewer states than requests")
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
-    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    _lib.call(_index_of(v.device), "rka_gated_delta_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+    o = v.new_empty(v.shape)
+    _lib.call(v.get_device(), "rka_gated_delta_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
               beta.data_ptr(), state.data_ptr(), _lib.ptr(slots), state.size(0), o.data_ptr(), batch, q.size(1),
               v.size(1), key_dim, v.size(2), _strides(q, k, v, g, beta), _DTYPES[q.dtype], _DTYPES[g.dtype],
               int(normalize), key_dim ** -0.5 if scale is None else float(scale))

@@ -32,6 +32,8 @@ def _index_of(device) -> int:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as a matrix whose rows are dense (any distance apart)."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     m = t if t.dim() == 2 else t.reshape(-1, t.size(-1))
     return m if (m.size(1) == 1 or m.stride(1) == 1) and (m.size(0) <= 1 or m.stride(0) >= m.size(1)) else m.contiguous()
 
@@ -41,14 +43,15 @@ def _ld(m: torch.Tensor) -> int:
 
 
 def _check(x, weight, bias, residual, activation) -> None:
+    index, dtype = x.get_device(), x.dtype
     for t, name in ((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual")):
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"linear: {name} must be a CUDA/HIP tensor")
-        if t.device != x.device:
+        if t.get_device() != index:
             raise RuntimeError("linear: all tensors must be on one device")
-        if t.dtype not in _DTYPES or t.dtype != x.dtype:
+        if t.dtype != dtype or dtype not in _DTYPES:
             raise RuntimeError("linear: tensors must be all float32 or all bfloat16")
     if activation not in _ACTS:
         raise ValueError(f"linear: activation must be one of {', '.join(ACTIVATIONS)}")
@@ -72,12 +75,12 @@ def _forward(x, weight, bias, residual, act: int, keep_z: bool):
     rows, outputs, inputs = xm.size(0), wm.size(0), wm.size(1)
     bm = None if bias is None else bias.contiguous()
     rm = None if residual is None else _rows(residual)
-    y = torch.empty(*x.shape[:-1], outputs, dtype=x.dtype, device=x.device)
-    z = torch.empty(rows, outputs, dtype=x.dtype, device=x.device) if keep_z else None
+    y = x.new_empty((*x.shape[:-1], outputs))
+    z = x.new_empty((rows, outputs)) if keep_z else None
     dtype = _DTYPES[x.dtype]
     nbytes = lib.rka_linear_forward_workspace_bytes(rows, outputs, inputs, dtype)
     ws = _bytes(nbytes, x.device) if nbytes else None
-    _lib.call(_index_of(x.device), "rka_linear_forward", xm.data_ptr(), _ld(xm), wm.data_ptr(), _ld(wm), _lib.ptr(bm),
+    _lib.call(x.get_device(), "rka_linear_forward", xm.data_ptr(), _ld(xm), wm.data_ptr(), _ld(wm), _lib.ptr(bm),
               _lib.ptr(rm), 0 if rm is None else _ld(rm), y.data_ptr(), _lib.ptr(z), _lib.ptr(ws), nbytes, rows, outputs,
               inputs, act, dtype)
     return y, z, xm, wm
