@@ -97,7 +97,7 @@ def test_answers_continue_a_prompt(gpu, dtype):
 
 
 def test_the_command_trains_and_answers(gpu):
-    from rnn_kernel_amd.delta_layer import main
+    from rnn_kernel_amd.delta_train import main
 
     r = main(["--size", "64", "--heads", "2", "--key-heads", "1", "--head-dim", "32", "--batch-size", "4", "--seq-len", "100",
               "--steps", "40", "--answer", "9"])

@@ -57,7 +57,7 @@ def test_linear_has_nn_linears_parameters():
 
 
 def test_the_command_needs_a_gpu():
-    from rnn_kernel_amd.delta_layer import main
+    from rnn_kernel_amd.delta_train import main
 
     with pytest.raises(RuntimeError, match="runs on a GPU"):
         main(["--device", "cpu"])
