@@ -578,7 +578,9 @@ __global__ __launch_bounds__(256) void slices_kernel(Args p) {
 // The weight goes from memory to the matrix instructions' operands directly, every
 // element once.  4 rows of 4096 over 2048 bf16 (16.8 MB, which the chip's caches hold
 // between calls): 5.7 us.
-template <typename T, int MT>
+// SWAP: few columns instead, 16 rows of x per workgroup: a is the weight, b is x, and the
+// output is written the other way round.
+template <typename T, int MT, bool SWAP>
 __global__ __launch_bounds__(512) void rows_kernel(Args p) {
     constexpr int kV = kVec<T>, kK = 4 * kV, kWaves = 8, kDeep = 4;
     __shared__ float sums[kWaves][MT][16][17];
@@ -631,18 +633,26 @@ __global__ __launch_bounds__(512) void rows_kernel(Args p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) sums[wave][t][4 * hi + r][i16] = acc[t][r];
     __syncthreads();
+    Args out = p;
+    if (SWAP) out.n = p.m;
     for (int i = threadIdx.x; i < MT * 256; i += 512) {
-        const int t = i / 256, r = i / 16 % 16, c = i % 16;
-        if (16 * t + r >= p.m) continue;
+        const int t = SWAP ? i / 16 % MT : i / 256, r = SWAP ? i % 16 : i / 16 % 16, c = SWAP ? i / (16 * MT) : i % 16;
+        if (16 * t + r >= p.m || n0 + c >= p.n) continue;
         float sum[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) sum[0] += sums[k][t][r][c];
-        finish<T, 1>(p, 16 * t + r, n0 + c, sum);
+        if (SWAP)
+            finish<T, 1>(out, n0 + c, 16 * t + r, sum);
+        else
+            finish<T, 1>(out, 16 * t + r, n0 + c, sum);
     }
 }
 
 // dz = dy act'(z) and the sums of its columns over a range of rows: 8 rows of 32
-// threads per workgroup, kVec columns each.
+// threads per workgroup, kVec columns each.  z comes, and dz goes, as T: the products that
+// take dz are products of T, and in bf16 z is half of what the forward keeps; dx and dW
+// are then off by 0.0024 instead of 0.0017 (db, summed before the rounding, by less).
+// Bound by memory: 8192 x 2048 bf16 (100 MB) 20 us, 5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long long lddy, const T* z, T* dz, float* sums, int m,
                                                     int n, int rows_per_block, int act) {
@@ -721,6 +731,7 @@ enum Tile { TILE_256, TILE_128, TILE_64 };
 struct Plan {
     Tile tile;
     int slices, stages;
+    double cost;
 };
 
 // Tile and slices of a product: the least of a model of the time in us.  A stage of a
@@ -740,8 +751,7 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
     };
     static const Cost costs[] = {
         {TILE_256, 256, 1, 1.8, 1.8, 1.2, 4}, {TILE_128, 128, 2, 0.7, 0.55, 1.2, 3.1}, {TILE_64, 64, 4, 0.35, 0.165, 1.25, 2.95}};
-    Plan best{TILE_64, 1, all};
-    double least = 1e30;
+    Plan best{TILE_64, 1, all, 1e30};
     for (const Cost& c : costs) {
         const double tiles = (double)((m - 1) / c.edge + 1) * ((n - 1) / c.edge + 1);
         for (int want = 1; want <= 64 && want <= all; want *= 2) {
@@ -752,10 +762,7 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
             if (esize == 4) stage *= c.f32;
             double cost = (stages + 3) * stage;
             if (slices > 1) cost += 3 + 0.15 * slices + (double)slices * m * n * 8 / 6e6;
-            if (cost < least) {
-                least = cost;
-                best = Plan{c.tile, slices, stages};
-            }
+            if (cost < best.cost) best = Plan{c.tile, slices, stages, cost};
         }
     }
     return best;
@@ -763,15 +770,20 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
 size_t partial_bytes(int m, int n, const Plan& p) {
     return p.slices > 1 ? align_up((size_t)p.slices * m * n * sizeof(float), 256) : 0;
 }
-// The rows' kernel, whose workgroup goes through the whole sum, or tiles, in slices where
-// those are few, which go through the weight at 6 TB/s (out of the caches; models of the
-// measured times in us).  Rows' kernel and tiles, bf16, 4096 columns over 2048: 1 row 4.9 and
-// 9.3, 16 5.8 and 10.1, 32 7.7 and 10.7, 64 12.1 and 10.4; 256 columns over 4096: 8 rows 7.5
-// and 10.0, 32 12.5 and 10.9.  float32, 64 columns over 4096: 1 row 11.8 and 9.6.
-bool few_rows(int m, int n, int k, int esize) {
-    if (m > 32) return false;
-    const double row = (double)k * esize;
-    return 4 + row / 1024 * (m <= 16 ? 0.5 : 1.15) < 9.3 + n * row / 6e6;
+// The rows' kernel, whose workgroup goes through the whole sum, for few rows or few columns
+// (with a workgroup for 16 of the others), or tiles, in slices where those are few: models of
+// the measured times in us.  Rows and tiles, bf16, 4096 columns over 2048: 1 row 4.9 and 9.3, 16
+// 5.8 and 10.1, 32 7.7 and 10.7, 64 12.1 and 10.4; 256 columns over 4096: 8 rows 7.5 and 10.0, 32
+// 12.5 and 10.9.  float32, 64 columns over 4096: 1 row 11.8 and 9.6.  Columns and tiles, bf16, over
+// 2048: 16 columns of 2048 rows 5.5 and 9.1, of 8192 9.4 and 11.6, of 65536 65 and 41; 32 of 8192
+// 13.4 and 12.1.  float32: 16 of 8192 18.9 and 25.1, 32 30 and 26.
+enum Few { FEW_NONE, FEW_ROWS, FEW_COLUMNS };
+Few few_of(int m, int n, int k, int esize) {
+    const double row = (double)k * esize, kb = row / 1024;
+    if (m <= 32) return 4 + kb * (m <= 16 ? 0.5 : 1.15) < 9.3 + n * row / 6e6 ? FEW_ROWS : FEW_NONE;
+    if (n > 32) return FEW_NONE;
+    const double rounds = ((m - 1) / 16 + 1) / 512.0, at_once = n <= 16 ? std::max(0.5, 1.5 * rounds) : std::max(1.15, 2.5 * rounds);
+    return 4 + kb * at_once * (esize == 4 ? 1.4 : 1) < 2.5 + plan_product(m, n, k, esize, false).cost ? FEW_COLUMNS : FEW_NONE;
 }
 
 template <int N>
@@ -831,13 +843,13 @@ int product(int m, int n, int k, const Operand& a, const Operand& b, void* c, co
 template <typename T>
 int forward(int m, int n, int k, const Operand& x, const Operand& w, void* y, const Epilogue& ep, float* partial,
             hipStream_t s) {
-    if (!few_rows(m, n, k, sizeof(T))) return product<T, false, false>(m, n, k, x, w, y, ep, partial, s);
-    const Args p{m, n, k, x, w, y, nullptr, 1, 0, ep};
-    const dim3 grid((unsigned)((n - 1) / 16 + 1));
-    if (m <= 16)
-        hipLaunchKernelGGL((rows_kernel<T, 1>), grid, dim3(512), 0, s, p);
-    else
-        hipLaunchKernelGGL((rows_kernel<T, 2>), grid, dim3(512), 0, s, p);
+    const Few few = few_of(m, n, k, sizeof(T));
+    if (few == FEW_NONE) return product<T, false, false>(m, n, k, x, w, y, ep, partial, s);
+    const bool swap = few == FEW_COLUMNS;
+    const Args p = swap ? Args{n, m, k, w, x, y, nullptr, 1, 0, ep} : Args{m, n, k, x, w, y, nullptr, 1, 0, ep};
+    const auto kernel = p.m <= 16 ? (swap ? &rows_kernel<T, 1, true> : &rows_kernel<T, 1, false>)
+                                  : (swap ? &rows_kernel<T, 2, true> : &rows_kernel<T, 2, false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n - 1) / 16 + 1)), dim3(512), 0, s, p);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
@@ -913,7 +925,7 @@ extern "C" {
 
 size_t rka_linear_forward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {
     const int esize = dtype == RKA_DTYPE_F32 ? 4 : 2;
-    if (rows < 1 || outputs < 1 || inputs < 1 || few_rows(rows, outputs, inputs, esize)) return 0;
+    if (rows < 1 || outputs < 1 || inputs < 1 || few_of(rows, outputs, inputs, esize) != FEW_NONE) return 0;
     return partial_bytes(rows, outputs, plan_product(rows, outputs, inputs, esize, false));
 }
 

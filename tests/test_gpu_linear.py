@@ -115,6 +115,13 @@ def test_few_rows(gpu, m, n, k, dtype):
     _check(gpu, m, n, k, dtype, "relu")
 
 
+# and few columns, on either side of its rule
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(33, 1, 64), (300, 8, 513), (2000, 16, 2048), (4096, 17, 1000), (70, 32, 200), (700, 33, 200)])
+def test_few_columns(gpu, m, n, k, dtype):
+    _check(gpu, m, n, k, dtype, "logsigmoid")
+
+
 @pytest.mark.parametrize("m,n,k", [(4100, 4104, 320), (16384, 1032, 64)])
 def test_aligned_large_tiles(gpu, m, n, k):
     _check(gpu, m, n, k, torch.bfloat16, "silu")
