@@ -49,12 +49,17 @@ struct Pair<bf16> {
     __device__ __forceinline__ float k() const { return __uint_as_float(here() & 0xffff0000u); }
 };
 
-// Sum over the 16 lanes that hold a row of a 16x16 block.
+// Sum over the 16 lanes that hold a row of a 16x16 block, by rotations within them (which
+// pass no LDS, as shuffles do).
+template <int N>
+__device__ __forceinline__ float rotate(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 1);
-    x += __shfl_xor(x, 2);
-    x += __shfl_xor(x, 4);
-    x += __shfl_xor(x, 8);
+    x += rotate<8>(x);
+    x += rotate<4>(x);
+    x += rotate<2>(x);
+    x += rotate<1>(x);
     return x;
 }
 
