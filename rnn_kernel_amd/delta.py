@@ -87,8 +87,10 @@ def _dense_heads(t: torch.Tensor) -> torch.Tensor:
 
 
 def _strides(q, k, v, g, beta):
+    """What the C entries take; ``v`` None: it is not read (the backward)."""
     if q.dim() == 4:
-        return (ctypes.c_longlong * 15)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
+        of_v = (0, 0, 0) if v is None else v.stride()[:3]
+        return (ctypes.c_longlong * 15)(*q.stride()[:3], *k.stride()[:3], *of_v, *g.stride(), *beta.stride())
     (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
     (gb, gh), (bb, bh) = g.stride(), beta.stride()
     return (ctypes.c_longlong * 15)(qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh, bb, 0, bh)
@@ -123,7 +125,6 @@ class GatedDeltaFunction(torch.autograd.Function):
         o, final_state, reserve = _forward(q, k, v, g, beta, initial_state, lengths, scale, normalize, training=True)
         ctx.save_for_backward(q, k, g, beta, lengths, reserve)
         ctx.sizes = (*q.shape[:3], v.size(2), q.size(3), v.size(3))
-        ctx.strides = _strides(q, k, v, g, beta)
         ctx.scale, ctx.normalize, ctx.has_state = scale, normalize, initial_state is not None
         ctx.set_materialize_grads(False)
         return o, final_state
@@ -131,7 +132,10 @@ class GatedDeltaFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_o, grad_state):
+        # (hooks may have given them back in another layout than they were saved in)
         q, k, g, beta, lengths, reserve = ctx.saved_tensors
+        q, k, reserve = _dense_heads(q), _dense_heads(k), reserve.contiguous()
+        lengths = None if lengths is None else lengths.contiguous()
         batch, tokens, _, value_heads, key_dim, value_dim = ctx.sizes
         lib, device = _lib.load(), q.device
         grad_o = None if grad_o is None else grad_o.contiguous()
@@ -147,7 +151,7 @@ class GatedDeltaFunction(torch.autograd.Function):
         _lib.call(_index_of(device), "rka_gated_delta_backward", q.data_ptr(), k.data_ptr(), g.data_ptr(),
                   beta.data_ptr(), _lib.ptr(lengths), reserve.data_ptr(), _lib.ptr(grad_o), _lib.ptr(grad_state),
                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), _lib.ptr(ds0),
-                  ws.data_ptr(), ws_bytes, *ctx.sizes, ctx.strides, _DTYPES[q.dtype], _DTYPES[g.dtype],
+                  ws.data_ptr(), ws_bytes, *ctx.sizes, _strides(q, k, None, g, beta), _DTYPES[q.dtype], _DTYPES[g.dtype],
                   int(ctx.normalize), ctx.scale)
         return dq, dk, dv, dg, dbeta, ds0, None, None, None
 

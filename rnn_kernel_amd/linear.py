@@ -102,7 +102,9 @@ class LinearFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
+        # (hooks may have given them back in another layout than they were saved in)
         xm, wm, z = ctx.saved_tensors
+        xm, wm, z = _rows(xm), _rows(wm), None if z is None else z.contiguous()
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         rows, outputs, inputs = xm.size(0), wm.size(0), wm.size(1)
         dx = torch.empty(ctx.shape, dtype=xm.dtype, device=xm.device) if need_x else None
