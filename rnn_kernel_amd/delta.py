@@ -100,9 +100,20 @@ def _bytes(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
 
 
-def _forward(q, k, v, g, beta, initial_state, lengths, scale: float, normalize: bool, training: bool):
-    lib = _lib.load()
+def _forward(q, k, v, g, beta, initial_state, lengths, scale: Optional[float], normalize: bool, training: bool):
+    """Checks, and the forward: o, final_state, what is saved if ``training``, and q, k,
+    lengths and scale as they were used."""
+    _check_inputs(q, k, v, g, beta, tokens=True)
     batch, tokens, key_heads, key_dim = q.shape
+    if initial_state is not None:
+        _check_state(initial_state, (batch, v.size(2), key_dim, v.size(3)), "initial_state", q.device)
+        initial_state = initial_state.contiguous()
+    if lengths is not None:
+        _check_ints(lengths, batch, "lengths", q.device)
+        lengths = lengths.contiguous()
+    scale = key_dim ** -0.5 if scale is None else float(scale)
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    lib = _lib.load()
     sizes = (batch, tokens, key_heads, v.size(2), key_dim, v.size(3))
     o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     final_state = torch.empty(batch, v.size(2), key_dim, v.size(3), dtype=torch.float32, device=v.device)
@@ -113,7 +124,7 @@ def _forward(q, k, v, g, beta, initial_state, lengths, scale: float, normalize: 
               beta.data_ptr(), _lib.ptr(initial_state), _lib.ptr(lengths), o.data_ptr(), final_state.data_ptr(),
               _lib.ptr(reserve), ws.data_ptr(), ws_bytes, *sizes, _strides(q, k, v, g, beta), _DTYPES[q.dtype],
               _DTYPES[g.dtype], int(normalize), scale)
-    return o, final_state, reserve
+    return o, final_state, reserve, (q, k, lengths, scale)
 
 
 class GatedDeltaFunction(torch.autograd.Function):
@@ -122,7 +133,8 @@ class GatedDeltaFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial_state, lengths, scale, normalize):
-        o, final_state, reserve = _forward(q, k, v, g, beta, initial_state, lengths, scale, normalize, training=True)
+        o, final_state, reserve, (q, k, lengths, scale) = _forward(q, k, v, g, beta, initial_state, lengths, scale,
+                                                                   normalize, training=True)
         ctx.save_for_backward(q, k, g, beta, lengths, reserve)
         ctx.sizes = (*q.shape[:3], v.size(2), q.size(3), v.size(3))
         ctx.scale, ctx.normalize, ctx.has_state = scale, normalize, initial_state is not None
@@ -173,20 +185,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     Tokens are taken in chunks of 64, so a NaN or an infinity in a token may reach
     the outputs of the earlier tokens of its chunk."""
-    _check_inputs(q, k, v, g, beta, tokens=True)
-    batch, _, _, key_dim = q.shape
-    if initial_state is not None:
-        _check_state(initial_state, (batch, v.size(2), key_dim, v.size(3)), "initial_state", q.device)
-        initial_state = initial_state.contiguous()
-    if lengths is not None:
-        _check_ints(lengths, batch, "lengths", q.device)
-        lengths = lengths.contiguous()
-    scale = key_dim ** -0.5 if scale is None else float(scale)
-    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, lengths, scale, normalize)
-    o, final_state, _ = _forward(q, k, v, g, beta, initial_state, lengths, scale, normalize, training=False)
-    return o, final_state
+    return _forward(q, k, v, g, beta, initial_state, lengths, scale, normalize, training=False)[:2]
 
 
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,

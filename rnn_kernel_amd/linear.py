@@ -69,7 +69,10 @@ def _bytes(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
 
 
-def _forward(x, weight, bias, residual, act: int, keep_z: bool):
+def _forward(x, weight, bias, residual, activation, keep_z: bool):
+    _check(x, weight, bias, residual, activation)
+    act = _ACTS[activation]
+    keep_z = keep_z and act != 0
     lib = _lib.load()
     xm, wm = _rows(x), _rows(weight)
     rows, outputs, inputs = xm.size(0), wm.size(0), wm.size(1)
@@ -93,10 +96,9 @@ class LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        act = _ACTS[activation]
-        y, z, xm, wm = _forward(x, weight, bias, residual, act, keep_z=act != 0 and any(ctx.needs_input_grad[:3]))
+        y, z, xm, wm = _forward(x, weight, bias, residual, activation, keep_z=any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(xm, wm, z)
-        ctx.act, ctx.shape = act, x.shape
+        ctx.act, ctx.shape = _ACTS[activation], x.shape
         return y
 
     @staticmethod
@@ -131,10 +133,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     one of ACTIVATIONS (gelu is the one with the error function) or None.  Rows may
     be any distance (up to 2^21 elements) apart.  Sums, bias, activation and residual
     are in float32; y is rounded once."""
-    _check(x, weight, bias, residual, activation)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, activation)
-    return _forward(x, weight, bias, residual, _ACTS[activation], keep_z=False)[0]
+    return _forward(x, weight, bias, residual, activation, keep_z=False)[0]
 
 
 class Linear(nn.Module):
