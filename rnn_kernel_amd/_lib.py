@@ -121,6 +121,21 @@ def ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def refuse_tangents(what: str, *tensors) -> None:
+    """RuntimeError if one of ``tensors`` (or None) carries a forward-mode tangent, which the
+    library's results would be without."""
+    global _forward_ad
+    if _forward_ad is None:
+        from torch.autograd import forward_ad as _forward_ad
+    # (a level below 0: there are no tangents; where torch does not say, every tensor is asked)
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
+_forward_ad = None
+
+
 def raw_stream(index: int) -> int:
     """Handle of torch's current stream on CUDA device ``index`` (without
     building a Stream object, where torch offers that)."""

@@ -185,6 +185,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     Tokens are taken in chunks of 64, so a NaN or an infinity in a token may reach
     the outputs of the earlier tokens of its chunk."""
+    _lib.refuse_tangents("gated_delta_rule", q, k, v, g, beta, initial_state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, lengths, scale, normalize)
     return _forward(q, k, v, g, beta, initial_state, lengths, scale, normalize, training=False)[:2]
@@ -201,6 +202,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     request without a state (padding): its output is 0; a slot from N up gives NaN;
     neither touches a state.  No gradients: with grad mode on, inputs that require
     them are refused."""
+    _lib.refuse_tangents("gated_delta_step", q, k, v, g, beta, state)
     _check_inputs(q, k, v, g, beta, tokens=False)
     batch, _, key_dim = q.shape
     if state.dim() != 4:

@@ -133,6 +133,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     one of ACTIVATIONS (gelu is the one with the error function) or None.  Rows may
     be any distance (up to 2^21 elements) apart.  Sums, bias, activation and residual
     are in float32; y is rounded once."""
+    _lib.refuse_tangents("linear", x, weight, bias, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, activation)
     return _forward(x, weight, bias, residual, activation, keep_z=False)[0]
