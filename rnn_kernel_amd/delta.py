@@ -223,6 +223,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
               beta.data_ptr(), state.data_ptr(), _lib.ptr(slots), state.size(0), o.data_ptr(), batch, q.size(1),
               v.size(1), key_dim, v.size(2), _strides(q, k, v, g, beta), _DTYPES[q.dtype], _DTYPES[g.dtype],
               int(normalize), key_dim ** -0.5 if scale is None else float(scale))
+    torch.autograd.graph.increment_version(state)  # (a graph that saved it would be wrong)
     return o
 
 
