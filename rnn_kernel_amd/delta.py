@@ -24,6 +24,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 MAX_KEY_DIM = 256
+MAX_SIZE = 2 ** 31 - 1  # of a dimension: the library takes them as 32-bit integers
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -60,6 +61,9 @@ def _check_inputs(q, k, v, g, beta, tokens: bool) -> None:
         raise ValueError("gated delta rule: v's heads must be a multiple of q's and k's")
     if not 1 <= qs[-1] <= MAX_KEY_DIM or vs[-1] < 1:
         raise ValueError(f"gated delta rule: key dim must be in [1, {MAX_KEY_DIM}] and value dim at least 1")
+    # (a size that large shows in the number of elements, or is hidden by a size of 0)
+    if not (0 < q.numel() <= MAX_SIZE and 0 < v.numel() <= MAX_SIZE) and max(*qs, *vs) > MAX_SIZE:
+        raise ValueError("gated delta rule: sizes must be below 2^31")
     gates = vs[:-1]
     if g.shape != gates or beta.shape != gates:
         raise ValueError("gated delta rule: g and beta must have v's shape without its last dimension")
@@ -208,6 +212,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     if state.dim() != 4:
         raise ValueError("gated delta rule: state must have shape [slots, heads, key dim, value dim]")
     _check_state(state, (state.size(0), v.size(1), key_dim, v.size(2)), "state", q.device)
+    if state.size(0) > MAX_SIZE:
+        raise ValueError("gated delta rule: sizes must be below 2^31")
     if not state.is_contiguous():
         raise ValueError("gated delta rule: state must be contiguous")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):

@@ -21,6 +21,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+MAX_SIZE = 2 ** 31 - 1  # of rows, inputs and outputs: the library takes them as 32-bit integers
 ACTIVATIONS = ("none", "relu", "gelu", "silu", "sigmoid", "logsigmoid")
 _ACTS = {name: i for i, name in enumerate(ACTIVATIONS)}
 _ACTS[None] = 0
@@ -59,6 +60,8 @@ def _check(x, weight, bias, residual, activation) -> None:
         raise ValueError("linear: weight must have shape [outputs, inputs]")
     if x.dim() < 1 or x.size(-1) != weight.size(1):
         raise ValueError(f"linear: x must have shape [..., {weight.size(1)}]")
+    if (x.numel() > MAX_SIZE or weight.numel() > MAX_SIZE) and max(x.numel() // x.size(-1), *weight.shape) > MAX_SIZE:
+        raise ValueError("linear: rows, inputs and outputs must be below 2^31")
     if bias is not None and bias.shape != (weight.size(0),):
         raise ValueError(f"linear: bias must have shape [{weight.size(0)}]")
     if residual is not None and residual.shape != (*x.shape[:-1], weight.size(0)):
