@@ -463,6 +463,16 @@ int rka_linear_backward(const void* grad_y, long long ldy, const void* x, long l
                         const void* z, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                         size_t workspace_bytes, int rows, int outputs, int inputs, int act, int dtype, void* stream);
 
+/* The form that a product of these calls takes (host only), for tests and tuning.
+ * `product`: 0 for x W^T, 1 for grad_x, 2 for grad_weight; `aligned`: whether addresses
+ * and row strides are multiples of 16 bytes.  Writes the first min(n_out, 4) of {form, edge
+ * of a tile, slices of the sum, workgroups}. */
+#define RKA_LINEAR_FORM_ROWS 0    /* 16 columns to a workgroup, at most 32 rows */
+#define RKA_LINEAR_FORM_COLUMNS 1 /* 16 rows to a workgroup, at most 32 columns */
+#define RKA_LINEAR_FORM_DIRECT 2  /* tiles, operands from memory to LDS */
+#define RKA_LINEAR_FORM_TILES 3   /* tiles, operands through registers */
+int rka_describe_linear(int product, int rows, int outputs, int inputs, int dtype, int aligned, int* out, int n_out);
+
 #ifdef __cplusplus
 }
 #endif

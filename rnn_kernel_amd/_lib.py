@@ -70,6 +70,7 @@ SIGNATURES = {
     "rka_linear_backward_workspace_bytes": (_SZ, [_I] * 4),
     "rka_linear_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
     "rka_linear_backward": (_I, [_P, _LL, _P, _LL, _P, _LL] + [_P] * 5 + [_SZ] + [_I] * 5 + [_P]),
+    "rka_describe_linear": (_I, [_I] * 6 + [ctypes.POINTER(_I), _I]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
 }
 NUM_STAGES = 6
@@ -228,6 +229,19 @@ def describe_weight_gradients(batch: int, seq_len: int, input_size: int, hidden:
     check(load().rka_describe_weight_gradients(batch, seq_len, input_size, hidden, out, 4),
           "rka_describe_weight_gradients")
     return dict(form=GEMM_FORMS[out[0]], slices_hh=out[1], slices_ih=out[2], direct=bool(out[3]))
+
+
+LINEAR_FORMS = {0: "rows", 1: "columns", 2: "direct", 3: "tiles"}
+LINEAR_PRODUCTS = {"y": 0, "grad_x": 1, "grad_weight": 2}
+
+
+def describe_linear(product: str, rows: int, outputs: int, inputs: int, dtype: int, aligned: bool = True) -> dict:
+    """Form, tile edge, slices and workgroups of one of a linear layer's products;
+    see rka_describe_linear."""
+    out = (ctypes.c_int * 4)()
+    check(load().rka_describe_linear(LINEAR_PRODUCTS[product], rows, outputs, inputs, dtype, int(aligned), out, 4),
+          "rka_describe_linear")
+    return dict(form=LINEAR_FORMS[out[0]], edge=out[1], slices=out[2], workgroups=out[3])
 
 
 def set_exchange_stores(mode: int) -> None:

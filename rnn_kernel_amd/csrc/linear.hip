@@ -580,9 +580,10 @@ __global__ __launch_bounds__(256) void slices_kernel(Args p) {
 // between calls): 5.7 us.
 // SWAP: few columns instead, 16 rows of x per workgroup: a is the weight, b is x, and the
 // output is written the other way round.
+constexpr int kRowsThreads = 512;
 template <typename T, int MT, bool SWAP>
-__global__ __launch_bounds__(512) void rows_kernel(Args p) {
-    constexpr int kV = kVec<T>, kK = 4 * kV, kWaves = 8, kDeep = 4;
+__global__ __launch_bounds__(kRowsThreads) void rows_kernel(Args p) {
+    constexpr int kV = kVec<T>, kK = 4 * kV, kWaves = kRowsThreads / 64, kDeep = 4;
     __shared__ float sums[kWaves][MT][16][17];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, i16 = lane % 16, hi = lane / 16;
     const int n0 = blockIdx.x * 16;
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(512) void rows_kernel(Args p) {
     __syncthreads();
     Args out = p;
     if (SWAP) out.n = p.m;
-    for (int i = threadIdx.x; i < MT * 256; i += 512) {
+    for (int i = threadIdx.x; i < MT * 256; i += kRowsThreads) {
         const int t = SWAP ? i / 16 % MT : i / 256, r = SWAP ? i % 16 : i / 16 % 16, c = SWAP ? i / (16 * MT) : i % 16;
         if (16 * t + r >= p.m || n0 + c >= p.n) continue;
         float sum[1] = {0.f};
@@ -728,6 +729,7 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* sums, int ranges
 
 // ------------------------------------------------------------- choices ---
 enum Tile { TILE_256, TILE_128, TILE_64 };
+constexpr long long kLaunchThreads = 1LL << 32;  // a launch has fewer
 struct Plan {
     Tile tile;
     int slices, stages;
@@ -746,16 +748,17 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
     const int kk = kRowBytes / esize, all = std::max(1, (k + kk - 1) / kk);
     struct Cost {
         Tile tile;
-        int edge;
+        int edge, threads;
         double share, least, work, turn, f32;
     };
     static const Cost costs[] = {
-        {TILE_256, 256, 1, 1.8, 1.8, 1.2, 4}, {TILE_128, 128, 2, 0.7, 0.55, 1.2, 3.1}, {TILE_64, 64, 4, 0.35, 0.165, 1.25, 2.95}};
+        {TILE_256, 256, 512, 1, 1.8, 1.8, 1.2, 4}, {TILE_128, 128, 256, 2, 0.7, 0.55, 1.2, 3.1}, {TILE_64, 64, 256, 4, 0.35, 0.165, 1.25, 2.95}};
     Plan best{TILE_64, 1, all, 1e30};
     for (const Cost& c : costs) {
         const double tiles = (double)((m - 1) / c.edge + 1) * ((n - 1) / c.edge + 1);
         for (int want = 1; want <= 64 && want <= all; want *= 2) {
             const int stages = (all + want - 1) / want, slices = (all + stages - 1) / stages;
+            if (tiles * slices * c.threads >= kLaunchThreads) continue;
             const double to_a_cu = std::ceil(tiles * slices / 256), rounds = std::floor(to_a_cu / c.share), rest = to_a_cu - rounds * c.share;
             double stage = rounds * std::max(c.least, c.share * c.work) + (rest > 0 ? std::max(c.least, rest * c.work) : 0);
             if (across) stage *= c.turn;
@@ -778,13 +781,18 @@ size_t partial_bytes(int m, int n, const Plan& p) {
 // 2048: 16 columns of 2048 rows 5.5 and 9.1, of 8192 9.4 and 11.6, of 65536 65 and 41; 32 of 8192
 // 13.4 and 12.1.  float32: 16 of 8192 18.9 and 25.1, 32 30 and 26.
 enum Few { FEW_NONE, FEW_ROWS, FEW_COLUMNS };
+// (tiles also where a launch may not have a workgroup for 16 of the others)
 Few few_of(int m, int n, int k, int esize) {
+    if ((long long)((m <= 32 ? n : m) - 1) / 16 + 1 >= kLaunchThreads / kRowsThreads) return FEW_NONE;
     const double row = (double)k * esize, kb = row / 1024;
     if (m <= 32) return 4 + kb * (m <= 16 ? 0.5 : 1.15) < 9.3 + n * row / 6e6 ? FEW_ROWS : FEW_NONE;
     if (n > 32) return FEW_NONE;
     const double rounds = ((m - 1) / 16 + 1) / 512.0, at_once = n <= 16 ? std::max(0.5, 1.5 * rounds) : std::max(1.15, 2.5 * rounds);
     return 4 + kb * at_once * (esize == 4 ? 1.4 : 1) < 2.5 + plan_product(m, n, k, esize, false).cost ? FEW_COLUMNS : FEW_NONE;
 }
+
+// Whether a sum is whole stages, which direct_kernel takes.
+bool whole_stages(int k, int esize) { return k % (kRowBytes / esize) == 0; }
 
 template <int N>
 using Int = std::integral_constant<int, N>;
@@ -794,7 +802,7 @@ int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
     auto go = [&](auto kernel, bool direct, int edge, int wm, int wn) {
         const int threads = edge / wm * edge / wn * 64;
         const long long blocks = (long long)((p.m - 1) / edge + 1) * ((p.n - 1) / edge + 1) * p.slices;
-        if (blocks * threads >= (1LL << 32)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, "linear: more workgroups than a launch may have");
+        if (blocks * threads >= kLaunchThreads) return fail(RKA_ERR_UNSUPPORTED_SHAPE, "linear: more workgroups than a launch may have");
         const size_t lds = direct ? 0 : std::max<size_t>((size_t)4 * edge * kRowBytes, (size_t)threads / 64 * 32 * (wn + 4) * 4);
         if (lds > (64 << 10))
             RKA_RETURN_IF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
@@ -818,7 +826,7 @@ int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
     bool done = false;
     if constexpr (!A && !B) {
         const auto on16 = [](const Operand& o) { return (reinterpret_cast<uintptr_t>(o.ptr) | (size_t)o.ld * sizeof(T)) % 16 == 0; };
-        if (p.k % (8 * kVec<T>) == 0 && on16(p.a) && on16(p.b)) {
+        if (whole_stages(p.k, sizeof(T)) && on16(p.a) && on16(p.b)) {
             RKA_RETURN_IF_ERR(either(std::true_type{}));
             done = true;
         }
@@ -849,7 +857,7 @@ int forward(int m, int n, int k, const Operand& x, const Operand& w, void* y, co
     const Args p = swap ? Args{n, m, k, w, x, y, nullptr, 1, 0, ep} : Args{m, n, k, x, w, y, nullptr, 1, 0, ep};
     const auto kernel = p.m <= 16 ? (swap ? &rows_kernel<T, 1, true> : &rows_kernel<T, 1, false>)
                                   : (swap ? &rows_kernel<T, 2, true> : &rows_kernel<T, 2, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n - 1) / 16 + 1)), dim3(512), 0, s, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n - 1) / 16 + 1)), dim3(kRowsThreads), 0, s, p);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
@@ -932,6 +940,30 @@ size_t rka_linear_forward_workspace_bytes(int rows, int outputs, int inputs, int
 size_t rka_linear_backward_workspace_bytes(int rows, int outputs, int inputs, int dtype) {
     if (rows < 1 || outputs < 1 || inputs < 1) return 0;
     return backward_layout(rows, outputs, inputs, dtype == RKA_DTYPE_F32 ? 4 : 2).total;
+}
+
+int rka_describe_linear(int product, int rows, int outputs, int inputs, int dtype, int aligned, int* out, int n_out) {
+    clear_error();
+    if (product < 0 || product > 2 || !out || n_out < 1)
+        return fail(RKA_ERR_INVALID_ARGUMENT, "describe_linear: product must be 0, 1 or 2, out non-NULL and n_out >= 1");
+    RKA_RETURN_IF_ERR(check("describe_linear", rows, outputs, inputs, 0, 0, 0, RKA_ACT_NONE, dtype));
+    const int esize = dtype == RKA_DTYPE_F32 ? 4 : 2;
+    const int m = product == 2 ? outputs : rows, n = product == 0 ? outputs : inputs;
+    const int k = product == 0 ? inputs : product == 1 ? outputs : rows;
+    const Few few = product == 0 ? few_of(m, n, k, esize) : FEW_NONE;
+    int v[4] = {few == FEW_ROWS ? RKA_LINEAR_FORM_ROWS : RKA_LINEAR_FORM_COLUMNS, 16, 1,
+                ((few == FEW_ROWS ? n : m) - 1) / 16 + 1};
+    if (few == FEW_NONE) {
+        const Plan p = plan_product(m, n, k, esize, product != 0);
+        const int edge = p.tile == TILE_256 ? 256 : p.tile == TILE_128 ? 128 : 64;
+        const long long blocks = (long long)((m - 1) / edge + 1) * ((n - 1) / edge + 1) * p.slices;
+        v[0] = product == 0 && aligned && whole_stages(k, esize) ? RKA_LINEAR_FORM_DIRECT : RKA_LINEAR_FORM_TILES;
+        v[1] = edge;
+        v[2] = p.slices;
+        v[3] = (int)std::min<long long>(blocks, 0x7fffffff);
+    }
+    for (int i = 0; i < 4 && i < n_out; ++i) out[i] = v[i];
+    return 0;
 }
 
 int rka_linear_forward(const void* x, long long ldx, const void* weight, long long ldw, const void* bias,
