@@ -920,7 +920,7 @@ int check(const char* what, int m, int n, int k, long long ld0, long long ld1, l
     // a tile's 32-bit offsets: 256 rows of a leading dimension
     constexpr long long kMost = 1LL << 21;
     for (const long long ld : {ld0, ld1, ld2, (long long)n, (long long)k})
-        if (ld < 0 || ld > kMost) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": row strides must be at most 2^21 elements");
+        if (ld < 0 || ld > kMost) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": row strides, inputs and outputs must be at most 2^21 elements");
     return 0;
 }
 

@@ -22,6 +22,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MAX_SIZE = 2 ** 31 - 1  # of rows, inputs and outputs: the library takes them as 32-bit integers
+MAX_ROW_STRIDE = 2 ** 21  # elements: the kernels' offsets within a tile are 32-bit
 ACTIVATIONS = ("none", "relu", "gelu", "silu", "sigmoid", "logsigmoid")
 _ACTS = {name: i for i, name in enumerate(ACTIVATIONS)}
 _ACTS[None] = 0
@@ -32,11 +33,14 @@ def _index_of(device) -> int:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as a matrix whose rows are dense (any distance apart)."""
+    """``t`` as a matrix whose rows are dense and at most MAX_ROW_STRIDE apart: a copy where
+    they are not."""
     if t.dim() == 2 and t.is_contiguous():
         return t
     m = t if t.dim() == 2 else t.reshape(-1, t.size(-1))
-    return m if (m.size(1) == 1 or m.stride(1) == 1) and (m.size(0) <= 1 or m.stride(0) >= m.size(1)) else m.contiguous()
+    if (m.size(1) == 1 or m.stride(1) == 1) and (m.size(0) <= 1 or m.size(1) <= m.stride(0) <= MAX_ROW_STRIDE):
+        return m
+    return m.contiguous()
 
 
 def _ld(m: torch.Tensor) -> int:
@@ -62,6 +66,8 @@ def _check(x, weight, bias, residual, activation) -> None:
         raise ValueError(f"linear: x must have shape [..., {weight.size(1)}]")
     if (x.numel() > MAX_SIZE or weight.numel() > MAX_SIZE) and max(x.numel() // x.size(-1), *weight.shape) > MAX_SIZE:
         raise ValueError("linear: rows, inputs and outputs must be below 2^31")
+    if weight.numel() > MAX_ROW_STRIDE and max(weight.shape) > MAX_ROW_STRIDE:
+        raise ValueError("linear: inputs and outputs must be at most 2^21")
     if bias is not None and bias.shape != (weight.size(0),):
         raise ValueError(f"linear: bias must have shape [{weight.size(0)}]")
     if residual is not None and residual.shape != (*x.shape[:-1], weight.size(0)):
@@ -133,9 +139,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x W^T + b) + r:  x [..., inputs], weight [outputs, inputs], bias [outputs]
     or None, residual [..., outputs] or None, all float32 or all bfloat16; activation
-    one of ACTIVATIONS (gelu is the one with the error function) or None.  Rows may
-    be any distance (up to 2^21 elements) apart.  Sums, bias, activation and residual
-    are in float32; y is rounded once."""
+    one of ACTIVATIONS (gelu is the one with the error function) or None.  Inputs
+    and outputs are at most 2^21.  Rows may be any distance apart (more than 2^21 elements:
+    they are copied).  Sums, bias, activation and residual are in float32; y is rounded
+    once."""
     _lib.refuse_tangents("linear", x, weight, bias, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, activation)
