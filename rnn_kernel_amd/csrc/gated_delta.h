@@ -166,11 +166,20 @@ __device__ __forceinline__ f32x4 mul(const u32x4 (&a)[NA], const u32x4 (&b)[NB],
     return c;
 }
 
-// Waits until the last product of a sum is in its registers.  The compiler counts the
-// wait states between a matrix instruction and the reader of its result only within a
-// basic block (clang 22 of ROCm 7.2; where a branch came between, the reader saw the old
-// value now and then), so every sum that is read behind a branch ends with this.
+// Waits until the last product of a sum is in its registers.  Between a matrix
+// instruction and the reader of its result the compiler (clang 22 of ROCm 7.2) counts the
+// wait states on most paths, but has missed some that pass a branch: there the reader
+// came after one state instead of eight and saw the old value now and then.  So every sum
+// that is read in another basic block than its last product's ends with this.
 __device__ __forceinline__ void settle(f32x4& c) { asm volatile("s_nop 9" : "+v"(c)); }
+// The same, right behind the product, for sums that may be in accumulation registers: an
+// operand of it would be copied out of them before the wait, and behind a branch they may
+// have been copied already.
+__device__ __forceinline__ void settle_all() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 9" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // A value that is made whether or not it is used: without this the compiler puts loads
 // and exponentials whose result is then selected away under branches, one each.

@@ -172,6 +172,7 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
             for (int i = 0; i < NP; ++i) y[i] = fk[((j * steps + u) * NP + i) * kFragLanes];
             kk[j] = mul(a, y, kk[j]);
             qk[j] = mul(aq, y, qk[j]);
+            settle_all();
         }
     }
     __syncthreads();
@@ -232,8 +233,12 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
         f32x4 sum{};
         for (int m = 0; m <= i; ++m) {
             f32x4 y{};
-            for (int l = j; l < 2; ++l) y = block_product(at(nb, 2 + m, l), at(ti, l, j), n, hi, y);
+            for (int l = j; l < 2; ++l) {
+                y = block_product(at(nb, 2 + m, l), at(ti, l, j), n, hi, y);
+                settle_all();
+            }
             sum = block_product(at(ti, 2 + i, 2 + m), y, n, hi, sum);
+            settle_all();
         }
         put_result(at(ti, 2 + i, j), -sum, n, hi);
     }
@@ -275,7 +280,10 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, c
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             m[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int l = j; l <= wave; ++l) m[j] = block_product(at(nb, wave, l), at(ti, l, j), n, hi, m[j]);
+            for (int l = j; l <= wave; ++l) {
+                m[j] = block_product(at(nb, wave, l), at(ti, l, j), n, hi, m[j]);
+                settle_all();
+            }
         }
         __syncthreads();
 #pragma unroll

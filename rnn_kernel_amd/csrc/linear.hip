@@ -277,6 +277,17 @@ __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
     }
 }
 
+// Waits until the last products of a wavefront's sums are in their registers, before sums
+// are stored in another basic block than their last product's: between a matrix instruction
+// and the reader of its result the compiler has missed wait states on paths that pass a
+// branch.  18 states, what 32x32x2 float32 asks for, the most of those here.  (The sums are
+// no operands of it: that copies them out of accumulation registers, before the wait.)
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 1" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // Results of V neighbouring columns, with the epilogue.
 template <typename T, int V>
 __device__ __forceinline__ void finish(const Args& p, long long row, int col, const float (&sum)[V]) {
@@ -436,6 +447,7 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(Args p) {
         }
         __syncthreads();
     }
+    settle();
     put_out<T, WM, WN>(p, acc, reinterpret_cast<float*>(lds + wave * kOutBytes<WN>), m0 + wm, n0 + wn, slice);
 }
 
@@ -535,8 +547,12 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(Args p) 
     }
     if (s + 1 < stages) load(odd, s + 1, 0, kLoads);
     compute(even, nullptr, 0);
+    settle();
     arrive();
-    if (s + 1 < stages) compute(odd, nullptr, 0);
+    if (s + 1 < stages) {
+        compute(odd, nullptr, 0);
+        settle();
+    }
     __syncthreads();
     float* out = reinterpret_cast<float*>((wave < W / 2 ? even : odd) + wave % (W / 2) * kOutBytes<WN>);
     put_out<T, WM, WN>(p, acc, out, m0 + wm, n0 + wn, slice);
@@ -629,6 +645,7 @@ __global__ __launch_bounds__(kRowsThreads) void rows_kernel(Args p) {
                 }
             }
     }
+    settle();
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
