@@ -768,10 +768,13 @@ Plan plan_product(int m, int n, int k, int esize, bool across) {
         int edge, threads;
         double share, least, work, turn, f32;
     };
-    static const Cost costs[] = {
-        {TILE_256, 256, 512, 1, 1.8, 1.8, 1.2, 4}, {TILE_128, 128, 256, 2, 0.7, 0.55, 1.2, 3.1}, {TILE_64, 64, 256, 4, 0.35, 0.165, 1.25, 2.95}};
+    // (float32: four 128 tiles, two to a CU, are faster than a 256 tile at any count)
+    static const Cost costs[] = {{TILE_256, 256, 512, 1, 1.8, 1.8, 1.2, 0},
+                                 {TILE_128, 128, 256, 2, 0.7, 0.55, 1.2, 3.1},
+                                 {TILE_64, 64, 256, 4, 0.35, 0.165, 1.25, 2.95}};
     Plan best{TILE_64, 1, all, 1e30};
     for (const Cost& c : costs) {
+        if (esize == 4 && c.tile == TILE_256) continue;
         const double tiles = (double)((m - 1) / c.edge + 1) * ((n - 1) / c.edge + 1);
         for (int want = 1; want <= 64 && want <= all; want *= 2) {
             const int stages = (all + want - 1) / want, slices = (all + stages - 1) / stages;
@@ -836,7 +839,8 @@ int launch_tiles(const Args& p, Tile tile, hipStream_t s) {
             else
                 return &tile_kernel<T, BM, BM, WM, WN, A, B>;
         };
-        if (tile == TILE_256) return go(kernel(Int<256>{}, Int<128>{}, Int<64>{}), D, 256, 128, 64);
+        if constexpr (sizeof(T) == 2)
+            if (tile == TILE_256) return go(kernel(Int<256>{}, Int<128>{}, Int<64>{}), D, 256, 128, 64);
         if (tile == TILE_128) return go(kernel(Int<128>{}, Int<64>{}, Int<64>{}), D, 128, 64, 64);
         return go(kernel(Int<64>{}, Int<32>{}, Int<32>{}), D, 64, 32, 32);
     };
