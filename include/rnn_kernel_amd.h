@@ -434,6 +434,11 @@ int rka_gated_delta_step(const void* q, const void* k, const void* v, const void
                          int key_dim, int value_dim, const long long* strides, int dtype, int gate_dtype, int normalize,
                          double scale, void* stream);
 
+/* The form that the chain over a call's chunks takes (host only), for tests and tuning.
+ * Writes the first min(n_out, 3) of {32-wide steps over key_dim, blocks of 16 columns of a
+ * state per workgroup, workgroups}. */
+int rka_describe_gated_delta(int batch, int value_heads, int key_dim, int value_dim, int dtype, int* out, int n_out);
+
 /*
  * The matrix product with its epilogue, y = act(x W^T + b) + r: x [rows, inputs],
  * W [outputs, inputs], b [outputs] or NULL, r [rows, outputs] or NULL and y [rows,

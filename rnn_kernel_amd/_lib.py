@@ -70,6 +70,7 @@ SIGNATURES = {
     "rka_linear_backward_workspace_bytes": (_SZ, [_I] * 4),
     "rka_linear_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
     "rka_linear_backward": (_I, [_P, _LL, _P, _LL, _P, _LL] + [_P] * 5 + [_SZ] + [_I] * 5 + [_P]),
+    "rka_describe_gated_delta": (_I, [_I] * 5 + [ctypes.POINTER(_I), _I]),
     "rka_describe_linear": (_I, [_I] * 6 + [ctypes.POINTER(_I), _I]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
 }
@@ -229,6 +230,15 @@ def describe_weight_gradients(batch: int, seq_len: int, input_size: int, hidden:
     check(load().rka_describe_weight_gradients(batch, seq_len, input_size, hidden, out, 4),
           "rka_describe_weight_gradients")
     return dict(form=GEMM_FORMS[out[0]], slices_hh=out[1], slices_ih=out[2], direct=bool(out[3]))
+
+
+def describe_gated_delta(batch: int, value_heads: int, key_dim: int, value_dim: int, dtype: int) -> dict:
+    """Steps, column blocks per workgroup and workgroups of the gated delta rule's
+    chains; see rka_describe_gated_delta."""
+    out = (ctypes.c_int * 3)()
+    check(load().rka_describe_gated_delta(batch, value_heads, key_dim, value_dim, dtype, out, 3),
+          "rka_describe_gated_delta")
+    return dict(steps=out[0], columns=out[1], workgroups=out[2])
 
 
 LINEAR_FORMS = {0: "rows", 1: "columns", 2: "direct", 3: "tiles"}

@@ -327,6 +327,23 @@ struct BackwardData {
     float* dx;            // [B][T][Hv][Dv]
 };
 
+// Blocks of 16 columns that a chain's workgroup takes, one or two.  Two halve what is read
+// of K, Q, T and P per column, one has the shorter chain: two where one to a workgroup would
+// not have a CU for each.  Measured, the whole forward in us with one and two (bf16,
+// 128x128): 256 workgroups of one (2048 tokens) 113 and 131, 320 163 and 140, 512 260 and
+// 225, 1024 (1024 tokens) 325 and 230; 128 (16384 tokens) 690 and 810.  float32 (512
+// tokens): 256 57 and 61, 384 84 and 71.  (Float32 operands of the largest Dk leave no
+// registers for two.)
+inline int chain_columns(const Dims& d, int pieces) {
+    constexpr int kCus = 256;
+    if (pieces > 1 && chain_steps(d.Dk) == 8) return 1;
+    return d.Dv > 16 && (long long)d.B * d.Hv * column_blocks(d.Dv) > kCus ? 2 : 1;
+}
+// A chain's workgroups with that many blocks each (grid: 8 x heads per XCD x blocks).
+inline long long chain_blocks(const Dims& d, int columns) {
+    return (((long long)d.B * d.Hv + 7) / 8) * 8 * ((d.Dv - 1) / (16 * columns) + 1);
+}
+
 // The launches below take lengths == nullptr for rows of T tokens each.
 // states, e: saved for the backward, or both null.
 template <typename T>

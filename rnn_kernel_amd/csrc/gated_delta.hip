@@ -542,6 +542,19 @@ size_t rka_gated_delta_backward_workspace_bytes(int batch, int tokens, int key_h
     return backward_layout(d, dtype == RKA_DTYPE_F32).total;
 }
 
+int rka_describe_gated_delta(int batch, int value_heads, int key_dim, int value_dim, int dtype, int* out, int n_out) {
+    clear_error();
+    if (!out || n_out < 1) return fail(RKA_ERR_INVALID_ARGUMENT, "describe_gated_delta: out must be non-NULL and n_out >= 1");
+    if (dtype != RKA_DTYPE_F32 && dtype != RKA_DTYPE_BF16)
+        return fail(RKA_ERR_INVALID_ARGUMENT, "describe_gated_delta: dtype must be RKA_DTYPE_F32 or RKA_DTYPE_BF16");
+    Dims d;
+    RKA_RETURN_IF_ERR(make_dims("describe_gated_delta", batch, 0, 1, value_heads, key_dim, value_dim, &d));
+    const int columns = chain_columns(d, dtype == RKA_DTYPE_F32 ? kPieces<float> : kPieces<bf16>);
+    const int v[3] = {chain_steps(d.Dk), columns, (int)std::min<long long>(chain_blocks(d, columns), 0x7fffffff)};
+    for (int i = 0; i < 3 && i < n_out; ++i) out[i] = v[i];
+    return 0;
+}
+
 int rka_gated_delta_forward(const void* q, const void* k, const void* v, const void* g, const void* beta,
                             const float* initial_state, const int* lengths, void* o, float* final_state, void* reserve,
                             void* workspace, size_t workspace_bytes, int batch, int tokens, int key_heads,

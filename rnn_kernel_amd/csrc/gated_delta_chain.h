@@ -74,9 +74,6 @@ __device__ __forceinline__ bool head_and_block(int heads, int* bh, int* blk) {
     *blk = i / per;
     return *bh < heads;
 }
-inline long long chain_blocks(const Dims& d, int nc) {
-    return (((long long)d.B * d.Hv + 7) / 8) * 8 * ((d.Dv - 1) / (16 * nc) + 1);
-}
 
 // What both directions share of a workgroup's place.
 template <int KU, int NC>
@@ -614,18 +611,11 @@ __global__ __launch_bounds__(kChainThreads, 1) void chain_backward_kernel(Dims d
 }
 
 // Calls f with the chain's steps over Dk and its column blocks as integral constants.
-// Two blocks halve what is read of K, Q, T and P per column, one has the shorter chain:
-// two where one to a workgroup would not have a CU for each.  Measured, the whole forward
-// in us with one and two (bf16, 128x128): 256 workgroups of one (2048 tokens) 113 and 131,
-// 320 163 and 140, 512 260 and 225, 1024 (1024 tokens) 325 and 230; 128 (16384 tokens) 690
-// and 810.  float32 (512 tokens): 256 57 and 61, 384 84 and 71.  (Float32 operands of the
-// largest Dk leave no registers for two.)
 template <typename T, typename F>
 int with_chain(const Dims& d, F f) {
-    constexpr int kCus = 256;
-    const bool two = d.Dv > 16 && (long long)d.B * d.Hv * ((d.Dv + 15) / 16) > kCus;
+    const bool two = chain_columns(d, kPieces<T>) == 2;
     auto pick = [&](auto ku) {
-        if constexpr (kPieces<T> == 1 || decltype(ku)::value < 8)
+        if constexpr (kPieces<T> == 1 || decltype(ku)::value < 8)  // (as chain_columns has it)
             if (two) return f(ku, std::integral_constant<int, 2>{});
         return f(ku, std::integral_constant<int, 1>{});
     };
