@@ -38,9 +38,11 @@
 // (24 bits in three rounded pieces of 8), a bf16 is one; of the products of pieces
 // those up to 2^-16 of the largest are taken, smallest first, each exact and summed in
 // float32: three where one operand is bf16, six where neither is.  The error is that
-// of a float32 product (lower pieces of numbers under some 2^-110 are lost).  One
-// 16x16x32 bf16 instruction takes 16 clocks, the eight 16x16x4 float32 ones for the same
-// block 256.
+// of a float32 product (lower pieces of numbers under some 2^-110 are lost; a number past
+// bf16's largest, 3.39e38, has no first piece and becomes NaN, as an infinity does).  What
+// only reaches a bf16 o is taken in two pieces of S, E and P: 16 bits, of which o keeps 8.
+// One 16x16x32 bf16 instruction takes 16 clocks, the eight 16x16x4 float32 ones for the
+// same block 256.
 #pragma once
 
 #include "rka_internal.h"
@@ -330,10 +332,10 @@ struct BackwardData {
 // Blocks of 16 columns that a chain's workgroup takes, one or two.  Two halve what is read
 // of K, Q, T and P per column, one has the shorter chain: two where one to a workgroup would
 // not have a CU for each.  Measured, the whole forward in us with one and two (bf16,
-// 128x128): 256 workgroups of one (2048 tokens) 113 and 131, 320 163 and 140, 512 260 and
-// 225, 1024 (1024 tokens) 325 and 230; 128 (16384 tokens) 690 and 810.  float32 (512
-// tokens): 256 57 and 61, 384 84 and 71.  (Float32 operands of the largest Dk leave no
-// registers for two.)
+// 128x128): 256 workgroups of one (2048 tokens) 107 and 122, 320 160 and 138, 512 262 and
+// 226, 1024 (1024 tokens) 307 and 229; 128 (16384 tokens) 733 and 847.  float32 (512
+// tokens): 256 57 and 61, 320 81 and 68, 512 91 and 80.  (Float32 operands of the largest
+// Dk leave no registers for two.)
 inline int chain_columns(const Dims& d, int pieces) {
     constexpr int kCus = 256;
     if (pieces > 1 && chain_steps(d.Dk) == 8) return 1;

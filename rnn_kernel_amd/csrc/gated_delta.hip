@@ -13,7 +13,8 @@ constexpr int kThreads = 256;
 // A chunk's q (which = 1) or k (0) as fragments, by rows and transposed, and what
 // normalises its rows.  The chunk is staged in LDS once, as it is.  VEC: Dk is a multiple
 // of eight.  Bound by memory and the launch's ends: 16384 tokens of 8 heads of 128 bf16
-// (67 MB read, 100 written) 40 us, 4.2 TB/s.
+// (67 MB read, 102 written) 40 us, 4.2 TB/s.  (In bf16 the fragments by rows are
+// q's and k's own 16 bytes, two thirds of what is written.)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void rows_kernel(Dims d, const T* q, const T* k, const int* lengths, ChunkData out) {
     constexpr int NP = kPieces<T>;
@@ -108,9 +109,9 @@ __device__ __forceinline__ void put_result(float* to, f32x4 x, int n, int hi) {
 // `x`: v, or (backward) dO, which may be null.  VEC: Dv is a multiple of eight.
 //
 // Bound by what it writes: of a chunk and head of 128x128 bf16 32 KB of `own` (float32, as
-// the chain adds it), 48 KB of `read` and 18 KB of `p` in three pieces; 16384 tokens of 16
-// heads (408 MB written, 219 read) 160 us, 3.9 TB/s; the inverse, a chain of its own, is
-// hidden by the other workgroups of the CU.  Written in the form that the chain's
+// the chain adds it), 48 KB of `read` and 18 KB of `p` in three pieces, of which the bf16
+// chain reads two; 16384 tokens of 16 heads (418 MB written, 225 read) 160 us, 4.0 TB/s; the
+// inverse, a chain of its own, is hidden by the other workgroups of the CU.  Written in the form that the chain's
 // registers take, since the chain, which is serial, would pay for every conversion.
 template <typename T, bool BACKWARD, bool VEC>
 __global__ __launch_bounds__(kThreads) void prepare_kernel(Dims d, const T* x, const void* g, const void* beta,

@@ -21,7 +21,10 @@
 // make E spend 1500 on its products with the loads between them, 250 on handing it on, 600
 // on the state's update and 1300 at the two barriers, where the other four arrive last.
 // Without its loads of rows (a copy, with wrong results) the same takes 280 us.
-// 64 heads of 2048 tokens with two blocks: 151 us forward and 155 backward.
+// 64 heads of 2048 tokens with two blocks: 151 us forward and 155 backward.  In float32 the
+// operands of a Dk above 128 do not fit the registers: 48 to 236 bytes of a lane are spilled
+// to memory in the forward, 236 to 352 in the backward (bf16: 52 in the backward of a Dk
+// above 192 with two blocks, else none).
 #pragma once
 
 #include <algorithm>

@@ -8,11 +8,15 @@
 // memory to the operand registers, the blocks of S, dS' and E are split into bf16 pieces
 // once and shared through LDS, loaded a step ahead.
 //
-// Bound by latency, with one workgroup to a CU, as the sums and the operands fill its
-// registers and LDS: 8192 tokens of 16 heads of 128x128 bf16 282 us, in which the matrix
-// instructions are busy for 16% of the clocks and 710 MB are read and written, 150 us of a
-// copy.  Holding the next head's first loads through what follows a head's last step
-// spills registers and took 347 us.
+// Bound by latency, with one workgroup to a CU, whose registers and LDS the sums and the
+// operands more than fill: 8192 tokens of 16 heads of 128x128 bf16 282 us, in which the matrix
+// instructions are busy for 16% of the clocks.  624 MB are read and 99 written, 150 us of a
+// copy; 65 of the MB written are registers spilled to memory (1024 workgroups of 512 lanes, 124
+// bytes each), dq, dk, dg and dbeta are 35.  Bytes that a lane spills, with 16-byte loads
+// and without: bf16 none at Dk up to 64, 124 and 188 to 128, 716 and 784 to 192, 1076 and
+// 1176 to 256; float32 160 and 256, 504 and 548, 1068 and 1148, 1464 and 1512.  Holding the
+// next head's first loads through what follows a head's last step spills more and took
+// 347 us.
 #include "gated_delta.h"
 
 namespace rka {

@@ -7,7 +7,7 @@
 //
 // Bound by memory: 256 requests on 32 heads of 128x128 (1.07 GB) 225 us, 4.8 TB/s, the rate of
 // a large copy.  Blocks of 32 columns give one request on 8 heads of 64x64 16 workgroups;
-// that call is 12 us, 11 of them the host's.
+// that call is 13 us, 12 of them the host's.
 #include "gated_delta.h"
 
 namespace rka {

@@ -758,9 +758,10 @@ struct Plan {
 // measured with 1, 2 and 4 workgroups to a CU, bf16: 256: 1.8; 128: 0.7, 1.1; 64: 0.25-0.5,
 // 0.4, 0.73.  `across`: an operand is turned on its way.  Slices write and read float32 sums.
 // Of 24 products measured with every choice, the one taken costs at most a tenth more than
-// the best: 8192 x 2048 x 2048's gradient of the weight 92 us with 256 tiles in 4 slices,
-// 147 and 234 with 64 and 256 tiles unsliced; 8192 x 32 over 2048 12 and 17 us with 64 tiles
-// in 4 slices and one.
+// the best for 23: 8192 x 2048 x 2048's gradient of the weight 91 us with 256 tiles in 4
+// slices, 148 and 234 with 64 and 256 tiles unsliced; 8192 x 32 over 2048 12 and 19 us with 64
+// tiles in 4 slices and one.  The 24th: float32's gradient of a 1024 x 1024 weight over 4096
+// rows, 118 us with 64 tiles in 2 slices, 85 with 128 tiles in 8.
 Plan plan_product(int m, int n, int k, int esize, bool across) {
     const int kk = kRowBytes / esize, all = std::max(1, (k + kk - 1) / kk);
     struct Cost {
@@ -795,11 +796,11 @@ size_t partial_bytes(int m, int n, const Plan& p) {
 }
 // The rows' kernel, whose workgroup goes through the whole sum, for few rows or few columns
 // (with a workgroup for 16 of the others), or tiles, in slices where those are few: models of
-// the measured times in us.  Rows and tiles, bf16, 4096 columns over 2048: 1 row 4.9 and 9.3, 16
-// 5.8 and 10.1, 32 7.7 and 10.7, 64 12.1 and 10.4; 256 columns over 4096: 8 rows 7.5 and 10.0, 32
-// 12.5 and 10.9.  float32, 64 columns over 4096: 1 row 11.8 and 9.6.  Columns and tiles, bf16, over
-// 2048: 16 columns of 2048 rows 5.5 and 9.1, of 8192 9.4 and 11.6, of 65536 65 and 41; 32 of 8192
-// 13.4 and 12.1.  float32: 16 of 8192 18.9 and 25.1, 32 30 and 26.
+// the measured times in us.  Rows and tiles, bf16, 4096 columns over 2048: 1 row 4.6 and 8.6, 16
+// 5.7 and 9.7, 32 7.6 and 10.7; 256 columns over 4096: 8 rows 7.4 and 9.9, 32 12.3 and 10.7.
+// float32, 64 columns over 4096: 1 row 11.5 and 8.7.  Columns and tiles, bf16, over 2048: 16
+// columns of 2048 rows 5.5 and 9.1, of 8192 9.2 and 11.2, of 65536 65 and 40; 32 of 8192 13.9
+// and 11.8.  float32: 16 of 8192 18.9 and 25.0, 32 29.5 and 25.0.
 enum Few { FEW_NONE, FEW_ROWS, FEW_COLUMNS };
 // (tiles also where a launch may not have a workgroup for 16 of the others)
 Few few_of(int m, int n, int k, int esize) {

@@ -188,7 +188,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     final state is float32.  Sums and states are held in float32 throughout.
 
     Tokens are taken in chunks of 64, so a NaN or an infinity in a token may reach
-    the outputs of the earlier tokens of its chunk."""
+    the outputs of the earlier tokens of its chunk (as NaN; a float32 above 3.39e38, the
+    largest bfloat16, counts as an infinity).  Tensors with forward-mode tangents are
+    refused."""
     _lib.refuse_tangents("gated_delta_rule", q, k, v, g, beta, initial_state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, lengths, scale, normalize)
@@ -205,7 +207,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     (int32 [B], distinct), or b if ``slots`` is None.  A negative slot marks a
     request without a state (padding): its output is 0; a slot from N up gives NaN;
     neither touches a state.  No gradients: with grad mode on, inputs that require
-    them are refused."""
+    them are refused, and so are forward-mode tangents.  Autograd counts the call as a
+    change of ``state``."""
     _lib.refuse_tangents("gated_delta_step", q, k, v, g, beta, state)
     _check_inputs(q, k, v, g, beta, tokens=False)
     batch, _, key_dim = q.shape
