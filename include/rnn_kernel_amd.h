@@ -443,7 +443,7 @@ int rka_describe_gated_delta(int batch, int value_heads, int key_dim, int value_
  * The matrix product with its epilogue, y = act(x W^T + b) + r: x [rows, inputs],
  * W [outputs, inputs], b [outputs] or NULL, r [rows, outputs] or NULL and y [rows,
  * outputs], all of `dtype`; y and z are dense, the others' rows lie ldx, ldw and ldr
- * elements apart (at most 2^21).  Sums, bias, activation and residual are in float32.
+ * elements apart.  Those, inputs and outputs are at most 2^21.  Sums, bias, activation and residual are in float32.
  * (The reference's F.linear, src/rnn_kernel/a100/prod/gru.py:519-523, has neither.)
  */
 #define RKA_ACT_NONE 0
