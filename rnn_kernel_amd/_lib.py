@@ -138,6 +138,16 @@ def refuse_tangents(what: str, *tensors) -> None:
 _forward_ad = None
 
 
+def check_saved(what: str, device, *expected) -> None:
+    """RuntimeError if a tensor that was saved for a backward came back (hooks may hand
+    back what they like) on another device, of another type or size: ``expected`` are
+    (tensor or None, type, shape)."""
+    for t, dtype, shape in expected:
+        if t is not None and (t.device != device or t.dtype != dtype or t.shape != shape):
+            raise RuntimeError(f"{what}: a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}, not as "
+                               f"{dtype} {list(shape)} on {device}")
+
+
 def raw_stream(index: int) -> int:
     """Handle of torch's current stream on CUDA device ``index`` (without
     building a Stream object, where torch offers that)."""

@@ -141,6 +141,7 @@ class GatedDeltaFunction(torch.autograd.Function):
                                                                    normalize, training=True)
         ctx.save_for_backward(q, k, g, beta, lengths, reserve)
         ctx.sizes = (*q.shape[:3], v.size(2), q.size(3), v.size(3))
+        ctx.device, ctx.dtype, ctx.gate_dtype = q.device, q.dtype, g.dtype
         ctx.scale, ctx.normalize, ctx.has_state = scale, normalize, initial_state is not None
         ctx.set_materialize_grads(False)
         return o, final_state
@@ -148,12 +149,16 @@ class GatedDeltaFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_o, grad_state):
-        # (hooks may have given them back in another layout than they were saved in)
         q, k, g, beta, lengths, reserve = ctx.saved_tensors
+        batch, tokens, key_heads, value_heads, key_dim, value_dim = ctx.sizes
+        lib, device, dtype, gate_dtype = _lib.load(), ctx.device, ctx.dtype, ctx.gate_dtype
+        keys, gates = (batch, tokens, key_heads, key_dim), (batch, tokens, value_heads)
+        _lib.check_saved("gated delta rule", device, (q, dtype, keys), (k, dtype, keys), (g, gate_dtype, gates),
+                         (beta, gate_dtype, gates), (lengths, torch.int32, (batch,)),
+                         (reserve, torch.uint8, (max(lib.rka_gated_delta_reserve_bytes(*ctx.sizes), 1),)))
+        # (and hooks may have given them back in another layout than they were saved in)
         q, k, reserve = _dense_heads(q), _dense_heads(k), reserve.contiguous()
         lengths = None if lengths is None else lengths.contiguous()
-        batch, tokens, _, value_heads, key_dim, value_dim = ctx.sizes
-        lib, device = _lib.load(), q.device
         grad_o = None if grad_o is None else grad_o.contiguous()
         grad_state = None if grad_state is None else grad_state.contiguous()
         dq, dk = (torch.empty(q.shape, dtype=q.dtype, device=device) for _ in range(2))

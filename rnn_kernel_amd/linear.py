@@ -107,17 +107,20 @@ class LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation):
         y, z, xm, wm = _forward(x, weight, bias, residual, activation, keep_z=any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(xm, wm, z)
-        ctx.act, ctx.shape = _ACTS[activation], x.shape
+        ctx.act, ctx.shape, ctx.device, ctx.dtype = _ACTS[activation], x.shape, x.device, x.dtype
+        ctx.sizes = (xm.size(0), wm.size(0), wm.size(1))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        # (hooks may have given them back in another layout than they were saved in)
         xm, wm, z = ctx.saved_tensors
+        rows, outputs, inputs = ctx.sizes
+        _lib.check_saved("linear", ctx.device, (xm, ctx.dtype, (rows, inputs)), (wm, ctx.dtype, (outputs, inputs)),
+                         (z, ctx.dtype, (rows, outputs)))
+        # (and hooks may have given them back in another layout than they were saved in)
         xm, wm, z = _rows(xm), _rows(wm), None if z is None else z.contiguous()
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        rows, outputs, inputs = xm.size(0), wm.size(0), wm.size(1)
         dx = torch.empty(ctx.shape, dtype=xm.dtype, device=xm.device) if need_x else None
         dw = torch.empty(outputs, inputs, dtype=xm.dtype, device=xm.device) if need_w else None
         db = torch.empty(outputs, dtype=xm.dtype, device=xm.device) if need_b else None

@@ -88,3 +88,44 @@ def test_the_products_backward_goes_by_the_unpacked_tensors(hip_lib, monkeypatch
             assert change is _apart and args[at + 1] == cols
     if change is _apart:
         assert args[6] not in given  # the sums before the activation
+
+
+@pytest.mark.parametrize("change", [lambda t: t.to("meta"), lambda t: t.double() if t.is_floating_point() else t.long(),
+                                    lambda t: t[:1] if t.size(0) > 1 else t])
+def test_what_comes_back_as_something_else_is_refused(hip_lib, monkeypatch, change):
+    """As torch's own operators refuse it: on another device, of another type or size."""
+    from rnn_kernel_amd import delta
+
+    linear = importlib.import_module("rnn_kernel_amd.linear")
+    calls = _recorded(monkeypatch, delta, ("_check_inputs", "_check_state", "_check_ints"))
+    _recorded(monkeypatch, linear, ("_check",))
+    monkeypatch.setattr(linear._lib, "call", lambda index, name, *args: calls.__setitem__(name, args))
+    q, k, v = (torch.randn(2, 3, h, d, requires_grad=True) for h, d in ((1, 4), (1, 4), (2, 5)))
+    gates = [torch.rand(2, 3, 2) for _ in range(2)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), change):
+        o, _ = delta.GatedDeltaFunction.apply(q, k, v, *gates, None, torch.tensor([3, 1], dtype=torch.int32), 1.0, False)
+        y = linear.LinearFunction.apply(torch.randn(4, 5), torch.randn(3, 5, requires_grad=True), None, None, "silu")
+    for t in (o, y):
+        with pytest.raises(RuntimeError, match="saved tensor"):
+            t.sum().backward()
+    assert not any("backward" in name for name in calls)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_each_saved_tensor_of_the_rule_is_looked_at(hip_lib, monkeypatch, which):
+    from rnn_kernel_amd import delta
+
+    calls = _recorded(monkeypatch, delta, ("_check_inputs", "_check_state", "_check_ints"))
+    seen = []
+
+    def unpack(t):
+        seen.append(t)
+        return t.to("meta") if len(seen) == which + 1 else t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+        o, _ = delta.GatedDeltaFunction.apply(torch.randn(2, 3, 1, 4), torch.randn(2, 3, 1, 4),
+                                              torch.randn(2, 3, 2, 5, requires_grad=True), torch.rand(2, 3, 2),
+                                              torch.rand(2, 3, 2), None, torch.tensor([3, 1], dtype=torch.int32), 1.0, False)
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        o.sum().backward()
+    assert len(seen) == 6 and "rka_gated_delta_backward" not in calls
