@@ -478,6 +478,46 @@ int rka_linear_backward(const void* grad_y, long long ldy, const void* x, long l
 #define RKA_LINEAR_FORM_TILES 3   /* tiles, operands through registers */
 int rka_describe_linear(int product, int rows, int outputs, int inputs, int dtype, int aligned, int* out, int n_out);
 
+/*
+ * Layer norm over rows: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps).  x
+ * [rows, size], its rows ldx elements apart, y dense; weight and bias [size] or NULL; all of
+ * `dtype`, statistics in float32.  size is at most 16384.  (The reference has no norm.)
+ */
+/* `mean` and `rstd` [rows] receive the statistics for the backward, or are both NULL. */
+int rka_layer_norm_forward(const void* x, long long ldx, const void* weight, const void* bias, void* y, float* mean,
+                           float* rstd, int rows, int size, double eps, int dtype, void* stream);
+size_t rka_layer_norm_backward_workspace_bytes(int rows, int size, int dtype);
+/* Its gradients, dense, or NULL if one is not wanted; the workspace is for those of weight
+ * and bias, whose sums have a fixed order. */
+int rka_layer_norm_backward(const void* grad_y, long long ldy, const void* x, long long ldx, const void* weight,
+                            const float* mean, const float* rstd, void* grad_x, void* grad_weight, void* grad_bias,
+                            void* workspace, size_t workspace_bytes, int rows, int size, int dtype, void* stream);
+
+/*
+ * The causal convolution of each channel over `width` tokens (2 to 8):
+ * y_t = act(bias + sum_j weight[j] x_{t - width + 1 + j}), act RKA_ACT_NONE or RKA_ACT_SILU.
+ * x [batch, tokens, channels] with dense channels, y [batch, tokens, channels] dense, weight
+ * [channels, width], bias [channels] or NULL, states [batch, width - 1, channels] (the inputs
+ * before the first token, or NULL for zeros; a row's last width - 1 inputs), all of `dtype`.
+ * lengths as in rka_gated_delta_forward.  batch is at most 65535.  (The reference has none.)
+ */
+int rka_causal_conv_forward(const void* x, long long x_batch_stride, long long x_token_stride, const void* weight,
+                            const void* bias, const void* initial_state, const int* lengths, void* y, void* final_state,
+                            int batch, int tokens, int channels, int width, int act, int dtype, void* stream);
+size_t rka_causal_conv_backward_workspace_bytes(int batch, int tokens, int channels, int width);
+/* Its gradients, dense, or NULL if one is not wanted.  grad_y and grad_final_state may be NULL
+ * (zeros).  The workspace is for the gradients of weight and bias, whose sums have a fixed
+ * order. */
+int rka_causal_conv_backward(const void* grad_y, const void* grad_final_state, const void* x, long long x_batch_stride,
+                             long long x_token_stride, const void* weight, const void* bias, const void* initial_state,
+                             const int* lengths, void* grad_x, void* grad_weight, void* grad_bias, void* grad_initial_state,
+                             void* workspace, size_t workspace_bytes, int batch, int tokens, int channels, int width, int act,
+                             int dtype, void* stream);
+/* One token of each of `batch` requests: x [batch, channels], its rows ldx apart; state
+ * [num_slots, width - 1, channels] is updated in place, slots as in rka_gated_delta_step. */
+int rka_causal_conv_step(const void* x, long long ldx, const void* weight, const void* bias, void* state, const int* slots,
+                         int num_slots, void* y, int batch, int channels, int width, int act, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 """MI355X (gfx950) fp32 GRU training path: hand-written HIP kernels behind a
 C ABI (librnn_kernel_amd.so), with an nn.GRU-compatible PyTorch front end."""
+from .conv import CausalConvFunction, causal_conv, causal_conv_step
 from .delta import GatedDeltaFunction, gated_delta_rule, gated_delta_step
 from .delta_layer import GatedDelta
 from .gru import (
@@ -15,9 +16,16 @@ from .gru import (
     set_strict,
 )
 from .linear import Linear, LinearFunction, linear
+from .norm import LayerNorm, LayerNormFunction, layer_norm
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "LayerNorm",
+    "LayerNormFunction",
+    "layer_norm",
+    "CausalConvFunction",
+    "causal_conv",
+    "causal_conv_step",
     "Linear",
     "LinearFunction",
     "linear",

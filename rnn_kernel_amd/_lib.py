@@ -70,6 +70,13 @@ SIGNATURES = {
     "rka_linear_backward_workspace_bytes": (_SZ, [_I] * 4),
     "rka_linear_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
     "rka_linear_backward": (_I, [_P, _LL, _P, _LL, _P, _LL] + [_P] * 5 + [_SZ] + [_I] * 5 + [_P]),
+    "rka_layer_norm_forward": (_I, [_P, _LL] + [_P] * 5 + [_I, _I, ctypes.c_double, _I, _P]),
+    "rka_layer_norm_backward_workspace_bytes": (_SZ, [_I] * 3),
+    "rka_layer_norm_backward": (_I, [_P, _LL, _P, _LL] + [_P] * 7 + [_SZ] + [_I] * 3 + [_P]),
+    "rka_causal_conv_forward": (_I, [_P, _LL, _LL] + [_P] * 6 + [_I] * 6 + [_P]),
+    "rka_causal_conv_backward_workspace_bytes": (_SZ, [_I] * 4),
+    "rka_causal_conv_backward": (_I, [_P, _P, _P, _LL, _LL] + [_P] * 9 + [_SZ] + [_I] * 6 + [_P]),
+    "rka_causal_conv_step": (_I, [_P, _LL] + [_P] * 4 + [_I, _P] + [_I] * 5 + [_P]),
     "rka_describe_gated_delta": (_I, [_I] * 5 + [ctypes.POINTER(_I), _I]),
     "rka_describe_linear": (_I, [_I] * 6 + [ctypes.POINTER(_I), _I]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
