@@ -518,6 +518,53 @@ int rka_causal_conv_backward(const void* grad_y, const void* grad_final_state, c
 int rka_causal_conv_step(const void* x, long long ldx, const void* weight, const void* bias, void* state, const int* slots,
                          int num_slots, void* y, int batch, int channels, int width, int act, int dtype, void* stream);
 
+/*
+ * The selective scan.  Per batch row, channel d of group g = d / (channels / groups) and state
+ * n, the state h in float32 and s = dt + dt_bias, or with `softplus` log(1 + exp(.)) of it:
+ *
+ *   h_t = exp(s_t A[d, n]) h_{t-1} + s_t x_t B_t[g, n];
+ *   y_t = (sum_n C_t[g, n] h_t + skip[d] x_t) silu(gate_t).
+ *
+ * x, dt, gate (or NULL: no gate) [batch, tokens, channels], B and C [batch, tokens, groups,
+ * states] and y (dense) are of `dtype`; A [channels, states], skip and dt_bias [channels] (or
+ * NULL) and the states [batch, channels, states] dense float32.  states is at most 64.
+ * `strides` is a host array of 12 element strides: (batch row, token) of x, dt and gate, (batch
+ * row, token, group) of B and C; channels and states are contiguous.  lengths as in
+ * rka_gated_delta_forward.  (No counterpart in the reference.)
+ */
+/* Workspace of the calls below, and what a forward saves for its backward (0 for sizes that
+ * the calls refuse). */
+size_t rka_selective_scan_forward_workspace_bytes(int batch, int tokens, int channels, int states, int groups);
+size_t rka_selective_scan_reserve_bytes(int batch, int tokens, int channels, int states, int groups);
+size_t rka_selective_scan_backward_workspace_bytes(int batch, int tokens, int channels, int states, int groups);
+
+/* Whole sequences.  initial_state NULL: zeros.  `reserve` non-NULL saves what the backward
+ * needs. */
+int rka_selective_scan_forward(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* skip,
+                               const void* gate, const float* dt_bias, const float* initial_state, const int* lengths, void* y,
+                               float* final_state, void* reserve, void* workspace, size_t workspace_bytes, int batch, int tokens,
+                               int channels, int states, int groups, const long long* strides, int softplus, int dtype,
+                               void* stream);
+
+/* Its gradients, dense; those of tokens behind a row's length are 0.  grad_y and
+ * grad_final_state may be NULL (zeros), grad_A, grad_skip, grad_dt_bias and grad_initial_state
+ * NULL (not wanted); grad_gate is written where there is a gate.  Every sum has a fixed
+ * order. */
+int rka_selective_scan_backward(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* skip,
+                                const void* gate, const float* dt_bias, const int* lengths, const void* reserve,
+                                const void* grad_y, const float* grad_final_state, void* grad_x, void* grad_dt, float* grad_A,
+                                void* grad_B, void* grad_C, float* grad_skip, void* grad_gate, float* grad_dt_bias,
+                                float* grad_initial_state, void* workspace, size_t workspace_bytes, int batch, int tokens,
+                                int channels, int states, int groups, const long long* strides, int softplus, int dtype,
+                                void* stream);
+
+/* One token of each of `batch` requests (x [batch, channels] and so on; the token strides are
+ * not used).  state [num_slots, channels, states] is updated in place, slots as in
+ * rka_gated_delta_step. */
+int rka_selective_step(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* skip,
+                       const void* gate, const float* dt_bias, float* state, const int* slots, int num_slots, void* y, int batch,
+                       int channels, int states, int groups, const long long* strides, int softplus, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

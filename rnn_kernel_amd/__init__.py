@@ -17,9 +17,13 @@ from .gru import (
 )
 from .linear import Linear, LinearFunction, linear
 from .norm import LayerNorm, LayerNormFunction, layer_norm
+from .scan import SelectiveScanFunction, selective_scan, selective_step
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "SelectiveScanFunction",
+    "selective_scan",
+    "selective_step",
     "LayerNorm",
     "LayerNormFunction",
     "layer_norm",

@@ -1,0 +1,140 @@
+// The selective scan: a recurrence of N numbers per channel whose decay and input are made
+// of the token.  Per batch row, channel d (of group g) and state n, with the step size
+// s = softplus(dt + bias) or dt + bias:
+//
+//   h_t = exp(s A[d, n]) h_{t-1} + s x_t B_t[g, n]
+//   y_t = (sum_n C_t[g, n] h_t + skip[d] x_t) silu(gate_t)
+//
+// and, with r_t = dy_t silu(gate_t) and H_t the gradient of h_t,
+//
+//   H_t = C_t r_t + a_{t+1} H_{t+1},  a_t = exp(s_t A)
+//   dC_t = sum_d r_t h_t;  dB_t = sum_d s x_t H_t;  q_t = sum_n H_t B_t
+//   dx_t = s q_t + skip r_t;  ds_t = x_t q_t + sum_n H_t a_t h_{t-1} A;  dA = sum_t H_t a_t h_{t-1} s
+//   dskip = sum_t r_t x_t;  dgate_t = dy_t (sum_n C h + skip x) silu'(gate_t)
+//
+// Tokens are split over chunks that run at once.  A chunk's state from nothing and the sum of
+// its s (its decay is exp(A sum s)) come first, then the states at the chunks' starts one
+// after another, then the chunks themselves; the gradients the same backwards.  With enough
+// channels there is one chunk and only the last of the three.
+//
+// A wavefront takes 16 channels through tiles of 16 tokens: lane l has channel l % 16 and of
+// every 16 states the four from 4 (l / 16) on.  What a tile needs of its tokens is loaded and
+// made by all lanes at once, a lane four tokens of its channel, as the 16x16x4 float32 matrix
+// instruction's result lies in registers, and handed round through LDS.  That instruction
+// adds a token's sums over n up: its second operand are the lanes' parts, its first is 1 in
+// the token's row and 0 in the others, so that tile's sums end where its x and gate are.
+#pragma once
+
+#include "elementwise.h"
+
+namespace rka {
+namespace scan {
+
+using namespace elem;
+
+constexpr int kTile = 16;       // tokens of a tile, channels of a wavefront's block, states of a block
+constexpr int kMaxStates = 64;  // N
+
+struct Dims {
+    int B, T, D, N, G;
+    int softplus;
+    int chunk, chunks;  // tokens of a chunk, a multiple of kTile; chunks of T, at least one
+    const int* lengths;
+    const float *A, *skip, *bias;
+    const void *x, *dt, *gate, *Bm, *C;
+    long long xs[2], ts[2], zs[2], bs[3], cs[3];  // element strides: batch row, token (, group)
+};
+
+inline int tiles_of(int tokens) { return tokens <= 0 ? 1 : (tokens - 1) / kTile + 1; }
+inline int state_blocks(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+// Blocks of `width` channels, each within a group.
+inline long long channel_blocks(const Dims& d, int width) { return (long long)d.G * ((d.D / d.G - 1) / width + 1); }
+
+// Workgroups of the same tokens follow one another on one XCD (consecutive workgroups go to
+// the eight in turn): neighbouring channels share lines of memory, all channels of a group B
+// and C.
+__device__ __forceinline__ long long in_order() {
+    const unsigned total = gridDim.x, per = total / 8, rest = total % 8, xcd = blockIdx.x % 8, i = blockIdx.x / 8;
+    return (long long)xcd * per + min(xcd, rest) + i;
+}
+
+// log(1 + exp(r)) as max(r, 0) + log(1 + u), u = exp(-|r|), and log(1 + u) = 2 artanh(z), z =
+// u / (2 + u) <= 1/3, by its series up to z^15 (the rest is under 2e-9 of it): small steps keep
+// their 24 bits.  slope: its derivative.
+__device__ __forceinline__ float softplus(float r, float* slope) {
+    const float u = exp_fast(-fabsf(r)), z = u * __builtin_amdgcn_rcpf(2.f + u), q = z * z;
+    float p = 1.f / 15.f;
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    *slope = (r < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(1.f + u);
+    // (NaN stays)
+    return (r < 0.f ? 0.f : r) + 2.f * z * p;
+}
+
+// The values of a tile that a lane holds: tokens t0 + 4 (lane / 16) + r of channel lane % 16,
+// and of B and C the same tokens of state lane % 16 of each block.
+template <typename T>
+struct Rows {
+    T v[4];
+    // Element (token, column) at p[token * stride]; tokens from `len` on repeat the last.
+    __device__ __forceinline__ void load(const T* p, long long stride, int t0, int len) {
+        const int first = t0 + threadIdx.x % 64 / 16 * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = p[(long long)min(first + r, len - 1) * stride];
+    }
+};
+
+// Adds, for each state of a block, a token's sum over the lanes of a channel to row t of c.
+__device__ __forceinline__ f32x4 add_row(float part, int t, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32((int)(threadIdx.x % 16) == t ? 1.f : 0.f, part, c, 0, 0, 0);
+}
+// Waits until the last such sums are in their registers, before they are read in another
+// basic block than the instruction's (11 states: eight passes, and three to be read).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 1" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// A lane's states of a block: rows 4 (lane / 16) .. + 3 of [states][channels].
+__device__ __forceinline__ f32x4 load_states(const float* p, int n0, int N, long long D, int ch) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = n0 + i < N ? p[(n0 + i) * D + ch] : 0.f;
+    return v;
+}
+__device__ __forceinline__ void store_states(float* p, int n0, int N, long long D, int ch, f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n0 + i < N) p[(n0 + i) * D + ch] = v[i];
+}
+// The same of [channels][states].
+__device__ __forceinline__ f32x4 load_states_of(const float* p, int n0, int N) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = n0 + i < N ? p[n0 + i] : 0.f;
+    return v;
+}
+__device__ __forceinline__ void store_states_of(float* p, int n0, int N, f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n0 + i < N) p[n0 + i] = v[i];
+}
+
+// Tokens of a chunk for channel blocks that give `waves` wavefronts per chunk.
+int chunk_tokens(int tokens, long long waves);
+int make_dims(const char* what, int batch, int tokens, int channels, int states, int groups, Dims* d);
+int set_call(const char* what, Dims* d, const void* x, const void* dt, const float* A, const void* Bm, const void* C,
+             const float* skip, const void* gate, const float* bias, const int* lengths, const long long* strides, int softplus,
+             int dtype);
+// States at the chunks' starts (forward) or the gradients at their ends (backward), in place
+// of the chunks' own: h_{c+1} = exp(A sum_c) h_c + own_c, from `first` ([batch, D, N] or null).
+int launch_join(const Dims& d, float* own, const float* sums, const float* first, bool backward, hipStream_t s);
+
+}  // namespace scan
+}  // namespace rka

@@ -1,0 +1,321 @@
+// The selective scan of whole sequences (selective_scan.h has the formulas and the split).
+#include "selective_scan.h"
+
+#include <algorithm>
+
+namespace rka {
+namespace scan {
+namespace {
+
+template <typename T, int NB>
+struct Tile {
+    Rows<T> x, dt, gate, b[NB], c[NB];
+};
+
+// One block of channels through one chunk.  STATES_ONLY: from nothing to the chunk's own state
+// and the sum of its steps; else from the state at its start to the outputs.
+template <typename T, int NB, bool STATES_ONLY>
+__global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float* sums, const float* initial, T* y,
+                                                   float* final_state, float* kept) {
+    __shared__ float2 steps[kTile][16];  // s, s x
+    __shared__ __attribute__((aligned(16))) float bt[kTile][NB * 16], ct[STATES_ONLY ? 1 : kTile][NB * 16];
+    const int lane = threadIdx.x, c = lane % 16, nl = lane / 16;
+    const int Dg = d.D / d.G, per_group = (Dg - 1) / 16 + 1, blocks = d.G * per_group;
+    const int chunks = STATES_ONLY ? d.chunks - 1 : d.chunks;
+    const long long id = in_order();
+    const int block = (int)(id % blocks), chunk = (int)(id / blocks % chunks), b = (int)(id / blocks / chunks);
+    const int g = block / per_group, in = block % per_group * 16 + c;
+    const bool on = in < Dg;
+    const int ch = g * Dg + min(in, Dg - 1);
+    const int len = row_length(d.lengths, b, d.T);
+    const int t0 = chunk * d.chunk, t_end = min(d.T, t0 + d.chunk), t1 = min(len, t_end);
+    const size_t at = (size_t)b * d.chunks + chunk;
+
+    f32x4 a2[NB], h[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        const int n0 = 16 * k + 4 * nl;
+        a2[k] = kLog2e * load_states_of(d.A + (size_t)ch * d.N, n0, d.N);
+        if (STATES_ONLY)
+            h[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        else if (d.chunks > 1)
+            h[k] = load_states(states + at * d.N * d.D, n0, d.N, d.D, ch);
+        else
+            h[k] = initial ? load_states_of(initial + ((size_t)b * d.D + ch) * d.N, n0, d.N) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float bias = d.bias ? d.bias[ch] : 0.f, skip = !STATES_ONLY && d.skip ? d.skip[ch] : 0.f;
+    const T* px = static_cast<const T*>(d.x) + b * d.xs[0] + ch;
+    const T* pt = static_cast<const T*>(d.dt) + b * d.ts[0] + ch;
+    const T* pz = static_cast<const T*>(d.gate) + b * d.zs[0] + ch;
+    const T* pb = static_cast<const T*>(d.Bm) + b * d.bs[0] + g * d.bs[2];
+    const T* pc = static_cast<const T*>(d.C) + b * d.cs[0] + g * d.cs[2];
+    float sum = 0.f;
+    Tile<T, NB> next;
+    auto load = [&](int t) {
+        next.x.load(px, d.xs[1], t, len);
+        next.dt.load(pt, d.ts[1], t, len);
+        if (!STATES_ONLY && d.gate) next.gate.load(pz, d.zs[1], t, len);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const int n = min(16 * k + c, d.N - 1);
+            next.b[k].load(pb + n, d.bs[1], t, len);
+            if (!STATES_ONLY) next.c[k].load(pc + n, d.cs[1], t, len);
+        }
+    };
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; t += kTile) {
+        if (!STATES_ONLY && kept) {
+            float* to = kept + ((size_t)b * ((d.T - 1) / kTile + 1) + t / kTile) * d.N * d.D;
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+                if (on) store_states(to, 16 * k + 4 * nl, d.N, d.D, ch, h[k]);
+        }
+        float x[4], gate[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 4 * nl + r;
+            const bool live = t + row < t1;
+            float slope, s = to_f32(next.dt.v[r]) + bias;
+            if (d.softplus) s = softplus(s, &slope);
+            s = live ? s : 0.f;
+            x[r] = live ? to_f32(next.x.v[r]) : 0.f;
+            gate[r] = !STATES_ONLY && d.gate ? to_f32(next.gate.v[r]) : 0.f;
+            sum += s;
+            steps[row][c] = float2{s, s * x[r]};
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                const bool is = live && 16 * k + c < d.N;
+                bt[row][16 * k + c] = is ? to_f32(next.b[k].v[r]) : 0.f;
+                if (!STATES_ONLY) ct[row][16 * k + c] = is ? to_f32(next.c[k].v[r]) : 0.f;
+            }
+        }
+        __syncthreads();
+        if (t + kTile < t1) load(t + kTile);
+        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < kTile; ++i) {
+            const float2 s = steps[i][c];
+            float part = 0.f;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                const f32x4 bv = *reinterpret_cast<const f32x4*>(&bt[i][16 * k + 4 * nl]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = fmaf(__builtin_amdgcn_exp2f(s.x * a2[k][j]), h[k][j], s.y * bv[j]);
+                if (!STATES_ONLY) {
+                    const f32x4 cv = *reinterpret_cast<const f32x4*>(&ct[i][16 * k + 4 * nl]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) part = fmaf(cv[j], h[k][j], part);
+                }
+            }
+            if (!STATES_ONLY) acc = add_row(part, i, acc);
+        }
+        if (!STATES_ONLY) {
+            settle();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int token = t + 4 * nl + r;
+                float v = fmaf(skip, x[r], acc[r]);
+                if (d.gate) v *= gate[r] * sigmoid_fast(gate[r]);
+                if (on && token < t_end) y[((size_t)b * d.T + token) * d.D + ch] = from_f32<T>(token < t1 ? v : 0.f);
+            }
+        }
+        __syncthreads();
+    }
+    if (STATES_ONLY) {
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (on && nl == 0) sums[at * d.D + ch] = sum;
+    } else {
+        // tiles behind the row's end
+        const int rest = t1 <= t0 ? t0 : t0 + ((t1 - t0 - 1) / kTile + 1) * kTile;
+        for (int t = rest + nl; t < t_end; t += 4)
+            if (on) y[((size_t)b * d.T + t) * d.D + ch] = from_f32<T>(0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        const int n0 = 16 * k + 4 * nl;
+        if (!on) continue;
+        if (STATES_ONLY)
+            store_states(states + at * d.N * d.D, n0, d.N, d.D, ch, h[k]);
+        else if (chunk == d.chunks - 1)
+            store_states_of(final_state + ((size_t)b * d.D + ch) * d.N, n0, d.N, h[k]);
+    }
+}
+
+__global__ __launch_bounds__(256) void join_kernel(Dims d, float* own, const float* sums, const float* first, int backward) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, per = (long long)d.N * d.D;
+    if (i >= per * d.B) return;
+    const int b = (int)(i / per), n = (int)(i % per / d.D), ch = (int)(i % d.D);
+    const float a2 = kLog2e * d.A[(size_t)ch * d.N + n];
+    float h = first ? first[((size_t)b * d.D + ch) * d.N + n] : 0.f;
+    const long long start = backward ? d.chunks - 1 : 0, step = backward ? -1 : 1;
+    float* p = own + ((size_t)b * d.chunks + start) * per + (size_t)n * d.D + ch;
+    const float* ps = sums + ((size_t)b * d.chunks + start) * d.D + ch;
+    constexpr int kDeep = 8;
+    for (int c0 = 0; c0 < d.chunks; c0 += kDeep) {
+        float mine[kDeep], sum[kDeep];
+        const int left = d.chunks - c0;
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j) {
+            // (the last chunk's own is not made)
+            const long long of = step * min(j, max(0, left - 2));
+            mine[j] = left > 1 ? p[of * per] : 0.f;
+            sum[j] = left > 1 ? ps[of * d.D] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j) {
+            if (j >= left) break;
+            p[step * j * per] = h;
+            h = fmaf(__builtin_amdgcn_exp2f(sum[j] * a2), h, mine[j]);
+        }
+        p += step * kDeep * per;
+        ps += step * kDeep * d.D;
+    }
+}
+
+struct Layout {
+    size_t states, sums, total;
+};
+Layout forward_layout(const Dims& d) {
+    Layout l{};
+    if (d.chunks > 1) {
+        l.sums = align_up((size_t)d.B * d.chunks * d.N * d.D * sizeof(float), 256);
+        l.total = l.sums + align_up((size_t)d.B * d.chunks * d.D * sizeof(float), 256);
+    }
+    return l;
+}
+
+template <typename T, int NB>
+int forward(const Dims& d, const float* initial, T* y, float* final_state, float* kept, char* ws, hipStream_t s) {
+    const Layout l = forward_layout(d);
+    float *states = reinterpret_cast<float*>(ws + l.states), *sums = reinterpret_cast<float*>(ws + l.sums);
+    const long long blocks = channel_blocks(d, 16) * d.B;
+    RKA_RETURN_IF_ERR(check_grid(blocks * d.chunks, 64, "selective_scan_forward"));
+    if (d.chunks > 1) {
+        hipLaunchKernelGGL((chunk_kernel<T, NB, true>), dim3((unsigned)(blocks * (d.chunks - 1))), dim3(64), 0, s, d, states,
+                           sums, nullptr, nullptr, nullptr, nullptr);
+        RKA_RETURN_IF_HIP(hipGetLastError());
+        RKA_RETURN_IF_ERR(launch_join(d, states, sums, initial, false, s));
+    }
+    hipLaunchKernelGGL((chunk_kernel<T, NB, false>), dim3((unsigned)(blocks * d.chunks)), dim3(64), 0, s, d, states, nullptr,
+                       initial, y, final_state, kept);
+    RKA_RETURN_IF_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T>
+int forward(const Dims& d, const float* initial, void* y, float* final_state, float* kept, char* ws, hipStream_t s) {
+    T* out = static_cast<T*>(y);
+    switch (state_blocks(d.N)) {
+        case 1: return forward<T, 1>(d, initial, out, final_state, kept, ws, s);
+        case 2: return forward<T, 2>(d, initial, out, final_state, kept, ws, s);
+        default: return forward<T, 4>(d, initial, out, final_state, kept, ws, s);
+    }
+}
+
+}  // namespace
+
+int chunk_tokens(int tokens, long long waves) {
+    constexpr long long kWant = 4096;
+    const long long chunks = std::max(1LL, kWant / std::max(1LL, waves));
+    if (chunks == 1) return std::max(1, tiles_of(tokens)) * kTile;
+    const int tiles = std::max(4, (int)((tiles_of(tokens) + chunks - 1) / chunks));
+    return tiles * kTile;
+}
+
+int launch_join(const Dims& d, float* own, const float* sums, const float* first, bool backward, hipStream_t s) {
+    const long long blocks = ((long long)d.B * d.N * d.D + 255) / 256;
+    RKA_RETURN_IF_ERR(check_grid(blocks, 256, "selective_scan"));
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, d, own, sums, first, backward ? 1 : 0);
+    RKA_RETURN_IF_HIP(hipGetLastError());
+    return 0;
+}
+
+int make_dims(const char* what, int batch, int tokens, int channels, int states, int groups, Dims* d) {
+    const std::string name(what);
+    if (batch < 0 || tokens < 0) return fail(RKA_ERR_INVALID_ARGUMENT, name + ": batch and tokens must be >= 0");
+    if (channels < 1 || states < 1 || groups < 1 || channels % groups != 0)
+        return fail(RKA_ERR_INVALID_ARGUMENT, name + ": channels and states must be >= 1, channels a multiple of groups");
+    if (states > kMaxStates) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": more than 64 states per channel");
+    *d = Dims{};
+    d->B = batch;
+    d->T = tokens;
+    d->D = channels;
+    d->N = states;
+    d->G = groups;
+    d->chunk = chunk_tokens(tokens, channel_blocks(*d, 16) * std::max(batch, 1));
+    d->chunks = tokens > 0 ? (tokens - 1) / d->chunk + 1 : 1;
+    // (what a kernel counts in 32 bits)
+    if (tokens > (1 << 30)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": more than 2^30 tokens");
+    return 0;
+}
+
+int set_call(const char* what, Dims* d, const void* x, const void* dt, const float* A, const void* Bm, const void* C,
+             const float* skip, const void* gate, const float* bias, const int* lengths, const long long* strides, int softplus,
+             int dtype) {
+    RKA_RETURN_IF_ERR(check_dtype(dtype, what));
+    if (!strides) return fail(RKA_ERR_INVALID_ARGUMENT, std::string(what) + ": null strides");
+    if (!A || (d->B > 0 && d->T > 0 && (!x || !dt || !Bm || !C)))
+        return fail(RKA_ERR_INVALID_ARGUMENT, std::string(what) + ": null tensor pointer");
+    d->x = x;
+    d->dt = dt;
+    d->A = A;
+    d->Bm = Bm;
+    d->C = C;
+    d->skip = skip;
+    d->gate = gate;
+    d->bias = bias;
+    d->lengths = lengths;
+    d->softplus = softplus;
+    for (int i = 0; i < 2; ++i) {
+        d->xs[i] = strides[i];
+        d->ts[i] = strides[2 + i];
+        d->zs[i] = strides[4 + i];
+    }
+    for (int i = 0; i < 3; ++i) {
+        d->bs[i] = strides[6 + i];
+        d->cs[i] = strides[9 + i];
+    }
+    return 0;
+}
+
+}  // namespace scan
+}  // namespace rka
+
+using namespace rka;
+using namespace rka::scan;
+
+extern "C" {
+
+size_t rka_selective_scan_forward_workspace_bytes(int batch, int tokens, int channels, int states, int groups) {
+    Dims d;
+    if (make_dims("selective_scan", batch, tokens, channels, states, groups, &d) != 0) return 0;
+    return forward_layout(d).total;
+}
+
+size_t rka_selective_scan_reserve_bytes(int batch, int tokens, int channels, int states, int groups) {
+    Dims d;
+    if (make_dims("selective_scan", batch, tokens, channels, states, groups, &d) != 0) return 0;
+    return (size_t)batch * tiles_of(tokens) * states * channels * sizeof(float);
+}
+
+int rka_selective_scan_forward(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* skip,
+                               const void* gate, const float* dt_bias, const float* initial_state, const int* lengths, void* y,
+                               float* final_state, void* reserve, void* workspace, size_t workspace_bytes, int batch, int tokens,
+                               int channels, int states, int groups, const long long* strides, int softplus, int dtype,
+                               void* stream) {
+    clear_error();
+    Dims d;
+    RKA_RETURN_IF_ERR(make_dims("selective_scan_forward", batch, tokens, channels, states, groups, &d));
+    RKA_RETURN_IF_ERR(set_call("selective_scan_forward", &d, x, dt, A, B, C, skip, gate, dt_bias, lengths, strides, softplus, dtype));
+    if (batch == 0) return 0;
+    if ((tokens > 0 && !y) || !final_state) return fail(RKA_ERR_INVALID_ARGUMENT, "selective_scan_forward: null tensor pointer");
+    RKA_RETURN_IF_ERR(check_workspace(workspace, workspace_bytes, forward_layout(d).total, "selective_scan_forward"));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    float* kept = static_cast<float*>(reserve);
+    return dtype == RKA_DTYPE_F32 ? forward<float>(d, initial_state, y, final_state, kept, ws, s)
+                                  : forward<bf16>(d, initial_state, y, final_state, kept, ws, s);
+}
+
+}  // extern "C"
