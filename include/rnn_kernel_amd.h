@@ -565,6 +565,39 @@ int rka_selective_step(const void* x, const void* dt, const float* A, const void
                        const void* gate, const float* dt_bias, float* state, const int* slots, int num_slots, void* y, int batch,
                        int channels, int states, int groups, const long long* strides, int softplus, int dtype, void* stream);
 
+/*
+ * The cross entropy of a product with a vocabulary: l = x W^T + b, loss = log sum exp(l) -
+ * l[target] of each row, or their sum, or their mean over the rows with a target.  x [rows,
+ * inputs] and W [outputs, inputs], their rows ldx and ldw elements apart, and b [outputs] or
+ * NULL are of `dtype`; target [rows] 64-bit or 32-bit integers; the losses float32.  A row whose
+ * target is ignore_index has no part in anything: its loss and gradient are 0 and its x is not
+ * read; the mean of no rows is 0.  One whose target lies outside the vocabulary gives NaN.  The
+ * logits are not kept: the backward makes them again, for a piece of the vocabulary at a
+ * time.  rows, inputs, outputs and ldw are at most 2^21.  (The reference's one loss is
+ * F.mse_loss, rnn_benchmark.py:636.)
+ */
+#define RKA_REDUCE_NONE 0
+#define RKA_REDUCE_MEAN 1
+#define RKA_REDUCE_SUM 2
+
+/* What a forward leaves for its backward (its calls need it in any case), and workspaces (0
+ * for sizes that the calls refuse). */
+size_t rka_cross_entropy_reserve_bytes(int rows);
+size_t rka_cross_entropy_forward_workspace_bytes(int rows, int inputs, int outputs, int dtype);
+size_t rka_cross_entropy_backward_workspace_bytes(int rows, int inputs, int outputs, int dtype);
+
+/* loss: [rows] without reduction, else one. */
+int rka_cross_entropy_forward(const void* x, long long ldx, const void* weight, long long ldw, const void* bias,
+                              const void* target, int target_is_64bit, long long ignore_index, float* loss, void* reserve,
+                              void* workspace, size_t workspace_bytes, int rows, int inputs, int outputs, int reduction, int dtype,
+                              void* stream);
+/* grad_loss as loss.  The gradients are dense, or NULL if one is not wanted.  Every sum has a
+ * fixed order. */
+int rka_cross_entropy_backward(const float* grad_loss, const void* x, long long ldx, const void* weight, long long ldw,
+                               const void* bias, const void* reserve, void* grad_x, void* grad_weight, void* grad_bias,
+                               void* workspace, size_t workspace_bytes, int rows, int inputs, int outputs, int reduction, int dtype,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,11 +16,15 @@ from .gru import (
     set_strict,
 )
 from .linear import Linear, LinearFunction, linear
+from .loss import LinearCrossEntropy, LinearCrossEntropyFunction, linear_cross_entropy
 from .norm import LayerNorm, LayerNormFunction, layer_norm
 from .scan import SelectiveScanFunction, selective_scan, selective_step
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "LinearCrossEntropy",
+    "LinearCrossEntropyFunction",
+    "linear_cross_entropy",
     "SelectiveScanFunction",
     "selective_scan",
     "selective_step",

@@ -83,6 +83,11 @@ SIGNATURES = {
     "rka_selective_scan_forward": (_I, [_P] * 14 + [_SZ] + [_I] * 5 + [_LLP, _I, _I, _P]),
     "rka_selective_scan_backward": (_I, [_P] * 22 + [_SZ] + [_I] * 5 + [_LLP, _I, _I, _P]),
     "rka_selective_step": (_I, [_P] * 10 + [_I, _P] + [_I] * 4 + [_LLP, _I, _I, _P]),
+    "rka_cross_entropy_reserve_bytes": (_SZ, [_I]),
+    "rka_cross_entropy_forward_workspace_bytes": (_SZ, [_I] * 4),
+    "rka_cross_entropy_backward_workspace_bytes": (_SZ, [_I] * 4),
+    "rka_cross_entropy_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _I, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
+    "rka_cross_entropy_backward": (_I, [_P, _P, _LL, _P, _LL] + [_P] * 6 + [_SZ] + [_I] * 5 + [_P]),
     "rka_describe_gated_delta": (_I, [_I] * 5 + [ctypes.POINTER(_I), _I]),
     "rka_describe_linear": (_I, [_I] * 6 + [ctypes.POINTER(_I), _I]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),

@@ -22,7 +22,7 @@ SOURCES = ["rka_capi.hip", "gemm_f32.hip", "gru_recurrence.hip", "gru_rec_tiled.
            "gated_delta.hip", "gated_delta_grad.hip",
            "gated_delta_chain_fwd_bf16.hip", "gated_delta_chain_fwd_f32.hip", "gated_delta_chain_bwd_bf16.hip",
            "gated_delta_chain_bwd_f32.hip", "gated_delta_step.hip", "linear.hip", "layer_norm.hip", "causal_conv.hip",
-           "selective_scan.hip", "selective_scan_grad.hip", "selective_scan_step.hip"]
+           "selective_scan.hip", "selective_scan_grad.hip", "selective_scan_step.hip", "cross_entropy.hip"]
 ARCH = "gfx950"
 # Flags of single sources on top of compile_flags().  The machine-scheduler
 # strategy is an option per translation unit: the one-row kernels that

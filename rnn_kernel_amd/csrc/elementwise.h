@@ -98,6 +98,8 @@ inline int check_workspace(const void* workspace, size_t bytes, size_t need, con
     if (bytes < need || (need > 0 && !workspace))
         return fail(RKA_ERR_WORKSPACE_TOO_SMALL, std::string(what) + ": workspace needs " + std::to_string(need) +
                                                      " bytes, got " + std::to_string(bytes));
+    if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+        return fail(RKA_ERR_INVALID_ARGUMENT, std::string(what) + ": the workspace must begin at a multiple of 16 bytes");
     return 0;
 }
 
