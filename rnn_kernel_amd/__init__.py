@@ -19,9 +19,11 @@ from .linear import Linear, LinearFunction, linear
 from .loss import LinearCrossEntropy, LinearCrossEntropyFunction, linear_cross_entropy
 from .norm import LayerNorm, LayerNormFunction, layer_norm
 from .scan import SelectiveScanFunction, selective_scan, selective_step
+from .scan_layer import SelectiveScan
 from .train import AdamW, HeadFunction, LinearHead, MSELossFunction, mse_loss
 
 __all__ = [
+    "SelectiveScan",
     "LinearCrossEntropy",
     "LinearCrossEntropyFunction",
     "linear_cross_entropy",
