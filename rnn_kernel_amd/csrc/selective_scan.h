@@ -34,6 +34,7 @@ using namespace elem;
 
 constexpr int kTile = 16;       // tokens of a tile, channels of a wavefront's block, states of a block
 constexpr int kMaxStates = 64;  // N
+constexpr long long kMaxStride = 1 << 21;  // of a token, in elements: a tile's offsets are 32-bit
 
 struct Dims {
     int B, T, D, N, G;
@@ -58,34 +59,33 @@ __device__ __forceinline__ long long in_order() {
     return (long long)xcd * per + min(xcd, rest) + i;
 }
 
-// log(1 + exp(r)) as max(r, 0) + log(1 + u), u = exp(-|r|), and log(1 + u) = 2 artanh(z), z =
-// u / (2 + u) <= 1/3, by its series up to z^15 (the rest is under 2e-9 of it): small steps keep
-// their 24 bits.  slope: its derivative.
+// log(1 + exp(r)) as max(r, 0) + log(1 + u), u = exp(-|r|).  1 + u is rounded; what it lost,
+// (u - (w - 1)) / w, is added to log(w), without the division, as it matters where w is next to
+// 1: small steps keep their 24 bits.  slope: its derivative.
 __device__ __forceinline__ float softplus(float r, float* slope) {
-    const float u = exp_fast(-fabsf(r)), z = u * __builtin_amdgcn_rcpf(2.f + u), q = z * z;
-    float p = 1.f / 15.f;
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
-    p = fmaf(p, q, 1.f);
-    *slope = (r < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(1.f + u);
+    const float u = exp_fast(-fabsf(r)), w = 1.f + u;
+    *slope = (r < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(w);
     // (NaN stays)
-    return (r < 0.f ? 0.f : r) + 2.f * z * p;
+    return (r < 0.f ? 0.f : r) + fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, u - (w - 1.f));
 }
 
-// The values of a tile that a lane holds: tokens t0 + 4 (lane / 16) + r of channel lane % 16,
-// and of B and C the same tokens of state lane % 16 of each block.
+// Offsets in bytes of the values of a tile that a lane holds: tokens 4 (lane / 16) + r of one
+// column, rows from `rows` on as the last.  (Strides are at most kMaxStride elements: they fit.)
+struct Offsets {
+    unsigned at[4];
+    __device__ __forceinline__ void set(long long stride, int column, int rows, int esize) {
+        const int first = threadIdx.x % 64 / 16 * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) at[r] = ((unsigned)min(first + r, rows - 1) * (unsigned)stride + (unsigned)column) * (unsigned)esize;
+    }
+};
+// The values themselves; `p` is the tile's first token's row.
 template <typename T>
 struct Rows {
     T v[4];
-    // Element (token, column) at p[token * stride]; tokens from `len` on repeat the last.
-    __device__ __forceinline__ void load(const T* p, long long stride, int t0, int len) {
-        const int first = t0 + threadIdx.x % 64 / 16 * 4;
+    __device__ __forceinline__ void load(const T* p, const Offsets& o) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = p[(long long)min(first + r, len - 1) * stride];
+        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + o.at[r]);
     }
 };
 

@@ -7,11 +7,6 @@ namespace rka {
 namespace scan {
 namespace {
 
-template <typename T, int NB>
-struct Tile {
-    Rows<T> x, dt, gate, b[NB], c[NB];
-};
-
 // One block of channels through one chunk.  STATES_ONLY: from nothing to the chunk's own state
 // and the sum of its steps; else from the state at its start to the outputs.
 template <typename T, int NB, bool STATES_ONLY>
@@ -44,24 +39,39 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
             h[k] = initial ? load_states_of(initial + ((size_t)b * d.D + ch) * d.N, n0, d.N) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float bias = d.bias ? d.bias[ch] : 0.f, skip = !STATES_ONLY && d.skip ? d.skip[ch] : 0.f;
-    const T* px = static_cast<const T*>(d.x) + b * d.xs[0] + ch;
-    const T* pt = static_cast<const T*>(d.dt) + b * d.ts[0] + ch;
-    const T* pz = static_cast<const T*>(d.gate) + b * d.zs[0] + ch;
+    const T* px = static_cast<const T*>(d.x) + b * d.xs[0];
+    const T* pt = static_cast<const T*>(d.dt) + b * d.ts[0];
+    const T* pz = static_cast<const T*>(d.gate) + b * d.zs[0];
     const T* pb = static_cast<const T*>(d.Bm) + b * d.bs[0] + g * d.bs[2];
     const T* pc = static_cast<const T*>(d.C) + b * d.cs[0] + g * d.cs[2];
-    float sum = 0.f;
-    Tile<T, NB> next;
-    auto load = [&](int t) {
-        next.x.load(px, d.xs[1], t, len);
-        next.dt.load(pt, d.ts[1], t, len);
-        if (!STATES_ONLY && d.gate) next.gate.load(pz, d.zs[1], t, len);
+    T* py = STATES_ONLY ? nullptr : y + (size_t)b * d.T * d.D;
+    Rows<T> x, dt, gate, bv[NB], cv[NB];
+    Offsets ox, ot, oz, ob[NB], oc[NB], oy;
+    auto set = [&](int rows) {
+        ox.set(d.xs[1], ch, rows, sizeof(T));
+        ot.set(d.ts[1], ch, rows, sizeof(T));
+        if (!STATES_ONLY && d.gate) oz.set(d.zs[1], ch, rows, sizeof(T));
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             const int n = min(16 * k + c, d.N - 1);
-            next.b[k].load(pb + n, d.bs[1], t, len);
-            if (!STATES_ONLY) next.c[k].load(pc + n, d.cs[1], t, len);
+            ob[k].set(d.bs[1], n, rows, sizeof(T));
+            if (!STATES_ONLY) oc[k].set(d.cs[1], n, rows, sizeof(T));
         }
     };
+    auto load = [&](int t) {
+        if (t1 - t < kTile) set(t1 - t);
+        x.load(px + t * d.xs[1], ox);
+        dt.load(pt + t * d.ts[1], ot);
+        if (!STATES_ONLY && d.gate) gate.load(pz + t * d.zs[1], oz);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            bv[k].load(pb + t * d.bs[1], ob[k]);
+            if (!STATES_ONLY) cv[k].load(pc + t * d.cs[1], oc[k]);
+        }
+    };
+    float sum = 0.f;
+    set(kTile);
+    oy.set(d.D, ch, kTile, sizeof(T));
     if (t0 < t1) load(t0);
     for (int t = t0; t < t1; t += kTile) {
         if (!STATES_ONLY && kept) {
@@ -70,23 +80,22 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
             for (int k = 0; k < NB; ++k)
                 if (on) store_states(to, 16 * k + 4 * nl, d.N, d.D, ch, h[k]);
         }
-        float x[4], gate[4];
+        // (a token behind the last has a step of 0, which changes nothing, and is no output)
+        const int rows = t1 - t - 4 * nl;
+        float xf[4], zf[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 4 * nl + r;
-            const bool live = t + row < t1;
-            float slope, s = to_f32(next.dt.v[r]) + bias;
+            float slope, s = to_f32(dt.v[r]) + bias;
             if (d.softplus) s = softplus(s, &slope);
-            s = live ? s : 0.f;
-            x[r] = live ? to_f32(next.x.v[r]) : 0.f;
-            gate[r] = !STATES_ONLY && d.gate ? to_f32(next.gate.v[r]) : 0.f;
+            s = r < rows ? s : 0.f;
+            xf[r] = r < rows ? to_f32(x.v[r]) : 0.f;
+            zf[r] = !STATES_ONLY && d.gate ? to_f32(gate.v[r]) : 0.f;
             sum += s;
-            steps[row][c] = float2{s, s * x[r]};
+            steps[4 * nl + r][c] = float2{s, s * xf[r]};
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                const bool is = live && 16 * k + c < d.N;
-                bt[row][16 * k + c] = is ? to_f32(next.b[k].v[r]) : 0.f;
-                if (!STATES_ONLY) ct[row][16 * k + c] = is ? to_f32(next.c[k].v[r]) : 0.f;
+                bt[4 * nl + r][16 * k + c] = 16 * k + c < d.N ? to_f32(bv[k].v[r]) : 0.f;
+                if (!STATES_ONLY) ct[4 * nl + r][16 * k + c] = to_f32(cv[k].v[r]);
             }
         }
         __syncthreads();
@@ -98,25 +107,26 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
             float part = 0.f;
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                const f32x4 bv = *reinterpret_cast<const f32x4*>(&bt[i][16 * k + 4 * nl]);
+                const f32x4 q = *reinterpret_cast<const f32x4*>(&bt[i][16 * k + 4 * nl]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) h[k][j] = fmaf(__builtin_amdgcn_exp2f(s.x * a2[k][j]), h[k][j], s.y * bv[j]);
+                for (int j = 0; j < 4; ++j) h[k][j] = fmaf(__builtin_amdgcn_exp2f(s.x * a2[k][j]), h[k][j], s.y * q[j]);
                 if (!STATES_ONLY) {
-                    const f32x4 cv = *reinterpret_cast<const f32x4*>(&ct[i][16 * k + 4 * nl]);
+                    const f32x4 p = *reinterpret_cast<const f32x4*>(&ct[i][16 * k + 4 * nl]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) part = fmaf(cv[j], h[k][j], part);
+                    for (int j = 0; j < 4; ++j) part = fmaf(p[j], h[k][j], part);
                 }
             }
             if (!STATES_ONLY) acc = add_row(part, i, acc);
         }
         if (!STATES_ONLY) {
             settle();
+            char* to = reinterpret_cast<char*>(py + (size_t)t * d.D);
+            const int room = t_end - t - 4 * nl;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int token = t + 4 * nl + r;
-                float v = fmaf(skip, x[r], acc[r]);
-                if (d.gate) v *= gate[r] * sigmoid_fast(gate[r]);
-                if (on && token < t_end) y[((size_t)b * d.T + token) * d.D + ch] = from_f32<T>(token < t1 ? v : 0.f);
+                float v = fmaf(skip, xf[r], acc[r]);
+                if (d.gate) v *= zf[r] * sigmoid_fast(zf[r]);
+                if (on && r < room) *reinterpret_cast<T*>(to + oy.at[r]) = from_f32<T>(r < rows ? v : 0.f);
             }
         }
         __syncthreads();
@@ -129,7 +139,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
         // tiles behind the row's end
         const int rest = t1 <= t0 ? t0 : t0 + ((t1 - t0 - 1) / kTile + 1) * kTile;
         for (int t = rest + nl; t < t_end; t += 4)
-            if (on) y[((size_t)b * d.T + t) * d.D + ch] = from_f32<T>(0.f);
+            if (on) py[(size_t)t * d.D + ch] = from_f32<T>(0.f);
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -276,6 +286,10 @@ int set_call(const char* what, Dims* d, const void* x, const void* dt, const flo
         d->bs[i] = strides[6 + i];
         d->cs[i] = strides[9 + i];
     }
+    if (d->D > kMaxStride) return fail(RKA_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": more than 2^21 channels");
+    for (const long long of_token : {d->xs[1], d->ts[1], d->zs[1], d->bs[1], d->cs[1]})
+        if (d->T > 1 && (of_token < 0 || of_token > kMaxStride))
+            return fail(RKA_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": the strides of a token must be in [0, 2^21]");
     return 0;
 }
 

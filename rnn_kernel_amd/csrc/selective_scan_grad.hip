@@ -53,26 +53,39 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
         dh[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float bias = d.bias ? d.bias[p.ch] : 0.f;
-    const T* pt = static_cast<const T*>(d.dt) + p.b * d.ts[0] + p.ch;
-    const T* pz = static_cast<const T*>(d.gate) + p.b * d.zs[0] + p.ch;
-    const T* pd = dy ? dy + (size_t)p.b * d.T * d.D + p.ch : nullptr;
+    const T* pt = static_cast<const T*>(d.dt) + p.b * d.ts[0];
+    const T* pz = static_cast<const T*>(d.gate) + p.b * d.zs[0];
+    const T* pd = dy ? dy + (size_t)p.b * d.T * d.D : nullptr;
     const T* pc = static_cast<const T*>(d.C) + p.b * d.cs[0] + p.g * d.cs[2];
     float sum = 0.f;
     Rows<T> dt, gate, up, cv[NB];
-    auto load = [&](int t) {
-        dt.load(pt, d.ts[1], t, p.len);
-        if (d.gate) gate.load(pz, d.zs[1], t, p.len);
-        if (pd) up.load(pd, d.D, t, p.len);
+    Offsets ot, oz, od, oc[NB];
+    auto set = [&](int rows) {
+        ot.set(d.ts[1], p.ch, rows, sizeof(T));
+        if (d.gate) oz.set(d.zs[1], p.ch, rows, sizeof(T));
+        od.set(d.D, p.ch, rows, sizeof(T));
 #pragma unroll
-        for (int k = 0; k < NB; ++k) cv[k].load(pc + min(16 * k + c, d.N - 1), d.cs[1], t, p.len);
+        for (int k = 0; k < NB; ++k) oc[k].set(d.cs[1], min(16 * k + c, d.N - 1), rows, sizeof(T));
+    };
+    auto load = [&](int t) {
+        dt.load(pt + t * d.ts[1], ot);
+        if (d.gate) gate.load(pz + t * d.zs[1], oz);
+        if (pd) up.load(pd + (size_t)t * d.D, od);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) cv[k].load(pc + t * d.cs[1], oc[k]);
     };
     const int last = p.t0 + (p.t1 - 1 - p.t0) / kTile * kTile;
-    if (p.t0 < p.t1) load(last);
+    if (p.t0 < p.t1) {
+        set(p.t1 - last);
+        load(last);
+        set(kTile);
+    }
     for (int t = p.t0 < p.t1 ? last : p.t0 - 1; t >= p.t0; t -= kTile) {
+        const int rows = p.t1 - t - 4 * nl;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 4 * nl + r;
-            const bool live = t + row < p.t1;
+            const bool live = r < rows;
             float slope, s = to_f32(dt.v[r]) + bias;
             if (d.softplus) s = softplus(s, &slope);
             s = live ? s : 0.f;
@@ -81,7 +94,7 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
             sum += s;
             steps[row][c] = float2{s, live ? dr : 0.f};
 #pragma unroll
-            for (int k = 0; k < NB; ++k) ct[row][16 * k + c] = live && 16 * k + c < d.N ? to_f32(cv[k].v[r]) : 0.f;
+            for (int k = 0; k < NB; ++k) ct[row][16 * k + c] = 16 * k + c < d.N ? to_f32(cv[k].v[r]) : 0.f;
         }
         __syncthreads();
         if (t > p.t0) load(t - kTile);
@@ -155,42 +168,64 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             dh[k] = load_states_of(dfinal + ((size_t)p.b * d.D + p.ch) * d.N, n0, d.N);
     }
     const float bias = d.bias ? d.bias[p.ch] : 0.f, skip = d.skip ? d.skip[p.ch] : 0.f;
-    const T* px = static_cast<const T*>(d.x) + p.b * d.xs[0] + p.ch;
-    const T* pt = static_cast<const T*>(d.dt) + p.b * d.ts[0] + p.ch;
-    const T* pz = static_cast<const T*>(d.gate) + p.b * d.zs[0] + p.ch;
-    const T* pd = dy ? dy + (size_t)p.b * d.T * d.D + p.ch : nullptr;
+    const T* px = static_cast<const T*>(d.x) + p.b * d.xs[0];
+    const T* pt = static_cast<const T*>(d.dt) + p.b * d.ts[0];
+    const T* pz = static_cast<const T*>(d.gate) + p.b * d.zs[0];
+    const T* pd = dy ? dy + (size_t)p.b * d.T * d.D : nullptr;
     const T* pb = static_cast<const T*>(d.Bm) + p.b * d.bs[0] + p.g * d.bs[2];
     const T* pc = static_cast<const T*>(d.C) + p.b * d.cs[0] + p.g * d.cs[2];
     Rows<T> xv, dt, gate, up;
+    Offsets ox, ot, oz, od, oy;
     T bv[NB], cv[NB];
+    unsigned ob[NB], oc[NB], oh[4];
     const int btoken = threadIdx.x / 16;  // B and C are staged by all wavefronts
-    auto load = [&](int t) {
-        xv.load(px, d.xs[1], t, p.len);
-        dt.load(pt, d.ts[1], t, p.len);
-        if (d.gate) gate.load(pz, d.zs[1], t, p.len);
-        if (pd) up.load(pd, d.D, t, p.len);
-        const long long token = min(t + btoken, p.len - 1);
+    auto set = [&](int rows) {
+        ox.set(d.xs[1], p.ch, rows, sizeof(T));
+        ot.set(d.ts[1], p.ch, rows, sizeof(T));
+        if (d.gate) oz.set(d.zs[1], p.ch, rows, sizeof(T));
+        od.set(d.D, p.ch, rows, sizeof(T));
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const int n = min(16 * k + c, d.N - 1);
-            bv[k] = pb[token * d.bs[1] + n];
-            cv[k] = pc[token * d.cs[1] + n];
-            h[k] = load_states(kept + ((size_t)p.b * tiles + t / kTile) * d.N * d.D, 16 * k + 4 * nl, d.N, d.D, p.ch);
+            const unsigned n = min(16 * k + c, d.N - 1), row = min(btoken, rows - 1);
+            ob[k] = row * (unsigned)d.bs[1] + n;
+            oc[k] = row * (unsigned)d.cs[1] + n;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) oh[j] = (unsigned)(4 * nl + j) * (unsigned)d.D + (unsigned)p.ch;
+    auto load = [&](int t) {
+        xv.load(px + t * d.xs[1], ox);
+        dt.load(pt + t * d.ts[1], ot);
+        if (d.gate) gate.load(pz + t * d.zs[1], oz);
+        if (pd) up.load(pd + (size_t)t * d.D, od);
+        const float* from = kept + ((size_t)p.b * tiles + t / kTile) * d.N * d.D;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            bv[k] = (pb + t * d.bs[1])[ob[k]];
+            cv[k] = (pc + t * d.cs[1])[oc[k]];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[k][j] = 16 * k + 4 * nl + j < d.N ? (from + (size_t)16 * k * d.D)[oh[j]] : 0.f;
         }
     };
     float dskip = 0.f, dbias = 0.f;
     const int last = p.t0 + (p.t1 - 1 - p.t0) / kTile * kTile;
-    if (p.t0 < p.t1) load(last);
+    oy.set(d.D, p.ch, kTile, sizeof(T));
+    if (p.t0 < p.t1) {
+        set(p.t1 - last);
+        load(last);
+        set(kTile);
+    }
     for (int t = p.t0 < p.t1 ? last : p.t0 - 1; t >= p.t0; t -= kTile) {
+        const int rows = p.t1 - t - 4 * nl;
         float x[4], s[4], slope[4], z[4], u[4], dr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 4 * nl + r;
-            const bool live = t + row < p.t1 && p.on;
+            const bool live = r < rows && p.on;
             s[r] = to_f32(dt.v[r]) + bias;
             slope[r] = 1.f;
             if (d.softplus) s[r] = softplus(s[r], &slope[r]);
-            s[r] = t + row < p.t1 ? s[r] : 0.f;
+            s[r] = r < rows ? s[r] : 0.f;
             x[r] = live ? to_f32(xv.v[r]) : 0.f;
             z[r] = d.gate ? to_f32(gate.v[r]) : 0.f;
             u[r] = live && pd ? to_f32(up.v[r]) : 0.f;
@@ -200,7 +235,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const bool is = t + btoken < p.t1 && 16 * k + c < d.N;
+            const bool is = 16 * k + c < d.N;
             bt[btoken][16 * k + c] = is ? to_f32(bv[k]) : 0.f;
             ct[btoken][16 * k + c] = is ? to_f32(cv[k]) : 0.f;
         }
@@ -266,25 +301,25 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             }
         }
         settle();
+        const size_t first = ((size_t)p.b * d.T + t) * d.D;
+        const int room = p.t_end - t - 4 * nl;
+        auto put = [&](T* to, int r, float v) {
+            if (p.on && r < room) *reinterpret_cast<T*>(reinterpret_cast<char*>(to + first) + oy.at[r]) = from_f32<T>(r < rows ? v : 0.f);
+        };
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int token = t + 4 * nl + r;
-            const bool live = token < p.t1;
             const float dx = fmaf(s[r], q1[r], skip * dr[r]);
             // (a2 is A log2(e))
             const float ddt = slope[r] * fmaf(x[r], q1[r], 0.6931471805599453f * q2[r]);
-            if (live) {
+            if (r < rows) {
                 dskip = fmaf(dr[r], x[r], dskip);
                 dbias += ddt;
             }
-            if (!p.on || token >= p.t_end) continue;
-            const size_t i = ((size_t)p.b * d.T + token) * d.D + p.ch;
-            out.x[i] = from_f32<T>(live ? dx : 0.f);
-            out.dt[i] = from_f32<T>(live ? ddt : 0.f);
+            put(out.x, r, dx);
+            put(out.dt, r, ddt);
             if (d.gate) {
                 const float sig = sigmoid_fast(z[r]);
-                const float dz = u[r] * fmaf(skip, x[r], read[r]) * sig * (1.f + z[r] * (1.f - sig));
-                out.gate[i] = from_f32<T>(live ? dz : 0.f);
+                put(out.gate, r, u[r] * fmaf(skip, x[r], read[r]) * sig * (1.f + z[r] * (1.f - sig)));
             }
         }
     }

@@ -26,6 +26,7 @@ from . import _args, _lib
 
 MAX_STATES = 64
 MAX_TOKENS = 2 ** 30
+MAX_TOKEN_STRIDE = 2 ** 21  # elements: the kernels' offsets within a tile are 32-bit
 
 
 def _check(what: str, x, dt, A, B, C, skip, gate, dt_bias, tokens: bool) -> None:
@@ -49,8 +50,17 @@ def _check(what: str, x, dt, A, B, C, skip, gate, dt_bias, tokens: bool) -> None
     for t, name in ((skip, "skip"), (dt_bias, "dt_bias")):
         _args.check_shape(what, t, name, (channels,))
     _args.check_sizes(what, x)
+    if channels > MAX_TOKEN_STRIDE:
+        raise ValueError(f"{what}: at most 2^21 channels")
     if tokens and x.size(1) > MAX_TOKENS:
         raise ValueError(f"{what}: at most 2^30 tokens")
+
+
+def _near(t):
+    """``t`` with its last dimension's elements side by side and tokens at most MAX_TOKEN_STRIDE
+    apart: a copy where they are not."""
+    t = _args.dense_last(t)
+    return t if t is None or t.size(1) <= 1 or t.stride(1) <= MAX_TOKEN_STRIDE else t.contiguous()
 
 
 def _strides(x, dt, gate, B, C):
@@ -73,7 +83,7 @@ def _forward(x, dt, A, B, C, initial_state, skip, gate, dt_bias, softplus: bool,
     _args.check_tensors(what, x, (initial_state, "initial_state", torch.float32))
     _args.check_shape(what, initial_state, "initial_state", (batch, channels, states))
     _args.check_row_ints(what, lengths, "lengths", batch, x.device)
-    x, dt, gate, B, C = (_args.dense_last(t) for t in (x, dt, gate, B, C))
+    x, dt, gate, B, C = (_near(t) for t in (x, dt, gate, B, C))
     A, initial_state, skip, dt_bias, lengths = (_args.dense(t) for t in (A, initial_state, skip, dt_bias, lengths))
     lib, sizes = _lib.load(), (batch, tokens, channels, states, groups)
     y = torch.empty(batch, tokens, channels, dtype=x.dtype, device=x.device)
@@ -112,7 +122,7 @@ class SelectiveScanFunction(torch.autograd.Function):
                          (lengths, torch.int32, (batch,)),
                          (reserve, torch.uint8, (max(lib.rka_selective_scan_reserve_bytes(*ctx.sizes), 1),)))
         # (hooks may have given them back in another layout than they were saved in)
-        x, dt, gate, B, C = (_args.dense_last(t) for t in (x, dt, gate, B, C))
+        x, dt, gate, B, C = (_near(t) for t in (x, dt, gate, B, C))
         A, skip, dt_bias, lengths, reserve, grad_y, grad_state = (
             _args.dense(t) for t in (A, skip, dt_bias, lengths, reserve, grad_y, grad_state))
         dx, ddt = (torch.empty(wide, dtype=dtype, device=device) for _ in range(2))
