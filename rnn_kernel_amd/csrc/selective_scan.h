@@ -79,13 +79,29 @@ struct Offsets {
         for (int r = 0; r < 4; ++r) at[r] = ((unsigned)min(first + r, rows - 1) * (unsigned)stride + (unsigned)column) * (unsigned)esize;
     }
 };
+// Memory from an address that is the same for all lanes on, which a lane addresses by 32 bits:
+// with pointers the compiler keeps a 64-bit address of each load's from tile to tile.
+struct Memory {
+    __amdgpu_buffer_rsrc_t of;
+    __device__ __forceinline__ explicit Memory(const void* p)
+        : of(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)0xffffffffu, 0x27000)) {}
+    __device__ __forceinline__ void load(float* v, unsigned at) const {
+        *v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(of, (int)at, 0, 0));
+    }
+    __device__ __forceinline__ void load(bf16* v, unsigned at) const { v->bits = __builtin_amdgcn_raw_buffer_load_b16(of, (int)at, 0, 0); }
+    __device__ __forceinline__ void store(float v, unsigned at) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), of, (int)at, 0, 0);
+    }
+    __device__ __forceinline__ void store(bf16 v, unsigned at) const { __builtin_amdgcn_raw_buffer_store_b16(v.bits, of, (int)at, 0, 0); }
+};
 // The values themselves; `p` is the tile's first token's row.
 template <typename T>
 struct Rows {
     T v[4];
     __device__ __forceinline__ void load(const T* p, const Offsets& o) {
+        const Memory m(p);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + o.at[r]);
+        for (int r = 0; r < 4; ++r) m.load(&v[r], o.at[r]);
     }
 };
 

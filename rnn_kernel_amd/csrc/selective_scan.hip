@@ -120,13 +120,13 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
         }
         if (!STATES_ONLY) {
             settle();
-            char* to = reinterpret_cast<char*>(py + (size_t)t * d.D);
+            const Memory to(py + (size_t)t * d.D);
             const int room = t_end - t - 4 * nl;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float v = fmaf(skip, xf[r], acc[r]);
                 if (d.gate) v *= zf[r] * sigmoid_fast(zf[r]);
-                if (on && r < room) *reinterpret_cast<T*>(to + oy.at[r]) = from_f32<T>(r < rows ? v : 0.f);
+                if (on && r < room) to.store(from_f32<T>(r < rows ? v : 0.f), oy.at[r]);
             }
         }
         __syncthreads();
@@ -225,8 +225,11 @@ int forward(const Dims& d, const float* initial, void* y, float* final_state, fl
 
 }  // namespace
 
+// Chunks for some eight wavefronts to a SIMD: 16384 tokens of 2048 channels take 487, 322, 272,
+// 265 and 268 us with one, two, four, eight and sixteen.  At least four tiles: what a chunk's
+// state costs in memory is then a third of its tokens' at most.
 int chunk_tokens(int tokens, long long waves) {
-    constexpr long long kWant = 4096;
+    constexpr long long kWant = 8192;
     const long long chunks = std::max(1LL, kWant / std::max(1LL, waves));
     if (chunks == 1) return std::max(1, tiles_of(tokens)) * kTile;
     const int tiles = std::max(4, (int)((tiles_of(tokens) + chunks - 1) / chunks));

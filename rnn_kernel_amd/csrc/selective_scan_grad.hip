@@ -187,24 +187,30 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             const unsigned n = min(16 * k + c, d.N - 1), row = min(btoken, rows - 1);
-            ob[k] = row * (unsigned)d.bs[1] + n;
-            oc[k] = row * (unsigned)d.cs[1] + n;
+            ob[k] = (row * (unsigned)d.bs[1] + n) * (unsigned)sizeof(T);
+            oc[k] = (row * (unsigned)d.cs[1] + n) * (unsigned)sizeof(T);
         }
     };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) oh[j] = (unsigned)(4 * nl + j) * (unsigned)d.D + (unsigned)p.ch;
+    for (int j = 0; j < 4; ++j) oh[j] = ((unsigned)(4 * nl + j) * (unsigned)d.D + (unsigned)p.ch) * 4u;
     auto load = [&](int t) {
         xv.load(px + t * d.xs[1], ox);
         dt.load(pt + t * d.ts[1], ot);
         if (d.gate) gate.load(pz + t * d.zs[1], oz);
         if (pd) up.load(pd + (size_t)t * d.D, od);
         const float* from = kept + ((size_t)p.b * tiles + t / kTile) * d.N * d.D;
+        const Memory fb(pb + t * d.bs[1]), fc(pc + t * d.cs[1]);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            bv[k] = (pb + t * d.bs[1])[ob[k]];
-            cv[k] = (pc + t * d.cs[1])[oc[k]];
+            fb.load(&bv[k], ob[k]);
+            fc.load(&cv[k], oc[k]);
+            const Memory fh(from + (size_t)16 * k * d.D);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[k][j] = 16 * k + 4 * nl + j < d.N ? (from + (size_t)16 * k * d.D)[oh[j]] : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                float v = 0.f;
+                if (16 * k + 4 * nl + j < d.N) fh.load(&v, oh[j]);
+                h[k][j] = v;
+            }
         }
     };
     float dskip = 0.f, dbias = 0.f;
@@ -286,8 +292,10 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
                 q1 = add_row(of_b, i, q1);
                 q2 = add_row(of_a, i, q2);
                 const float sum = row_sums(v);
-                if (c % 2 == 0) reinterpret_cast<float*>(&before[wave][i][0])[nl * 8 + c / 2] = sum;
+                // (two lanes write the same: no branch between matrix instructions)
+                reinterpret_cast<float*>(&before[wave][i][0])[nl * 8 + c / 2] = sum;
             }
+            settle();
             __syncthreads();
             // 32 sums of 16 tokens, two to a thread
 #pragma unroll
@@ -300,11 +308,11 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
                     out.bc[(((size_t)p.block * d.B + p.b) * d.T + t + token) * 2 * d.N + (i / 4 % 2 ? d.N : 0) + n] = sum;
             }
         }
-        settle();
         const size_t first = ((size_t)p.b * d.T + t) * d.D;
         const int room = p.t_end - t - 4 * nl;
-        auto put = [&](T* to, int r, float v) {
-            if (p.on && r < room) *reinterpret_cast<T*>(reinterpret_cast<char*>(to + first) + oy.at[r]) = from_f32<T>(r < rows ? v : 0.f);
+        const Memory to_x(out.x + first), to_dt(out.dt + first), to_gate(out.gate + first);
+        auto put = [&](const Memory& to, int r, float v) {
+            if (p.on && r < room) to.store(from_f32<T>(r < rows ? v : 0.f), oy.at[r]);
         };
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -315,11 +323,11 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
                 dskip = fmaf(dr[r], x[r], dskip);
                 dbias += ddt;
             }
-            put(out.x, r, dx);
-            put(out.dt, r, ddt);
+            put(to_x, r, dx);
+            put(to_dt, r, ddt);
             if (d.gate) {
                 const float sig = sigmoid_fast(z[r]);
-                put(out.gate, r, u[r] * fmaf(skip, x[r], read[r]) * sig * (1.f + z[r] * (1.f - sig)));
+                put(to_gate, r, u[r] * fmaf(skip, x[r], read[r]) * sig * (1.f + z[r] * (1.f - sig)));
             }
         }
     }
