@@ -105,10 +105,11 @@ struct Rows {
     }
 };
 
-// Adds, for each state of a block, a token's sum over the lanes of a channel to row t of c.
-__device__ __forceinline__ f32x4 add_row(float part, int t, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32((int)(threadIdx.x % 16) == t ? 1.f : 0.f, part, c, 0, 0, 0);
+// Adds a token's sum over the lanes of a channel to the row of c whose lanes `is` marks.
+__device__ __forceinline__ f32x4 add_row(float part, bool is, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(is ? 1.f : 0.f, part, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 // Waits until the last such sums are in their registers, before they are read in another
 // basic block than the instruction's (11 states: eight passes, and three to be read).
 __device__ __forceinline__ void settle() {

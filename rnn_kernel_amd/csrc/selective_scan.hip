@@ -12,7 +12,7 @@ namespace {
 template <typename T, int NB, bool STATES_ONLY>
 __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float* sums, const float* initial, T* y,
                                                    float* final_state, float* kept) {
-    __shared__ float2 steps[kTile][16];  // s, s x
+    __shared__ __attribute__((aligned(16))) float steps[16][2 * kTile + 4];  // of a channel: s; s x
     __shared__ __attribute__((aligned(16))) float bt[kTile][NB * 16], ct[STATES_ONLY ? 1 : kTile][NB * 16];
     const int lane = threadIdx.x, c = lane % 16, nl = lane / 16;
     const int Dg = d.D / d.G, per_group = (Dg - 1) / 16 + 1, blocks = d.G * per_group;
@@ -42,8 +42,8 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
     const T* px = static_cast<const T*>(d.x) + b * d.xs[0];
     const T* pt = static_cast<const T*>(d.dt) + b * d.ts[0];
     const T* pz = static_cast<const T*>(d.gate) + b * d.zs[0];
-    const T* pb = static_cast<const T*>(d.Bm) + b * d.bs[0] + g * d.bs[2];
-    const T* pc = static_cast<const T*>(d.C) + b * d.cs[0] + g * d.cs[2];
+    const T* gb = static_cast<const T*>(d.Bm) + b * d.bs[0] + g * d.bs[2];
+    const T* gc = static_cast<const T*>(d.C) + b * d.cs[0] + g * d.cs[2];
     T* py = STATES_ONLY ? nullptr : y + (size_t)b * d.T * d.D;
     Rows<T> x, dt, gate, bv[NB], cv[NB];
     Offsets ox, ot, oz, ob[NB], oc[NB], oy;
@@ -65,8 +65,8 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
         if (!STATES_ONLY && d.gate) gate.load(pz + t * d.zs[1], oz);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            bv[k].load(pb + t * d.bs[1], ob[k]);
-            if (!STATES_ONLY) cv[k].load(pc + t * d.cs[1], oc[k]);
+            bv[k].load(gb + t * d.bs[1], ob[k]);
+            if (!STATES_ONLY) cv[k].load(gc + t * d.cs[1], oc[k]);
         }
     };
     float sum = 0.f;
@@ -91,7 +91,8 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
             xf[r] = r < rows ? to_f32(x.v[r]) : 0.f;
             zf[r] = !STATES_ONLY && d.gate ? to_f32(gate.v[r]) : 0.f;
             sum += s;
-            steps[4 * nl + r][c] = float2{s, s * xf[r]};
+            steps[c][4 * nl + r] = s;
+            steps[c][kTile + 4 * nl + r] = s * xf[r];
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
                 bt[4 * nl + r][16 * k + c] = 16 * k + c < d.N ? to_f32(bv[k].v[r]) : 0.f;
@@ -101,22 +102,28 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
         __syncthreads();
         if (t + kTile < t1) load(t + kTile);
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int i = 0; i < kTile; ++i) {
-            const float2 s = steps[i][c];
-            float part = 0.f;
+        // (addresses from one place for four tokens: each array's own would cost an addition a token)
+        const float *ps = &steps[c][0], *pb = &bt[0][4 * nl], *pc = &ct[0][4 * nl];
+        int row = c;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q, ps += 4, pb += 64 * NB, pc += 64 * NB, row -= 4) {
+            const f32x4 s4 = load4(ps), i4 = load4(ps + kTile);
 #pragma unroll
-            for (int k = 0; k < NB; ++k) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(&bt[i][16 * k + 4 * nl]);
+            for (int i = 0; i < 4; ++i) {
+                float part = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) h[k][j] = fmaf(__builtin_amdgcn_exp2f(s.x * a2[k][j]), h[k][j], s.y * q[j]);
-                if (!STATES_ONLY) {
-                    const f32x4 p = *reinterpret_cast<const f32x4*>(&ct[i][16 * k + 4 * nl]);
+                for (int k = 0; k < NB; ++k) {
+                    const f32x4 bq = load4(pb + 16 * (NB * i + k));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) part = fmaf(p[j], h[k][j], part);
+                    for (int j = 0; j < 4; ++j) h[k][j] = fmaf(__builtin_amdgcn_exp2f(s4[i] * a2[k][j]), h[k][j], i4[i] * bq[j]);
+                    if (!STATES_ONLY) {
+                        const f32x4 cq = load4(pc + 16 * (NB * i + k));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) part = fmaf(cq[j], h[k][j], part);
+                    }
                 }
+                if (!STATES_ONLY) acc = add_row(part, row == i, acc);
             }
-            if (!STATES_ONLY) acc = add_row(part, i, acc);
         }
         if (!STATES_ONLY) {
             settle();

@@ -42,7 +42,7 @@ __device__ __forceinline__ Place place(const Dims& d, int width, int skipped) {
 // A chunk's own part of the gradient of the state at its start, and the sum of its steps.
 template <typename T, int NB>
 __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* own, float* sums) {
-    __shared__ float2 steps[kTile][16];  // s, r
+    __shared__ __attribute__((aligned(16))) float steps[16][2 * kTile + 4];  // of a channel: s; r
     __shared__ __attribute__((aligned(16))) float ct[kTile][NB * 16];
     const int lane = threadIdx.x, c = lane % 16, nl = lane / 16;
     const Place p = place(d, 16, 1);
@@ -92,21 +92,25 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
             float dr = pd ? to_f32(up.v[r]) : 0.f;
             if (d.gate) dr *= to_f32(gate.v[r]) * sigmoid_fast(to_f32(gate.v[r]));
             sum += s;
-            steps[row][c] = float2{s, live ? dr : 0.f};
+            steps[c][row] = s;
+            steps[c][kTile + row] = live ? dr : 0.f;
 #pragma unroll
             for (int k = 0; k < NB; ++k) ct[row][16 * k + c] = 16 * k + c < d.N ? to_f32(cv[k].v[r]) : 0.f;
         }
         __syncthreads();
         if (t > p.t0) load(t - kTile);
-#pragma unroll 4
-        for (int i = kTile - 1; i >= 0; --i) {
-            const float2 s = steps[i][c];
+        const float *ps = &steps[c][kTile - 4], *pq = &ct[kTile - 4][4 * nl];
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q, ps -= 4, pq -= 64 * NB) {
+            const f32x4 s4 = load4(ps), r4 = load4(ps + kTile);
 #pragma unroll
-            for (int k = 0; k < NB; ++k) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(&ct[i][16 * k + 4 * nl]);
+            for (int i = 3; i >= 0; --i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) dh[k][j] = fmaf(s.y, q[j], dh[k][j]) * __builtin_amdgcn_exp2f(s.x * a2[k][j]);
-            }
+                for (int k = 0; k < NB; ++k) {
+                    const f32x4 cq = load4(pq + 16 * (NB * i + k));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dh[k][j] = fmaf(r4[i], cq[j], dh[k][j]) * __builtin_amdgcn_exp2f(s4[i] * a2[k][j]);
+                }
         }
         __syncthreads();
     }
@@ -150,8 +154,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
     // The states before each token; then, in each token's first 32 numbers, its dB and dC
     // over the wavefront's channels.
     __shared__ __attribute__((aligned(16))) f32x4 before[kWaves][kTile][64];
-    __shared__ float2 steps[kWaves][kTile][16];  // s, r
-    __shared__ float inputs[kWaves][kTile][16];  // s x
+    __shared__ __attribute__((aligned(16))) float steps[kWaves][16][3 * kTile + (NB == 1 ? 8 : 0)];  // of a channel: s; r; s x (two workgroups to a CU up to NB 2)
     __shared__ __attribute__((aligned(16))) float bt[kTile][NB * 16], ct[kTile][NB * 16];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, nl = lane / 16;
     const Place p = place(d, kChannels, 0);
@@ -236,8 +239,9 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             z[r] = d.gate ? to_f32(gate.v[r]) : 0.f;
             u[r] = live && pd ? to_f32(up.v[r]) : 0.f;
             dr[r] = d.gate && live ? u[r] * z[r] * sigmoid_fast(z[r]) : u[r];
-            steps[wave][row][c] = float2{s[r], dr[r]};
-            inputs[wave][row][c] = s[r] * x[r];
+            steps[wave][c][row] = s[r];
+            steps[wave][c][kTile + row] = dr[r];
+            steps[wave][c][2 * kTile + row] = s[r] * x[r];
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
@@ -256,44 +260,53 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             if (k > 0) __syncthreads();  // the sums of the block before are out
             f32x4 hk = start[k];
             const int n0 = 16 * k + 4 * nl;
-#pragma unroll 4
-            for (int i = 0; i < kTile; ++i) {
-                const float2 sr = steps[wave][i][c];
-                const float in = inputs[wave][i][c];
-                const f32x4 bq = *reinterpret_cast<const f32x4*>(&bt[i][n0]), cq = *reinterpret_cast<const f32x4*>(&ct[i][n0]);
-                before[wave][i][lane] = hk;
-                float part = 0.f;
+            // (addresses from one place for four tokens: each array's own would cost an addition a token)
+            const float *ps = &steps[wave][c][0], *pbt = &bt[0][n0], *pct = &ct[0][n0];
+            f32x4* ph = &before[wave][0][lane];
+            float* sums = reinterpret_cast<float*>(&before[wave][0][0]) + nl * 8 + c / 2;
+            int row = c;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q, ps += 4, pbt += 64 * NB, pct += 64 * NB, ph += 4 * 64, row -= 4) {
+                const f32x4 s4 = load4(ps), i4 = load4(ps + 2 * kTile);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    hk[j] = fmaf(__builtin_amdgcn_exp2f(sr.x * a2[k][j]), hk[j], in * bq[j]);
-                    part = fmaf(cq[j], hk[j], part);
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 bq = load4(pbt + 16 * NB * i), cq = load4(pct + 16 * NB * i);
+                    ph[64 * i] = hk;
+                    float part = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        hk[j] = fmaf(__builtin_amdgcn_exp2f(s4[i] * a2[k][j]), hk[j], i4[i] * bq[j]);
+                        part = fmaf(cq[j], hk[j], part);
+                    }
+                    read = add_row(part, row == i, read);
                 }
-                read = add_row(part, i, read);
             }
-#pragma unroll 4
-            for (int i = kTile - 1; i >= 0; --i) {
-                const float2 sr = steps[wave][i][c];
-                const float in = inputs[wave][i][c];
-                const f32x4 bq = *reinterpret_cast<const f32x4*>(&bt[i][n0]), cq = *reinterpret_cast<const f32x4*>(&ct[i][n0]);
-                const f32x4 hp = before[wave][i][lane];
-                float of_b = 0.f, of_a = 0.f, v[8];
+            sums += kTile * 256;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+                ps -= 4, pbt -= 64 * NB, pct -= 64 * NB, ph -= 4 * 64, sums -= 4 * 256, row += 4;
+                const f32x4 s4 = load4(ps), r4 = load4(ps + kTile), i4 = load4(ps + 2 * kTile);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float full = fmaf(sr.y, cq[j], dh[k][j]);
-                    v[j] = in * full;
-                    v[4 + j] = sr.y * hk[j];
-                    of_b = fmaf(full, bq[j], of_b);
-                    dh[k][j] = full * __builtin_amdgcn_exp2f(sr.x * a2[k][j]);
-                    const float w = dh[k][j] * hp[j];
-                    of_a = fmaf(w, a2[k][j], of_a);
-                    da[k][j] = fmaf(w, sr.x, da[k][j]);
+                for (int i = 3; i >= 0; --i) {
+                    const f32x4 bq = load4(pbt + 16 * NB * i), cq = load4(pct + 16 * NB * i), hp = ph[64 * i];
+                    float of_b = 0.f, of_a = 0.f, v[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float full = fmaf(r4[i], cq[j], dh[k][j]);
+                        v[j] = i4[i] * full;
+                        v[4 + j] = r4[i] * hk[j];
+                        of_b = fmaf(full, bq[j], of_b);
+                        dh[k][j] = full * __builtin_amdgcn_exp2f(s4[i] * a2[k][j]);
+                        const float w = dh[k][j] * hp[j];
+                        of_a = fmaf(w, a2[k][j], of_a);
+                        da[k][j] = fmaf(w, s4[i], da[k][j]);
+                    }
+                    hk = hp;
+                    q1 = add_row(of_b, row == i, q1);
+                    q2 = add_row(of_a, row == i, q2);
+                    // (two lanes write the same: no branch between matrix instructions)
+                    sums[256 * i] = row_sums(v);
                 }
-                hk = hp;
-                q1 = add_row(of_b, i, q1);
-                q2 = add_row(of_a, i, q2);
-                const float sum = row_sums(v);
-                // (two lanes write the same: no branch between matrix instructions)
-                reinterpret_cast<float*>(&before[wave][i][0])[nl * 8 + c / 2] = sum;
             }
             settle();
             __syncthreads();
