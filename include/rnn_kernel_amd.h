@@ -499,7 +499,8 @@ int rka_layer_norm_backward(const void* grad_y, long long ldy, const void* x, lo
  * x [batch, tokens, channels] with dense channels, y [batch, tokens, channels] dense, weight
  * [channels, width], bias [channels] or NULL, states [batch, width - 1, channels] (the inputs
  * before the first token, or NULL for zeros; a row's last width - 1 inputs), all of `dtype`.
- * lengths as in rka_gated_delta_forward.  batch is at most 65535.  (The reference has none.)
+ * lengths as in rka_gated_delta_forward.  batch is at most 65535, tokens 2^20.  (The reference
+ * has none.)
  */
 int rka_causal_conv_forward(const void* x, long long x_batch_stride, long long x_token_stride, const void* weight,
                             const void* bias, const void* initial_state, const int* lengths, void* y, void* final_state,

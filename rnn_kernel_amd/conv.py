@@ -107,7 +107,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The convolution over whole sequences: ``(y, final_state)``.
 
-    x [B, T, D] of any strides, B at most 65535 and T below 2^22 - 64, weight [D, W] with W in
+    x [B, T, D] of any strides, B at most 65535 and T at most 2^20, weight [D, W] with W in
     [2, 8], bias [D] or None, initial_state [B, W - 1, D] (the inputs before the first token)
     or None (zeros), all float32 or all bfloat16; activation "silu" or None.  ``lengths`` [B]
     int32: row b ends after lengths[b] tokens; what lies behind is not read, its outputs and

@@ -4,11 +4,12 @@
 //   dz = dy act'(z);  dx_s = sum_j w_j dz_{s+W-1-j};  dw_j = sum_t dz_t x_{t-W+1+j};  db = sum dz
 // The final state is a row's last W - 1 inputs; its gradient adds to theirs.
 //
-// A thread takes 16 bytes of channels through a run of tokens, the last W - 1 inputs (and
-// in the backward the last dz) in registers.  Bound by memory.
+// A thread takes four channels through a run of tokens, whose inputs it loads at once: what it
+// needs of its neighbours' tokens it loads and makes again (from L2).  Bound by memory.
 #include "elementwise.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rka {
 namespace conv {
@@ -17,8 +18,11 @@ namespace {
 using namespace elem;
 
 constexpr int kMaxWidth = 8;
-constexpr int kLanes = 64, kRuns = 4;  // channel groups and runs of a workgroup
-constexpr int kForwardRun = 32, kBackwardRun = 32;
+constexpr int kLanes = 64, kRuns = 4;  // groups of channels and runs of a workgroup
+constexpr int kGroup = 4;              // channels of a thread
+// Tokens of a run, of the forward and of the backward with those before it whose dz it makes
+// again: 4 x 2048 tokens of 2048 channels are then some 4000 wavefronts.
+constexpr int kForwardRun = 16, kBackwardSpan = 16;
 
 struct Dims {
     int B, T, D, act;
@@ -32,156 +36,168 @@ __device__ __forceinline__ float slope(float z, int act) {
     return act == RKA_ACT_SILU ? s * (1.f + z * (1.f - s)) : 1.f;
 }
 
-template <typename T, int W>
+// Four channels of a token.
+template <typename T>
+struct Quad {
+    T e[kGroup];
+};
+// SMALL: there are fewer than four channels, `left`.
+template <bool SMALL, typename T>
+__device__ __forceinline__ Quad<T> load_quad(const T* p, int left) {
+    struct __attribute__((packed, aligned(2))) Bytes {
+        unsigned w[sizeof(T)];
+    };
+    Quad<T> q;
+    if constexpr (SMALL) {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) q.e[e] = p[min(e, left - 1)];
+    } else {
+        const Bytes b = *reinterpret_cast<const Bytes*>(p);
+        q = __builtin_bit_cast(Quad<T>, b);
+    }
+    return q;
+}
+template <bool SMALL, typename T>
+__device__ __forceinline__ void store_quad(T* p, const Quad<T>& q, int left) {
+    struct __attribute__((packed, aligned(2))) Bytes {
+        unsigned w[sizeof(T)];
+    };
+    if constexpr (SMALL) {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e)
+            if (e < left) p[e] = q.e[e];
+    } else {
+        *reinterpret_cast<Bytes*>(p) = __builtin_bit_cast(Bytes, q);
+    }
+}
+
+template <bool SMALL, typename T, int W>
 struct Weights {
-    float w[W][kVec<T>], b[kVec<T>];
+    float w[W][kGroup], b[kGroup];
 
     __device__ __forceinline__ void load(const T* weight, const T* bias, int d0, int left) {
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) {
-            const int d = d0 + min(e, left - 1);
+        for (int e = 0; e < kGroup; ++e) {
+            const int d = d0 + (SMALL ? min(e, left - 1) : e);
 #pragma unroll
             for (int j = 0; j < W; ++j) w[j][e] = to_f32(weight[(long long)d * W + j]);
             b[e] = bias ? to_f32(bias[d]) : 0.f;
         }
     }
-    __device__ __forceinline__ float z(const float (&x)[W][kVec<T>], int e) const {
+    // x: the token's input and the W - 1 before it
+    __device__ __forceinline__ float z(const Quad<T>* x, int e) const {
         float sum = b[e];
 #pragma unroll
-        for (int j = 0; j < W; ++j) sum = fmaf(w[j][e], x[j][e], sum);
+        for (int j = 0; j < W; ++j) sum = fmaf(w[j][e], to_f32(x[j].e[e]), sum);
         return sum;
     }
 };
 
-// Input t of a row with `len` tokens: from the initial state before the first, 0 behind the
-// last.
-template <typename T, int W>
-__device__ __forceinline__ Piece<T> input(const Dims& d, const T* x, const T* initial, int b, int t, int len, int d0, int left) {
-    if (t >= 0 && t < len) return load_piece(x + b * d.xb + t * d.xt + d0, left);
-    if (t >= -(W - 1) && t < 0 && initial) return load_piece(initial + ((long long)b * (W - 1) + t + W - 1) * d.D + d0, left);
-    Piece<T> none;
-    none.u = u32x4{0, 0, 0, 0};
-    return none;
+// A thread's channels: the last four again where fewer are left (two threads then make, and
+// write, the same).
+__device__ __forceinline__ int first_channel(int D) { return min((int)(blockIdx.x * kLanes + threadIdx.x) * kGroup, max(0, D - kGroup)); }
+__device__ __forceinline__ bool has_channels(int D) { return (long long)(blockIdx.x * kLanes + threadIdx.x) * kGroup < D; }
+
+// Input t of a row with `len` tokens, those behind the last as the last; before the first, from
+// the initial state, and before that 0.
+template <bool SMALL, typename T, int W>
+__device__ __forceinline__ Quad<T> input(const Dims& d, const T* x, const T* initial, int b, int t, int len, int d0) {
+    if (t >= 0 && len > 0) return load_quad<SMALL>(x + b * d.xb + min(t, len - 1) * d.xt + d0, d.D);
+    if (t < 0 && t >= -(W - 1) && initial) return load_quad<SMALL>(initial + ((long long)b * (W - 1) + t + W - 1) * d.D + d0, d.D);
+    return Quad<T>{};
 }
 
-template <typename T, int W>
+template <bool SMALL, typename T, int W>
 __global__ __launch_bounds__(kLanes* kRuns) void forward_kernel(Dims d, const T* x, const T* weight, const T* bias,
                                                                 const T* initial, T* y, T* final_state) {
-    constexpr int V = kVec<T>;
-    const int b = blockIdx.z, d0 = (blockIdx.x * kLanes + threadIdx.x) * V, left = d.D - d0;
-    const int run = blockIdx.y * kRuns + threadIdx.y;
-    const long long first = (long long)run * kForwardRun;
-    if (left <= 0 || first > d.T) return;
-    const int t0 = (int)first, t1 = min(d.T, t0 + min(kForwardRun, d.T - t0)), len = row_length(d.lengths, b, d.T);
+    const int b = blockIdx.z, d0 = first_channel(d.D), run = blockIdx.y * kRuns + __builtin_amdgcn_readfirstlane(threadIdx.y);
+    if (!has_channels(d.D) || (long long)run * kForwardRun > d.T) return;
+    const int t0 = run * kForwardRun, len = row_length(d.lengths, b, d.T);
     if (run == 0) {
 #pragma unroll
         for (int j = 0; j < W - 1; ++j)
-            store_piece(final_state + ((long long)b * (W - 1) + j) * d.D + d0,
-                        input<T, W>(d, x, initial, b, len - (W - 1) + j, len, d0, left), left);
+            store_quad<SMALL>(final_state + ((long long)b * (W - 1) + j) * d.D + d0,
+                              input<SMALL, T, W>(d, x, initial, b, len - (W - 1) + j, len, d0), d.D);
     }
     if (t0 >= d.T) return;
-    Weights<T, W> wt;
-    wt.load(weight, bias, d0, left);
-    float win[W][V];
+    Weights<SMALL, T, W> wt;
+    wt.load(weight, bias, d0, d.D);
+    Quad<T> in[kForwardRun + W - 1];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-        const Piece<T> p = input<T, W>(d, x, initial, b, t0 - (W - 1) + j, len, d0, left);
-#pragma unroll
-        for (int e = 0; e < V; ++e) win[j][e] = to_f32(p.e[e]);
-    }
+    for (int i = 0; i < kForwardRun + W - 1; ++i) in[i] = input<SMALL, T, W>(d, x, initial, b, t0 - (W - 1) + i, len, d0);
     T* py = y + ((long long)b * d.T + t0) * d.D + d0;
-#pragma unroll 4
-    for (int t = t0; t < t1; ++t, py += d.D) {
-        const Piece<T> p = input<T, W>(d, x, initial, b, t, len, d0, left);
-        Piece<T> out;
 #pragma unroll
-        for (int e = 0; e < V; ++e) win[W - 1][e] = to_f32(p.e[e]);
+    for (int i = 0; i < kForwardRun; ++i, py += d.D) {
+        if (t0 + i >= d.T) break;
+        Quad<T> out;
 #pragma unroll
-        for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(t < len ? activate(wt.z(win, e), d.act) : 0.f);
-        store_piece(py, out, left);
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) win[j][e] = win[j + 1][e];
+        for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(t0 + i < len ? activate(wt.z(in + i, e), d.act) : 0.f);
+        store_quad<SMALL>(py, out, d.D);
     }
 }
 
-// Run r takes the dz of tokens [r R, r R + R) of [0, T + W - 1) (those from the length on
-// are 0) and the dx that the last of them completes, those of tokens [r R - W + 1,
-// r R + R - W + 1), where tokens before 0 are the initial state's; the dz before its first
-// it makes again.  Sums of dw and db: [batch row][workgroup's runs][W + 1][channels].
-template <typename T, int W>
+// Run r takes the dz of R = kBackwardSpan - W + 1 tokens of [0, T + W - 1) (those from the
+// length on are 0) and the dx that they complete, of the tokens W - 1 before, where tokens before
+// 0 are the initial state's.  Sums of dw and db: [batch row][workgroup's runs][W + 1][channels].
+template <bool SMALL, typename T, int W>
 __global__ __launch_bounds__(kLanes* kRuns) void backward_kernel(Dims d, const T* dy, const T* dstate, const T* x,
                                                                  const T* weight, const T* bias, const T* initial, T* dx,
                                                                  T* dinitial, float* sums) {
-    constexpr int V = kVec<T>;
-    __shared__ float part[kRuns - 1][V][kLanes];
-    const int b = blockIdx.z, d0 = (blockIdx.x * kLanes + threadIdx.x) * V, left = d.D - d0;
+    constexpr int R = kBackwardSpan - W + 1;
+    __shared__ float part[kRuns - 1][kGroup][kLanes];
+    const int b = blockIdx.z, d0 = first_channel(d.D), wave = __builtin_amdgcn_readfirstlane(threadIdx.y);
+    const bool on = has_channels(d.D);
     const int len = row_length(d.lengths, b, d.T);
-    const long long first = (long long)(blockIdx.y * kRuns + threadIdx.y) * kBackwardRun;
-    float dw[W][V] = {}, db[V] = {};
-    if (left > 0 && first < (long long)d.T + W - 1) {
-        const int t0 = (int)first, t1 = (int)min(first + kBackwardRun, (long long)d.T + W - 1);
-        Weights<T, W> wt;
-        wt.load(weight, bias, d0, left);
-        float win[W][V], dz[W][V] = {};  // inputs up to t; dz up to t
+    const long long first = (long long)(blockIdx.y * kRuns + wave) * R;
+    float dw[W][kGroup] = {}, db[kGroup] = {};
+    if (on && first < (long long)d.T + W - 1) {
+        const int t0 = (int)first - (W - 1);  // the first whose dz is made
+        Weights<SMALL, T, W> wt;
+        wt.load(weight, bias, d0, d.D);
+        Quad<T> in[kBackwardSpan + W - 1], up[kBackwardSpan];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-            const Piece<T> p = input<T, W>(d, x, initial, b, t0 - 2 * (W - 1) + j, len, d0, left);
+        for (int i = 0; i < kBackwardSpan + W - 1; ++i) in[i] = input<SMALL, T, W>(d, x, initial, b, t0 - (W - 1) + i, len, d0);
+        const bool given = dy && len > 0;
+        if (given) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) win[j][e] = to_f32(p.e[e]);
+            for (int i = 0; i < kBackwardSpan; ++i)
+                up[i] = load_quad<SMALL>(dy + ((long long)b * d.T + max(0, min(t0 + i, len - 1))) * d.D + d0, d.D);
         }
-#pragma unroll 2
-        for (int t = t0 - (W - 1); t < t1; ++t) {
-            const Piece<T> p = input<T, W>(d, x, initial, b, t, len, d0, left);
+        float dz[kBackwardSpan][kGroup];
 #pragma unroll
-            for (int e = 0; e < V; ++e) win[W - 1][e] = to_f32(p.e[e]);
-            const bool on = t >= 0 && t < len && dy;
-            if (on) {
-                const Piece<T> g = load_piece(dy + ((long long)b * d.T + t) * d.D + d0, left);
+        for (int i = 0; i < kBackwardSpan; ++i) {
+            const int t = t0 + i;
+            const bool live = given && t >= 0 && t < len;
 #pragma unroll
-                for (int e = 0; e < V; ++e) dz[W - 1][e] = to_f32(g.e[e]) * slope(wt.z(win, e), d.act);
-            } else {
+            for (int e = 0; e < kGroup; ++e) dz[i][e] = live ? to_f32(up[i].e[e]) * slope(wt.z(in + i, e), d.act) : 0.f;
+            if (i < W - 1) continue;
+            if (live) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) dz[W - 1][e] = 0.f;
-            }
-            if (t >= t0) {
+                for (int e = 0; e < kGroup; ++e) {
+                    db[e] += dz[i][e];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    db[e] += dz[W - 1][e];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dz[W - 1][e], win[j][e], dw[j][e]);
-                }
-                const int s = t - (W - 1);
-                T* to = s >= 0 ? dx : dinitial;
-                if (to && s < d.T) {
-                    float sum[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        sum[e] = 0.f;
-#pragma unroll
-                        for (int j = 0; j < W; ++j) sum[e] = fmaf(wt.w[j][e], dz[W - 1 - j][e], sum[e]);
-                    }
-                    const int kept = s - (len - (W - 1));  // its place in the final state
-                    if (dstate && kept >= 0 && kept < W - 1) {
-                        const Piece<T> g = load_piece(dstate + ((long long)b * (W - 1) + kept) * d.D + d0, left);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) sum[e] += to_f32(g.e[e]);
-                    }
-                    Piece<T> out;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(sum[e]);
-                    to += s >= 0 ? ((long long)b * d.T + s) * d.D : ((long long)b * (W - 1) + s + W - 1) * d.D;
-                    store_piece(to + d0, out, left);
+                    for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dz[i][e], to_f32(in[i + j].e[e]), dw[j][e]);
                 }
             }
+            const int s = t - (W - 1);
+            T* to = s >= 0 ? dx : dinitial;
+            if (!to || s >= d.T) continue;
+            float sum[kGroup] = {};
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j)
+            for (int e = 0; e < kGroup; ++e)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    win[j][e] = win[j + 1][e];
-                    dz[j][e] = dz[j + 1][e];
-                }
+                for (int j = 0; j < W; ++j) sum[e] = fmaf(wt.w[j][e], dz[i - j][e], sum[e]);
+            const int kept = s - (len - (W - 1));  // its place in the final state
+            if (dstate && kept >= 0 && kept < W - 1) {
+                const Quad<T> g = load_quad<SMALL>(dstate + ((long long)b * (W - 1) + kept) * d.D + d0, d.D);
+#pragma unroll
+                for (int e = 0; e < kGroup; ++e) sum[e] += to_f32(g.e[e]);
+            }
+            Quad<T> out;
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(sum[e]);
+            to += s >= 0 ? ((long long)b * d.T + s) * d.D : ((long long)b * (W - 1) + s + W - 1) * d.D;
+            store_quad<SMALL>(to + d0, out, d.D);
         }
     }
     if (!sums) return;
@@ -190,18 +206,18 @@ __global__ __launch_bounds__(kLanes* kRuns) void backward_kernel(Dims d, const T
     for (int j = 0; j <= W; ++j) {
         float* own = j < W ? dw[j < W ? j : 0] : db;
         __syncthreads();
-        if (threadIdx.y > 0) {
+        if (wave > 0) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) part[threadIdx.y - 1][e][threadIdx.x] = own[e];
+            for (int e = 0; e < kGroup; ++e) part[wave - 1][e][threadIdx.x] = own[e];
         }
         __syncthreads();
-        if (threadIdx.y == 0) {
+        if (wave == 0 && on) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
+            for (int e = 0; e < kGroup; ++e) {
                 float s = own[e];
 #pragma unroll
                 for (int k = 0; k < kRuns - 1; ++k) s += part[k][e][threadIdx.x];
-                if (e < left) to[(long long)j * d.D + e] = s;
+                if (!SMALL || e < d.D) to[(long long)j * d.D + e] = s;
             }
         }
     }
@@ -229,58 +245,56 @@ __global__ __launch_bounds__(256) void sums_kernel(const float* sums, int count,
     }
 }
 
-template <typename T, int W>
+// (in place, so that no channel has two threads: element by element where the last of them would
+// have fewer than four)
+template <bool SMALL, typename T, int W>
 __global__ __launch_bounds__(kLanes) void step_kernel(int B, int D, int act, const T* x, long long ldx, const T* weight,
                                                       const T* bias, T* state, const int* slots, int num_slots, T* y) {
-    constexpr int V = kVec<T>;
-    const int groups = (D - 1) / (kLanes * V) + 1;
-    const int b = blockIdx.x / groups, d0 = (blockIdx.x % groups * kLanes + threadIdx.x) * V, left = D - d0;
+    const int groups = (D - 1) / (kLanes * kGroup) + 1;
+    const int b = blockIdx.x / groups, d0 = (blockIdx.x % groups * kLanes + threadIdx.x) * kGroup, left = D - d0;
     if (left <= 0) return;
     const int slot = slots ? slots[b] : b;
-    Piece<T> out;
+    Quad<T> out;
     T* py = y + (long long)b * D + d0;
     if (slot < 0 || slot >= num_slots) {
         // a request without a state: nothing is read or written but its output
 #pragma unroll
-        for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(slot < 0 ? 0.f : __builtin_nanf(""));
-        store_piece(py, out, left);
+        for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(slot < 0 ? 0.f : __builtin_nanf(""));
+        store_quad<SMALL>(py, out, left);
         return;
     }
     T* ps = state + (long long)slot * (W - 1) * D + d0;
-    Piece<T> p[W];
+    Quad<T> p[W];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) p[j] = load_piece(ps + (long long)j * D, left);
-    p[W - 1] = load_piece(x + b * ldx + d0, left);
-    Weights<T, W> wt;
+    for (int j = 0; j < W - 1; ++j) p[j] = load_quad<SMALL>(ps + (long long)j * D, left);
+    p[W - 1] = load_quad<SMALL>(x + b * ldx + d0, left);
+    Weights<SMALL, T, W> wt;
     wt.load(weight, bias, d0, left);
-    float win[W][V];
 #pragma unroll
-    for (int j = 0; j < W; ++j)
+    for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(activate(wt.z(p, e), act));
+    store_quad<SMALL>(py, out, left);
 #pragma unroll
-        for (int e = 0; e < V; ++e) win[j][e] = to_f32(p[j].e[e]);
-#pragma unroll
-    for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(activate(wt.z(win, e), act));
-    store_piece(py, out, left);
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_piece(ps + (long long)j * D, p[j + 1], left);
+    for (int j = 0; j < W - 1; ++j) store_quad<SMALL>(ps + (long long)j * D, p[j + 1], left);
 }
 
+// Calls f with `small` and the width as constants.
 template <typename F>
-int with_width(int width, F f) {
+int with_form(bool small, int width, F f) {
+    const auto go = [&](auto w) { return small ? f(std::true_type{}, w) : f(std::false_type{}, w); };
     switch (width) {
-        case 2: return f(std::integral_constant<int, 2>{});
-        case 3: return f(std::integral_constant<int, 3>{});
-        case 4: return f(std::integral_constant<int, 4>{});
-        case 5: return f(std::integral_constant<int, 5>{});
-        case 6: return f(std::integral_constant<int, 6>{});
-        case 7: return f(std::integral_constant<int, 7>{});
-        default: return f(std::integral_constant<int, 8>{});
+        case 2: return go(std::integral_constant<int, 2>{});
+        case 3: return go(std::integral_constant<int, 3>{});
+        case 4: return go(std::integral_constant<int, 4>{});
+        case 5: return go(std::integral_constant<int, 5>{});
+        case 6: return go(std::integral_constant<int, 6>{});
+        case 7: return go(std::integral_constant<int, 7>{});
+        default: return go(std::integral_constant<int, 8>{});
     }
 }
 
 int blocks_of_runs(long long tokens, int run) { return (int)((std::max(tokens, 1LL) - 1) / ((long long)run * kRuns) + 1); }
-dim3 grid(const Dims& d, int esize, int run_blocks) {
-    return dim3((unsigned)((d.D - 1) / (kLanes * (16 / esize)) + 1), (unsigned)run_blocks, (unsigned)d.B);
+dim3 grid(const Dims& d, int run_blocks) {
+    return dim3((unsigned)((d.D - 1) / (kLanes * kGroup) + 1), (unsigned)run_blocks, (unsigned)d.B);
 }
 // (65535 is the most of a grid's second and third size)
 int check_sizes(const char* what, const Dims& d, int width, int dtype) {
@@ -288,17 +302,17 @@ int check_sizes(const char* what, const Dims& d, int width, int dtype) {
     if (d.B < 0 || d.T < 0 || d.D < 1) return fail(RKA_ERR_INVALID_ARGUMENT, name + ": batch and tokens must be >= 0, channels >= 1");
     if (width < 2 || width > kMaxWidth) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": width must be in [2, 8]");
     if (d.act != RKA_ACT_NONE && d.act != RKA_ACT_SILU) return fail(RKA_ERR_INVALID_ARGUMENT, name + ": activation must be none or silu");
-    if (d.B > 65535 || d.T > 65535 * 64) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": batch exceeds 65535 or tokens 2^22 - 64");
+    if (d.B > 65535 || d.T > (1 << 20)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": batch exceeds 65535 or tokens 2^20");
     return check_dtype(dtype, what);
 }
 
 template <typename T>
 int forward(const Dims& d, const void* x, const void* weight, const void* bias, const void* initial, void* y,
             void* final_state, int width, hipStream_t s) {
-    const dim3 blocks = grid(d, sizeof(T), blocks_of_runs(d.T, kForwardRun));
+    const dim3 blocks = grid(d, blocks_of_runs(d.T, kForwardRun));
     RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_forward"));
-    return with_width(width, [&](auto w) {
-        hipLaunchKernelGGL((forward_kernel<T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d, static_cast<const T*>(x), static_cast<const T*>(weight),
+    return with_form(d.D < kGroup, width, [&](auto small, auto w) {
+        hipLaunchKernelGGL((forward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d, static_cast<const T*>(x), static_cast<const T*>(weight),
                            static_cast<const T*>(bias), static_cast<const T*>(initial), static_cast<T*>(y),
                            static_cast<T*>(final_state));
         RKA_RETURN_IF_HIP(hipGetLastError());
@@ -310,12 +324,12 @@ template <typename T>
 int backward(const Dims& d, const void* dy, const void* dstate, const void* x, const void* weight, const void* bias,
              const void* initial, void* dx, void* dweight, void* dbias, void* dinitial, float* sums, int width,
              hipStream_t s) {
-    const int runs = blocks_of_runs((long long)d.T + width - 1, kBackwardRun);
+    const int runs = blocks_of_runs((long long)d.T + width - 1, kBackwardSpan - width + 1);
     if (!dweight && !dbias) sums = nullptr;
-    const dim3 blocks = grid(d, sizeof(T), runs);
+    const dim3 blocks = grid(d, runs);
     RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_backward"));
-    RKA_RETURN_IF_ERR(with_width(width, [&](auto w) {
-        hipLaunchKernelGGL((backward_kernel<T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d,
+    RKA_RETURN_IF_ERR(with_form(d.D < kGroup, width, [&](auto small, auto w) {
+        hipLaunchKernelGGL((backward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d,
                            static_cast<const T*>(dy), static_cast<const T*>(dstate), static_cast<const T*>(x),
                            static_cast<const T*>(weight), static_cast<const T*>(bias), static_cast<const T*>(initial),
                            static_cast<T*>(dx), static_cast<T*>(dinitial), sums);
@@ -333,10 +347,10 @@ int backward(const Dims& d, const void* dy, const void* dstate, const void* x, c
 template <typename T>
 int step(int B, int D, int act, const void* x, long long ldx, const void* weight, const void* bias, void* state,
          const int* slots, int num_slots, void* y, int width, hipStream_t s) {
-    const long long blocks = (long long)B * ((D - 1) / (kLanes * kVec<T>) + 1);
+    const long long blocks = (long long)B * ((D - 1) / (kLanes * kGroup) + 1);
     RKA_RETURN_IF_ERR(check_grid(blocks, kLanes, "causal_conv_step"));
-    return with_width(width, [&](auto w) {
-        hipLaunchKernelGGL((step_kernel<T, decltype(w)::value>), dim3((unsigned)blocks), dim3(kLanes), 0, s, B, D, act,
+    return with_form(D % kGroup != 0, width, [&](auto small, auto w) {
+        hipLaunchKernelGGL((step_kernel<decltype(small)::value, T, decltype(w)::value>), dim3((unsigned)blocks), dim3(kLanes), 0, s, B, D, act,
                            static_cast<const T*>(x), ldx, static_cast<const T*>(weight), static_cast<const T*>(bias),
                            static_cast<T*>(state), slots, num_slots, static_cast<T*>(y));
         RKA_RETURN_IF_HIP(hipGetLastError());
@@ -369,7 +383,7 @@ int rka_causal_conv_forward(const void* x, long long x_batch_stride, long long x
 
 size_t rka_causal_conv_backward_workspace_bytes(int batch, int tokens, int channels, int width) {
     if (batch < 1 || tokens < 0 || channels < 1 || width < 2 || width > kMaxWidth) return 0;
-    return (size_t)batch * blocks_of_runs((long long)tokens + width - 1, kBackwardRun) * (width + 1) * channels * sizeof(float);
+    return (size_t)batch * blocks_of_runs((long long)tokens + width - 1, kBackwardSpan - width + 1) * (width + 1) * channels * sizeof(float);
 }
 
 int rka_causal_conv_backward(const void* grad_y, const void* grad_final_state, const void* x, long long x_batch_stride,
