@@ -85,14 +85,16 @@ __global__ __launch_bounds__(1024) void number_kernel(const I* target, long long
     if (tid == 0) *r.count = base;
 }
 
-// The numbered rows of x, padded with zeros to `width`.
+// The numbered rows of x, padded with zeros to `width`, and rows of zeros behind them to the end
+// of the largest tile: their logits are numbers.
 template <typename T>
-__global__ __launch_bounds__(256) void gather_kernel(const T* x, long long ldx, int inputs, int width, Rows r, T* out) {
+__global__ __launch_bounds__(256) void gather_kernel(const T* x, long long ldx, int inputs, int width, int rows, Rows r, T* out) {
     const int n = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
-    if (n >= *r.count) return;
-    const T* p = x + r.from[n] * ldx;
+    const int live = *r.count;
+    if (n >= min(rows, (live + 255) / 256 * 256)) return;
+    const T* p = x + (n < live ? r.from[n] : 0) * ldx;
     for (int k = lane * kVec<T>; k < width; k += 64 * kVec<T>)
-        store_piece(out + (size_t)n * width + k, load_piece(p + k, inputs - k), kVec<T>);
+        store_piece(out + (size_t)n * width + k, load_piece(p + k, n < live ? inputs - k : 0), kVec<T>);
 }
 
 // Rows (numbered ones where `r.from` is set, else `first` on) as columns: out[k][row], zeros
@@ -154,11 +156,19 @@ struct Logits : Product {
 
     template <typename T, int WM, int WN>
     __device__ __forceinline__ void put(const f32x16 (&acc)[WM / 32][WN / 32], float*, int row0, int col0, int) const {
+        if (col0 >= n) return;
+        if (!bias && col0 + WN <= n)
+            of_tile<true, T, WM, WN>(acc, row0, col0);
+        else
+            of_tile<false, T, WM, WN>(acc, row0, col0);
+    }
+    // PLAIN: no bias, and every column is the vocabulary's.
+    template <bool PLAIN, typename T, int WM, int WN>
+    __device__ __forceinline__ void of_tile(const f32x16 (&acc)[WM / 32][WN / 32], int row0, int col0) const {
         constexpr int MB = WM / 32, NB = WN / 32;
         const int live = live_rows(), i32 = threadIdx.x % 32;
-        if (col0 >= n) return;
         Bias<T, NB> b;
-        b.load(bias, col0, n);
+        if (!PLAIN) b.load(bias, col0, n);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
             const int row = row0 + 32 * i + i32;
@@ -168,7 +178,7 @@ struct Logits : Product {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
                     // (a sum past the last column is another column's again: finite or not, it is not one)
-                    l[j][x] = b.b[j][x] == -INFINITY ? -INFINITY : acc[i][j][x] + b.b[j][x];
+                    l[j][x] = PLAIN ? acc[i][j][x] : b.b[j][x] == -INFINITY ? -INFINITY : acc[i][j][x] + b.b[j][x];
                     top = fmaxf(top, l[j][x]);  // (NaN comes back in the sum)
                 }
             top *= kLog2e;
@@ -209,19 +219,28 @@ struct Slopes : Product {
 
     template <typename T, int WM, int WN>
     __device__ __forceinline__ void put(const f32x16 (&acc)[WM / 32][WN / 32], float* out, int row0, int col0, int) const {
+        if (row0 >= ldt || col0 >= ld) return;
+        if (!bias && col0 + WN <= n)
+            of_tile<true, T, WM, WN>(acc, out, row0, col0);
+        else
+            of_tile<false, T, WM, WN>(acc, out, row0, col0);
+    }
+    // PLAIN: no bias, and every column is the vocabulary's.
+    template <bool PLAIN, typename T, int WM, int WN>
+    __device__ __forceinline__ void of_tile(const f32x16 (&acc)[WM / 32][WN / 32], float* out, int row0, int col0) const {
         constexpr int MB = WM / 32, NB = WN / 32, kLd = WN + 4, kV = kVec<T>, kLanes = WN / kV, kRows = 64 / kLanes;
         const int live = live_rows(), lane = threadIdx.x % 64, i32 = lane % 32;
-        if (row0 >= ldt || col0 >= ld) return;
         Bias<T, NB> b;
-        b.load(bias, col0, n);
+        if (!PLAIN) b.load(bias, col0, n);
         float total[kV] = {};
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
             const int row = row0 + 32 * i + i32, at = min(row, live - 1);
             const int target = r.target[at];
-            float scale = of_rows ? grad[r.from[at]] : grad[0];
+            // (a row behind the last has a logit of 0 and this scale)
+            float scale = row >= live ? 0.f : of_rows ? grad[r.from[at]] : grad[0];
             if (mean) scale /= (float)live;
-            if (target < 0) scale = __builtin_nanf("");
+            if (target < 0 && row < live) scale = __builtin_nanf("");
             const float lse = r.lse[at];
             const int t = target - first - col0;
             __builtin_amdgcn_wave_barrier();
@@ -232,12 +251,14 @@ struct Slopes : Product {
                     f32x4 v;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float of = b.b[j][4 * q + e], p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e] + of, kLog2e, -lse));
-                        const int col = column(j, q, e);
-                        v[e] = row < live && col0 + col < n ? (p - (t == col ? 1.f : 0.f)) * scale : 0.f;
+                        const float l = PLAIN ? acc[i][j][4 * q + e] : acc[i][j][4 * q + e] + b.b[j][4 * q + e];
+                        v[e] = __builtin_amdgcn_exp2f(fmaf(l, kLog2e, -lse)) * scale;
+                        if (!PLAIN && (row >= live || col0 + column(j, q, e) >= n)) v[e] = 0.f;
                     }
                     *reinterpret_cast<f32x4*>(out + i32 * kLd + column(j, q, 0)) = v;
                 }
+            __builtin_amdgcn_wave_barrier();
+            if (row < live && t >= 0 && t < WN && lane < 32) out[i32 * kLd + t] -= scale;
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int x = 0; x < 32 / kRows; ++x) {
@@ -254,7 +275,8 @@ struct Slopes : Product {
             }
 #pragma unroll 1
             for (int x = lane; x < WN * 32 / kV; x += 64) {
-                const int c = x % WN, y = x / WN * kV;
+                // (neighbouring lanes along a column's 32 rows)
+                const int c = x / (32 / kV), y = x % (32 / kV) * kV;
                 Piece<T> p;
 #pragma unroll
                 for (int e = 0; e < kV; ++e) p.e[e] = from_f32<T>(out[(y + e) * kLd + c]);
@@ -492,7 +514,7 @@ int blocks_of(long long items) { return (int)std::max(1LL, std::min((items + 255
 
 template <typename T>
 int gather(const Sizes& z, const Rows& r, const T* x, long long ldx, T* out, hipStream_t s) {
-    hipLaunchKernelGGL((gather_kernel<T>), dim3((z.m - 1) / 4 + 1), dim3(256), 0, s, x, ldx, z.k, z.width, r, out);
+    hipLaunchKernelGGL((gather_kernel<T>), dim3((z.m - 1) / 4 + 1), dim3(256), 0, s, x, ldx, z.k, z.width, z.m, r, out);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
 }
