@@ -56,7 +56,11 @@ def check_row_ints(what: str, t, name: str, batch: int, device) -> None:
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def dense_last(t):

@@ -26,6 +26,13 @@ _ACTS = {None: 0, "none": 0, "silu": 3}
 
 
 def _check(what: str, x, weight, bias, activation, lead: int) -> None:
+    # (a call is a few us of the host: one expression for all that is right)
+    dtype, index, shape, of = x.dtype, x.get_device(), x.shape, weight.shape
+    if (x.is_cuda and dtype in _args.DTYPES and weight.dtype is dtype and weight.get_device() == index and activation in _ACTS
+            and len(shape) == lead + 1 and len(of) == 2 and of[0] == shape[-1] >= 1 and MIN_CONV_WIDTH <= of[1] <= MAX_CONV_WIDTH
+            and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == of[:1]))
+            and max(shape) <= _args.MAX_SIZE):
+        return
     _args.check_dtype(what, x, "x")
     _args.check_tensors(what, x, (weight, "weight", x.dtype), (bias, "bias", x.dtype))
     if x.dim() != lead + 1 or x.size(-1) < 1:
@@ -133,22 +140,27 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     _lib.refuse_tangents(what, x, state, weight, bias)
     _check(what, x, weight, bias, activation, 1)
     batch, channels = x.shape
-    width = weight.size(1)
-    _args.check_tensors(what, x, (state, "state", x.dtype))
-    if state.dim() != 3 or tuple(state.shape[1:]) != (width - 1, channels):
+    width, of = weight.size(1), state.shape
+    if len(of) != 3 or of[1] != width - 1 or of[2] != channels or state.dtype is not x.dtype or state.get_device() != x.get_device():
+        _args.check_tensors(what, x, (state, "state", x.dtype))
         raise ValueError(f"{what}: state must have shape [slots, {width - 1}, {channels}]")
-    _args.check_sizes(what, state)
+    slots_held = of[0]
+    if slots_held > _args.MAX_SIZE:
+        raise ValueError(f"{what}: sizes must be below 2^31")
     if not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous")
-    if _args.wants_grad(x, state, weight, bias):
+    if torch.is_grad_enabled() and _args.wants_grad(x, state, weight, bias):
         raise RuntimeError(f"{what} has no gradients; use causal_conv or torch.no_grad()")
-    _args.check_row_ints(what, slots, "slots", batch, x.device)
-    if slots is None and state.size(0) < batch:
+    if slots is not None:
+        _args.check_row_ints(what, slots, "slots", batch, x.device)
+        slots = slots.contiguous()
+    elif slots_held < batch:
         raise ValueError(f"{what}: fewer states than requests")
-    x, weight, bias, slots = _args.dense_last(x), _args.dense(weight), _args.dense(bias), _args.dense(slots)
-    y = torch.empty(batch, channels, dtype=x.dtype, device=x.device)
+    x, weight = _args.dense_last(x), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = x.new_empty((batch, channels))
     _lib.call(x.get_device(), "rka_causal_conv_step", x.data_ptr(), x.stride(0), weight.data_ptr(), _lib.ptr(bias),
-              state.data_ptr(), _lib.ptr(slots), state.size(0), y.data_ptr(), batch, channels, width, _ACTS[activation],
+              state.data_ptr(), _lib.ptr(slots), slots_held, y.data_ptr(), batch, channels, width, _ACTS[activation],
               _args.DTYPES[x.dtype])
     torch.autograd.graph.increment_version(state)  # (a graph that saved it would be wrong)
     return y

@@ -29,12 +29,32 @@ MAX_TOKENS = 2 ** 30
 MAX_TOKEN_STRIDE = 2 ** 21  # elements: the kernels' offsets within a tile are 32-bit
 
 
+def _fits(x, dt, A, B, C, skip, gate, dt_bias, lead: int) -> bool:
+    """Whether the arguments are what the operators take (a call is a few us of the host: one
+    expression for all that is right, `_check` to say what is not)."""
+    dtype, index, shape = x.dtype, x.get_device(), x.shape
+    a, b = A.shape, B.shape
+    if len(shape) != lead + 1 or len(a) != 2 or len(b) != lead + 2 or dtype not in _args.DTYPES or not x.is_cuda:
+        return False
+    channels, states, groups = shape[lead], a[1], b[lead]
+    return (index == dt.get_device() == A.get_device() == B.get_device() == C.get_device()
+            and dt.dtype is dtype and B.dtype is dtype and C.dtype is dtype and A.dtype is torch.float32
+            and dt.shape == shape and C.shape == b and b[:lead] == shape[:lead] and b[lead + 1] == states
+            and a[0] == channels and 1 <= states <= MAX_STATES and 1 <= channels <= MAX_TOKEN_STRIDE and groups >= 1
+            and channels % groups == 0 and (lead == 1 or shape[1] <= MAX_TOKENS) and shape[0] <= _args.MAX_SIZE
+            and (gate is None or (gate.shape == shape and gate.dtype is dtype and gate.get_device() == index))
+            and (skip is None or (skip.shape == a[:1] and skip.dtype is torch.float32 and skip.get_device() == index))
+            and (dt_bias is None or (dt_bias.shape == a[:1] and dt_bias.dtype is torch.float32 and dt_bias.get_device() == index)))
+
+
 def _check(what: str, x, dt, A, B, C, skip, gate, dt_bias, tokens: bool) -> None:
+    lead = 2 if tokens else 1
+    if _fits(x, dt, A, B, C, skip, gate, dt_bias, lead):
+        return
     _args.check_dtype(what, x, "x")
     f32 = torch.float32
     _args.check_tensors(what, x, (dt, "dt", x.dtype), (A, "A", f32), (B, "B", x.dtype), (C, "C", x.dtype), (skip, "skip", f32),
                         (gate, "gate", x.dtype), (dt_bias, "dt_bias", f32))
-    lead = 2 if tokens else 1
     if x.dim() != lead + 1 or x.size(-1) < 1:
         raise ValueError(f"{what}: x must have shape {'[batch, tokens, channels]' if tokens else '[batch, channels]'}")
     channels = x.size(-1)
@@ -49,11 +69,11 @@ def _check(what: str, x, dt, A, B, C, skip, gate, dt_bias, tokens: bool) -> None
         _args.check_shape(what, t, name, x.shape)
     for t, name in ((skip, "skip"), (dt_bias, "dt_bias")):
         _args.check_shape(what, t, name, (channels,))
-    _args.check_sizes(what, x)
     if channels > MAX_TOKEN_STRIDE:
         raise ValueError(f"{what}: at most 2^21 channels")
     if tokens and x.size(1) > MAX_TOKENS:
         raise ValueError(f"{what}: at most 2^30 tokens")
+    raise ValueError(f"{what}: sizes must be below 2^31")
 
 
 def _near(t):
@@ -180,27 +200,34 @@ def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     on, inputs that require them are refused, and so are forward-mode tangents.  Autograd
     counts the call as a change of ``state``."""
     what = "selective_step"
-    inputs = (x, dt, A, B, C, state, skip, gate, dt_bias)
-    _lib.refuse_tangents(what, *inputs)
+    _lib.refuse_tangents(what, x, dt, A, B, C, state, skip, gate, dt_bias)
     _check(what, x, dt, A, B, C, skip, gate, dt_bias, tokens=False)
     batch, channels = x.shape
-    groups, states = B.shape[1:]
-    _args.check_tensors(what, x, (state, "state", torch.float32))
-    if state.dim() != 3 or tuple(state.shape[1:]) != (channels, states):
+    _, groups, states = B.shape
+    of = state.shape
+    if len(of) != 3 or of[1] != channels or of[2] != states or state.dtype is not torch.float32 or state.get_device() != x.get_device():
+        _args.check_tensors(what, x, (state, "state", torch.float32))
         raise ValueError(f"{what}: state must have shape [slots, {channels}, {states}]")
-    _args.check_sizes(what, state)
+    slots_held = of[0]
+    if slots_held > _args.MAX_SIZE:
+        raise ValueError(f"{what}: sizes must be below 2^31")
     if not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous")
-    if _args.wants_grad(*inputs):
+    if torch.is_grad_enabled() and _args.wants_grad(x, dt, A, B, C, state, skip, gate, dt_bias):
         raise RuntimeError(f"{what} has no gradients; use selective_scan or torch.no_grad()")
-    _args.check_row_ints(what, slots, "slots", batch, x.device)
-    if slots is None and state.size(0) < batch:
+    if slots is not None:
+        _args.check_row_ints(what, slots, "slots", batch, x.device)
+        slots = slots.contiguous()
+    elif slots_held < batch:
         raise ValueError(f"{what}: fewer states than requests")
-    x, dt, gate, B, C = (_args.dense_last(t) for t in (x, dt, gate, B, C))
-    A, skip, dt_bias, slots = (_args.dense(t) for t in (A, skip, dt_bias, slots))
-    y = torch.empty(batch, channels, dtype=x.dtype, device=x.device)
+    last = _args.dense_last
+    x, dt, B, C, A = last(x), last(dt), last(B), last(C), A.contiguous()
+    gate = None if gate is None else last(gate)
+    skip = None if skip is None else skip.contiguous()
+    dt_bias = None if dt_bias is None else dt_bias.contiguous()
+    y = x.new_empty((batch, channels))
     _lib.call(x.get_device(), "rka_selective_step", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
-              _lib.ptr(skip), _lib.ptr(gate), _lib.ptr(dt_bias), state.data_ptr(), _lib.ptr(slots), state.size(0), y.data_ptr(),
+              _lib.ptr(skip), _lib.ptr(gate), _lib.ptr(dt_bias), state.data_ptr(), _lib.ptr(slots), slots_held, y.data_ptr(),
               batch, channels, states, groups, _strides(x, dt, gate, B, C), int(softplus), _args.DTYPES[x.dtype])
     torch.autograd.graph.increment_version(state)  # (a graph that saved it would be wrong)
     return y
