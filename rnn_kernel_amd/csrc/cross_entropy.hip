@@ -169,6 +169,9 @@ struct Logits : Product {
         const int live = live_rows(), i32 = threadIdx.x % 32;
         Bias<T, NB> b;
         if (!PLAIN) b.load(bias, col0, n);
+        int target[MB];  // (at once, ahead of what it is needed for)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) target[i] = r.target[min(row0 + 32 * i + i32, live - 1)];
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
             const int row = row0 + 32 * i + i32;
@@ -193,7 +196,7 @@ struct Logits : Product {
             sum += __shfl_xor(sum, 32);
             if (row >= live) continue;
             if (threadIdx.x % 64 < 32) stats[(size_t)(col0 / WN) * m + row] = float2{both, sum};
-            const int t = r.target[row] - col0;
+            const int t = target[i] - col0;
             if (t >= 0 && t < WN) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
@@ -232,17 +235,24 @@ struct Slopes : Product {
         const int live = live_rows(), lane = threadIdx.x % 64, i32 = lane % 32;
         Bias<T, NB> b;
         if (!PLAIN) b.load(bias, col0, n);
-        float total[kV] = {};
+        float total[kV] = {}, scales[MB], lses[MB];
+        int targets[MB];
+        // (ahead of all that goes through LDS: their latency is waited for once)
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
             const int row = row0 + 32 * i + i32, at = min(row, live - 1);
-            const int target = r.target[at];
+            targets[i] = r.target[at];
+            lses[i] = r.lse[at];
             // (a row behind the last has a logit of 0 and this scale)
-            float scale = row >= live ? 0.f : of_rows ? grad[r.from[at]] : grad[0];
+            scales[i] = row >= live ? 0.f : of_rows ? grad[r.from[at]] : grad[0];
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int row = row0 + 32 * i + i32, t = targets[i] - first - col0;
+            float scale = scales[i];
             if (mean) scale /= (float)live;
-            if (target < 0 && row < live) scale = __builtin_nanf("");
-            const float lse = r.lse[at];
-            const int t = target - first - col0;
+            if (targets[i] < 0 && row < live) scale = __builtin_nanf("");
+            const float lse = lses[i];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int j = 0; j < NB; ++j)
@@ -260,7 +270,7 @@ struct Slopes : Product {
             __builtin_amdgcn_wave_barrier();
             if (row < live && t >= 0 && t < WN && lane < 32) out[i32 * kLd + t] -= scale;
             __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
+#pragma unroll 2
             for (int x = 0; x < 32 / kRows; ++x) {
                 const int y = x * kRows + lane / kLanes, c = lane % kLanes * kV;
                 Piece<T> p;
@@ -273,10 +283,10 @@ struct Slopes : Product {
                 if (row0 + 32 * i + y < live && col0 + c < ld)
                     store16(static_cast<T*>(dl) + (row0 + 32 * i + y) * ld + col0 + c, p.u);
             }
-#pragma unroll 1
-            for (int x = lane; x < WN * 32 / kV; x += 64) {
+#pragma unroll 2
+            for (int z = 0; z < WN * 32 / kV / 64; ++z) {
                 // (neighbouring lanes along a column's 32 rows)
-                const int c = x / (32 / kV), y = x % (32 / kV) * kV;
+                const int x = z * 64 + lane, c = x / (32 / kV), y = x % (32 / kV) * kV;
                 Piece<T> p;
 #pragma unroll
                 for (int e = 0; e < kV; ++e) p.e[e] = from_f32<T>(out[(y + e) * kLd + c]);
