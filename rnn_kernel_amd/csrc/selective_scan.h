@@ -19,10 +19,10 @@
 //
 // A wavefront takes 16 channels through tiles of 16 tokens: lane l has channel l % 16 and of
 // every 16 states the four from 4 (l / 16) on.  What a tile needs of its tokens is loaded and
-// made by all lanes at once, a lane four tokens of its channel, as the 16x16x4 float32 matrix
-// instruction's result lies in registers, and handed round through LDS.  That instruction
-// adds a token's sums over n up: its second operand are the lanes' parts, its first is 1 in
-// the token's row and 0 in the others, so that tile's sums end where its x and gate are.
+// made by all lanes at once, a lane four tokens of its channel, and handed round through LDS.
+// A token's sums over n are added up between the four lanes of a channel for four tokens at a
+// time, by exchanges of half of the lanes after which each lane holds one token's: 2.5
+// instructions a token, and the tile's sums end where its x and gate are.
 #pragma once
 
 #include "elementwise.h"
@@ -105,18 +105,35 @@ struct Rows {
     }
 };
 
-// Adds a token's sum over the lanes of a channel to the row of c whose lanes `is` marks.
-__device__ __forceinline__ f32x4 add_row(float part, bool is, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(is ? 1.f : 0.f, part, c, 0, 0, 0);
+// Two values to a lane become others: of `a` the second half of the lanes (or the second of each
+// two rows of 16 lanes) changes places with the first half (or the first) of `b`.
+__device__ __forceinline__ void swap_halves(float* a, float* b) {
+    const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(*a), __float_as_uint(*b), false, false);
+    *a = __uint_as_float(v[0]), *b = __uint_as_float(v[1]);
+}
+__device__ __forceinline__ void swap_rows(float* a, float* b) {
+    const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(*a), __float_as_uint(*b), false, false);
+    *a = __uint_as_float(v[0]), *b = __uint_as_float(v[1]);
+}
+// Sums of four tokens' parts over a channel's four lanes: lanes of row i end with token i's.
+// (Matrix instructions would take a token's sum times 0 into the others': not where it is infinite.)
+__device__ __forceinline__ float token_sums(float v0, float v1, float v2, float v3) {
+    swap_halves(&v0, &v2);
+    swap_halves(&v1, &v3);
+    float a = v0 + v2, b = v1 + v3;
+    swap_rows(&a, &b);
+    return a + b;
+}
+// Of a tile's four such (w[q]: lanes of row i have token 4 q + i) the lane's own tokens, 4 (lane / 16) + r.
+__device__ __forceinline__ void own_tokens(f32x4* w) {
+    float v0 = (*w)[0], v1 = (*w)[1], v2 = (*w)[2], v3 = (*w)[3];
+    swap_halves(&v0, &v2);
+    swap_halves(&v1, &v3);
+    swap_rows(&v0, &v1);
+    swap_rows(&v2, &v3);
+    *w = f32x4{v0, v1, v2, v3};
 }
 __device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
-// Waits until the last such sums are in their registers, before they are read in another
-// basic block than the instruction's (11 states: eight passes, and three to be read).
-__device__ __forceinline__ void settle() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 15\n\ts_nop 1" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
 
 // A lane's states of a block: rows 4 (lane / 16) .. + 3 of [states][channels].
 __device__ __forceinline__ f32x4 load_states(const float* p, int n0, int N, long long D, int ch) {

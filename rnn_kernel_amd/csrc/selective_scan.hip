@@ -95,8 +95,9 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
             steps[c][kTile + 4 * nl + r] = s * xf[r];
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                bt[4 * nl + r][16 * k + c] = 16 * k + c < d.N ? to_f32(bv[k].v[r]) : 0.f;
-                if (!STATES_ONLY) ct[4 * nl + r][16 * k + c] = to_f32(cv[k].v[r]);
+                const bool is = r < rows && 16 * k + c < d.N;
+                bt[4 * nl + r][16 * k + c] = is ? to_f32(bv[k].v[r]) : 0.f;
+                if (!STATES_ONLY) ct[4 * nl + r][16 * k + c] = is ? to_f32(cv[k].v[r]) : 0.f;
             }
         }
         __syncthreads();
@@ -104,10 +105,10 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
         // (addresses from one place for four tokens: each array's own would cost an addition a token)
         const float *ps = &steps[c][0], *pb = &bt[0][4 * nl], *pc = &ct[0][4 * nl];
-        int row = c;
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q, ps += 4, pb += 64 * NB, pc += 64 * NB, row -= 4) {
+        for (int q = 0; q < 4; ++q, ps += 4, pb += 64 * NB, pc += 64 * NB) {
             const f32x4 s4 = load4(ps), i4 = load4(ps + kTile);
+            float parts[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float part = 0.f;
@@ -122,11 +123,12 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
                         for (int j = 0; j < 4; ++j) part = fmaf(cq[j], h[k][j], part);
                     }
                 }
-                if (!STATES_ONLY) acc = add_row(part, row == i, acc);
+                parts[i] = part;
             }
+            if (!STATES_ONLY) acc = f32x4{acc[1], acc[2], acc[3], token_sums(parts[0], parts[1], parts[2], parts[3])};
         }
         if (!STATES_ONLY) {
-            settle();
+            own_tokens(&acc);
             const Memory to(py + (size_t)t * d.D);
             const int room = t_end - t - 4 * nl;
 #pragma unroll

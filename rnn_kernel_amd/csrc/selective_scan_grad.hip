@@ -264,10 +264,11 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             const float *ps = &steps[wave][c][0], *pbt = &bt[0][n0], *pct = &ct[0][n0];
             f32x4* ph = &before[wave][0][lane];
             float* sums = reinterpret_cast<float*>(&before[wave][0][0]) + nl * 8 + c / 2;
-            int row = c;
+            f32x4 reads, q1s, q2s;
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q, ps += 4, pbt += 64 * NB, pct += 64 * NB, ph += 4 * 64, row -= 4) {
+            for (int q = 0; q < 4; ++q, ps += 4, pbt += 64 * NB, pct += 64 * NB, ph += 4 * 64) {
                 const f32x4 s4 = load4(ps), i4 = load4(ps + 2 * kTile);
+                float parts[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 bq = load4(pbt + 16 * NB * i), cq = load4(pct + 16 * NB * i);
@@ -278,37 +279,42 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
                         hk[j] = fmaf(__builtin_amdgcn_exp2f(s4[i] * a2[k][j]), hk[j], i4[i] * bq[j]);
                         part = fmaf(cq[j], hk[j], part);
                     }
-                    read = add_row(part, row == i, read);
+                    parts[i] = part;
                 }
+                reads = f32x4{reads[1], reads[2], reads[3], token_sums(parts[0], parts[1], parts[2], parts[3])};
             }
             sums += kTile * 256;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
-                ps -= 4, pbt -= 64 * NB, pct -= 64 * NB, ph -= 4 * 64, sums -= 4 * 256, row += 4;
+                ps -= 4, pbt -= 64 * NB, pct -= 64 * NB, ph -= 4 * 64, sums -= 4 * 256;
+                float of_b[4], of_a[4];
                 const f32x4 s4 = load4(ps), r4 = load4(ps + kTile), i4 = load4(ps + 2 * kTile);
 #pragma unroll
                 for (int i = 3; i >= 0; --i) {
                     const f32x4 bq = load4(pbt + 16 * NB * i), cq = load4(pct + 16 * NB * i), hp = ph[64 * i];
-                    float of_b = 0.f, of_a = 0.f, v[8];
+                    float v[8];
+                    of_b[i] = of_a[i] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float full = fmaf(r4[i], cq[j], dh[k][j]);
                         v[j] = i4[i] * full;
                         v[4 + j] = r4[i] * hk[j];
-                        of_b = fmaf(full, bq[j], of_b);
+                        of_b[i] = fmaf(full, bq[j], of_b[i]);
                         dh[k][j] = full * __builtin_amdgcn_exp2f(s4[i] * a2[k][j]);
                         const float w = dh[k][j] * hp[j];
-                        of_a = fmaf(w, a2[k][j], of_a);
+                        of_a[i] = fmaf(w, a2[k][j], of_a[i]);
                         da[k][j] = fmaf(w, s4[i], da[k][j]);
                     }
                     hk = hp;
-                    q1 = add_row(of_b, row == i, q1);
-                    q2 = add_row(of_a, row == i, q2);
-                    // (two lanes write the same: no branch between matrix instructions)
-                    sums[256 * i] = row_sums(v);
+                    sums[256 * i] = row_sums(v);  // (two lanes write the same)
                 }
+                q1s = f32x4{token_sums(of_b[0], of_b[1], of_b[2], of_b[3]), q1s[0], q1s[1], q1s[2]};
+                q2s = f32x4{token_sums(of_a[0], of_a[1], of_a[2], of_a[3]), q2s[0], q2s[1], q2s[2]};
             }
-            settle();
+            own_tokens(&reads);
+            own_tokens(&q1s);
+            own_tokens(&q2s);
+            read += reads, q1 += q1s, q2 += q2s;
             __syncthreads();
             // 32 sums of 16 tokens, two to a thread
 #pragma unroll

@@ -297,3 +297,47 @@ def test_graph_replays(gpu):
         want = _call(args)
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(s, want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [3, 16, 24, 64])
+def test_what_is_not_finite_stays_with_its_token(gpu, dtype, N):
+    """An infinite C is in one token's outputs, a NaN of one channel's x in that channel's from its
+    token on, a NaN of dy in the gradients up to its token; all else has the bits of a run without."""
+    B, T, D, G, at = 2, 45, 24, 2, 21
+    args, dy, _ = _inputs(B, T, D, N, G, dtype, seed=5, device=gpu)
+    y0, h0 = _call(args)
+    others = torch.arange(T, device=gpu) != at
+
+    C = args[4].clone()
+    C[0, at, 0, 0] = float("inf")
+    y, h = _call([*args[:4], C, *args[5:]])
+    assert torch.equal(y[:, others], y0[:, others]) and torch.equal(h, h0) and torch.equal(y[1], y0[1])
+    assert not torch.isfinite(y[0, at, :D // G]).any() and torch.equal(y[0, at, D // G:], y0[0, at, D // G:])
+
+    x = args[0].clone()
+    x[0, at, 3] = float("nan")
+    y, h = _call([x, *args[1:]])
+    assert torch.equal(y[:, :at], y0[:, :at]) and torch.equal(y[1], y0[1])
+    assert torch.isnan(y[0, at:, 3]).all() and torch.isnan(h[0, 3]).all()
+    rest = torch.arange(D, device=gpu) != 3
+    assert torch.equal(y[:, :, rest], y0[:, :, rest]) and torch.equal(h[:, rest], h0[:, rest])
+
+    # (the last token of a row: what lies behind is no part of its state)
+    lengths = torch.tensor([at + 1, T], dtype=torch.int32, device=gpu)
+    Bm = args[3].clone()
+    Bm[0, at, 0, 0] = float("inf")
+    _, h = _call([*args[:3], Bm, *args[4:]], lengths=lengths)
+    _, clean = _call(args, lengths=lengths)
+    assert torch.isinf(h[0, :D // G, 0]).all() and torch.equal(h[0, :, 1:], clean[0, :, 1:]) and torch.equal(h[1], clean[1])
+
+    leaves = [t.clone().requires_grad_(True) for t in args]
+    y, _ = _call(leaves)
+    pick = [leaves[i] for i in (0, 1, 3, 4, 7)]
+    want = torch.autograd.grad(y, pick, dy, retain_graph=True)
+    dy = dy.clone()
+    dy[0, at, 3] = float("nan")
+    for got, ref in zip(torch.autograd.grad(y, pick, dy), want):
+        assert torch.equal(got[:, at + 1:], ref[:, at + 1:]) and torch.equal(got[1], ref[1])
+        if got.shape[2] == D:
+            assert torch.equal(got[:, :, rest], ref[:, :, rest]) and torch.isnan(got[0, at, 3])
