@@ -223,12 +223,13 @@ struct Slopes : Product {
     template <typename T, int WM, int WN>
     __device__ __forceinline__ void put(const f32x16 (&acc)[WM / 32][WN / 32], float* out, int row0, int col0, int) const {
         if (row0 >= ldt || col0 >= ld) return;
-        if (!bias && col0 + WN <= n)
+        if (!bias && col0 + WN <= n && row0 + WM <= live_rows())
             of_tile<true, T, WM, WN>(acc, out, row0, col0);
         else
             of_tile<false, T, WM, WN>(acc, out, row0, col0);
     }
-    // PLAIN: no bias, and every column is the vocabulary's.
+    // PLAIN: no bias, every column is the vocabulary's, and every row one of the call's (dl behind
+    // the last is a 0 for dW: the exponential of a logit of no row is not always one).
     template <bool PLAIN, typename T, int WM, int WN>
     __device__ __forceinline__ void of_tile(const f32x16 (&acc)[WM / 32][WN / 32], float* out, int row0, int col0) const {
         constexpr int MB = WM / 32, NB = WN / 32, kLd = WN + 4, kV = kVec<T>, kLanes = WN / kV, kRows = 64 / kLanes;
@@ -243,8 +244,7 @@ struct Slopes : Product {
             const int row = row0 + 32 * i + i32, at = min(row, live - 1);
             targets[i] = r.target[at];
             lses[i] = r.lse[at];
-            // (a row behind the last has a logit of 0 and this scale)
-            scales[i] = row >= live ? 0.f : of_rows ? grad[r.from[at]] : grad[0];
+            scales[i] = of_rows ? grad[r.from[at]] : grad[0];
         }
 #pragma unroll
         for (int i = 0; i < MB; ++i) {

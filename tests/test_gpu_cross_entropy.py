@@ -277,3 +277,31 @@ def test_same_bits_twice_on_a_stream_and_in_a_graph(gpu):
             eager = head(fixed, t)
             torch.cuda.synchronize()
             assert torch.equal(loss, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [70, 300])
+def test_rows_behind_the_last_add_nothing(gpu, dtype, M):
+    """A tile's rows past the call's: where all logits are far below 0, or a column's are all
+    -infinity, what a row of zeros would have there is not a number.  (float32: logits are sums of 64
+    products of size 2, off by at most 2^-24 of each partial sum, 64 * 64 * 2^-24 = 2.5e-4
+    altogether, and p by that times p.)"""
+    from rnn_kernel_amd import linear_cross_entropy
+
+    gen = torch.Generator().manual_seed(11)
+    x = torch.ones(M, 64).to(dtype)
+    w = -(2 + 0.01 * torch.randn(256, 64, generator=gen)).to(dtype)
+    target = torch.randint(0, 256, (M,), generator=gen)
+    for low in (False, True):
+        if low:
+            x, w = x.clone(), w.clone()
+            target = torch.where(target == 9, 10, target)
+            w[9, 3] = float("-inf")
+        ref = [t.double().requires_grad_(True) for t in (x, w)]
+        got = [t.to(gpu).requires_grad_(True) for t in (x, w)]
+        want = torch.autograd.grad(_formula(*ref, target, None).mean(), ref[1])[0]
+        # (the -infinite column has no part in the others' gradients, nor a gradient)
+        dw = torch.autograd.grad(linear_cross_entropy(*got, target.to(gpu)), got[1])[0]
+        assert _rel(dw, want) <= (2.5e-4 if dtype == torch.float32 else BF16 + 2.5e-4)
+        if low:
+            assert (dw[9] == 0).all()
