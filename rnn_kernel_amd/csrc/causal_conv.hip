@@ -5,7 +5,11 @@
 // The final state is a row's last W - 1 inputs; its gradient adds to theirs.
 //
 // A thread takes four channels through a run of tokens, whose inputs it loads at once: what it
-// needs of its neighbours' tokens it loads and makes again (from L2).  Bound by memory.
+// needs of its neighbours' tokens it loads and makes again (from L2).  Bound by memory: 16 x 2048
+// tokens of 2048 channels, width 4, bf16 take 51 us forward (5.3 TB/s of x and y) and 100 backward
+// (4.0 TB/s of dy, x and dx); a quarter of them, which caches hold, 19 and 28 us, a third of it
+// the exponentials.  Token by token with one channel to a thread 98 us instead of the last two and
+// the sums.
 #include "elementwise.h"
 
 #include <algorithm>
@@ -21,7 +25,8 @@ constexpr int kMaxWidth = 8;
 constexpr int kLanes = 64, kRuns = 4;  // groups of channels and runs of a workgroup
 constexpr int kGroup = 4;              // channels of a thread
 // Tokens of a run, of the forward and of the backward with those before it whose dz it makes
-// again: 4 x 2048 tokens of 2048 channels are then some 4000 wavefronts.
+// again: 4 x 2048 tokens of 2048 channels are then some 4000 wavefronts.  16 x 2048 tokens take 56,
+// 51 and 58 us forward with 8, 16 and 32, and 142, 100 and 124 backward.
 constexpr int kForwardRun = 16, kBackwardSpan = 16;
 
 struct Dims {

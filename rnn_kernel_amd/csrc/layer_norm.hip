@@ -4,7 +4,9 @@
 //
 // A row is in registers between its one read and its one write: mean first, then the
 // squares of what is left, so that a large mean takes nothing from the variance.  Bound by
-// memory.
+// memory: 65536 rows of 2048 bf16 take 96 us forward (5.6 TB/s of x and y; a copy of 4 GiB 4.8)
+// and 162 us backward (5.0 TB/s of dy, x and dx, the columns' sums 5 us of it); 1000 rows of 385
+// float32 4 and 5 us, a launch's latency.
 #include "elementwise.h"
 
 #include <algorithm>
@@ -195,7 +197,10 @@ __global__ __launch_bounds__(256) void columns_kernel(const float* sums, int cou
     out[col] = from_f32<T>(s);
 }
 
-// Calls f with the wavefronts of a row and the pieces of a lane as constants.
+// Calls f with the wavefronts of a row and the pieces of a lane as constants: as few wavefronts
+// as hold a row in 64 registers or so, as sums between them wait at barriers.  2^27 elements of
+// bf16, forward and backward, in rows of 1024: one wavefront 98 and 152 us, four 185 and 416; of 2048
+// 96 and 162, 124 and 232; of 4096: four 112 and 203, sixteen 196 and 292.
 template <typename T, typename F>
 int with_form(int size, F f) {
     const int pieces = (size - 1) / kVec<T> + 1;
@@ -207,7 +212,8 @@ int with_form(int size, F f) {
     return form(std::integral_constant<int, 16>{}, std::integral_constant<int, kMaxSize / 1024 / kVec<T>>{});
 }
 
-// Workgroups of the backward.
+// Workgroups of the backward, each with sums of its own: 2^27 elements in rows of 2048 take 170,
+// 162 and 171 us with at most 256, 512 and 1024, in rows of 4096 304, 203 and 221.
 int backward_blocks(int rows, int size, int esize) {
     const int a_block = (size - 1) / (16 / esize) + 1 <= 256 ? 4 : 1;
     return (int)std::min<long long>(((long long)rows - 1) / a_block + 1, 512);

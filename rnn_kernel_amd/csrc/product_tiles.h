@@ -280,7 +280,10 @@ __device__ __forceinline__ int direct_turn(int row) { return (row ^ (row >> 3 & 
 // the matrix instructions are busy for 52% of the clocks, LDS for 21%; without the loads (a
 // copy, with wrong results) 344 us, with all of them from L2 461; half stages in a ring of four,
 // whose next fragments are read before the barrier, 494 (rows of 64 bytes); 128 x 128 to a
-// wavefront, with one wavefront to a SIMD, 565.
+// wavefront, with one wavefront to a SIMD, 565.  Loads issued between the products of a quarter
+// of a stage, the next stage's fragments read in its last quarter, as written-out instructions that
+// the compiler does not wait for: 473 beside 470 in one run, 545 at 128 x 128.  A good part is power: the
+// same product of zeros takes 377 (a library's 255, and 355 of random numbers).
 template <typename T, int BM, int BN, int WM, int WN, typename P>
 __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(P p) {
     constexpr int W = BM / WM * BN / WN, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;

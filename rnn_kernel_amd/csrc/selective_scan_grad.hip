@@ -5,8 +5,8 @@
 // the lanes of a channel block, then over a workgroup's four blocks in LDS, then over the
 // workgroups by a launch of their own, always in the same order.
 //
-// 4 x 2048 tokens of 2048 channels, 16 states, bf16: chunks' ends 60 us, gradients 283, the sums
-// behind them 12.  Bound by vector instructions, some 110 a token and lane (22 of them the sums
+// 4 x 2048 tokens of 2048 channels, 16 states, bf16: chunks' ends 60 us, gradients 270, the sums
+// behind them 12.  Bound by vector instructions, some 105 a token and lane (16 of them the sums
 // over channels), at two wavefronts to a SIMD, which is what the states in LDS leave.
 #include "selective_scan.h"
 

@@ -2,7 +2,9 @@
 // formulas): every state is read and written once, in place.
 //
 // A lane takes four states of a channel (16 bytes), as many neighbouring lanes as they need a
-// channel's; their sum over the states passes through those lanes.  Bound by memory.
+// channel's; their sum over the states passes through those lanes.  Bound by memory: 256 requests
+// of 4096 channels with 16 states take 31 us, 4.5 TB/s (a copy of 4 GiB 4.8), 62 with states that
+// are not on 16 bytes; one request of 256 channels 3 us.
 #include "selective_scan.h"
 
 namespace rka {
