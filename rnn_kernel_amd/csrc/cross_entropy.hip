@@ -154,6 +154,7 @@ struct Bias {
 };
 
 struct Logits : Product {
+    static constexpr bool kParts = true;  // (an exponential's relative error is its logit's absolute one)
     static constexpr bool kDynamic = true;
     Rows r;
     const void* bias;
@@ -230,6 +231,7 @@ struct Scale {
 
 // dl for a piece of the vocabulary, from column `first` of it on.
 struct Slopes : Product {
+    static constexpr bool kParts = true;
     static constexpr bool kDynamic = true;
     Rows r;
     const void* bias;

@@ -45,6 +45,10 @@ struct Operand {
 // m x n sums over k, in `slices` of `stages` stages.
 struct Product {
     static constexpr bool kDynamic = false;
+    // Whether long float32 sums are added up in parts of kPart stages, 512 terms, for sums whose
+    // absolute error is what counts: gradients of the loss of 17 rows of 2518 and 657 tokens are off by
+    // 2e-7, by 8e-7 without.  1 to 4% of a product's time (3000 x 1024 over 20000 tokens 980 us, 943).
+    static constexpr bool kParts = false;
     int m, n, k;
     Operand a, b;       // m rows, n rows
     int slices, stages; // stages of a slice
@@ -53,6 +57,26 @@ struct Product {
 };
 
 constexpr int kRowBytes = 128;  // of a stage's row
+constexpr int kPart = 16;
+
+// The parts of a wavefront's sums.
+template <bool ON, int MB, int NB>
+struct Parts {
+    f32x16 total[MB][NB] = {};
+    // (sums are read and set in another block than their products: states between, settle())
+    __device__ __forceinline__ void end_part(f32x16 (&acc)[MB][NB]);
+    __device__ __forceinline__ void end(f32x16 (&acc)[MB][NB]) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] += total[i][j];
+    }
+};
+template <int MB, int NB>
+struct Parts<false, MB, NB> {
+    __device__ __forceinline__ void end_part(f32x16 (&)[MB][NB]) {}
+    __device__ __forceinline__ void end(f32x16 (&)[MB][NB]) {}
+};
 
 __device__ __forceinline__ int piece_at(int row, int piece) {
     return row * kRowBytes + (((piece ^ row ^ (row >> 3)) & 7) << 4);
@@ -189,6 +213,20 @@ __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+template <bool ON, int MB, int NB>
+__device__ __forceinline__ void Parts<ON, MB, NB>::end_part(f32x16 (&acc)[MB][NB]) {
+    settle();
+    end(acc);
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            total[i][j] = acc[i][j];
+            acc[i][j] = f32x16{};
+        }
+    settle();
+}
+
 // The tile and slice of a workgroup: consecutive workgroups go to the eight XCDs in
 // turn, so each XCD takes a run of tiles, in groups of eight tile rows whose operands
 // then stay in its L2.
@@ -211,9 +249,10 @@ constexpr int kOutBytes = 32 * (WN + 4) * 4;
 // turned on their way and for rows of any address and length.  Bound by its waits: the
 // registers that hold the next stage leave those of one k step's fragments, so that
 // LDS's latency shows between the products.  8192 x 2048 over 2048 bf16, one operand
-// turned: 87 us, 790 TFLOP/s; direct_kernel: 69 us.
+// turned: 87 us, 790 TFLOP/s; direct_kernel: 69 us.  (Two wavefronts to a SIMD where parts are
+// held too: with one to a SIMD the 128 tile takes 38% longer.)
 template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, typename P>
-__global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(P p) {
+__global__ __launch_bounds__(BM / WM * BN / WN * 64, P::kParts && sizeof(T) == 4 ? 2 : 1) void tile_kernel(P p) {
     constexpr int NT = BM / WM * BN / WN * 64, kK = 8 * kVec<T>, MB = WM / 32, NB = WN / 32;
     constexpr int kStage = (BM + BN) * kRowBytes;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -230,6 +269,8 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(P p) {
     for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x16{};
+    constexpr bool kInParts = P::kParts && sizeof(T) == 4;
+    Parts<kInParts, MB, NB> parts;
     const int stages = (kend - kbeg + kK - 1) / kK;
     if (stages > 0) {
         sa.load(p.a, m0, p.m, kbeg, kend, tid);
@@ -264,8 +305,10 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void tile_kernel(P p) {
             sb.store(next + BM * kRowBytes, tid);
         }
         __syncthreads();
+        if (kInParts && (s + 1) % kPart == 0) parts.end_part(acc);
     }
     settle();
+    parts.end(acc);
     p.template put<T, WM, WN>(acc, reinterpret_cast<float*>(lds + wave * kOutBytes<WN>), m0 + wm, n0 + wn, slice);
 }
 
@@ -326,6 +369,8 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(P p) {
     for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x16{};
+    constexpr bool kInParts = P::kParts && sizeof(T) == 4;
+    Parts<kInParts, MB, NB> parts;
     // (the next stage's loads are issued in two lots, 1.5% faster than in one)
     auto compute = [&](const char* cur, char* next, int stage) {
         u32x4 fa[2][MB], fb[2][NB];
@@ -368,6 +413,7 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(P p) {
             arrive();
             compute(odd, even, s + 2);
             arrive();
+            if (kInParts && (s + 2) % kPart == 0) parts.end_part(acc);
         }
         if (s + 1 < stages) load(odd, s + 1, 0, kLoads);
         compute(even, nullptr, 0);
@@ -378,6 +424,7 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(P p) {
             settle();
         }
     }
+    parts.end(acc);
     __syncthreads();
     float* out = reinterpret_cast<float*>((wave < W / 2 ? even : odd) + wave % (W / 2) * kOutBytes<WN>);
     p.template put<T, WM, WN>(acc, out, m0 + wm, n0 + wn, slice);
