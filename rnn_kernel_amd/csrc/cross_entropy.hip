@@ -14,10 +14,10 @@
 // (W's piece and x are turned for that).  dx is summed over the pieces in float32.  Four
 // products in all, which bound it; logarithms are of base 2 throughout.
 //
-// 8192 rows, 7373 of them with a target, 2048 inputs, 64000 tokens, bf16: forward 1.69 ms, backward
-// 5.64; logits 1.71 ms (1130 TFLOP/s, a library's product of the sizes 1.40), dl 0.53 for each of
-// four pieces, dx 0.43, dW 0.44 (1100 to 1150).  What keeps the products from the library's rate is
-// in product_tiles.h; of dl's 0.53, 0.05 are the eighth round of tiles, 29 of 256.
+// 8192 rows, 7373 of them with a target, 2048 inputs, 64000 tokens, bf16: forward 1.7 to 1.8 ms,
+// backward 5.6; logits 1.71 ms (1130 TFLOP/s, a library's product of the sizes 1.40), dl 0.52 for
+// each of four pieces, dx 0.43, dW 0.44 (1100 to 1150).  What keeps the products from the library's rate is
+// in product_tiles.h; of dl's 0.52, 0.05 are the eighth round of tiles, 29 of 256.
 #include "product_tiles.h"
 
 namespace rka {
