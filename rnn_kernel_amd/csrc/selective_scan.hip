@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void join_kernel(Dims d, float* own, const flo
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, per = (long long)d.N * d.D;
     if (i >= per * d.B) return;
     const int b = (int)(i / per), n = (int)(i % per / d.D), ch = (int)(i % d.D);
-    const float a2 = kLog2e * d.A[(size_t)ch * d.N + n];
+    const float a2 = 0.5f * kLog2e * d.A[(size_t)ch * d.N + n];
     float h = first ? first[((size_t)b * d.D + ch) * d.N + n] : 0.f;
     const long long start = backward ? d.chunks - 1 : 0, step = backward ? -1 : 1;
     float* p = own + ((size_t)b * d.chunks + start) * per + (size_t)n * d.D + ch;
@@ -181,16 +181,19 @@ __global__ __launch_bounds__(256) void join_kernel(Dims d, float* own, const flo
         const int left = d.chunks - c0;
 #pragma unroll
         for (int j = 0; j < kDeep; ++j) {
-            // (the last chunk's own is not made)
+            // (the last chunk's own is not made: where it alone is left, what is loaded is not used)
             const long long of = step * min(j, max(0, left - 2));
-            mine[j] = left > 1 ? p[of * per] : 0.f;
-            sum[j] = left > 1 ? ps[of * d.D] : 0.f;
+            mine[j] = p[of * per];
+            sum[j] = ps[of * d.D];
         }
 #pragma unroll
         for (int j = 0; j < kDeep; ++j) {
             if (j >= left) break;
             p[step * j * per] = h;
-            h = fmaf(__builtin_amdgcn_exp2f(sum[j] * a2), h, mine[j]);
+            // (by its root twice, which stays finite: a growing chunk's factor may be infinite where what it
+            // makes of h, which may be 0, is not; where a sum is NaN so is the chunk's own state)
+            const float root = fminf(__builtin_amdgcn_exp2f(sum[j] * a2), 3e38f);
+            h = fmaf(root, root * h, mine[j]);
         }
         p += step * kDeep * per;
         ps += step * kDeep * d.D;

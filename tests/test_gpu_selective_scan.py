@@ -341,3 +341,24 @@ def test_what_is_not_finite_stays_with_its_token(gpu, dtype, N):
         assert torch.equal(got[:, at + 1:], ref[:, at + 1:]) and torch.equal(got[1], ref[1])
         if got.shape[2] == D:
             assert torch.equal(got[:, :, rest], ref[:, :, rest]) and torch.isnan(got[0, at, 3])
+
+
+def test_growing_states_over_chunks(gpu):
+    """A above 0: over a chunk (64 tokens here) the growth exp(128) is no float32, but there is no
+    state for it until the last 10 tokens, or one so small that the result is a float32."""
+    from rnn_kernel_amd import selective_scan
+
+    gen = torch.Generator().manual_seed(2)
+    x, B, C = torch.randn(1, 300, 32, generator=gen), torch.randn(1, 300, 1, 16, generator=gen), torch.randn(1, 300, 1, 16, generator=gen)
+    x[:, :290] = 0
+    dt, A = torch.ones(1, 300, 32), torch.full((32, 16), 2.0)
+    want, h = _formula(*(t.double() for t in (x, dt, A, B, C)), None, None, None, None, False, None)
+    y, s = selective_scan(*(t.to(gpu) for t in (x, dt, A, B, C)))
+    assert _rel(y, want) <= VALUE and _rel(s, h) <= VALUE
+
+    # exp(0.5 * 300) of 1e-30 is exp(81); each of 300 decays is off by 2^-24 or so: 300 * 2^-24 = 1.8e-5
+    s0, A = torch.full((1, 32, 16), 1e-30), torch.full((32, 16), 0.5)
+    x = torch.zeros_like(x)
+    _, h = _formula(*(t.double() for t in (x, dt, A, B, C)), s0.double(), None, None, None, False, None)
+    _, s = selective_scan(*(t.to(gpu) for t in (x, dt, A, B, C)), s0.to(gpu))
+    assert _rel(s, h) <= 300 * 2.0 ** -24 + VALUE
