@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
             steps[c][row] = s;
             steps[c][kTile + row] = live ? dr : 0.f;
 #pragma unroll
-            for (int k = 0; k < NB; ++k) ct[row][16 * k + c] = 16 * k + c < d.N ? to_f32(cv[k].v[r]) : 0.f;
+            for (int k = 0; k < NB; ++k) ct[row][16 * k + c] = live && 16 * k + c < d.N ? to_f32(cv[k].v[r]) : 0.f;
         }
         __syncthreads();
         if (t > p.t0) load(t - kTile);
@@ -245,6 +245,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
     }
     for (int t = p.t0 < p.t1 ? last : p.t0 - 1; t >= p.t0; t -= kTile) {
         const int rows = p.t1 - t - 4 * nl;
+        // (a token behind the last has a step, an upper gradient, B and C of 0: it adds nothing)
         float x[4], s[4], slope[4], z[4], u[4], dr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const bool is = 16 * k + c < d.N;
+            const bool is = t + btoken < p.t1 && 16 * k + c < d.N;
             bt[btoken][16 * k + c] = is ? to_f32(bv[k]) : 0.f;
             ct[btoken][16 * k + c] = is ? to_f32(cv[k]) : 0.f;
         }
