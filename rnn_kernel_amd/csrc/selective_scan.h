@@ -160,6 +160,16 @@ __device__ __forceinline__ void store_states_of(float* p, int n0, int N, f32x4 v
         if (n0 + i < N) p[n0 + i] = v[i];
 }
 
+// A log2(e) as a finite number (NaN stays): the step of a token behind a row's end is 0, and its
+// decay has to be 1 where A is -infinity, or next to it, too.
+__device__ __forceinline__ float finite_rate(float a, float log2e = kLog2e) {
+    const float v = log2e * a;
+    return fabsf(v) == INFINITY ? copysignf(3.4e38f, v) : v;
+}
+__device__ __forceinline__ f32x4 finite_rates(f32x4 a) {
+    return f32x4{finite_rate(a[0]), finite_rate(a[1]), finite_rate(a[2]), finite_rate(a[3])};
+}
+
 // Tokens of a chunk for channel blocks that give `waves` wavefronts per chunk.
 int chunk_tokens(int tokens, long long waves);
 int make_dims(const char* what, int batch, int tokens, int channels, int states, int groups, Dims* d);

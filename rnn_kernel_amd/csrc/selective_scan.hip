@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
         const int n0 = 16 * k + 4 * nl;
-        a2[k] = kLog2e * load_states_of(d.A + (size_t)ch * d.N, n0, d.N);
+        a2[k] = finite_rates(load_states_of(d.A + (size_t)ch * d.N, n0, d.N));
         if (STATES_ONLY)
             h[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         else if (d.chunks > 1)
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void join_kernel(Dims d, float* own, const flo
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, per = (long long)d.N * d.D;
     if (i >= per * d.B) return;
     const int b = (int)(i / per), n = (int)(i % per / d.D), ch = (int)(i % d.D);
-    const float a2 = 0.5f * kLog2e * d.A[(size_t)ch * d.N + n];
+    const float a2 = finite_rate(d.A[(size_t)ch * d.N + n], 0.5f * kLog2e);
     float h = first ? first[((size_t)b * d.D + ch) * d.N + n] : 0.f;
     const long long start = backward ? d.chunks - 1 : 0, step = backward ? -1 : 1;
     float* p = own + ((size_t)b * d.chunks + start) * per + (size_t)n * d.D + ch;

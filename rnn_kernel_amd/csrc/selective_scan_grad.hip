@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
     f32x4 a2[NB], dh[NB];
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
-        a2[k] = kLog2e * load_states_of(d.A + (size_t)p.ch * d.N, 16 * k + 4 * nl, d.N);
+        a2[k] = finite_rates(load_states_of(d.A + (size_t)p.ch * d.N, 16 * k + 4 * nl, d.N));
         dh[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float bias = d.bias ? d.bias[p.ch] : 0.f;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
         const int n0 = 16 * k + 4 * nl;
-        a2[k] = kLog2e * load_states_of(d.A + (size_t)p.ch * d.N, n0, d.N);
+        a2[k] = finite_rates(load_states_of(d.A + (size_t)p.ch * d.N, n0, d.N));
         dh[k] = da[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (d.chunks > 1)
             dh[k] = load_states(ends + p.at * d.N * d.D, n0, d.N, d.D, p.ch);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, float* state, co
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        h[j] = fmaf(exp_fast(s * a[j]), h[j], s * x * to_f32(bv[j]));
+        h[j] = fmaf(__builtin_amdgcn_exp2f(s * finite_rate(a[j])), h[j], s * x * to_f32(bv[j]));
         if (n0 + j < d.N) sum = fmaf(to_f32(cv[j]), h[j], sum);
     }
 #pragma unroll

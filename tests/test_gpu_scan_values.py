@@ -42,3 +42,31 @@ def test_an_infinite_C_in_the_last_token_gives_infinite_gradients(gpu, T, at, N,
     assert want[0, :at + 1].isinf().all() and not want.isnan().any()
     assert torch.equal(grad.isinf(), want.isinf()) and not grad.isnan().any()
     assert torch.equal(grad[want.isinf()].sign().double(), want[want.isinf()].sign())
+
+
+@pytest.mark.parametrize("T", [1, 16, 21, 200])
+@pytest.mark.parametrize("N", [5, 16, 40])
+def test_a_state_whose_A_is_minus_infinity_holds_its_last_token(gpu, T, N):
+    """As with A of -1e30, by which exp(s A) is 0 as well: outputs, states and gradients, for rows that
+    end inside a tile, at its end, and with a chunk or more behind them."""
+    from rnn_kernel_amd import selective_scan, selective_step
+
+    args, up = _inputs(3, T, 24, N, gpu, seed=1)
+    s0 = torch.randn(3, 24, N, generator=torch.Generator().manual_seed(2)).to(gpu)
+    lengths = torch.tensor([T, (T + 1) // 2, 0], dtype=torch.int32, device=gpu)
+    out = []
+    for of in (-1e30, float("-inf")):
+        leaves = [t.clone() for t in args]
+        leaves[2][:, :3] = of
+        leaves = [t.requires_grad_(True) for t in (*leaves, s0.clone())]
+        y, h = selective_scan(*leaves, lengths=lengths)
+        grads = torch.autograd.grad([y, h], leaves, [up, torch.ones_like(h)])
+        pool = s0.clone()
+        step = selective_step(*(t.detach()[:, 0] if i != 2 else t.detach() for i, t in enumerate(leaves[:5])), pool)
+        out.append([y, h, *grads, step, pool])
+    for a, b in zip(*out):
+        assert torch.isfinite(b).all() and torch.equal(a, b)
+    h = out[1][1]
+    assert torch.equal(h[2], s0[2])
+    last = (args[1] * args[0])[0, T - 1, :, None] * args[3][0, T - 1]
+    assert (h[0, :, :3] - last[:, :3]).abs().max() <= 2.0 ** -22 * last.abs().max()
