@@ -188,8 +188,9 @@ struct Logits : Product {
             for (int j = 0; j < NB; ++j)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    // (a sum past the last column is another column's again: finite or not, it is not one)
-                    l[j][x] = PLAIN ? acc[i][j][x] : b.b[j][x] == -INFINITY ? -INFINITY : acc[i][j][x] + b.b[j][x];
+                    // (a sum past the last column is another column's again: finite or not, it is not one;
+                    // a masked column's, whose bias is -infinity, is: NaN stays)
+                    l[j][x] = PLAIN ? acc[i][j][x] : col0 + column(j, x / 4, x % 4) >= n ? -INFINITY : acc[i][j][x] + b.b[j][x];
                     top = fmaxf(top, l[j][x]);  // (NaN comes back in the sum)
                 }
             top *= kLog2e;
