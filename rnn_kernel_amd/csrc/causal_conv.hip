@@ -188,10 +188,12 @@ __global__ __launch_bounds__(kLanes* kRuns) void backward_kernel(Dims d, const T
             T* to = s >= 0 ? dx : dinitial;
             if (!to || s >= d.T) continue;
             float sum[kGroup] = {};
+            if (given && s < len) {  // (else it is 0 whatever the weights)
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e)
+                for (int e = 0; e < kGroup; ++e)
 #pragma unroll
-                for (int j = 0; j < W; ++j) sum[e] = fmaf(wt.w[j][e], dz[i - j][e], sum[e]);
+                    for (int j = 0; j < W; ++j) sum[e] = fmaf(wt.w[j][e], dz[i - j][e], sum[e]);
+            }
             const int kept = s - (len - (W - 1));  // its place in the final state
             if (dstate && kept >= 0 && kept < W - 1) {
                 const Quad<T> g = load_quad<SMALL>(dstate + ((long long)b * (W - 1) + kept) * d.D + d0, d.D);
