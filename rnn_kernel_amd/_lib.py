@@ -102,6 +102,10 @@ class RKAError(RuntimeError):
     """A nonzero status returned by the HIP library."""
 
 
+class RKAShapeError(RKAError, ValueError):
+    """The status of sizes that the library does not take."""
+
+
 def load() -> ctypes.CDLL:
     """Load the library (after torch, so it binds torch's HIP runtime)."""
     global _lib
@@ -131,9 +135,12 @@ def last_error() -> str:
     return msg.decode() if msg else ""
 
 
+UNSUPPORTED_SHAPE = 1004  # RKA_ERR_UNSUPPORTED_SHAPE
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
-        raise RKAError(f"{what} failed with status {rc}: {last_error()}")
+        raise (RKAShapeError if rc == UNSUPPORTED_SHAPE else RKAError)(f"{what} failed with status {rc}: {last_error()}")
 
 
 def ptr(t) -> Optional[int]:

@@ -22,6 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _args, _lib
 
 MIN_CONV_WIDTH, MAX_CONV_WIDTH = 2, 8
+MAX_CONV_BATCH, MAX_CONV_TOKENS = 65535, 2 ** 20  # of whole sequences
 _ACTS = {None: 0, "none": 0, "silu": 3}
 
 
@@ -31,7 +32,7 @@ def _check(what: str, x, weight, bias, activation, lead: int) -> None:
     if (x.is_cuda and dtype in _args.DTYPES and weight.dtype is dtype and weight.get_device() == index and activation in _ACTS
             and len(shape) == lead + 1 and len(of) == 2 and of[0] == shape[-1] >= 1 and MIN_CONV_WIDTH <= of[1] <= MAX_CONV_WIDTH
             and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == of[:1]))
-            and max(shape) <= _args.MAX_SIZE):
+            and max(shape) <= _args.MAX_SIZE and (lead == 1 or (shape[0] <= MAX_CONV_BATCH and shape[1] <= MAX_CONV_TOKENS))):
         return
     _args.check_dtype(what, x, "x")
     _args.check_tensors(what, x, (weight, "weight", x.dtype), (bias, "bias", x.dtype))
@@ -42,7 +43,9 @@ def _check(what: str, x, weight, bias, activation, lead: int) -> None:
     _args.check_shape(what, bias, "bias", (x.size(-1),))
     if activation not in _ACTS:
         raise ValueError(f"{what}: activation must be none or silu")
-    _args.check_sizes(what, x)
+    if lead == 2 and (x.size(0) > MAX_CONV_BATCH or x.size(1) > MAX_CONV_TOKENS):
+        raise ValueError(f"{what}: at most {MAX_CONV_BATCH} rows and 2^20 tokens")
+    raise ValueError(f"{what}: sizes must be below 2^31")
 
 
 def _forward(x, weight, bias, initial_state, activation, lengths):
