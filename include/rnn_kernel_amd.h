@@ -574,8 +574,9 @@ int rka_selective_step(const void* x, const void* dt, const float* A, const void
  * target is ignore_index has no part in anything: its loss and gradient are 0 and its x is not
  * read; the mean of no rows is 0.  One whose target lies outside the vocabulary gives NaN.  The
  * logits are not kept: the backward makes them again, for a piece of the vocabulary at a
- * time.  rows, inputs, outputs and ldw are at most 2^21.  (The reference's one loss is
- * F.mse_loss, rnn_benchmark.py:636.)
+ * time.  rows, inputs, outputs and ldw are at most 2^21, and a launch has to take all logits (some
+ * 2^38 in float32, 2^39 in bfloat16).  (The reference's one loss is F.mse_loss,
+ * rnn_benchmark.py:636.)
  */
 #define RKA_REDUCE_NONE 0
 #define RKA_REDUCE_MEAN 1

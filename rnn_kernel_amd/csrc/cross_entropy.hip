@@ -637,6 +637,20 @@ int backward(const Sizes& z, const float* grad, const T* x, long long ldx, const
     return 0;
 }
 
+// Whether a launch takes all logits, of the forward, or of the backward's pieces, whose turned
+// operands are launches of a thread to 16 elements.
+bool launches(const Sizes& z, bool backward) {
+    if (!backward) return plan_product(z.m, z.v, z.k, z.esize, false, 1).cost < kNoPlan;
+    const Backward l = backward_layout(z);
+    for (const int rows : {z.m, l.piece})
+        if ((long long)up64(rows) * up64(z.k) / 16 >= kLaunchThreads) return false;
+    return plan_product(z.m, l.piece, z.k, z.esize, false, 1).cost < kNoPlan && l.of_x.cost < kNoPlan && l.of_w.cost < kNoPlan;
+}
+int check_launches(const char* what, const Sizes& z, bool backward) {
+    if (launches(z, backward)) return 0;
+    return fail(RKA_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": more logits than a launch may have (2^38 or so in float32, 2^39 in bfloat16)");
+}
+
 int check(const char* what, int rows, int inputs, int outputs, long long ldx, long long ldw, int reduction, int dtype) {
     const std::string name(what);
     if (rows < 1 || inputs < 1 || outputs < 1) return fail(RKA_ERR_INVALID_ARGUMENT, name + ": sizes must be >= 1");
@@ -647,8 +661,9 @@ int check(const char* what, int rows, int inputs, int outputs, long long ldx, lo
         return fail(RKA_ERR_INVALID_ARGUMENT, name + ": unknown reduction");
     return check_dtype(dtype, what);
 }
-bool fits(int rows, int inputs, int outputs) {
-    return rows >= 1 && inputs >= 1 && outputs >= 1 && rows <= kMost && inputs <= kMost && outputs <= kMost;
+bool fits(int rows, int inputs, int outputs, int dtype, bool backward) {
+    return rows >= 1 && inputs >= 1 && outputs >= 1 && rows <= kMost && inputs <= kMost && outputs <= kMost &&
+           launches(sizes_of(rows, inputs, outputs, dtype), backward);
 }
 
 }  // namespace
@@ -663,11 +678,11 @@ extern "C" {
 size_t rka_cross_entropy_reserve_bytes(int rows) { return rows < 1 || rows > kMost ? 0 : rows_bytes(rows); }
 
 size_t rka_cross_entropy_forward_workspace_bytes(int rows, int inputs, int outputs, int dtype) {
-    return fits(rows, inputs, outputs) ? forward_layout(sizes_of(rows, inputs, outputs, dtype)).total : 0;
+    return fits(rows, inputs, outputs, dtype, false) ? forward_layout(sizes_of(rows, inputs, outputs, dtype)).total : 0;
 }
 
 size_t rka_cross_entropy_backward_workspace_bytes(int rows, int inputs, int outputs, int dtype) {
-    return fits(rows, inputs, outputs) ? backward_layout(sizes_of(rows, inputs, outputs, dtype)).total : 0;
+    return fits(rows, inputs, outputs, dtype, true) ? backward_layout(sizes_of(rows, inputs, outputs, dtype)).total : 0;
 }
 
 int rka_cross_entropy_forward(const void* x, long long ldx, const void* weight, long long ldw, const void* bias,
@@ -678,6 +693,7 @@ int rka_cross_entropy_forward(const void* x, long long ldx, const void* weight, 
     RKA_RETURN_IF_ERR(check("cross_entropy_forward", rows, inputs, outputs, ldx, ldw, reduction, dtype));
     if (!x || !weight || !target || !loss || !reserve) return fail(RKA_ERR_INVALID_ARGUMENT, "cross_entropy_forward: null tensor pointer");
     const Sizes z = sizes_of(rows, inputs, outputs, dtype);
+    RKA_RETURN_IF_ERR(check_launches("cross_entropy_forward", z, false));
     RKA_RETURN_IF_ERR(check_workspace(workspace, workspace_bytes, forward_layout(z).total, "cross_entropy_forward"));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
@@ -697,6 +713,7 @@ int rka_cross_entropy_backward(const float* grad_loss, const void* x, long long 
     RKA_RETURN_IF_ERR(check("cross_entropy_backward", rows, inputs, outputs, ldx, ldw, reduction, dtype));
     if (!grad_loss || !x || !weight || !reserve) return fail(RKA_ERR_INVALID_ARGUMENT, "cross_entropy_backward: null tensor pointer");
     const Sizes z = sizes_of(rows, inputs, outputs, dtype);
+    RKA_RETURN_IF_ERR(check_launches("cross_entropy_backward", z, true));
     RKA_RETURN_IF_ERR(check_workspace(workspace, workspace_bytes, backward_layout(z).total, "cross_entropy_backward"));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);

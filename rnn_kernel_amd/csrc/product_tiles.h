@@ -433,10 +433,11 @@ __global__ __launch_bounds__(BM / WM * BN / WN * 64) void direct_kernel(P p) {
 // ------------------------------------------------------------- choices ---
 enum Tile { TILE_256, TILE_128, TILE_64 };
 constexpr long long kLaunchThreads = 1LL << 32;  // a launch has fewer
+constexpr double kNoPlan = 1e30;
 struct Plan {
     Tile tile;
     int slices, stages;
-    double cost;
+    double cost;  // kNoPlan: every tile would take more threads than a launch may have
 };
 
 // Tile and slices of a product: the least of a model of the time in us.  A stage of a
@@ -459,7 +460,7 @@ inline Plan plan_product(int m, int n, int k, int esize, bool across, int most_s
     static const Cost costs[] = {{TILE_256, 256, 512, 1, 1.8, 1.8, 1.2, 0},
                                  {TILE_128, 128, 256, 2, 0.7, 0.55, 1.2, 3.1},
                                  {TILE_64, 64, 256, 4, 0.35, 0.165, 1.25, 2.95}};
-    Plan best{TILE_64, 1, all, 1e30};
+    Plan best{TILE_64, 1, all, kNoPlan};
     for (const Cost& c : costs) {
         if (esize == 4 && c.tile == TILE_256) continue;
         const double tiles = (double)((m - 1) / c.edge + 1) * ((n - 1) / c.edge + 1);

@@ -59,13 +59,16 @@ def _forward(x, weight, target, bias, ignore_index: int, reduction: str):
     rows = target.numel()
     if max(rows, inputs, outputs) > MAX_LOSS_SIZE:
         raise ValueError(f"{_WHAT}: rows, inputs and vocabulary must be at most 2^21")
+    lib, dtype, nbytes = _lib.load(), _args.DTYPES[x.dtype], 0
+    if rows:
+        nbytes = lib.rka_cross_entropy_forward_workspace_bytes(rows, inputs, outputs, dtype)
+        if nbytes == 0:
+            raise ValueError(f"{_WHAT}: {rows} rows of {outputs} logits are more than a launch may have")
     xm, wm, bm, tm = _rows(x), _weight_rows(weight), _args.dense(bias), _args.dense(target)
     loss = torch.empty(target.shape if reduction == "none" else (), dtype=torch.float32, device=x.device)
     if rows == 0:
         return loss.zero_(), xm, wm, bm, None
-    lib, dtype = _lib.load(), _args.DTYPES[x.dtype]
     reserve = _args.workspace(lib.rka_cross_entropy_reserve_bytes(rows), x.device)
-    nbytes = lib.rka_cross_entropy_forward_workspace_bytes(rows, inputs, outputs, dtype)
     ws = _args.workspace(nbytes, x.device)
     _lib.call(x.get_device(), "rka_cross_entropy_forward", xm.data_ptr(), xm.stride(0), wm.data_ptr(), wm.stride(0), _lib.ptr(bm),
               tm.data_ptr(), int(tm.dtype == torch.int64), ignore_index, loss.data_ptr(), reserve.data_ptr(), ws.data_ptr(), nbytes,
@@ -122,9 +125,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     ``reduction``: "mean" over the rows with a target, "sum" or "none" (a loss for each row). A
     row whose target is ``ignore_index`` has no part in anything: its loss and gradient are 0
     and its x is not read; the mean of no rows is 0.  A row whose target lies outside the
-    vocabulary gives NaN.  Rows, inputs and vocabulary are at most 2^21.  The backward makes the
-    logits again, for a piece of the vocabulary at a time, and rounds their gradients to x's type
-    before the products.  Tensors with forward-mode tangents are refused."""
+    vocabulary gives NaN.  Rows, inputs and vocabulary are at most 2^21, and the logits 2^38 or so
+    in float32, 2^39 in bfloat16 (what a launch may have).  The backward makes the logits again, for a
+    piece of the vocabulary at a time, and rounds their gradients to x's type before the products.
+    Tensors with forward-mode tangents are refused."""
     _lib.refuse_tangents(_WHAT, x, weight, bias)
     if _args.wants_grad(x, weight, bias):
         return LinearCrossEntropyFunction.apply(x, weight, target, bias, ignore_index, reduction)

@@ -31,3 +31,33 @@ def test_sequences_that_the_convolution_does_not_take(gpu, shape):
     assert torch.cuda.max_memory_allocated() - before <= 4096
     with pytest.raises(ValueError, match="at most 65535 rows and 2\\^20 tokens"), torch.no_grad():
         SelectiveScan(4, device=gpu)(x)
+
+
+# rows, vocabulary, type (0: float32, 1: bfloat16), whether a launch takes their logits
+LOGITS = [(2 ** 21, 2 ** 18, 1, False), (2 ** 21, 2 ** 17, 0, False), (2 ** 20, 2 ** 21, 1, False), (2 ** 20, 2 ** 18, 1, True),
+          (2 ** 20, 2 ** 17, 0, True), (2 ** 21, 5, 1, True), (1, 2 ** 21, 0, True), (2 ** 21, 2 ** 21, 0, False)]
+
+
+@pytest.mark.parametrize("rows,vocabulary,dtype,taken", LOGITS)
+def test_more_logits_than_a_launch_has(hip_lib, rows, vocabulary, dtype, taken):
+    """The forward's are refused before anything is launched; the backward has them in pieces."""
+    sizes = (rows, 8, vocabulary)
+    assert (hip_lib.rka_cross_entropy_forward_workspace_bytes(*sizes, dtype) > 0) == taken
+    assert hip_lib.rka_cross_entropy_backward_workspace_bytes(*sizes, dtype) > 0
+    if not taken:
+        assert hip_lib.rka_cross_entropy_forward(4096, 8, 4096, 8, None, 4096, 1, -100, 4096, 4096, 4096, 2 ** 60, *sizes, 1, dtype,
+                                                 None) == 1004
+        assert "more logits than a launch" in hip_lib.rka_last_error().decode()
+
+
+@pytest.mark.gpu
+def test_more_logits_than_a_launch_has_in_python(gpu):
+    from rnn_kernel_amd import linear_cross_entropy
+
+    x, w = (torch.ones(1, 8, device=gpu, dtype=torch.bfloat16).expand(n, 8) for n in (2 ** 21, 2 ** 18))
+    target = torch.zeros(2 ** 21, dtype=torch.int32, device=gpu)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with pytest.raises(ValueError, match="more than a launch may have"):
+        linear_cross_entropy(x, w, target)
+    assert torch.cuda.max_memory_allocated() == before
