@@ -39,13 +39,6 @@ def check_shape(what: str, t, name: str, shape) -> None:
         raise ValueError(f"{what}: {name} must have shape {list(shape)}, not {list(t.shape)}")
 
 
-def check_sizes(what: str, *tensors) -> None:
-    # (a size that large shows in the number of elements, or is hidden by a size of 0)
-    for t in tensors:
-        if t is not None and not 0 < t.numel() <= MAX_SIZE and t.dim() and max(t.shape) > MAX_SIZE:
-            raise ValueError(f"{what}: sizes must be below 2^31")
-
-
 def check_row_ints(what: str, t, name: str, batch: int, device) -> None:
     if t is None:
         return
