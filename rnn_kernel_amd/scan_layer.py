@@ -24,8 +24,8 @@ class SelectiveScan(nn.Module):
         u' = silu(conv(u)),   d, B, C = W_x u',   dt = W_d d,   v = scan of u' with gate z
 
     (steps softplus(dt + b), ``states`` numbers of state per channel and ``groups`` of B and
-    C).  The scan's A = -exp(A_log), skip and b are float32, the other parameters of one type,
-    float32 or bfloat16.  A starts at -1 .. -states, steps at 0.001 to 0.1."""
+    C).  The scan's A = -exp(A_log), skip and b are float32, whatever the module is cast to, the
+    other parameters of one type, float32 or bfloat16.  A starts at -1 .. -states, steps at 0.001 to 0.1."""
 
     def __init__(self, size: int, channels: Optional[int] = None, states: int = 16, width: int = 4, groups: int = 1,
                  step_rank: Optional[int] = None, device=None, dtype=None) -> None:
@@ -52,6 +52,16 @@ class SelectiveScan(nn.Module):
         self.A_log = nn.Parameter(torch.arange(1, states + 1, dtype=torch.float32, device=device).log().repeat(channels, 1))
         self.skip = nn.Parameter(torch.ones(channels, dtype=torch.float32, device=device))
         self.step_bias = nn.Parameter((first + torch.log(-torch.expm1(-first))).to(torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        # (what casts a module casts its parameters here: the scan's stay float32, wherever they go)
+        wide = {id(t) for p in (self.A_log, self.skip, self.step_bias) for t in (p, p.grad) if t is not None}
+
+        def keep(t):
+            out = fn(t)
+            return out if out.dtype == t.dtype or id(t) not in wide else t.to(out.device)
+
+        return super()._apply(keep, recurse)
 
     def new_states(self, count: int) -> State:
         """States of ``count`` sequences that have not begun."""
