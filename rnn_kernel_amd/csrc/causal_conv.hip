@@ -35,9 +35,13 @@ struct Dims {
     const int* lengths;
 };
 
-__device__ __forceinline__ float activate(float z, int act) { return act == RKA_ACT_SILU ? z * sigmoid_fast(z) : z; }
+template <typename T>
+__device__ __forceinline__ float activate(float z, int act) {
+    return act == RKA_ACT_SILU ? z * sigmoid<T>(z) : z;
+}
+template <typename T>
 __device__ __forceinline__ float slope(float z, int act) {
-    const float s = sigmoid_fast(z);
+    const float s = sigmoid<T>(z);
     return act == RKA_ACT_SILU ? s * (1.f + z * (1.f - s)) : 1.f;
 }
 
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(kLanes* kRuns) void forward_kernel(Dims d, const T*
         if (t0 + i >= d.T) break;
         Quad<T> out;
 #pragma unroll
-        for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(t0 + i < len ? activate(wt.z(in + i, e), d.act) : 0.f);
+        for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(t0 + i < len ? activate<T>(wt.z(in + i, e), d.act) : 0.f);
         store_quad<SMALL>(py, out, d.D);
     }
 }
@@ -174,7 +178,7 @@ __global__ __launch_bounds__(kLanes* kRuns) void backward_kernel(Dims d, const T
             const int t = t0 + i;
             const bool live = given && t >= 0 && t < len;
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) dz[i][e] = live ? to_f32(up[i].e[e]) * slope(wt.z(in + i, e), d.act) : 0.f;
+            for (int e = 0; e < kGroup; ++e) dz[i][e] = live ? to_f32(up[i].e[e]) * slope<T>(wt.z(in + i, e), d.act) : 0.f;
             if (i < W - 1) continue;
             if (live) {
 #pragma unroll
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(kLanes) void step_kernel(int B, int D, int act, con
     Weights<SMALL, T, W> wt;
     wt.load(weight, bias, d0, left);
 #pragma unroll
-    for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(activate(wt.z(p, e), act));
+    for (int e = 0; e < kGroup; ++e) out.e[e] = from_f32<T>(activate<T>(wt.z(p, e), act));
     store_quad<SMALL>(py, out, left);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) store_quad<SMALL>(ps + (long long)j * D, p[j + 1], left);

@@ -74,10 +74,26 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-// The hardware's exponential and reciprocal, off by a rounding or so (results under 2^-126
-// are 0).
-__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(kLog2e * x); }
-__device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-x)); }
+// exp and 1/x for results of type T: for bf16 the hardware's own, whose relative error (of a
+// rounded product, 1e-6 at |x| = 20; results under 2^-126 are 0) is far below its last bit.
+template <typename T>
+__device__ __forceinline__ float exp_for(float x) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_amdgcn_exp2f(kLog2e * x);
+    else
+        return expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float inverse_for(float x) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_amdgcn_rcpf(x);
+    else
+        return 1.f / x;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+    return inverse_for<T>(1.f + exp_for<T>(-z));
+}
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int tokens) {
     return lengths ? max(0, min(tokens, lengths[b])) : tokens;

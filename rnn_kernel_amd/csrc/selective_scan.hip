@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float slope, s = to_f32(dt.v[r]) + bias;
-            if (d.softplus) s = softplus(s, &slope);
+            if (d.softplus) s = softplus<T>(s, &slope);
             s = r < rows ? s : 0.f;
             xf[r] = r < rows ? to_f32(x.v[r]) : 0.f;
             zf[r] = !STATES_ONLY && d.gate ? to_f32(gate.v[r]) : 0.f;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float v = fmaf(skip, xf[r], acc[r]);
-                if (d.gate) v *= zf[r] * sigmoid_fast(zf[r]);
+                if (d.gate) v *= zf[r] * sigmoid<T>(zf[r]);
                 if (on && r < room) to.store(from_f32<T>(r < rows ? v : 0.f), oy.at[r]);
             }
         }

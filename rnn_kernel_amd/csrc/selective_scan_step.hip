@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, float* state, co
     const float gate = d.gate ? to_f32(static_cast<const T*>(d.gate)[b * d.zs[0] + ch]) : 0.f;
     float slope, s = to_f32(static_cast<const T*>(d.dt)[b * d.ts[0] + ch]) + (d.bias ? d.bias[ch] : 0.f);
     const float skip = d.skip ? d.skip[ch] : 0.f;
-    if (d.softplus) s = softplus(s, &slope);
+    if (d.softplus) s = softplus<T>(s, &slope);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, float* state, co
     if (in >= d.D) return;
     if (n0 == 0) {
         float v = fmaf(skip, x, sum);
-        if (d.gate) v *= gate * sigmoid_fast(gate);
+        if (d.gate) v *= gate * sigmoid<T>(gate);
         y[(size_t)b * d.D + ch] = from_f32<T>(v);
     }
     if constexpr (VEC) {

@@ -1,0 +1,93 @@
+"""The exponentials of float32 calls element by element, far from 0 too, where a rounded exponent
+would cost bits: SiLU of the convolution and of the scan's gate, their slopes, and small steps.
+
+Tolerances, of each element, by arithmetic: an exponential 2^-23, 1 + it 2^-24 and the
+exponential's own, a division and a product 2^-24 each: 5 * 2^-24.  The slope s (1 + z (1 - s)): s
+4 * 2^-24; for z <= -3, where s is below 1/20, z (1 - s) three roundings and s's, of which 1 +
+leaves at most 3/2; two more products: 13 * 2^-24.  For z >= 3 s is next to 1, off by two roundings
+or 2 * 2^-24, and 1 - s (a difference without rounding) by as much in absolute terms; z times that,
+beside a result of 1 or more: (2 z + 8) * 2^-24 with the roundings of the products and sums, as in any
+float32 arithmetic of this formula.  softplus far below 0: an exponential, a logarithm, a product of
+them and the sum: 4 * 2^-23."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+VALUE, STEP = 5 * 2.0 ** -24, 4 * 2.0 ** -23
+
+
+def _z(least, device):
+    gen = torch.Generator().manual_seed(5)
+    low = -80 + (80 - least) * torch.rand(4000, generator=gen)
+    return torch.cat([low, least + 20 * torch.rand(1000, generator=gen)]).to(device)
+
+
+def _silu(z):
+    z = z.double()
+    return z * torch.sigmoid(z)
+
+
+def _slope(z):
+    s = torch.sigmoid(z.double())
+    return s * (1 + z.double() * torch.sigmoid(-z.double()))
+
+
+def _slopes_fit(a, z):
+    off = (a.double() / _slope(z) - 1).abs()
+    return bool((off <= torch.where(z < 0, 13, 2 * z + 8) * 2.0 ** -24).all())
+
+
+def _off(a, ref):
+    return float((a.double() / ref - 1).abs().max())
+
+
+def test_silu_of_the_convolution(gpu):
+    from rnn_kernel_amd import causal_conv, causal_conv_step
+
+    z = _z(3, gpu)
+    w = torch.tensor([[0.0, 1.0]], device=gpu).expand(z.numel(), 2)
+    x = z.view(1, 1, -1).clone().requires_grad_(True)
+    y = causal_conv(x, w, activation="silu")[0]
+    dx = torch.autograd.grad(y.sum(), x)[0]
+    assert _off(y.detach().view(-1), _silu(z)) <= VALUE and _slopes_fit(dx.view(-1), z)
+    state = torch.zeros(1, 1, z.numel(), device=gpu)
+    with torch.no_grad():
+        assert torch.equal(causal_conv_step(z.view(1, -1), state, w, activation="silu").view(-1), y.view(-1))
+
+
+def test_silu_of_the_gate(gpu):
+    """(B and C are 0: y = skip x silu(gate).)"""
+    from rnn_kernel_amd import selective_scan, selective_step
+
+    z = _z(3, gpu)
+    n = z.numel()
+    one, none, A = torch.ones(1, 1, n, device=gpu), torch.zeros(1, 1, 1, 2, device=gpu), -torch.ones(n, 2, device=gpu)
+    skip, gate = torch.ones(n, device=gpu), z.view(1, 1, -1).clone().requires_grad_(True)
+    x = one.clone().requires_grad_(True)
+    y = selective_scan(x, one, A, none, none, skip=skip, gate=gate)[0]
+    dx, dgate = torch.autograd.grad(y.sum(), [x, gate])
+    assert _off(y.detach().view(-1), _silu(z)) <= VALUE and _off(dx.view(-1), _silu(z)) <= VALUE
+    assert _slopes_fit(dgate.view(-1), z)
+    with torch.no_grad():
+        step = selective_step(one[0], one[0], A, none[0], none[0], torch.zeros(1, n, 2, device=gpu), skip=skip, gate=gate[0])
+    assert torch.equal(step.view(-1), y.view(-1))
+
+
+def test_small_steps(gpu):
+    """A state of one token is the step: softplus(dt), and its gradient sigmoid(dt)."""
+    from rnn_kernel_amd import selective_scan, selective_step
+
+    z = -12 - 68 * torch.rand(4000, generator=torch.Generator().manual_seed(6)).to(gpu)
+    n = z.numel()
+    one, A = torch.ones(1, 1, n, device=gpu), -torch.ones(n, 1, device=gpu)
+    unit = torch.ones(1, 1, 1, 1, device=gpu)
+    dt = z.view(1, 1, -1).clone().requires_grad_(True)
+    h = selective_scan(one, dt, A, unit, unit, softplus=True)[1]
+    grad = torch.autograd.grad(h.sum(), dt)[0]
+    assert _off(h.detach().view(-1), torch.log1p(z.double().exp())) <= STEP
+    assert _off(grad.view(-1), torch.sigmoid(z.double())) <= STEP
+    pool = torch.zeros(1, n, 1, device=gpu)
+    with torch.no_grad():
+        selective_step(one[0], dt[0], A, unit[0], unit[0], pool, softplus=True)
+    assert torch.equal(pool.view(-1), h.view(-1))
