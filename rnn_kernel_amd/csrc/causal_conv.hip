@@ -37,11 +37,11 @@ struct Dims {
 
 template <typename T>
 __device__ __forceinline__ float activate(float z, int act) {
-    return act == RKA_ACT_SILU ? z * sigmoid<T>(z) : z;
+    return act == RKA_ACT_SILU ? z * sigmoid_of<T>(z) : z;
 }
 template <typename T>
 __device__ __forceinline__ float slope(float z, int act) {
-    const float s = sigmoid<T>(z);
+    const float s = sigmoid_of<T>(z);
     return act == RKA_ACT_SILU ? s * (1.f + z * (1.f - s)) : 1.f;
 }
 

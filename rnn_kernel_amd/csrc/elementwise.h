@@ -74,25 +74,28 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-// exp and 1/x for results of type T: for bf16 the hardware's own, whose relative error (of a
-// rounded product, 1e-6 at |x| = 20; results under 2^-126 are 0) is far below its last bit.
+// exp(x) for results of type T (those under 2^-126 are 0).  The hardware's exponential takes a
+// product, whose rounding is worth |x| 2^-24 of the result: nothing beside bf16's last bit.  float32
+// puts it back: e^x = 2^hi (1 + ln(2) lo).  (expf and a division cost the float32 scan 8% and the
+// convolution's gradients 17% more.)
 template <typename T>
-__device__ __forceinline__ float exp_for(float x) {
-    if constexpr (sizeof(T) == 2)
-        return __builtin_amdgcn_exp2f(kLog2e * x);
-    else
-        return expf(x);
+__device__ __forceinline__ float exp_of(float x) {
+    const float hi = kLog2e * x, e = __builtin_amdgcn_exp2f(hi);
+    if constexpr (sizeof(T) == 2) {
+        return e;
+    } else {
+        const float lo = fmaf(x, 1.925963e-8f, fmaf(x, kLog2e, -hi));  // (NaN where hi is infinite: e is right then)
+        return fmaf(e, fminf(0.6931471805599453f * lo, 1.f), e);
+    }
 }
+// 1 / (1 + exp(-z)), in float32 with a step of Newton's for the reciprocal's last bit.
 template <typename T>
-__device__ __forceinline__ float inverse_for(float x) {
+__device__ __forceinline__ float sigmoid_of(float z) {
+    const float w = 1.f + exp_of<T>(-z), r = __builtin_amdgcn_rcpf(w);
     if constexpr (sizeof(T) == 2)
-        return __builtin_amdgcn_rcpf(x);
+        return r;
     else
-        return 1.f / x;
-}
-template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-    return inverse_for<T>(1.f + exp_for<T>(-z));
+        return fmaf(fminf(fmaf(-w, r, 1.f), 1.f), r, r);  // (w infinite: r is 0)
 }
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int tokens) {

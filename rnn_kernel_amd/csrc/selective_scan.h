@@ -64,7 +64,7 @@ __device__ __forceinline__ long long in_order() {
 // 1: small steps keep their 24 bits.  slope: its derivative.
 template <typename T>
 __device__ __forceinline__ float softplus(float r, float* slope) {
-    const float u = exp_for<T>(-fabsf(r)), w = 1.f + u;
+    const float u = exp_of<T>(-fabsf(r)), w = 1.f + u;
     *slope = (r < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(w);
     // (NaN stays)
     return (r < 0.f ? 0.f : r) + fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, u - (w - 1.f));

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(Dims d, float* states, float*
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float v = fmaf(skip, xf[r], acc[r]);
-                if (d.gate) v *= zf[r] * sigmoid<T>(zf[r]);
+                if (d.gate) v *= zf[r] * sigmoid_of<T>(zf[r]);
                 if (on && r < room) to.store(from_f32<T>(r < rows ? v : 0.f), oy.at[r]);
             }
         }

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64) void ends_kernel(Dims d, const T* dy, float* ow
             if (d.softplus) s = softplus<T>(s, &slope);
             s = live ? s : 0.f;
             float dr = pd ? to_f32(up.v[r]) : 0.f;
-            if (d.gate) dr *= to_f32(gate.v[r]) * sigmoid<T>(to_f32(gate.v[r]));
+            if (d.gate) dr *= to_f32(gate.v[r]) * sigmoid_of<T>(to_f32(gate.v[r]));
             sum += s;
             steps[c][row] = s;
             steps[c][kTile + row] = live ? dr : 0.f;
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             x[r] = live ? to_f32(xv.v[r]) : 0.f;
             z[r] = d.gate ? to_f32(gate.v[r]) : 0.f;
             u[r] = live && pd ? to_f32(up.v[r]) : 0.f;
-            dr[r] = d.gate && live ? u[r] * z[r] * sigmoid<T>(z[r]) : u[r];
+            dr[r] = d.gate && live ? u[r] * z[r] * sigmoid_of<T>(z[r]) : u[r];
             steps[wave][c][row] = s[r];
             steps[wave][c][kTile + row] = dr[r];
             steps[wave][c][2 * kTile + row] = s[r] * x[r];
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
             put(to_x, r, dx);
             put(to_dt, r, ddt);
             if (d.gate) {
-                const float sig = sigmoid<T>(z[r]);
+                const float sig = sigmoid_of<T>(z[r]);
                 put(to_gate, r, u[r] * fmaf(skip, x[r], read[r]) * sig * (1.f + z[r] * (1.f - sig)));
             }
         }

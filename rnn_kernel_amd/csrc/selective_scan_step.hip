@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Dims d, float* state, co
     if (in >= d.D) return;
     if (n0 == 0) {
         float v = fmaf(skip, x, sum);
-        if (d.gate) v *= gate * sigmoid<T>(gate);
+        if (d.gate) v *= gate * sigmoid_of<T>(gate);
         y[(size_t)b * d.D + ch] = from_f32<T>(v);
     }
     if constexpr (VEC) {

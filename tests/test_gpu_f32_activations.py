@@ -91,3 +91,26 @@ def test_small_steps(gpu):
     with torch.no_grad():
         selective_step(one[0], dt[0], A, unit[0], unit[0], pool, softplus=True)
     assert torch.equal(pool.view(-1), h.view(-1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_is_not_finite_or_far(gpu, dtype):
+    """As the formulas have it: silu(inf) = inf, of -inf and NaN NaN, of -1e30 0; steps inf, 0 and NaN."""
+    from rnn_kernel_amd import causal_conv, selective_scan
+
+    z = torch.tensor([float("inf"), -float("inf"), float("nan"), 1e30, -1e30, 300.0, -300.0, 0.0, -0.0], device=gpu).to(dtype)
+    n = z.numel()
+    want = torch.nan_to_num(_silu(z).to(dtype).double(), nan=7.0)
+    w = torch.ones(n, 2, device=gpu, dtype=dtype)
+    y = causal_conv(z.view(1, 1, -1), w, activation="silu")[0]
+    one, none, A = torch.ones(1, 1, n, device=gpu, dtype=dtype), torch.zeros(1, 1, 1, 2, device=gpu, dtype=dtype), -torch.ones(n, 2, device=gpu)
+    gated = selective_scan(one, one, A, none, none, skip=torch.ones(n, device=gpu), gate=z.view(1, 1, -1))[0]
+    for got in (y, gated):
+        assert torch.equal(torch.nan_to_num(got.view(-1).double(), nan=7.0), want)
+    unit = torch.ones(1, 1, 1, 1, device=gpu, dtype=dtype)
+    h = selective_scan(one, z.view(1, 1, -1), A[:, :1], unit, unit, softplus=True)[1].view(-1).double()
+    z = z.double()
+    s = torch.where(z > 0, z, 0 * z.clamp(-1, 1)) + torch.log1p((-z.abs()).exp())
+    assert torch.equal(h.isnan(), s.isnan()) and torch.equal(h.isinf(), s.isinf())
+    rest = torch.isfinite(s)
+    assert ((h - s)[rest].abs() <= STEP * s[rest].abs() + 2.0 ** -126).all()
