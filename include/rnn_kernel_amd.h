@@ -531,7 +531,9 @@ int rka_causal_conv_step(const void* x, long long ldx, const void* weight, const
  * NULL) and the states [batch, channels, states] dense float32.  states is at most 64.
  * `strides` is a host array of 12 element strides: (batch row, token) of x, dt and gate, (batch
  * row, token, group) of B and C; channels and states are contiguous.  lengths as in
- * rka_gated_delta_forward.  (No counterpart in the reference.)
+ * rka_gated_delta_forward.  tokens is at most 2^30, channels and the strides of a token 2^21; sizes of
+ * which a launch would have 2^32 threads are refused (2^26 rows of up to 16 channels, 2^24 of up to
+ * 64 by a forward with a reserve and the backward).  (No counterpart in the reference.)
  */
 /* Workspace of the calls below, and what a forward saves for its backward (0 for sizes that
  * the calls refuse). */

@@ -34,6 +34,7 @@ using namespace elem;
 
 constexpr int kTile = 16;       // tokens of a tile, channels of a wavefront's block, states of a block
 constexpr int kMaxStates = 64;  // N
+constexpr int kWaves = 4, kChannels = 16 * kWaves;  // of a workgroup of the gradients
 constexpr long long kMaxStride = 1 << 21;  // of a token, in elements: a tile's offsets are 32-bit
 
 struct Dims {
@@ -177,6 +178,9 @@ int make_dims(const char* what, int batch, int tokens, int channels, int states,
 int set_call(const char* what, Dims* d, const void* x, const void* dt, const float* A, const void* Bm, const void* C,
              const float* skip, const void* gate, const float* bias, const int* lengths, const long long* strides, int softplus,
              int dtype);
+// Whether every launch of a forward takes its size, and of the backward that it saves for: a call is
+// refused whole, and where it is for training.
+int check_launches(const char* what, const Dims& d, bool training);
 // States at the chunks' starts (forward) or the gradients at their ends (backward), in place
 // of the chunks' own: h_{c+1} = exp(A sum_c) h_c + own_c, from `first` ([batch, D, N] or null).
 int launch_join(const Dims& d, float* own, const float* sums, const float* first, bool backward, hipStream_t s);

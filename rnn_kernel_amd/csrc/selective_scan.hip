@@ -217,7 +217,6 @@ int forward(const Dims& d, const float* initial, T* y, float* final_state, float
     const Layout l = forward_layout(d);
     float *states = reinterpret_cast<float*>(ws + l.states), *sums = reinterpret_cast<float*>(ws + l.sums);
     const long long blocks = channel_blocks(d, 16) * d.B;
-    RKA_RETURN_IF_ERR(check_grid(blocks * d.chunks, 64, "selective_scan_forward"));
     if (d.chunks > 1) {
         hipLaunchKernelGGL((chunk_kernel<T, NB, true>), dim3((unsigned)(blocks * (d.chunks - 1))), dim3(64), 0, s, d, states,
                            sums, nullptr, nullptr, nullptr, nullptr);
@@ -254,9 +253,15 @@ int chunk_tokens(int tokens, long long waves) {
     return tiles * kTile;
 }
 
+int check_launches(const char* what, const Dims& d, bool training) {
+    const long long chunks = (long long)d.B * d.chunks;
+    RKA_RETURN_IF_ERR(check_grid(channel_blocks(d, 16) * chunks, 64, what));
+    if (d.chunks > 1) RKA_RETURN_IF_ERR(check_grid(((long long)d.B * d.N * d.D + 255) / 256, 256, what));
+    return training ? check_grid(channel_blocks(d, kChannels) * chunks, kWaves * 64, what) : 0;
+}
+
 int launch_join(const Dims& d, float* own, const float* sums, const float* first, bool backward, hipStream_t s) {
     const long long blocks = ((long long)d.B * d.N * d.D + 255) / 256;
-    RKA_RETURN_IF_ERR(check_grid(blocks, 256, "selective_scan"));
     hipLaunchKernelGGL(join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, d, own, sums, first, backward ? 1 : 0);
     RKA_RETURN_IF_HIP(hipGetLastError());
     return 0;
@@ -268,6 +273,8 @@ int make_dims(const char* what, int batch, int tokens, int channels, int states,
     if (channels < 1 || states < 1 || groups < 1 || channels % groups != 0)
         return fail(RKA_ERR_INVALID_ARGUMENT, name + ": channels and states must be >= 1, channels a multiple of groups");
     if (states > kMaxStates) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": more than 64 states per channel");
+    // (what a kernel counts in 32 bits)
+    if (tokens > (1 << 30)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": more than 2^30 tokens");
     *d = Dims{};
     d->B = batch;
     d->T = tokens;
@@ -276,8 +283,6 @@ int make_dims(const char* what, int batch, int tokens, int channels, int states,
     d->G = groups;
     d->chunk = chunk_tokens(tokens, channel_blocks(*d, 16) * std::max(batch, 1));
     d->chunks = tokens > 0 ? (tokens - 1) / d->chunk + 1 : 1;
-    // (what a kernel counts in 32 bits)
-    if (tokens > (1 << 30)) return fail(RKA_ERR_UNSUPPORTED_SHAPE, name + ": more than 2^30 tokens");
     return 0;
 }
 
@@ -345,6 +350,7 @@ int rka_selective_scan_forward(const void* x, const void* dt, const float* A, co
     RKA_RETURN_IF_ERR(set_call("selective_scan_forward", &d, x, dt, A, B, C, skip, gate, dt_bias, lengths, strides, softplus, dtype));
     if (batch == 0) return 0;
     if ((tokens > 0 && !y) || !final_state) return fail(RKA_ERR_INVALID_ARGUMENT, "selective_scan_forward: null tensor pointer");
+    RKA_RETURN_IF_ERR(check_launches("selective_scan_forward", d, reserve != nullptr));
     RKA_RETURN_IF_ERR(check_workspace(workspace, workspace_bytes, forward_layout(d).total, "selective_scan_forward"));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);

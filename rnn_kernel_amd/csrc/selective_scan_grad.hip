@@ -16,8 +16,6 @@ namespace rka {
 namespace scan {
 namespace {
 
-constexpr int kWaves = 4, kChannels = 16 * kWaves;  // of a workgroup
-
 // Where a workgroup stands.
 struct Place {
     int g, ch, b, chunk, len, t0, t1, t_end, block;
@@ -399,18 +397,19 @@ __global__ __launch_bounds__(kWaves * 64) void grads_kernel(Dims d, const float*
 // dB and dC [B][T][G][N] over a group's channel blocks.
 template <typename T>
 __global__ __launch_bounds__(256) void inputs_kernel(Dims d, const float* bc, int per_group, T* dB, T* dC) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, width = 2LL * d.N;
-    if (i >= (long long)d.B * d.T * d.G * width) return;
-    const int in = (int)(i % width), g = (int)(i / width % d.G);
-    const long long row = i / width / d.G;
-    const int b = (int)(row / d.T), t = (int)(row % d.T);
-    float sum = 0.f;
-    if (t < row_length(d.lengths, b, d.T)) {
-        const float* p = bc + ((size_t)g * per_group * d.B * d.T + row) * width + in;
+    const long long width = 2LL * d.N, total = (long long)d.B * d.T * d.G * width;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int in = (int)(i % width), g = (int)(i / width % d.G);
+        const long long row = i / width / d.G;
+        const int b = (int)(row / d.T), t = (int)(row % d.T);
+        float sum = 0.f;
+        if (t < row_length(d.lengths, b, d.T)) {
+            const float* p = bc + ((size_t)g * per_group * d.B * d.T + row) * width + in;
 #pragma unroll 8
-        for (int k = 0; k < per_group; ++k) sum += p[(size_t)k * d.B * d.T * width];
+            for (int k = 0; k < per_group; ++k) sum += p[(size_t)k * d.B * d.T * width];
+        }
+        (in < d.N ? dB : dC)[(row * d.G + g) * d.N + in % d.N] = from_f32<T>(sum);
     }
-    (in < d.N ? dB : dC)[(row * d.G + g) * d.N + in % d.N] = from_f32<T>(sum);
 }
 
 // dA, dskip and dbias over batch rows and chunks.
@@ -460,8 +459,6 @@ int backward(const Dims& d, const float* kept, const T* dy, const float* dfinal,
     out.a = reinterpret_cast<float*>(ws + l.a);
     out.vec = reinterpret_cast<float*>(ws + l.vec);
     const long long small = channel_blocks(d, 16) * d.B * d.chunks, large = channel_blocks(d, kChannels) * d.B * d.chunks;
-    RKA_RETURN_IF_ERR(check_grid(small, 64, "selective_scan_backward"));
-    RKA_RETURN_IF_ERR(check_grid(large, kWaves * 64, "selective_scan_backward"));
     if (d.chunks > 1) {
         hipLaunchKernelGGL((ends_kernel<T, NB>), dim3((unsigned)(small / d.chunks * (d.chunks - 1))), dim3(64), 0, s, d, dy, ends,
                            sums);
@@ -470,9 +467,8 @@ int backward(const Dims& d, const float* kept, const T* dy, const float* dfinal,
     }
     hipLaunchKernelGGL((grads_kernel<T, NB>), dim3((unsigned)large), dim3(kWaves * 64), 0, s, d, kept, ends, dfinal, dy, out);
     RKA_RETURN_IF_HIP(hipGetLastError());
-    const long long items = ((long long)d.B * d.T * d.G * 2 * d.N + 255) / 256;
+    const long long items = std::min(((long long)d.B * d.T * d.G * 2 * d.N + 255) / 256, 1LL << 23);
     if (items > 0) {
-        RKA_RETURN_IF_ERR(check_grid(items, 256, "selective_scan_backward"));
         hipLaunchKernelGGL((inputs_kernel<T>), dim3((unsigned)items), dim3(256), 0, s, d, out.bc,
                            (int)(channel_blocks(d, kChannels) / d.G), dB, dC);
         RKA_RETURN_IF_HIP(hipGetLastError());
@@ -525,6 +521,7 @@ int rka_selective_scan_backward(const void* x, const void* dt, const float* A, c
     if (batch < 1) return fail(RKA_ERR_INVALID_ARGUMENT, "selective_scan_backward: batch must be >= 1");
     if (!reserve || (tokens > 0 && (!grad_x || !grad_dt || !grad_B || !grad_C || (gate && !grad_gate))))
         return fail(RKA_ERR_INVALID_ARGUMENT, "selective_scan_backward: null tensor pointer");
+    RKA_RETURN_IF_ERR(check_launches("selective_scan_backward", d, true));
     RKA_RETURN_IF_ERR(check_workspace(workspace, workspace_bytes, backward_layout(d).total, "selective_scan_backward"));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const float* kept = static_cast<const float*>(reserve);

@@ -61,3 +61,32 @@ def test_more_logits_than_a_launch_has_in_python(gpu):
     with pytest.raises(ValueError, match="more than a launch may have"):
         linear_cross_entropy(x, w, target)
     assert torch.cuda.max_memory_allocated() == before
+
+
+def test_a_scan_for_training_is_refused_where_its_gradients_would_be(hip_lib):
+    """(2^24 rows of one token: a launch of the gradients has four wavefronts where the forward's has one.)"""
+    import ctypes
+
+    strides, P, sizes = (ctypes.c_longlong * 12)(), 4096, (2 ** 24, 1, 16, 1, 1)
+    assert hip_lib.rka_selective_scan_forward(P, P, P, P, P, None, None, None, None, None, P, P, P, P, 2 ** 60, *sizes, strides, 0, 0,
+                                              None) == 1004
+    assert "more workgroups than a launch may have" in hip_lib.rka_last_error().decode()
+    assert hip_lib.rka_selective_scan_backward(P, P, P, P, P, None, None, None, None, P, P, None, P, P, P, P, P, None, None, None, None,
+                                               P, 2 ** 60, *sizes, strides, 0, 0, None) == 1004
+
+
+@pytest.mark.gpu
+def test_more_gradients_of_B_and_C_than_a_launch_has_threads(gpu):
+    """2^32 of them, of 2^19 tokens that are all alike and forget at once: every token's are those of the
+    first, which are products of powers of two."""
+    from rnn_kernel_amd import selective_scan
+
+    T, G = 2 ** 19, 64
+    x, dt = (torch.full((1, 1, G), v, device=gpu, dtype=torch.bfloat16).expand(1, T, G) for v in (2.0, 1.0))
+    Bm, C = (torch.full((1, 1, G, 64), v, device=gpu, dtype=torch.bfloat16).expand(1, T, G, 64).detach() for v in (0.5, 0.25))
+    Bm.requires_grad_(True), C.requires_grad_(True)
+    y, _ = selective_scan(x, dt, torch.full((G, 64), -1e4, device=gpu), Bm, C)
+    dB, dC = torch.autograd.grad(y, [Bm, C], torch.ones(1, 1, 1, device=gpu, dtype=torch.bfloat16).expand(1, T, G))
+    for g, want in ((dB, 0.5), (dC, 1.0)):
+        assert g.shape == (1, T, G, 64)
+        assert all(bool((part == want).all()) for part in g.split(2 ** 16, 1))
