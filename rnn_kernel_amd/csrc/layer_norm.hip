@@ -224,12 +224,16 @@ int forward(const void* x, long long ldx, const void* weight, const void* bias, 
             int size, double eps, hipStream_t s) {
     return with_form<T>(size, [&](auto waves, auto p) {
         constexpr int W = decltype(waves)::value, P = decltype(p)::value, kRows = W == 1 ? 4 : 1;
-        const long long blocks = ((long long)rows - 1) / kRows + 1;
-        RKA_RETURN_IF_ERR(check_grid(blocks, kThreads<W>, "layer_norm_forward"));
-        hipLaunchKernelGGL((forward_kernel<T, W, P>), dim3((unsigned)blocks), dim3(kThreads<W>), 0, s,
-                           static_cast<const T*>(x), ldx, static_cast<const T*>(weight), static_cast<const T*>(bias),
-                           static_cast<T*>(y), mean, rstd, rows, size, (float)eps);
-        RKA_RETURN_IF_HIP(hipGetLastError());
+        // (as many rows to a launch as it may have threads for)
+        constexpr int kMost = (int)(((1LL << 32) - 1) / kThreads<W>) * kRows;
+        for (long long row = 0; row < rows; row += kMost) {
+            const int some = (int)std::min<long long>(kMost, rows - row);
+            hipLaunchKernelGGL((forward_kernel<T, W, P>), dim3((unsigned)((some - 1) / kRows + 1)), dim3(kThreads<W>), 0, s,
+                               static_cast<const T*>(x) + row * ldx, ldx, static_cast<const T*>(weight), static_cast<const T*>(bias),
+                               static_cast<T*>(y) + row * size, mean ? mean + row : nullptr, rstd ? rstd + row : nullptr, some, size,
+                               (float)eps);
+            RKA_RETURN_IF_HIP(hipGetLastError());
+        }
         return 0;
     });
 }
