@@ -317,16 +317,37 @@ int check_sizes(const char* what, const Dims& d, int width, int dtype) {
     return check_dtype(dtype, what);
 }
 
+// Batch rows of a launch, of as many as it may have threads for.
+int rows_of(const dim3& blocks) {
+    return (int)std::max(1LL, std::min<long long>(blocks.z, ((1LL << 32) - 1) / (kLanes * kRuns) / ((long long)blocks.x * blocks.y)));
+}
+// `d`, and a tensor of `row` elements to a batch row, from row b on.
+Dims rows_from(const Dims& d, int b, int rows) {
+    Dims e = d;
+    e.B = std::min(rows, d.B - b);
+    if (d.lengths) e.lengths = d.lengths + b;
+    return e;
+}
+template <typename T>
+T* from(const void* p, long long b, long long row) {
+    return p ? static_cast<T*>(const_cast<void*>(p)) + b * row : nullptr;
+}
+
 template <typename T>
 int forward(const Dims& d, const void* x, const void* weight, const void* bias, const void* initial, void* y,
             void* final_state, int width, hipStream_t s) {
-    const dim3 blocks = grid(d, blocks_of_runs(d.T, kForwardRun));
-    RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_forward"));
+    const int runs = blocks_of_runs(d.T, kForwardRun), rows = rows_of(grid(d, runs));
+    const long long all = (long long)d.T * d.D, kept = (long long)(width - 1) * d.D;
     return with_form(d.D < kGroup, width, [&](auto small, auto w) {
-        hipLaunchKernelGGL((forward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d, static_cast<const T*>(x), static_cast<const T*>(weight),
-                           static_cast<const T*>(bias), static_cast<const T*>(initial), static_cast<T*>(y),
-                           static_cast<T*>(final_state));
-        RKA_RETURN_IF_HIP(hipGetLastError());
+        for (int b = 0; b < d.B; b += rows) {
+            const Dims e = rows_from(d, b, rows);
+            const dim3 blocks = grid(e, runs);
+            RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_forward"));
+            hipLaunchKernelGGL((forward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, e,
+                               from<T>(x, b, d.xb), from<T>(weight, 0, 0), from<T>(bias, 0, 0), from<T>(initial, b, kept),
+                               from<T>(y, b, all), from<T>(final_state, b, kept));
+            RKA_RETURN_IF_HIP(hipGetLastError());
+        }
         return 0;
     });
 }
@@ -335,16 +356,20 @@ template <typename T>
 int backward(const Dims& d, const void* dy, const void* dstate, const void* x, const void* weight, const void* bias,
              const void* initial, void* dx, void* dweight, void* dbias, void* dinitial, float* sums, int width,
              hipStream_t s) {
-    const int runs = blocks_of_runs((long long)d.T + width - 1, kBackwardSpan - width + 1);
+    const int runs = blocks_of_runs((long long)d.T + width - 1, kBackwardSpan - width + 1), rows = rows_of(grid(d, runs));
+    const long long all = (long long)d.T * d.D, kept = (long long)(width - 1) * d.D, of_sums = (long long)runs * (width + 1) * d.D;
     if (!dweight && !dbias) sums = nullptr;
-    const dim3 blocks = grid(d, runs);
-    RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_backward"));
     RKA_RETURN_IF_ERR(with_form(d.D < kGroup, width, [&](auto small, auto w) {
-        hipLaunchKernelGGL((backward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, d,
-                           static_cast<const T*>(dy), static_cast<const T*>(dstate), static_cast<const T*>(x),
-                           static_cast<const T*>(weight), static_cast<const T*>(bias), static_cast<const T*>(initial),
-                           static_cast<T*>(dx), static_cast<T*>(dinitial), sums);
-        RKA_RETURN_IF_HIP(hipGetLastError());
+        for (int b = 0; b < d.B; b += rows) {
+            const Dims e = rows_from(d, b, rows);
+            const dim3 blocks = grid(e, runs);
+            RKA_RETURN_IF_ERR(check_grid((long long)blocks.x * blocks.y * blocks.z, kLanes * kRuns, "causal_conv_backward"));
+            hipLaunchKernelGGL((backward_kernel<decltype(small)::value, T, decltype(w)::value>), blocks, dim3(kLanes, kRuns), 0, s, e,
+                               from<T>(dy, b, all), from<T>(dstate, b, kept), from<T>(x, b, d.xb), from<T>(weight, 0, 0),
+                               from<T>(bias, 0, 0), from<T>(initial, b, kept), from<T>(dx, b, all), from<T>(dinitial, b, kept),
+                               from<float>(sums, b, of_sums));
+            RKA_RETURN_IF_HIP(hipGetLastError());
+        }
         return 0;
     }));
     if (sums) {
