@@ -602,6 +602,13 @@ int rka_cross_entropy_backward(const float* grad_loss, const void* x, long long 
                                void* workspace, size_t workspace_bytes, int rows, int inputs, int outputs, int reduction, int dtype,
                                void* stream);
 
+/* The forms that these calls take (host only), for tests and tuning.  `aligned`: whether the
+ * weight's address and row stride are multiples of 16 bytes.  Writes the first min(n_out, 9) of
+ * {RKA_LINEAR_FORM_DIRECT or _TILES of the logits and dl, edge of a tile of the forward's logits,
+ * pieces of the vocabulary, columns of a piece at most, edges of dl's tiles and of grad_x's, its slices,
+ * edge of grad_weight's, its slices}. */
+int rka_describe_cross_entropy(int rows, int inputs, int outputs, int dtype, int aligned, int* out, int n_out);
+
 #ifdef __cplusplus
 }
 #endif

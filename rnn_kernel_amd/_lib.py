@@ -88,6 +88,7 @@ SIGNATURES = {
     "rka_cross_entropy_backward_workspace_bytes": (_SZ, [_I] * 4),
     "rka_cross_entropy_forward": (_I, [_P, _LL, _P, _LL, _P, _P, _I, _LL, _P, _P, _P, _SZ] + [_I] * 5 + [_P]),
     "rka_cross_entropy_backward": (_I, [_P, _P, _LL, _P, _LL] + [_P] * 6 + [_SZ] + [_I] * 5 + [_P]),
+    "rka_describe_cross_entropy": (_I, [_I] * 5 + [ctypes.POINTER(_I), _I]),
     "rka_describe_gated_delta": (_I, [_I] * 5 + [ctypes.POINTER(_I), _I]),
     "rka_describe_linear": (_I, [_I] * 6 + [ctypes.POINTER(_I), _I]),
     "rka_gated_delta_step": (_I, [_P] * 7 + [_I, _P] + [_I] * 5 + [_LLP] + [_I] * 3 + [ctypes.c_double, _P]),
@@ -287,6 +288,15 @@ def describe_linear(product: str, rows: int, outputs: int, inputs: int, dtype: i
     check(load().rka_describe_linear(LINEAR_PRODUCTS[product], rows, outputs, inputs, dtype, int(aligned), out, 4),
           "rka_describe_linear")
     return dict(form=LINEAR_FORMS[out[0]], edge=out[1], slices=out[2], workgroups=out[3])
+
+
+def describe_cross_entropy(rows: int, inputs: int, outputs: int, dtype: int, aligned: bool = True) -> dict:
+    """Form, tile edges, pieces of the vocabulary and slices of the cross entropy's products;
+    see rka_describe_cross_entropy."""
+    out = (ctypes.c_int * 9)()
+    check(load().rka_describe_cross_entropy(rows, inputs, outputs, dtype, int(aligned), out, 9), "rka_describe_cross_entropy")
+    keys = ("form", "forward", "pieces", "piece", "slopes", "grad_x", "slices_x", "grad_weight", "slices_weight")
+    return dict(zip(keys, (LINEAR_FORMS[out[0]], *out[1:])))
 
 
 def set_exchange_stores(mode: int) -> None:

@@ -685,6 +685,26 @@ size_t rka_cross_entropy_backward_workspace_bytes(int rows, int inputs, int outp
     return fits(rows, inputs, outputs, dtype, true) ? backward_layout(sizes_of(rows, inputs, outputs, dtype)).total : 0;
 }
 
+int rka_describe_cross_entropy(int rows, int inputs, int outputs, int dtype, int aligned, int* out, int n_out) {
+    clear_error();
+    if (!out || n_out < 1) return fail(RKA_ERR_INVALID_ARGUMENT, "describe_cross_entropy: out must be non-NULL and n_out >= 1");
+    RKA_RETURN_IF_ERR(check("describe_cross_entropy", rows, inputs, outputs, 0, 0, RKA_REDUCE_MEAN, dtype));
+    const Sizes z = sizes_of(rows, inputs, outputs, dtype);
+    const Backward l = backward_layout(z);
+    const auto edge = [](Tile t) { return t == TILE_256 ? 256 : t == TILE_128 ? 128 : 64; };
+    const int v[9] = {aligned && whole_stages(inputs, z.esize) ? RKA_LINEAR_FORM_DIRECT : RKA_LINEAR_FORM_TILES,
+                      edge(z.tile),
+                      (outputs - 1) / l.piece + 1,
+                      l.piece,
+                      edge(l.tile),
+                      edge(l.of_x.tile),
+                      l.of_x.slices,
+                      edge(l.of_w.tile),
+                      l.of_w.slices};
+    for (int i = 0; i < 9 && i < n_out; ++i) out[i] = v[i];
+    return 0;
+}
+
 int rka_cross_entropy_forward(const void* x, long long ldx, const void* weight, long long ldw, const void* bias,
                               const void* target, int target_is_64bit, long long ignore_index, float* loss, void* reserve,
                               void* workspace, size_t workspace_bytes, int rows, int inputs, int outputs, int reduction, int dtype,
