@@ -9,7 +9,7 @@ namespace {
 
 // One block of channels through one chunk.  STATES_ONLY: from nothing to the chunk's own state
 // and the sum of its steps; else from the state at its start to the outputs.  16384 tokens of 2048
-// channels, 16 states, bf16: 101 and 159 us.  Bound by vector instructions: a token takes 20 for
+// channels, 16 states, bf16: 101 and 156 us.  Bound by vector instructions: a token takes 20 for
 // its four states of a lane (and the exponentials twice an instruction's time), 2.5 for its sum
 // and a share of some 10 of what the tile makes of its inputs; they issue in three quarters of the
 // clocks.  Memory alone would take 56.  Four wavefronts to a SIMD hold the registers; five with

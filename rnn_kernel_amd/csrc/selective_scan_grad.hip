@@ -7,7 +7,9 @@
 //
 // 4 x 2048 tokens of 2048 channels, 16 states, bf16: chunks' ends 60 us, gradients 270, the sums
 // behind them 12.  Bound by vector instructions, some 105 a token and lane (16 of them the sums
-// over channels), at two wavefronts to a SIMD, which is what the states in LDS leave.
+// over channels), at two wavefronts to a SIMD, which is what the states in LDS leave.  From 33 states
+// on LDS and registers leave one: 4 x 2048 tokens of 1024 channels 177 us backward with 16 states, 304 with
+// 32, 803 with 48, 818 with 64.
 #include "selective_scan.h"
 
 #include <algorithm>

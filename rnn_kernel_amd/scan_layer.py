@@ -78,7 +78,8 @@ class SelectiveScan(nn.Module):
     def forward(self, x: torch.Tensor, state: Optional[State] = None,
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, State]:
         """(y, state) of x [batch, tokens, size], as causal_conv and selective_scan have states
-        and lengths; batch at most 65535 and tokens at most 2^20, as causal_conv takes them."""
+        and lengths; batch at most 65535 and tokens at most 2^20, as causal_conv takes them. Behind a
+        row's end y is x, which has to be finite there for gradients of the weights."""
         if x.dim() != 3 or x.size(-1) != self.size:
             raise ValueError(f"SelectiveScan: x must have shape [batch, tokens, {self.size}]")
         before, h = (None, None) if state is None else state
