@@ -114,3 +114,34 @@ def test_what_is_not_finite_or_far(gpu, dtype):
     assert torch.equal(h.isnan(), s.isnan()) and torch.equal(h.isinf(), s.isinf())
     rest = torch.isfinite(s)
     assert ((h - s)[rest].abs() <= STEP * s[rest].abs() + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_far_below_0_everywhere(gpu, dtype):
+    """Where exp(-z) is no float32 (z below -88.7), and next to it: silu and its slope are below 2^-115 there,
+    and no NaN; steps of as much are the number itself, or 0."""
+    from rnn_kernel_amd import causal_conv, causal_conv_step, selective_scan, selective_step
+
+    z = torch.cat([torch.linspace(-400, -87, 20001), -torch.logspace(2, 38, 5001)]).to(gpu, dtype)
+    n = z.numel()
+    w = torch.tensor([[0.0, 1.0]], device=gpu, dtype=dtype).expand(n, 2)
+    x = z.view(1, 1, -1).clone().requires_grad_(True)
+    y = causal_conv(x, w, activation="silu")[0]
+    found = [y, torch.autograd.grad(y.sum(), x)[0]]
+    one, none = torch.ones(1, 1, n, device=gpu, dtype=dtype), torch.zeros(1, 1, 1, 2, device=gpu, dtype=dtype)
+    A, skip = -torch.ones(n, 2, device=gpu), torch.ones(n, device=gpu)
+    v, gate = one.clone().requires_grad_(True), z.view(1, 1, -1).clone().requires_grad_(True)
+    y = selective_scan(v, one, A, none, none, skip=skip, gate=gate)[0]
+    found += [y, *torch.autograd.grad(y.sum(), [v, gate])]
+    with torch.no_grad():
+        found.append(causal_conv_step(z.view(1, -1), torch.zeros(1, 1, n, device=gpu, dtype=dtype), w, activation="silu"))
+        found.append(selective_step(one[0], one[0], A, none[0], none[0], torch.zeros(1, n, 2, device=gpu), skip=skip, gate=z.view(1, -1)))
+    for t in found:
+        assert (t.abs() <= 2.0 ** -115).all()
+    unit = torch.ones(1, 1, 1, 1, device=gpu, dtype=dtype)
+    for sign in (1, -1):
+        raw = (sign * z).view(1, 1, -1).clone().requires_grad_(True)
+        h = selective_scan(one, raw, A[:, :1], unit, unit, softplus=True)[1].view(-1)
+        (grad,) = torch.autograd.grad(h.sum(), raw)
+        want, slope = (torch.zeros_like(z), 0.0) if sign > 0 else (-z, 1.0)
+        assert ((h - want.float()).abs() <= 2.0 ** -115).all() and ((grad.float() - slope).abs() <= 2.0 ** -115).all()
